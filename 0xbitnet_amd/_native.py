@@ -113,6 +113,22 @@ SIGNATURES = {
     "oxb_attn_decode_head": (C.c_int, [vp, vp, vp, vp, i32, C.c_size_t, i32, i32, i32, i32, i32,
                                        i32, vp, vp]),
     "oxb_attn_prefill": (C.c_int, [vp, vp, vp, i32, i32, i32, i32, i32, i32, vp, vp]),
+    "oxb_kv8_bytes": (sz, [i32, i32, i32]),
+    "oxb_kv8_append": (C.c_int, [vp, sz, i32, i32, i32, i32, i32, vp, vp, sz, sz, i32, vp, i32, i32,
+                                 i32, vp, vp]),
+    "oxb_kv8_read": (C.c_int, [vp, sz, i32, i32, i32, i32, i32, vp, i32, i32, i32, vp, i32, vp, vp,
+                               vp]),
+    "oxb_attn_decode_kv8_ws_bytes": (sz, [i32, i32, i32, i32, i32]),
+    "oxb_attn_decode_kv8": (C.c_int, [vp, vp, sz, i32, vp, i32, i32, i32, i32, i32, i32, i32, vp, vp,
+                                      sz, vp]),
+    "oxb_attn_prefill_kv8_ws_bytes": (sz, [i32, i32, i32, i32, i32, i32]),
+    "oxb_attn_prefill_kv8": (C.c_int, [vp, vp, i32, i32, i32, i32, i32, i32, i32, i32, vp, vp, sz,
+                                       vp]),
+    "oxb_kv8_evict_ws_bytes": (sz, [i32, i32, i32, i32]),
+    "oxb_kv8_evict": (C.c_int, [vp, sz, i32, vp, sz, i32, vp, i32, vp, i32, i32, i32, i32, i32, i32,
+                                i32, vp, sz, vp]),
+    "oxb_logits_rules": (C.c_int, [vp, sz, i32, i32, vp, vp, vp, i32, vp, vp, vp, i32, vp, sz, vp,
+                                   sz, vp]),
     "oxb_embedding": (C.c_int, [vp, i32, i32, vp, i32, vp, vp, vp]),
     "oxb_lm_head_argmax": (C.c_int, [vp, vp, f32, vp, i32, i32, vp, vp, vp, i32, vp]),
     "oxb_repack_lm": (C.c_int, [vp, vp, i32, i32, vp]),

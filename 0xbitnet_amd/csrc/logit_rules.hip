@@ -1,0 +1,126 @@
+// Rules on logits for gfx950: penalties for tokens that a sequence's history
+// holds, biases on single ids and a mask of allowed ids, for a batch of rows
+// before the draw (oxb_sample_device) or an argmax.  The reference knows the
+// repetition penalty alone, one row at a time on the host
+// (rs/sampling.rs:14-24).
+//
+// One pass: a workgroup takes kLrChunk logits of a row, counts the row's
+// history ids that fall among them and finds each id's last bias entry in LDS,
+// and writes the ruled values.  Bound by the logits' bytes once there are
+// rows enough; every workgroup of a row reads its whole history (from L2).
+#include "oxb_common.h"
+#include "oxb_kernels.h"
+
+namespace oxb {
+
+constexpr int kLrThreads = 512;
+constexpr int kLrPer = 8;                        // logits per thread
+constexpr int kLrChunk = kLrThreads * kLrPer;
+
+struct RulesArgs {
+    const float *logits;
+    size_t stride;
+    int V;
+    const float *pen;       // [rows][3] repeat, frequency, presence
+    const int *hist, *hist_off;
+    int n_hist;
+    const int *bias_ids;
+    const float *bias;
+    const int *bias_off;
+    int n_bias;
+    const uint32_t *mask;
+    size_t mask_stride;
+    float *out;
+    size_t out_stride;
+};
+
+__global__ __launch_bounds__(kLrThreads) void logit_rules_kernel(RulesArgs a) {
+    __shared__ int cnt[kLrChunk];    // occurrences in the history
+    __shared__ int last[kLrChunk];   // 1 + the last bias entry of the id
+    const int r = blockIdx.y, base = blockIdx.x * kLrChunk, tid = threadIdx.x;
+    const int n = min(kLrChunk, a.V - base);
+    const float *lg = a.logits + (size_t)r * a.stride + base;
+    float x[kLrPer];
+#pragma unroll
+    for (int u = 0; u < kLrPer; ++u) {
+        x[u] = lg[min(tid + u * kLrThreads, n - 1)];
+        cnt[tid + u * kLrThreads] = 0;
+        last[tid + u * kLrThreads] = 0;
+    }
+    // ranges of this row, kept inside the lists whatever the offsets say
+    int h0 = 0, h1 = 0, b0 = 0, b1 = 0;
+    if (a.pen && a.n_hist > 0) {
+        h0 = min(max(a.hist_off[r], 0), a.n_hist);
+        h1 = min(a.hist_off[r + 1], a.n_hist);
+    }
+    if (a.n_bias > 0) {
+        b0 = min(max(a.bias_off[r], 0), a.n_bias);
+        b1 = min(a.bias_off[r + 1], a.n_bias);
+    }
+    lds_barrier();
+    for (int j = h0 + tid; j < h1; j += kLrThreads) {
+        const unsigned i = (unsigned)a.hist[j] - (unsigned)base;
+        if (i < (unsigned)n) atomicAdd(&cnt[i], 1);
+    }
+    for (int j = b0 + tid; j < b1; j += kLrThreads) {
+        const unsigned i = (unsigned)a.bias_ids[j] - (unsigned)base;
+        if (i < (unsigned)n) atomicMax(&last[i], j + 1);
+    }
+    lds_barrier();
+    float rep = 1.0f, freq = 0.0f, pres = 0.0f;
+    if (a.pen) {
+        rep = a.pen[3 * r];
+        freq = a.pen[3 * r + 1];
+        pres = a.pen[3 * r + 2];
+    }
+    const uint32_t *mask = a.mask ? a.mask + (size_t)r * a.mask_stride : nullptr;
+    float *out = a.out + (size_t)r * a.out_stride + base;
+#pragma unroll
+    for (int u = 0; u < kLrPer; ++u) {
+        const int i = tid + u * kLrThreads;
+        if (i >= n) continue;
+        float y = x[u];
+        const int c = cnt[i], b = last[i];
+        if (c > 0) {
+            y = y > 0.0f ? y / rep : y * rep;
+            y = y - (freq * (float)c + pres);
+        }
+        if (b > 0) y = y + a.bias[b - 1];
+        if (mask && !(mask[(base + i) >> 5] >> ((base + i) & 31) & 1)) y = -__builtin_inff();
+        out[i] = y;
+    }
+}
+
+}  // namespace oxb
+
+using namespace oxb;
+
+extern "C" int oxb_logits_rules(const float *logits, size_t stride, int n_rows, int V,
+                                const float *penalties, const int32_t *history,
+                                const int *history_off, int n_history, const int32_t *bias_ids,
+                                const float *bias, const int *bias_off, int n_bias,
+                                const uint32_t *mask, size_t mask_stride, float *out,
+                                size_t out_stride, void *stream) {
+    clear_error();
+    OXB_REQUIRE(logits && out, "logit rules: logits or out is NULL");
+    OXB_REQUIRE(n_rows >= 1 && n_rows <= 65535, "logit rules: %d rows", n_rows);
+    OXB_REQUIRE(V >= 1 && V <= (1 << 30), "logit rules: vocabulary %d", V);
+    OXB_REQUIRE(n_rows == 1 || (stride >= (size_t)V && out_stride >= (size_t)V),
+                "logit rules: row strides %zu and %zu below the vocabulary", stride, out_stride);
+    OXB_REQUIRE(n_history >= 0 && (!penalties || n_history == 0 || (history && history_off)),
+                "logit rules: a history of %d tokens without ids or offsets", n_history);
+    OXB_REQUIRE(n_bias >= 0 && (n_bias == 0 || (bias_ids && bias && bias_off)),
+                "logit rules: %d biases without ids, values or offsets", n_bias);
+    OXB_REQUIRE(!mask || mask_stride == 0 || mask_stride >= ((size_t)V + 31) / 32,
+                "logit rules: mask rows of %zu words for %d ids", mask_stride, V);
+    const uintptr_t s = (uintptr_t)logits, d = (uintptr_t)out;
+    const size_t sb = 4 * ((n_rows - 1) * stride + V), db = 4 * ((n_rows - 1) * out_stride + V);
+    OXB_REQUIRE((s == d && (n_rows == 1 || stride == out_stride)) || s + sb <= d || d + db <= s,
+                "logit rules: out overlaps the logits without being them");
+    RulesArgs a{logits, stride, V, penalties, history, history_off, n_history, bias_ids, bias,
+                bias_off, n_bias, mask, mask_stride, out, out_stride};
+    hipLaunchKernelGGL(logit_rules_kernel, dim3((V + kLrChunk - 1) / kLrChunk, n_rows),
+                       dim3(kLrThreads), 0, (hipStream_t)stream, a);
+    OXB_CHECK_HIP(hipGetLastError());
+    return 0;
+}

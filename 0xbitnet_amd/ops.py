@@ -263,6 +263,118 @@ def attn_prefill(q: np.ndarray, kcache: np.ndarray, vcache: np.ndarray, n_tok: i
     return out.download()
 
 
+KV8_INT8, KV8_E4M3, KV8_BLOCK = 0, 1, 32   # include/oxbitnet_ops.h OXB_KV8_*
+
+
+class Kv8Cache:
+    """A batch's 8-bit KV cache (oxb_kv8_*, oxb_attn_*_kv8): numpy rows in, numpy out."""
+
+    def __init__(self, batch: int, Hkv: int, max_seq: int, fmt: int = KV8_INT8, hd: int = 128):
+        self.batch, self.Hkv, self.max_seq, self.fmt, self.hd = batch, Hkv, max_seq, fmt, hd
+        self.stride = lib().oxb_kv8_bytes(Hkv, hd, max_seq)
+        if not self.stride:
+            raise NativeError(f"no 8-bit cache of {Hkv} heads of {hd}, {max_seq} positions")
+        self.data = DeviceArray((batch, self.stride), np.uint8)
+
+    def append(self, k: np.ndarray, v: np.ndarray, pos, counts=None, stream=None) -> None:
+        """f16 rows [batch][Hkv][n][128] at each sequence's position."""
+        k, v = (np.ascontiguousarray(x, np.float16) for x in (k, v))
+        n = k.shape[2]
+        dk, dv = (DeviceArray.from_host(x.view(np.uint16)) for x in (k, v))
+        dp = DeviceArray.from_host(np.ascontiguousarray(pos, np.int32))
+        dc = DeviceArray.from_host(np.ascontiguousarray(counts, np.int32)) if counts is not None else None
+        check(lib().oxb_kv8_append(self.data.ptr, self.stride, self.fmt, self.batch, self.Hkv, self.hd,
+                                   self.max_seq, dk.ptr, dv.ptr, self.Hkv * n * self.hd, n * self.hd, 0,
+                                   dp.ptr, 1, 0, n, _p(dc), stream), "kv8_append")
+        sync()
+
+    def read(self, pos, n: int, length=None):
+        """The values of n positions from each sequence's pos on: k, v f32 [batch][Hkv][n][128]."""
+        dp = DeviceArray.from_host(np.ascontiguousarray(pos, np.int32))
+        dl = DeviceArray.from_host(np.ascontiguousarray(length, np.int32)) if length is not None else None
+        k, v = (DeviceArray((self.batch, self.Hkv, n, self.hd), np.float32) for _ in "kv")
+        check(lib().oxb_kv8_read(self.data.ptr, self.stride, self.fmt, self.batch, self.Hkv, self.hd,
+                                 self.max_seq, dp.ptr, 1, 0, n, _p(dl), 1, k.ptr, v.ptr, None), "kv8_read")
+        sync()
+        return k.download(), v.download()
+
+    def weights(self) -> np.ndarray:
+        """Each block's accumulated attention weight [batch][Hkv][blocks]."""
+        nb, al = (self.max_seq + KV8_BLOCK - 1) // KV8_BLOCK, lambda b: (b + 255) // 256 * 256
+        at = al(self.Hkv * nb * 8192) + al(self.Hkv * nb * 8)
+        raw = self.data.download()[:, at:at + self.Hkv * nb * 4]
+        return np.ascontiguousarray(raw).view(np.float32).reshape(self.batch, self.Hkv, nb)
+
+    def attn_decode(self, q: np.ndarray, pos, add_weights: bool = False) -> np.ndarray:
+        """q f32 [batch][H*128]; sequence z attends over pos[z] + 1 positions."""
+        q = np.ascontiguousarray(q, np.float32).reshape(self.batch, -1)
+        H = q.shape[1] // self.hd
+        dq, dp = DeviceArray.from_host(q), DeviceArray.from_host(np.ascontiguousarray(pos, np.int32))
+        out = DeviceArray(q.shape, np.float32)
+        n = lib().oxb_attn_decode_kv8_ws_bytes(self.batch, H, self.Hkv, self.hd, self.max_seq)
+        ws = DeviceArray((max(n, 16),), np.uint8)
+        check(lib().oxb_attn_decode_kv8(dq.ptr, self.data.ptr, self.stride, self.fmt, dp.ptr, 1, self.batch,
+                                        H, self.Hkv, self.hd, self.max_seq, int(add_weights), out.ptr,
+                                        ws.ptr, n, None), "attn_decode_kv8")
+        sync()
+        return out.download()
+
+    def attn_prefill(self, q: np.ndarray, pos0: int, slot: int = 0, add_weights: bool = False) -> np.ndarray:
+        """q f32 [n][H*128] of sequence `slot` at positions pos0.., causal."""
+        q = np.ascontiguousarray(np.atleast_2d(q), np.float32)
+        n, H = q.shape[0], q.shape[1] // self.hd
+        dq, out = DeviceArray.from_host(q), DeviceArray(q.shape, np.float32)
+        b = lib().oxb_attn_prefill_kv8_ws_bytes(n, pos0, H, self.Hkv, self.hd, int(add_weights))
+        ws = DeviceArray((max(b, 16),), np.uint8)
+        check(lib().oxb_attn_prefill_kv8(dq.ptr, self.data.offset(slot * self.stride), self.fmt, n, pos0, H,
+                                         self.Hkv, self.hd, self.max_seq, int(add_weights), out.ptr, ws.ptr,
+                                         b, None), "attn_prefill_kv8")
+        sync()
+        return out.download()
+
+    def evict(self, length, budget: int, sink: int = 1, recent: int = 1, dst: "Kv8Cache | None" = None):
+        """Cut to `budget` blocks, in place or into dst; returns the new lengths."""
+        dst = dst or self
+        dl = DeviceArray.from_host(np.ascontiguousarray(length, np.int32))
+        n = lib().oxb_kv8_evict_ws_bytes(self.batch, self.Hkv, self.max_seq, budget)
+        ws = DeviceArray((max(n, 16),), np.uint8)
+        check(lib().oxb_kv8_evict(self.data.ptr, self.stride, self.max_seq, dst.data.ptr, dst.stride,
+                                  dst.max_seq, dl.ptr, 1, dl.ptr, 1, self.batch, self.Hkv, self.hd, budget,
+                                  sink, recent, ws.ptr, n, None), "kv8_evict")
+        sync()
+        return dl.download()
+
+
+def logits_rules(logits: np.ndarray, penalties=None, history=None, bias=None, mask=None) -> np.ndarray:
+    """Rules on logits [n][V] (oxb_logits_rules).  penalties: [n][3] repeat, frequency,
+    presence; history: a list of ids per row; bias: a list of (id, value) per row;
+    mask: uint32 words [n][w], or [w] for every row."""
+    x = np.ascontiguousarray(np.atleast_2d(logits), np.float32)
+    n, V = x.shape
+
+    def csr(lists, dtype):
+        off = np.concatenate([[0], np.cumsum([len(r) for r in lists])]).astype(np.int32)
+        flat = np.concatenate([np.asarray(r, dtype).reshape(-1) for r in lists]).astype(dtype)
+        return flat, off
+
+    up = lambda a: DeviceArray.from_host(np.ascontiguousarray(a)) if a is not None and a.size else None  # noqa: E731
+    dx = DeviceArray.from_host(x)
+    dpen = up(np.asarray(penalties, np.float32).reshape(n, 3)) if penalties is not None else None
+    h, ho = csr(history, np.int32) if history is not None else (np.empty(0, np.int32), None)
+    bi, bo = csr([[i for i, _ in r] for r in bias], np.int32) if bias is not None else (np.empty(0, np.int32), None)
+    bv = csr([[b for _, b in r] for r in bias], np.float32)[0] if bias is not None else None
+    dh, dho, dbi, dbo, dbv = up(h), up(ho), up(bi), up(bo), up(bv)
+    dm, words = None, 0
+    if mask is not None:
+        mask = np.ascontiguousarray(mask, np.uint32)
+        dm, words = up(mask), mask.shape[1] if mask.ndim == 2 else 0
+    out = DeviceArray((n, V), np.float32)
+    check(lib().oxb_logits_rules(dx.ptr, V, n, V, _p(dpen), _p(dh), _p(dho), h.size, _p(dbi), _p(dbv),
+                                 _p(dbo), bi.size, _p(dm), words, out.ptr, V, None), "logits_rules")
+    sync()
+    return out.download()
+
+
 def lm_head_argmax(x: np.ndarray, gamma: np.ndarray, eps: float, E_f16: np.ndarray):
     """Returns (logits [V], token, state)."""
     V, D = E_f16.shape

@@ -47,6 +47,13 @@ extern "C" {
  * a score and a probability row per query in LDS. */
 #define OXB_KV_F32_MAX_SEQ 16384
 
+/* The 8-bit KV cache (oxb_kv8_*): its code formats, the positions that share a
+ * scale, and the longest cache. */
+#define OXB_KV8_INT8 0
+#define OXB_KV8_E4M3 1
+#define OXB_KV8_BLOCK 32
+#define OXB_KV8_MAX_SEQ (1 << 24)
+
 /* ---- errors, device memory, streams, events (plumbing) ----------------- */
 const char *oxb_last_error(void);
 void *oxb_device_malloc(size_t bytes);
@@ -267,6 +274,99 @@ int oxb_attn_decode_noalloc(const float *q, const uint16_t *kcache, const uint16
 int oxb_attn_prefill(const float *q, const uint16_t *kcache, const uint16_t *vcache, int n_tok,
                      int pos0, int H, int Hkv, int hd, int max_seq, float *out, void *stream);
 
+/* ---- 8-bit KV cache --------------------------------------------------------- */
+/* K and V in 8 bits with one scale per block of 32 positions, KV head and
+ * tensor: half the bytes of the f16 cache, which is what decode attention
+ * reads.  value = code * scale, where a is the largest |x| among the block's
+ * rows so far:
+ *   OXB_KV8_INT8: scale = a / 127, code = 127 x / a to the nearest whole number
+ *   OXB_KV8_E4M3: scale = a / 448, code = 448 x / a to the nearest e4m3 number
+ * (ties to even; the code is that of the real quotient).  A block that holds
+ * an Inf or NaN has the scale NaN, and so has whatever reads it.
+ *
+ * One sequence's cache is one allocation of oxb_kv8_bytes(Hkv, 128, max_seq)
+ * bytes, 256-byte aligned, which needs no clearing; a batch is sequences
+ * cache_stride bytes apart (a multiple of 256).  With nb = ceil(max_seq / 32)
+ * blocks, each part 256-byte aligned:
+ *   codes   [Hkv][nb][8192]: 4096 K codes [32 positions][128 dims], then 4096
+ *           V codes [128 dims][32], position t of a V row at byte
+ *           16 (t/4 % 2) + 8 (t/16) + 4 (t/8 % 2) + t % 4; an int8 code q is
+ *           the byte q + 128
+ *   scales  [Hkv][nb][2] f32: K, V
+ *   weights [Hkv][nb] f32: accumulated attention weight (see the attention
+ *           calls), 0 when the block is begun
+ *   tails   [Hkv][2][32][128] f16: the K and V rows of the unfinished block,
+ *           from which the block is quantized again as it grows
+ * No counterpart in the reference (nn/attention.rs:23-48: f32 rows). */
+size_t oxb_kv8_bytes(int Hkv, int hd, int max_seq);
+
+/* Appends rows to each sequence: sequence z's counts[z] rows (n where counts
+ * is NULL; clamped to 0..n) at positions p = (pos ? pos[z*pos_stride] : 0) +
+ * pos0 and up.  pos and counts are device pointers.  Row i of head h is
+ * k + z*src_stride + h*src_head_stride + r*128 (f16; strides in elements,
+ * 16-byte aligned rows), r = i, or p + i with src_at_pos, which takes rows
+ * where the q|k|v projections leave them (a f16 cache [Hkv][max_seq][128] that
+ * all layers may share as scratch).  p is the position after the last one
+ * appended, or less within the same block (its later rows are dropped), or the
+ * start of any block.  The cache's content depends on the rows alone, not on how
+ * they were split over calls.  Positions past max_seq are dropped; p < 0 skips
+ * the sequence. */
+int oxb_kv8_append(void *cache, size_t cache_stride, int fmt, int batch, int Hkv, int hd,
+                   int max_seq, const uint16_t *k, const uint16_t *v, size_t src_stride,
+                   size_t src_head_stride, int src_at_pos, const int *pos, int pos_stride, int pos0,
+                   int n, const int *counts, void *stream);
+
+/* The values of n positions from p (as above, any p) on, as f32 rows k, v
+ * [batch][Hkv][n][128]; zeros for positions before 0, past max_seq or, where
+ * the device array len is given, from len[z*len_stride] on. */
+int oxb_kv8_read(const void *cache, size_t cache_stride, int fmt, int batch, int Hkv, int hd,
+                 int max_seq, const int *pos, int pos_stride, int pos0, int n, const int *len,
+                 int len_stride, float *k, float *v, void *stream);
+
+/* Decode attention over the 8-bit cache for a batch: sequence z's query
+ * q + z*H*128 attends over positions 0..pos[z*pos_stride] (device, at most
+ * max_seq - 1; below 0: the output is zeros), any H that is a multiple of Hkv,
+ * any length.  f32 in and out: codes are exact in f16, q and the softmax
+ * weights go through f16 MFMA as two parts each, sums are f32; not the
+ * reference's summation order (oxb_attn_decode keeps that).  With
+ * add_weights, the softmax weights of each block's positions, summed over the
+ * KV head's query heads, are added to the block's weight.  The result does not
+ * depend on timing.  ws: a device workspace of oxb_attn_decode_kv8_ws_bytes
+ * bytes, 256-byte aligned, any contents; calls that share one must not run
+ * concurrently.  Replaces nn/attention.rs:109-118 over this cache. */
+size_t oxb_attn_decode_kv8_ws_bytes(int batch, int H, int Hkv, int hd, int max_seq);
+int oxb_attn_decode_kv8(const float *q, void *cache, size_t cache_stride, int fmt, const int *pos,
+                        int pos_stride, int batch, int H, int Hkv, int hd, int max_seq,
+                        int add_weights, float *out, void *ws, size_t ws_bytes, void *stream);
+
+/* Causal prefill attention over one sequence's 8-bit cache: query i (q, out:
+ * [n_tok][H*128]) attends over positions 0..pos0 + i, which the cache holds
+ * already (append first).  Arithmetic, weights and workspace as above; the
+ * workspace may be 0 bytes and NULL for some shapes. */
+size_t oxb_attn_prefill_kv8_ws_bytes(int n_tok, int pos0, int H, int Hkv, int hd, int add_weights);
+int oxb_attn_prefill_kv8(const float *q, void *cache, int fmt, int n_tok, int pos0, int H, int Hkv,
+                         int hd, int max_seq, int add_weights, float *out, void *ws,
+                         size_t ws_bytes, void *stream);
+
+/* Cuts each sequence's cache to a budget of blocks.  A sequence of len[z] (device)
+ * positions in more than `budget` blocks keeps, per KV head, its first `sink`
+ * and last `recent` (>= 1: the unfinished one too) blocks and, of the others,
+ * those of the largest accumulated weight (ties: the first; NaN counts as the
+ * least), in their order; a shorter one keeps all.  len_out[z] = len[z] less
+ * 32 per dropped block.  Blocks move whole, with scale and weight: no value is
+ * rounded again.  Keys hold their rotation, so positions of later tokens go on
+ * counting for RoPE while the cache position is len_out (a rope table shifted by
+ * the dropped rows serves oxb_bitlinear_qkv / oxb_gemm_qkv).  dst is the cache
+ * itself, with the same max_seq and stride (cut in place), or another one
+ * without overlap that holds the budget or the whole length; len_out may be
+ * len.  ws: oxb_kv8_evict_ws_bytes bytes, 16-byte aligned, any contents, not
+ * shared by calls that run concurrently.  Format-independent. */
+size_t oxb_kv8_evict_ws_bytes(int batch, int Hkv, int max_seq, int budget);
+int oxb_kv8_evict(const void *cache, size_t cache_stride, int max_seq, void *dst, size_t dst_stride,
+                  int dst_max_seq, const int *len, int len_stride, int *len_out, int len_out_stride,
+                  int batch, int Hkv, int hd, int budget, int sink, int recent, void *ws,
+                  size_t ws_bytes, void *stream);
+
 /* ---- sampling ---------------------------------------------------------------- */
 /* One draw of rs/sampling.rs:4-80 over logits[V] (modified in place):
  * repetition penalty over recent[n_recent] (positive logits divided, others
@@ -292,6 +392,28 @@ size_t oxb_sample_ws_bytes(int V);
 int oxb_sample_device(const float *logits, int V, float temperature, size_t top_k,
                       float repeat_penalty, const int32_t *recent, int n_recent, const float *u,
                       int32_t *token, void *ws, size_t ws_bytes, void *stream);
+
+/* Rules on a batch's logits before the draw: logits row r (V values at
+ * logits + r*stride) to out row r (out may be logits).  All pointers are device
+ * memory.  For id i of row r, in this order, each step rounded to f32:
+ *   c = occurrences of i in history[history_off[r] .. history_off[r+1]);
+ *       where c > 0: x = x > 0 ? x / repeat : x * repeat, once however large c
+ *       is (oxb_sample_logits does it once per occurrence, the reference's
+ *       way), then x - (frequency * c + presence)
+ *   x + bias of the row's last entry j in bias_off[r] .. bias_off[r+1] with
+ *       bias_ids[j] == i
+ *   -inf unless bit i % 32 of word i / 32 of mask + r*mask_stride is set
+ *       (mask_stride 0: one mask for all rows)
+ * penalties: [n_rows][3] repeat, frequency, presence (NULL: none, the history
+ * is not read).  mask may be NULL; n_history, n_bias: entries of the whole
+ * lists, which bound what the offsets may reach; ids outside 0..V-1 are
+ * ignored.  Penalties extend rs/sampling.rs:14-24; biases and masks have no
+ * counterpart in the reference. */
+int oxb_logits_rules(const float *logits, size_t stride, int n_rows, int V, const float *penalties,
+                     const int32_t *history, const int *history_off, int n_history,
+                     const int32_t *bias_ids, const float *bias, const int *bias_off, int n_bias,
+                     const uint32_t *mask, size_t mask_stride, float *out, size_t out_stride,
+                     void *stream);
 
 /* ---- tokenizer (host) ------------------------------------------------------- */
 /* The tokenizer of a GGUF file from its metadata alone (no weights, no GPU):
