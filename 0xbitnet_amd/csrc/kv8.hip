@@ -343,23 +343,18 @@ __global__ __launch_bounds__(kKvThreads) void kv8_move_kernel(Kv8EvictArgs a) {
     const uint8_t *src = seq + (size_t)h * a.nb * kKv8Codes + off;
     uint8_t *dst = dseq + (size_t)h * a.dst_nb * kKv8Codes + off;
     for (int j0 = 0; j0 < kept; j0 += kMvRows * kMvUnroll) {
-        uint4 v[kMvUnroll];
-        bool move[kMvUnroll];
+        u32x4_t v[kMvUnroll];
+        int from[kMvUnroll];
 #pragma unroll
-        for (int u = 0; u < kMvUnroll; ++u) {
-            const int j = j0 + u * kMvRows + tid / kMvLanes;
-            move[u] = false;
-            if (j < kept) {
-                const int i = list[j];
-                move[u] = !inplace || i != j;
-                if (move[u]) v[u] = *(const uint4 *)(src + (size_t)i * kKv8Codes);
-            }
-        }
+        for (int u = 0; u < kMvUnroll; ++u)   // (clamped; not written past the kept ones)
+            from[u] = list[min(j0 + u * kMvRows + tid / kMvLanes, kept - 1)];
+#pragma unroll
+        for (int u = 0; u < kMvUnroll; ++u) v[u] = *(const u32x4_t *)(src + (size_t)from[u] * kKv8Codes);
         __syncthreads();   // the group is read before any of it is overwritten
 #pragma unroll
         for (int u = 0; u < kMvUnroll; ++u) {
             const int j = j0 + u * kMvRows + tid / kMvLanes;
-            if (move[u]) *(uint4 *)(dst + (size_t)j * kKv8Codes) = v[u];
+            if (j < kept && !(inplace && from[u] == j)) *(u32x4_t *)(dst + (size_t)j * kKv8Codes) = v[u];
         }
     }
     if (!inplace) {   // the unfinished block's f16 rows: 512 B of 16 KB each

@@ -29,6 +29,7 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 constexpr float kScoreUnit = 1.44269504088896340736f * 0.08838834764831844f;   // log2(e) / sqrt(128)
+constexpr int kArrivals = 1024; // arrival counters at a workspace's start
 constexpr float kStep = 8.0f;      // a score may pass the reference by this much
 constexpr int kQExp = 14;          // q rows are scaled below 2^kQExp
 
@@ -79,8 +80,9 @@ __device__ __forceinline__ int kv8_row_exp(float a) {
 // ---------------------------------------------------------------------------
 // decode
 // ---------------------------------------------------------------------------
-// Workgroup: four waves over a run of blocks, wave w taking every fourth; one
-// KV head, up to 8 of its query heads (K and V are read once for all of them).
+// Workgroup: four waves over a run of a KV head's blocks, wave w taking every
+// fourth, for up to 8 of its query heads at a time (K and V are read once for
+// all of them; more than 8 go round again over the run, which L2 then holds).
 // 16x16x32 MFMA: the 16 columns are the 8 heads' hi and lo parts, for q and
 // for p' alike, so the two-part products cost nothing over one.
 //   scores: A = 16 K rows x 32 dims, B = q; column c + (c ^ 8) is the score.
@@ -88,9 +90,13 @@ __device__ __forceinline__ int kv8_row_exp(float a) {
 //   the positions that bytes 8g .. 8g + 7 of a V row hold;
 //   P.V: A = 16 dims x the block's 32 positions (8 bytes a lane), B = the lane's
 //   own eight p' -- no exchange between lanes.
+// Bound by the cache's bytes; a wave keeps its next block's 8 KB in flight
+// under the current one's arithmetic.  A sequence's runs meet in the workspace:
+// each stores its part and counts in, and the last one joins them in order, so
+// the sum does not depend on which is last.
 constexpr int kDecWaves = 4;
 constexpr int kDecThreads = 64 * kDecWaves;
-constexpr int kDecRows = 8;            // query heads of a workgroup
+constexpr int kDecRows = 8;            // query heads of a pass
 constexpr int kDecQs = kKv8Hd + 8;     // q row stride in LDS (f16)
 constexpr float kDecBase = 6.0f;       // p' <= 2^(6 + kStep)
 
@@ -99,21 +105,46 @@ struct Kv8DecodeArgs {
     uint8_t *cache;
     size_t stride;
     const int *pos;
-    int pos_stride, H, Hkv, G, HC, max_seq, nb, splits, weights;
+    int pos_stride, H, Hkv, G, max_seq, nb, splits;
     float *out;
-    float2 *ml;      // [batch][Hkv * HC][splits][8] reference and sum
-    float *o;        // [batch][Hkv * HC][splits][8][128]
-    float2 *bw;      // [batch][H][nb] a block's sum of p' and its reference
+    int *cnt;        // [batch * Hkv] zero between calls
+    uint64_t *ml;    // [batch][H][splits] reference and sum (two floats)
+    uint64_t *o;     // [batch][H][splits][64] pairs of dims
+    uint64_t *bw;    // [batch][H][nb] a block's sum of p' and its reference
 };
 
-__device__ __forceinline__ int kv8_len(const Kv8DecodeArgs &a, int z) {
-    const int64_t p = (int64_t)a.pos[(size_t)z * a.pos_stride] + 1;
-    return (int)(p < 0 ? 0 : p > a.max_seq ? a.max_seq : p);
+__device__ __forceinline__ uint64_t kv8_pair(float a, float b) {
+    return (uint64_t)__float_as_uint(a) | ((uint64_t)__float_as_uint(b) << 32);
 }
-// Blocks of a workgroup: the sequence's blocks over all workgroups, at least
-// one per wave.
-__device__ __forceinline__ int kv8_per(int nblk, int splits) {
-    return max(kDecWaves, (nblk + splits - 1) / splits);
+__device__ __forceinline__ float2 kv8_unpair(uint64_t p) {
+    return make_float2(__uint_as_float((uint32_t)p), __uint_as_float((uint32_t)(p >> 32)));
+}
+// Hand-over between workgroups (and, for a block's weight, between the threads
+// of one) goes through agent-scope stores and loads.
+__device__ __forceinline__ void kv8_put(uint64_t *p, float a, float b) {
+    __hip_atomic_store(p, kv8_pair(a, b), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ float2 kv8_get(const uint64_t *p) {
+    return kv8_unpair(__hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+}
+
+// The softmax weights of a pass's heads (rows' references and sums in sml) join
+// the weights of the sequence's blocks, the heads in order.
+__device__ __forceinline__ void kv8_add_weights(const Kv8DecodeArgs &a, int z, int kvh, int g0, int ng,
+                                                int nblk, const float2 *sml) {
+    uint8_t *seq = a.cache + (size_t)z * a.stride;
+    float *w = (float *)(seq + kv8_layout(a.Hkv, a.nb).weights) + (size_t)kvh * a.nb;
+    const uint64_t *bw = a.bw + ((size_t)z * a.H + g0) * a.nb;
+    for (int b = threadIdx.x; b < nblk; b += kDecThreads) {
+        float add = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kDecRows; ++i) {
+            if (i >= ng) break;
+            const float2 p = kv8_get(bw + (size_t)i * a.nb + b);
+            add += p.x * __builtin_amdgcn_exp2f(p.y - sml[i].x) / sml[i].y;
+        }
+        w[b] += add;
+    }
 }
 
 template <int FMT, bool WEIGHTS>
@@ -122,53 +153,30 @@ __global__ __launch_bounds__(kDecThreads) void kv8_decode_kernel(Kv8DecodeArgs a
     __shared__ float sqs[kDecRows];
     __shared__ float2 sml[kDecWaves][kDecRows];
     __shared__ float4 so[kDecWaves][kDecRows][kKv8Hd / 4];
+    __shared__ float2 stot[kDecRows];
+    __shared__ int s_last;
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int z = blockIdx.z, hv = blockIdx.y, kvh = hv / a.HC, split = blockIdx.x;
-    const int g0 = kvh * a.G + (hv % a.HC) * kDecRows;      // first query head
-    const int ng = min(kDecRows, (kvh + 1) * a.G - g0);
-    const int len = kv8_len(a, z), nblk = kv8_blocks(len), per = kv8_per(nblk, a.splits);
+    const int z = blockIdx.z, kvh = blockIdx.y, split = blockIdx.x;
+    const int64_t p1 = (int64_t)a.pos[(size_t)z * a.pos_stride] + 1;
+    const int len = (int)(p1 < 0 ? 0 : p1 > a.max_seq ? a.max_seq : p1), nblk = kv8_blocks(len);
+    // blocks of a run: an even share, at least one per wave
+    const int per = max(kDecWaves, (nblk + a.splits - 1) / a.splits), runs = (nblk + per - 1) / per;
     const int b0 = split * per, b1 = min(nblk, b0 + per);
-    const bool direct = a.splits == 1 && !WEIGHTS;
-    const int orow = tid >> 5, od = (tid & 31) * 4;         // the row and dims a thread writes
-    float *out = a.out + ((size_t)z * a.H + g0 + orow) * kKv8Hd + od;
     if (b0 >= b1) {
-        if (direct && orow < ng) *(float4 *)out = make_float4(0, 0, 0, 0);
+        if (split == 0)
+            for (int i = tid; i < a.G * kKv8Hd; i += kDecThreads)
+                a.out[((size_t)z * a.H + kvh * a.G) * kKv8Hd + i] = 0.0f;
         return;
     }
-    {   // q rows: scaled, split, and their score units
-        float4 v = make_float4(0, 0, 0, 0);
-        if (orow < ng) v = *(const float4 *)(a.q + ((size_t)z * a.H + g0 + orow) * kKv8Hd + od);
-        float m = fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w)));
-#pragma unroll
-        for (int s = 16; s > 0; s >>= 1) m = fmaxf(m, __shfl_xor(m, s, 64));
-        const int e = kv8_row_exp(m);
-        const float f[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const float x = ldexpf(f[j], -e);
-            const _Float16 hi = (_Float16)x;
-            sq[orow * kDecQs + od + j] = hi;
-            sq[(orow + kDecRows) * kDecQs + od + j] = (_Float16)(x - (float)hi);
-        }
-        if ((tid & 31) == 0) sqs[orow] = ldexpf(kScoreUnit, e);
-    }
-    __syncthreads();
-    const int rr = lane & 15, g = lane >> 4;
-    half8_t qf[4];
-#pragma unroll
-    for (int s = 0; s < 4; ++s)
-        qf[s] = *(const half8_t *)(sq + rr * kDecQs + 64 * (s >> 1) + 16 * g + 8 * (s & 1));
-    const float qs = sqs[rr & 7];
-
     const Kv8Layout l = kv8_layout(a.Hkv, a.nb);
     const uint8_t *seq = a.cache + (size_t)z * a.stride;
     const uint8_t *codes = seq + (size_t)kvh * a.nb * kKv8Codes;
     const float2 *sc = (const float2 *)(seq + l.scales) + (size_t)kvh * a.nb;
+    const int rr = lane & 15, g = lane >> 4;
     // K row of this lane in 16-row tile 0 (tile 1: 8 positions on), V bytes of dim rr
     const int krow = ((rr >> 2) & 1) * 16 + (rr >> 3) * 4 + (rr & 3);
     const int koff = krow * kKv8Hd + 16 * g, voff = kKv8Half + rr * kKv8Block + 8 * g;
-
     struct Blk {
         uint4 k[4];
         uint2 v[8];
@@ -185,199 +193,241 @@ __global__ __launch_bounds__(kDecThreads) void kv8_decode_kernel(Kv8DecodeArgs a
         x.s = sc[b];
         return x;
     };
+    const int orow = tid >> 5, od = (tid & 31) * 4;         // the row and dims a thread joins
 
-    f32x4 o[8];
+    for (int hc = 0; hc < a.G; hc += kDecRows) {
+        const int g0 = kvh * a.G + hc, ng = min(kDecRows, a.G - hc);
+        // the first block is on its way while q is made ready
+        Blk cur = load(min(b0 + wave, b1 - 1));
+        {   // q rows: scaled, split, and their score units
+            float4 v = make_float4(0, 0, 0, 0);
+            if (orow < ng) v = *(const float4 *)(a.q + ((size_t)z * a.H + g0 + orow) * kKv8Hd + od);
+            float m = fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w)));
 #pragma unroll
-    for (int i = 0; i < 8; ++i) o[i] = f32x4{0, 0, 0, 0};
-    Kv8Ref ref;
-    float lsum = 0.0f;
+            for (int s = 16; s > 0; s >>= 1) m = fmaxf(m, __shfl_xor(m, s, 64));
+            const int e = kv8_row_exp(m);
+            const float f[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float x = ldexpf(f[j], -e);
+                const _Float16 hi = (_Float16)x;
+                sq[orow * kDecQs + od + j] = hi;
+                sq[(orow + kDecRows) * kDecQs + od + j] = (_Float16)(x - (float)hi);
+            }
+            if ((tid & 31) == 0) sqs[orow] = ldexpf(kScoreUnit, e);
+        }
+        lds_barrier();
+        half8_t qf[4];
+#pragma unroll
+        for (int s = 0; s < 4; ++s)
+            qf[s] = *(const half8_t *)(sq + rr * kDecQs + 64 * (s >> 1) + 16 * g + 8 * (s & 1));
+        const float qs = sqs[rr & 7];
 
-    Blk cur;
-    if (b0 + wave < b1) cur = load(b0 + wave);
-    for (int b = b0 + wave; b < b1; b += kDecWaves) {
-        const Blk nxt = load(min(b + kDecWaves, b1 - 1));
-        f32x4 s0{0, 0, 0, 0}, s1{0, 0, 0, 0};
+        f32x4 o[8];
 #pragma unroll
-        for (int s = 0; s < 4; ++s) {
-            const uint4 k0 = cur.k[s >> 1], k1 = cur.k[2 + (s >> 1)];
-            const half8_t f0 = (s & 1) ? kv8_unpack8<FMT>(k0.z, k0.w) : kv8_unpack8<FMT>(k0.x, k0.y);
-            const half8_t f1 = (s & 1) ? kv8_unpack8<FMT>(k1.z, k1.w) : kv8_unpack8<FMT>(k1.x, k1.y);
-            s0 = __builtin_amdgcn_mfma_f32_16x16x32_f16(f0, qf[s], s0, 0, 0, 0);
-            s1 = __builtin_amdgcn_mfma_f32_16x16x32_f16(f1, qf[s], s1, 0, 0, 0);
-        }
-        float x[8];
+        for (int i = 0; i < 8; ++i) o[i] = f32x4{0, 0, 0, 0};
+        Kv8Ref ref;
+        float lsum = 0.0f;
+        for (int b = b0 + wave; b < b1; b += kDecWaves) {
+            const Blk nxt = load(min(b + kDecWaves, b1 - 1));
+            f32x4 s0{0, 0, 0, 0}, s1{0, 0, 0, 0};
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            x[i] = s0[i] + kv8_ror8(s0[i]);
-            x[4 + i] = s1[i] + kv8_ror8(s1[i]);
-        }
-        // lane's positions in the block: slot 4 t + i is (g & 1) 16 + 8 t + (g >> 1) 4 + i
-        const int left = len - b * kKv8Block - ((g & 1) * 16 + (g >> 1) * 4);
-        const bool partial = len - b * kKv8Block < kKv8Block;
-        const float ck = cur.s.x * qs;
-        float mx = -__builtin_inff();
+            for (int s = 0; s < 4; ++s) {
+                const uint4 k0 = cur.k[s >> 1], k1 = cur.k[2 + (s >> 1)];
+                const half8_t f0 = (s & 1) ? kv8_unpack8<FMT>(k0.z, k0.w) : kv8_unpack8<FMT>(k0.x, k0.y);
+                const half8_t f1 = (s & 1) ? kv8_unpack8<FMT>(k1.z, k1.w) : kv8_unpack8<FMT>(k1.x, k1.y);
+                s0 = __builtin_amdgcn_mfma_f32_16x16x32_f16(f0, qf[s], s0, 0, 0, 0);
+                s1 = __builtin_amdgcn_mfma_f32_16x16x32_f16(f1, qf[s], s1, 0, 0, 0);
+            }
+            float x[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float v = x[i] * ck;
-            if (!partial || (i >> 2) * 8 + (i & 3) < left) mx = fmaxf(mx, v);
-        }
-        const float mx2 = mx + kv8_scale_exp(cur.s.y);
-        if (ref.passed(mx, mx2)) {
-            float al, al2;
-            ref.raise<4>(mx, mx2, al, al2);
-            lsum *= al;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) o[i] *= al2;
-        }
-        const float moff = ref.off() - kDecBase, vs = cur.s.y * ref.r;
-        float ps = 0.0f;
-        half8_t pf;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            float p = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i], ck, -moff));
-            if (partial && (i >> 2) * 8 + (i & 3) >= left) p = 0.0f;
-            ps += p;
-            p *= vs;
-            const _Float16 hi = (_Float16)p;
-            pf[i] = rr < kDecRows ? hi : (_Float16)(p - (float)hi);
-        }
-        lsum += ps;
-        if constexpr (WEIGHTS) {
-            ps += __shfl_xor(ps, 16, 64);
-            ps += __shfl_xor(ps, 32, 64);
-            if (lane < ng) a.bw[((size_t)z * a.H + g0 + lane) * a.nb + b] = make_float2(ps, moff);
-        }
-        if (partial) {   // bytes behind the last position may hold anything
-            uint32_t mk[2] = {0, 0};
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-                if ((i >> 2) * 8 + (i & 3) < left) mk[i >> 2] |= 0xffu << (8 * (i & 3));
+            for (int i = 0; i < 4; ++i) {
+                x[i] = s0[i] + kv8_ror8(s0[i]);
+                x[4 + i] = s1[i] + kv8_ror8(s1[i]);
+            }
+            // lane's positions in the block: slot 4 t + i is (g & 1) 16 + 8 t + (g >> 1) 4 + i
+            const int left = len - b * kKv8Block - ((g & 1) * 16 + (g >> 1) * 4);
+            const bool partial = len - b * kKv8Block < kKv8Block;
+            const float ck = cur.s.x * qs;
+            float mx = -__builtin_inff();
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                cur.v[i].x &= mk[0];
-                cur.v[i].y &= mk[1];
+                const float v = x[i] * ck;
+                if (!partial || (i >> 2) * 8 + (i & 3) < left) mx = fmaxf(mx, v);
             }
+            const float mx2 = mx + kv8_scale_exp(cur.s.y);
+            if (ref.passed(mx, mx2)) {
+                float al, al2;
+                ref.raise<4>(mx, mx2, al, al2);
+                lsum *= al;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) o[i] *= al2;
+            }
+            const float moff = ref.off() - kDecBase, vs = cur.s.y * ref.r;
+            float ps = 0.0f;
+            half8_t pf;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                float p = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i], ck, -moff));
+                if (partial && (i >> 2) * 8 + (i & 3) >= left) p = 0.0f;
+                ps += p;
+                // hi and lo of p' vs, each rounded once from the exact product
+                const _Float16 hi = (_Float16)__builtin_fmaf(p, vs, 0.0f);
+                pf[i] = rr < kDecRows ? hi : (_Float16)__builtin_fmaf(p, vs, -(float)hi);
+            }
+            lsum += ps;
+            if constexpr (WEIGHTS) {
+                ps += __shfl_xor(ps, 16, 64);
+                ps += __shfl_xor(ps, 32, 64);
+                if (lane < ng) kv8_put(a.bw + ((size_t)z * a.H + g0 + lane) * a.nb + b, ps, moff);
+            }
+            if (partial) {   // bytes behind the last position may hold anything
+                uint32_t mk[2] = {0, 0};
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if ((i >> 2) * 8 + (i & 3) < left) mk[i >> 2] |= 0xffu << (8 * (i & 3));
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    cur.v[i].x &= mk[0];
+                    cur.v[i].y &= mk[1];
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kv8_unpack8<FMT>(cur.v[i].x, cur.v[i].y), pf,
+                                                              o[i], 0, 0, 0);
+            cur = nxt;
         }
+        // the four waves' parts
+        lsum += __shfl_xor(lsum, 16, 64);
+        lsum += __shfl_xor(lsum, 32, 64);
+        const bool some = b0 + wave < b1;
+        if (lane < kDecRows)
+            sml[wave][lane] = make_float2(some ? ref.off() - kDecBase : -__builtin_inff(), lsum);
+        const float ri = 1.0f / ref.r;   // o in l's units
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-            o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kv8_unpack8<FMT>(cur.v[i].x, cur.v[i].y), pf,
-                                                          o[i], 0, 0, 0);
-        cur = nxt;
+        for (int i = 0; i < 8; ++i) {
+            float4 t;
+            t.x = (o[i][0] + kv8_ror8(o[i][0])) * ri;
+            t.y = (o[i][1] + kv8_ror8(o[i][1])) * ri;
+            t.z = (o[i][2] + kv8_ror8(o[i][2])) * ri;
+            t.w = (o[i][3] + kv8_ror8(o[i][3])) * ri;
+            if (rr < kDecRows) so[wave][rr][4 * i + g] = t;
+        }
+        lds_barrier();
+        float M = -__builtin_inff();
+#pragma unroll
+        for (int w = 0; w < kDecWaves; ++w) M = fmaxf(M, sml[w][orow].x);
+        float lt = 0.0f;
+        float4 t = make_float4(0, 0, 0, 0);
+#pragma unroll
+        for (int w = 0; w < kDecWaves; ++w) {
+            const float2 p = sml[w][orow];
+            const float f = __builtin_amdgcn_exp2f(p.x - M);
+            const float4 v = so[w][orow][od >> 2];
+            lt = __builtin_fmaf(p.y, f, lt);
+            t.x = __builtin_fmaf(v.x, f, t.x);
+            t.y = __builtin_fmaf(v.y, f, t.y);
+            t.z = __builtin_fmaf(v.z, f, t.z);
+            t.w = __builtin_fmaf(v.w, f, t.w);
+        }
+        const size_t row = (size_t)z * a.H + g0 + orow;
+        if (runs == 1) {
+            if (orow < ng)
+                *(float4 *)(a.out + row * kKv8Hd + od) =
+                    make_float4(t.x / lt, t.y / lt, t.z / lt, t.w / lt);
+            if constexpr (WEIGHTS) {
+                if (od == 0) stot[orow] = make_float2(M, lt);
+                __syncthreads();
+                kv8_add_weights(a, z, kvh, g0, ng, nblk, stot);
+            }
+        } else if (orow < ng) {
+            const size_t part = row * a.splits + split;
+            kv8_put(a.o + part * 64 + (od >> 1), t.x, t.y);
+            kv8_put(a.o + part * 64 + (od >> 1) + 1, t.z, t.w);
+            if (od == 0) kv8_put(a.ml + part, M, lt);
+        }
+        lds_barrier();   // LDS is free for the next heads
     }
-    // the four waves' parts
-    lsum += __shfl_xor(lsum, 16, 64);
-    lsum += __shfl_xor(lsum, 32, 64);
-    const bool some = b0 + wave < b1;
-    if (lane < kDecRows)
-        sml[wave][lane] = make_float2(some ? ref.off() - kDecBase : -__builtin_inff(), lsum);
-    const float ri = 1.0f / ref.r;   // o in l's units
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        float4 t;
-        t.x = (o[i][0] + kv8_ror8(o[i][0])) * ri;
-        t.y = (o[i][1] + kv8_ror8(o[i][1])) * ri;
-        t.z = (o[i][2] + kv8_ror8(o[i][2])) * ri;
-        t.w = (o[i][3] + kv8_ror8(o[i][3])) * ri;
-        if (rr < kDecRows) so[wave][rr][4 * i + g] = t;
+    if (runs == 1) return;
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();   // every thread's part has arrived
+    if (tid == 0) {
+        int *cnt = a.cnt + (size_t)z * a.Hkv + kvh;
+        const int old = __hip_atomic_fetch_add(cnt, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        s_last = old == runs - 1;
+        if (s_last) __hip_atomic_store(cnt, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
     __syncthreads();
-    float M = -__builtin_inff();
+    if (!s_last) return;
+    for (int hc = 0; hc < a.G; hc += kDecRows) {
+        const int g0 = kvh * a.G + hc, ng = min(kDecRows, a.G - hc);
+        if (orow < ng) {   // 32 lanes a row: lane i holds every 32nd run's factor
+            const size_t row = (size_t)z * a.H + g0 + orow;
+            const uint64_t *ml = a.ml + row * a.splits, *op = a.o + row * a.splits * 64 + (od >> 1);
+            const int i = tid & 31;
+            float M = -__builtin_inff();
+            for (int s = i; s < runs; s += 32) M = fmaxf(M, kv8_get(ml + s).x);
 #pragma unroll
-    for (int w = 0; w < kDecWaves; ++w) M = fmaxf(M, sml[w][orow].x);
-    float lt = 0.0f;
-    float4 t = make_float4(0, 0, 0, 0);
+            for (int s = 16; s > 0; s >>= 1) M = fmaxf(M, __shfl_xor(M, s, 64));
+            float lt = 0.0f;
+            float4 t = make_float4(0, 0, 0, 0);
+            for (int s0 = 0; s0 < runs; s0 += 32) {
+                float f = 0.0f, lf = 0.0f;
+                if (s0 + i < runs) {
+                    const float2 p = kv8_get(ml + s0 + i);
+                    f = __builtin_amdgcn_exp2f(p.x - M);
+                    lf = p.y * f;
+                }
+                const int n = min(32, runs - s0);
+                for (int j0 = 0; j0 < n; j0 += 8) {
+                    float2 lo[8], hi[8];
 #pragma unroll
-    for (int w = 0; w < kDecWaves; ++w) {
-        const float2 p = sml[w][orow];
-        const float f = __builtin_amdgcn_exp2f(p.x - M);
-        const float4 v = so[w][orow][od >> 2];
-        lt = __builtin_fmaf(p.y, f, lt);
-        t.x = __builtin_fmaf(v.x, f, t.x);
-        t.y = __builtin_fmaf(v.y, f, t.y);
-        t.z = __builtin_fmaf(v.z, f, t.z);
-        t.w = __builtin_fmaf(v.w, f, t.w);
+                    for (int j = 0; j < 8; ++j) {   // (clamped; its factor is 0)
+                        const uint64_t *p = op + (size_t)min(s0 + j0 + j, runs - 1) * 64;
+                        lo[j] = kv8_get(p);
+                        hi[j] = kv8_get(p + 1);
+                    }
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        if (j0 + j >= n) break;
+                        const float fj = __shfl(f, (j0 + j) | (lane & 32), 64);
+                        lt += __shfl(lf, (j0 + j) | (lane & 32), 64);
+                        t.x = __builtin_fmaf(lo[j].x, fj, t.x);
+                        t.y = __builtin_fmaf(lo[j].y, fj, t.y);
+                        t.z = __builtin_fmaf(hi[j].x, fj, t.z);
+                        t.w = __builtin_fmaf(hi[j].y, fj, t.w);
+                    }
+                }
+            }
+            *(float4 *)(a.out + row * kKv8Hd + od) = make_float4(t.x / lt, t.y / lt, t.z / lt, t.w / lt);
+            if (od == 0) stot[orow] = make_float2(M, lt);
+        }
+        if constexpr (WEIGHTS) {
+            lds_barrier();
+            kv8_add_weights(a, z, kvh, g0, ng, nblk, stot);
+            lds_barrier();
+        }
     }
-    if (direct) {
-        if (orow < ng) *(float4 *)out = make_float4(t.x / lt, t.y / lt, t.z / lt, t.w / lt);
-        return;
-    }
-    const size_t part = (((size_t)z * a.Hkv * a.HC + hv) * a.splits + split) * kDecRows + orow;
-    *(float4 *)(a.o + part * kKv8Hd + od) = t;
-    if (od == 0) a.ml[part] = make_float2(M, lt);
 }
 
-// Joins the splits: workgroup y < H writes a query head's output; the others
-// add to 128 blocks' weights each (their KV head's query heads in order).
-constexpr int kJoinThreads = 128;
-__global__ __launch_bounds__(kJoinThreads) void kv8_decode_join_kernel(Kv8DecodeArgs a) {
-    const int z = blockIdx.y, tid = threadIdx.x;
-    const int len = kv8_len(a, z), nblk = kv8_blocks(len), per = kv8_per(nblk, a.splits);
-    const int ns = (nblk + per - 1) / per;
-    auto row = [&](int h) {   // the first split's part of a query head
-        const int kvh = h / a.G, i = h % a.G, hv = kvh * a.HC + i / kDecRows;
-        return (((size_t)z * a.Hkv * a.HC + hv) * a.splits) * kDecRows + i % kDecRows;
-    };
-    auto total = [&](size_t r, float &M, float &lt) {
-        M = -__builtin_inff();
-        for (int s = 0; s < ns; ++s) M = fmaxf(M, a.ml[r + (size_t)s * kDecRows].x);
-        lt = 0.0f;
-        for (int s = 0; s < ns; ++s) {
-            const float2 p = a.ml[r + (size_t)s * kDecRows];
-            lt = __builtin_fmaf(p.y, __builtin_amdgcn_exp2f(p.x - M), lt);
-        }
-    };
-    if ((int)blockIdx.x < a.H) {
-        const int h = blockIdx.x;
-        float *out = a.out + ((size_t)z * a.H + h) * kKv8Hd + tid;
-        if (len == 0) {
-            *out = 0.0f;
-            return;
-        }
-        const size_t r = row(h);
-        float M, lt, t = 0.0f;
-        total(r, M, lt);
-        for (int s = 0; s < ns; ++s) {
-            const size_t p = r + (size_t)s * kDecRows;
-            t = __builtin_fmaf(a.o[p * kKv8Hd + tid], __builtin_amdgcn_exp2f(a.ml[p].x - M), t);
-        }
-        *out = t / lt;
-        return;
-    }
-    const int chunks = (a.nb + kJoinThreads - 1) / kJoinThreads;
-    const int c = blockIdx.x - a.H, kvh = c / chunks, b = (c % chunks) * kJoinThreads + tid;
-    if (b >= nblk) return;
-    float add = 0.0f;
-    for (int i = 0; i < a.G; ++i) {
-        const int h = kvh * a.G + i;
-        float M, lt;
-        total(row(h), M, lt);
-        const float2 p = a.bw[((size_t)z * a.H + h) * a.nb + b];
-        add += p.x * __builtin_amdgcn_exp2f(p.y - M) / lt;
-    }
-    uint8_t *seq = a.cache + (size_t)z * a.stride;
-    float *w = (float *)(seq + kv8_layout(a.Hkv, a.nb).weights) + (size_t)kvh * a.nb + b;
-    *w += add;
-}
-
-// Workgroups per KV head and sequence: about four per CU over the launch, none
-// with fewer than one block per wave.
-static int decode_splits(int batch, int Hkv, int HC, int nb) {
-    const int64_t target = 4 * (int64_t)device_cus(), rows = (int64_t)batch * Hkv * HC;
-    int64_t s = (target + rows - 1) / rows;
-    const int64_t most = (nb + kDecWaves - 1) / kDecWaves;
+// Runs per KV head and sequence: two workgroups per CU over the launch (what
+// the registers let reside), none with fewer blocks than waves.
+static int decode_splits(int batch, int Hkv, int nb) {
+    const int64_t rows = (int64_t)batch * Hkv, most = (nb + kDecWaves - 1) / kDecWaves;
+    int64_t s = 2 * (int64_t)device_cus() / rows;
     if (s > most) s = most;
-    return (int)(s < 1 ? 1 : s);
+    return (int)(s < 1 || rows > kArrivals ? 1 : s);
 }
 
 struct DecodeWs {
     size_t ml, o, bw, bytes;
 };
 static DecodeWs decode_ws(int batch, int H, int Hkv, int nb) {
-    const int HC = (H / Hkv + kDecRows - 1) / kDecRows;
-    const size_t parts = (size_t)batch * Hkv * HC * decode_splits(batch, Hkv, HC, nb) * kDecRows;
+    const size_t parts = (size_t)batch * H * decode_splits(batch, Hkv, nb);
     DecodeWs w;
-    w.ml = 0;
-    w.o = kv8_align(parts * 8);
+    w.ml = kArrivals * 4;
+    w.o = w.ml + kv8_align(parts * 8);
     w.bw = w.o + kv8_align(parts * kKv8Hd * 4);
     w.bytes = w.bw + kv8_align((size_t)batch * H * nb * 8);
     return w;
@@ -387,28 +437,35 @@ static DecodeWs decode_ws(int batch, int H, int Hkv, int nb) {
 // prefill
 // ---------------------------------------------------------------------------
 // Rows of a KV head are (token, query head of the group) pairs, token-major, so
-// that a K/V tile serves all of the group's heads.  A workgroup takes 128 rows,
-// 32 per wave, and a run of 64-position tiles.  Each tile's codes are unpacked
-// to f16 once, by all four waves, into LDS in the order the MFMA operands are
-// read (every read is 1 KB contiguous); the next tile's codes are in flight
-// meanwhile.
+// that a block of K and V serves all of the group's heads.  A workgroup takes
+// 128 rows, 32 per wave, and a run of blocks.  A block's codes are unpacked to
+// f16 once, a quarter by each wave, into LDS in the order the MFMA operands are
+// read (every read is 1 KB contiguous).
 //   scores: 32x32x16 MFMA, A = 32 K rows, B = q (in registers, hi and lo);
 //   P.V: A = 32 dims x 16 positions, B = the lane's own p' (kv8_v_byte's order).
-// Rows that see different lengths finish at different tiles; long rows are
-// split over workgroups where the rows alone leave CUs idle, and joined after.
+// Bound by the MFMAs (32 of 32 cycles per wave and block, twice the one-part
+// products) as long as the softmax's VALU work runs under them: the next
+// block's score products alternate with this block's exponentials, and P.V with
+// the rest of them and the unpacking, instruction by instruction (a wave that
+// issues 16 MFMAs and then 128 VALU instructions takes 395 ns, one that
+// alternates them 349, the MFMAs alone 261; two waves per SIMD).  K runs a
+// block ahead of V; rings of four blocks of each leave one barrier per two
+// blocks.
+// Row tiles see different lengths and finish apart; where they alone leave CUs
+// idle, their runs are split and a second launch joins the parts.
 constexpr int kPreWaves = 4;
 constexpr int kPreThreads = 64 * kPreWaves;
 constexpr int kPreRows = 32 * kPreWaves;
-constexpr int kPreTile = 2 * kKv8Block;
-constexpr int kPreTileBytes = 2 * 2 * kKv8Codes;   // a tile's K and V as f16
-constexpr float kPreBase = 6.0f;                   // p' <= 2^(6 + kStep)
+constexpr int kPreRing = 4;
+constexpr int kPreOps = kKv8Half * 2 / 16;   // 16-byte operands of a block's K (or V) as f16
+constexpr float kPreBase = 6.0f;             // p' <= 2^(6 + kStep)
 
 struct Kv8PrefillArgs {
     const float *q;
     uint8_t *cache;
-    int n, pos0, H, Hkv, G, nb, rows, splits, per, weights;
+    int n, pos0, H, Hkv, G, nb, rows, rtiles, splits, per, weights;
     float *out;
-    float2 *ml;     // [splits][Hkv][rows]
+    float2 *ml;     // [splits][Hkv][rows] a row's reference and sum
     float *o;       // [splits][Hkv][rows][128]
     float2 *lse;    // [Hkv][rows32] log2 of the row's softmax sum, its score unit
     uint4 *qf;      // [Hkv][rows32 / 32][8][2][64] q as MFMA operands
@@ -417,25 +474,69 @@ struct Kv8PrefillArgs {
 };
 
 __host__ __device__ inline int pre_rows32(int rows) { return (rows + 31) & ~31; }
+// The first row tile that sees a block of run `split`: its last row's token is at
+// position 32 per split at least.
+__device__ __forceinline__ int pre_first_tile(const Kv8PrefillArgs &a, int split) {
+    const int64_t tok = (int64_t)split * a.per * kKv8Block - a.pos0;
+    return tok <= 0 ? 0 : (int)min(tok * a.G / kPreRows, (int64_t)a.rtiles);
+}
 
 template <int FMT>
 __global__ __launch_bounds__(kPreThreads, 2) void kv8_prefill_kernel(Kv8PrefillArgs a) {
-    extern __shared__ uint4 sbuf[];   // two tiles: K operands [2][8][64], V operands [2][4][2][64]
+    // rings of K [8][64] and V operands [4 dims][2][64]: block b of the run in slot b % 4
+    __shared__ uint4 sk[kPreRing][kPreOps], sv[kPreRing][kPreOps];
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int kvh = blockIdx.y;
-    const int rtile = gridDim.x - 1 - blockIdx.x;   // the longest rows first
-    const int split = blockIdx.z;
+    // The grid holds the workgroups that have work and no others: run 0 of every
+    // row tile, then run 1 of those that have one, .., each from the last row
+    // tile (the longest rows) on, the KV heads side by side.
+    const int kvh = blockIdx.x % a.Hkv;
+    int at = blockIdx.x / a.Hkv, split = 0;
+    for (int n; at >= (n = a.rtiles - pre_first_tile(a, split)); at -= n) ++split;
+    const int rtile = a.rtiles - 1 - at;
     const int r0 = rtile * kPreRows, row = r0 + wave * 32 + (lane & 31), h = lane >> 5;
     const int total = a.pos0 + a.n;
     const int lastrow = min(r0 + kPreRows, a.rows) - 1;
-    const int seen = a.pos0 + lastrow / a.G + 1;    // positions the tile's last row sees
-    const int tiles = (seen + kPreTile - 1) / kPreTile;
-    const int t0 = split * a.per, t1 = min(tiles, t0 + a.per);
-    if (t0 >= t1) return;
-    const bool live = row < a.rows;
+    const int blocks = kv8_blocks(a.pos0 + lastrow / a.G + 1);   // that the tile's last row sees
+    const int b0 = split * a.per, b1 = min(blocks, b0 + a.per);
     const int tok = min(row, a.rows - 1) / a.G, head = kvh * a.G + min(row, a.rows - 1) % a.G;
     const int qpos = a.pos0 + tok;
+
+    const Kv8Layout l = kv8_layout(a.Hkv, a.nb);
+    const uint8_t *codes = a.cache + (size_t)kvh * a.nb * kKv8Codes;
+    const float2 *sc = (const float2 *)(a.cache + l.scales) + (size_t)kvh * a.nb;
+    // a wave unpacks 32 dims of K and of V of each block: operands 2 wave, 2 wave + 1
+    const uint32_t koff = (lane & 31) * kKv8Hd + 32 * wave + 16 * h;
+    const uint32_t voff = kKv8Half + (32 * wave + (lane & 31)) * kKv8Block + 16 * h;
+    uint4 ck4[2], cv4[2];
+    // (buffer loads: a scalar address and one register of offset)
+    auto fetch = [&](int b, uint32_t off) {
+        const uint8_t *p = codes + (size_t)__builtin_amdgcn_readfirstlane(min(b, b1 - 1)) * kKv8Codes;
+        const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc((void *)p, 0, kKv8Codes, 0x00027000);
+        return __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, 0));
+    };
+    const int slot = 128 * wave + lane;
+    auto stage = [&](uint4 *ring, const uint4 &c) {
+        ring[slot] = __builtin_bit_cast(uint4, kv8_unpack8<FMT>(c.x, c.y));
+        ring[slot + 64] = __builtin_bit_cast(uint4, kv8_unpack8<FMT>(c.z, c.w));
+    };
+    auto clear_v = [&](int b, uint4 &c) {   // bytes behind the last position may hold anything
+        const int left = total - b * kKv8Block, hh = 4 * h + opaque_zero();
+        if (left >= kKv8Block) return;   // uniform
+        uint32_t mk[4] = {0, 0, 0, 0};
+#pragma unroll
+        for (int p = 0; p < 16; ++p)   // byte 16 h + p: position 16 (p / 8) + 8 (p / 4 % 2) + 4 h + p % 4
+            if (16 * (p >> 3) + 8 * (p >> 2 & 1) + (p & 3) + hh < left) mk[p >> 2] |= 0xffu << (8 * (p & 3));
+        c.x &= mk[0];
+        c.y &= mk[1];
+        c.z &= mk[2];
+        c.w &= mk[3];
+    };
+    ck4[0] = fetch(b0, koff);
+    ck4[1] = fetch(b0 + 1, koff);
+    cv4[0] = fetch(b0, voff);
+    cv4[1] = fetch(b0 + 1, voff);
+    const uint4 ck2 = fetch(b0 + 2, koff);
 
     // q: dims 32 c + 16 h + 8 e + j are operand s = 2 c + e
     half8_t qh[8], ql[8];
@@ -478,49 +579,13 @@ __global__ __launch_bounds__(kPreThreads, 2) void kv8_prefill_kernel(Kv8PrefillA
                 f[(2 * s) * 64] = __builtin_bit_cast(uint4, qh[s]);
                 f[(2 * s + 1) * 64] = __builtin_bit_cast(uint4, ql[s]);
             }
-            if (h == 0) a.lse[(size_t)kvh * r32 + row].y = qs;
-        }
-    }
-
-    const Kv8Layout l = kv8_layout(a.Hkv, a.nb);
-    const uint8_t *codes = a.cache + (size_t)kvh * a.nb * kKv8Codes;
-    const float2 *sc = (const float2 *)(a.cache + l.scales) + (size_t)kvh * a.nb;
-    const int lastblk = kv8_blocks(total) - 1;
-    // wave 0, 1: K of the tile's blocks; 2, 3: V
-    const int lb = wave & 1, isv = wave >> 1;
-    const int goff = isv ? kKv8Half + (lane & 31) * kKv8Block + 16 * h : (lane & 31) * kKv8Hd + 16 * h;
-    const int gstep = isv ? 32 * kKv8Block : 32;
-    uint4 c[4];
-    auto fetch = [&](int t) {
-        const int b = min(2 * t + lb, lastblk);
-        const uint8_t *p = codes + (size_t)b * kKv8Codes + goff;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) c[i] = *(const uint4 *)(p + i * gstep);
-    };
-    auto stage = [&](int t, int buf) {
-        const int b = min(2 * t + lb, lastblk), left = total - b * kKv8Block;
-        if (isv && left < kKv8Block) {   // bytes behind the last position may hold anything
-            uint32_t mk[4] = {0, 0, 0, 0};
-#pragma unroll
-            for (int p = 0; p < 16; ++p)   // byte 16 h + p: position 16 (p / 8) + 8 (p / 4 % 2) + 4 h + p % 4
-                if (16 * (p >> 3) + 8 * (p >> 2 & 1) + 4 * h + (p & 3) < left)
-                    mk[p >> 2] |= 0xffu << (8 * (p & 3));
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                c[i].x &= mk[0];
-                c[i].y &= mk[1];
-                c[i].z &= mk[2];
-                c[i].w &= mk[3];
+            if (h == 0) {
+                float2 *ls = a.lse + (size_t)kvh * r32 + row;
+                ls->y = qs;
+                if (row >= a.rows) ls->x = __builtin_inff();   // weighs nothing
             }
         }
-        // operands 2 i and 2 i + 1 of the block
-        uint4 *s = sbuf + buf * (kPreTileBytes / 16) + (isv * 2 + lb) * 512 + lane;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            s[(2 * i) * 64] = __builtin_bit_cast(uint4, kv8_unpack8<FMT>(c[i].x, c[i].y));
-            s[(2 * i + 1) * 64] = __builtin_bit_cast(uint4, kv8_unpack8<FMT>(c[i].z, c[i].w));
-        }
-    };
+    }
 
     f32x16 o[4];
 #pragma unroll
@@ -532,132 +597,240 @@ __global__ __launch_bounds__(kPreThreads, 2) void kv8_prefill_kernel(Kv8PrefillA
     const int wseen = a.pos0 + min(r0 + wave * 32 + 31, a.rows - 1) / a.G + 1;   // the wave's last row
     const int wfull = a.pos0 + min(r0 + wave * 32, a.rows - 1) / a.G + 1;        // its first row
 
-    fetch(t0);
-    stage(t0, 0);
-    __syncthreads();
-    for (int t = t0; t < t1; ++t) {
-        const int buf = (t - t0) & 1;
-        if (t + 1 < t1) fetch(t + 1);
-        if (t * kPreTile < wseen) {   // uniform over the wave
-            const uint4 *kb = sbuf + buf * (kPreTileBytes / 16) + lane;
-            const uint4 *vb = kb + 1024;
-            f32x16 s[2];
+    clear_v(b0, cv4[0]);
+    clear_v(b0 + 1, cv4[1]);
+    stage(sk[0], ck4[0]);
+    stage(sk[1], ck4[1]);
+    stage(sv[0], cv4[0]);
+    stage(sv[1], cv4[1]);
+    stage(sk[2], ck2);
+    // codes in flight at the start of a pair b, b + 1: K of b + 3, b + 4, V of b + 2, b + 3
+    auto fetch_pair = [&](int b) {
+        ck4[0] = fetch(b + 3, koff);
+        ck4[1] = fetch(b + 4, koff);
+        cv4[0] = fetch(b + 2, voff);
+        cv4[1] = fetch(b + 3, voff);
+    };
+    fetch_pair(b0);
+    lds_barrier();
+    f32x16 s0, s1;
 #pragma unroll
-            for (int b = 0; b < 2; ++b) {
+    for (int i = 0; i < 16; ++i) s0[i] = 0.0f;
 #pragma unroll
-                for (int i = 0; i < 16; ++i) s[b][i] = 0.0f;
+    for (int i = 0; i < 8; ++i) {
+        const half8_t k = __builtin_bit_cast(half8_t, sk[0][i * 64 + lane]);
+        s0 = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, qh[i], s0, 0, 0, 0);
+        s0 = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, ql[i], s0, 0, 0, 0);
+    }
+    lds_barrier();   // the first K slot is free
+    const int wb = min(b1, kv8_blocks(wseen));   // blocks that some row of the wave sees
+    float2 sb = sc[b0];
+    auto top = [&](const f32x16 &s, int i) {   // of four scores
+        return fmaxf(fmaxf(s[i], s[i + 1]), fmaxf(s[i + 2], s[i + 3]));
+    };
+    float smax = fmaxf(fmaxf(top(s0, 0), top(s0, 4)), fmaxf(top(s0, 8), top(s0, 12)));
+    // Block b, its scores in s and their maximum in smax; the next one's go to sn.
+    // r: b's place in the run; stage0, stage1: what is unpacked under it.
+    auto block = [&](int b, int r, f32x16 &s, f32x16 &sn, auto stage0, auto stage1) {
+        const int p0 = b * kKv8Block;
+        // (units of 0, of zero blocks, are made positive: hidden scores are -inf)
+        float ck = sb.x * qs, vs = sb.y;
+        sb = sc[min(b + 1, b1 - 1)];
+        ck = ck < 1.2e-38f ? 1.2e-38f : ck;
+        if (p0 + kKv8Block > wfull) {   // some rows do not see all of it (uniform)
+            // positions of the lane's scores: (i & 3) + 8 (i >> 2) + 4 h
+            const int left = qpos + 1 - p0 - 4 * h + opaque_zero();   // (a branch, not 32 selects)
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const half8_t k = __builtin_bit_cast(half8_t, kb[(b * 8 + i) * 64]);
-                    s[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, qh[i], s[b], 0, 0, 0);
-                    s[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, ql[i], s[b], 0, 0, 0);
-                }
+            for (int i = 0; i < 16; ++i) s[i] = (i & 3) + 8 * (i >> 2) < left ? s[i] : -__builtin_inff();
+            if (qpos < p0) {   // a row that sees none: the block's scales, NaN or not, are nothing to it
+                ck = 1.2e-38f;
+                vs = 0.0f;
             }
-            const float2 sc0 = sc[min(2 * t, lastblk)], sc1 = sc[min(2 * t + 1, lastblk)];
-            const float ck[2] = {sc0.x * qs, sc1.x * qs};
-            // positions of the lane's scores: 32 b + (i & 3) + 8 (i >> 2) + 4 h
-            const bool masked = (t + 1) * kPreTile > wfull;
-            const int left = qpos + 1 - t * kPreTile - 4 * h;
-            float mb[2];
-#pragma unroll
-            for (int b = 0; b < 2; ++b) {
-                mb[b] = -__builtin_inff();
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const float v = s[b][i] * ck[b];
-                    if (!masked || 32 * b + (i & 3) + 8 * (i >> 2) < left) mb[b] = fmaxf(mb[b], v);
-                }
-            }
-            const float mx = fmaxf(mb[0], mb[1]);
-            const float mx2 = fmaxf(mb[0] + kv8_scale_exp(sc0.y), mb[1] + kv8_scale_exp(sc1.y));
-            if (ref.passed(mx, mx2)) {
-                float al, al2;
-                ref.raise<2>(mx, mx2, al, al2);
-                lsum *= al;
-#pragma unroll
-                for (int d = 0; d < 4; ++d)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) o[d][i] *= al2;
-            }
-            const float moff = ref.off() - kPreBase;
-            const float vs[2] = {sc0.y * ref.r, sc1.y * ref.r};
-#pragma unroll
-            for (int b = 0; b < 2; ++b)
-#pragma unroll
-                for (int gr = 0; gr < 2; ++gr) {
-                    half8_t ph, pl;
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        const int i = 8 * gr + j;
-                        float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][i], ck[b], -moff));
-                        const bool hide = masked && 32 * b + (i & 3) + 8 * (i >> 2) >= left;
-                        lsum += hide ? 0.0f : p;
-                        p = hide ? 0.0f : p * vs[b];   // (vs may be NaN)
-                        const _Float16 hi = (_Float16)p;
-                        ph[j] = hi;
-                        pl[j] = (_Float16)(p - (float)hi);
-                    }
-#pragma unroll
-                    for (int d = 0; d < 4; ++d) {
-                        const half8_t v = __builtin_bit_cast(half8_t, vb[((b * 4 + d) * 2 + gr) * 64]);
-                        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, ph, o[d], 0, 0, 0);
-                        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, pl, o[d], 0, 0, 0);
-                    }
-                }
+            smax = fmaxf(fmaxf(top(s, 0), top(s, 4)), fmaxf(top(s, 8), top(s, 12)));
         }
-        if (t + 1 < t1) stage(t + 1, buf ^ 1);
-        __syncthreads();
+        const float mx = smax * ck;
+        const float mx2 = mx + kv8_scale_exp(vs);
+        if (ref.passed(mx, mx2)) {
+            float al, al2;
+            ref.raise<2>(mx, mx2, al, al2);
+            lsum *= al;
+#pragma unroll
+            for (int d = 0; d < 4; ++d)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) o[d][i] *= al2;
+        }
+        const float moff = ref.off() - kPreBase;
+        vs *= ref.r;
+        // From here on the order is the one written: SLOT ends what may run under
+        // the MFMA before it.
+#define SLOT() __builtin_amdgcn_sched_barrier(0)
+        const uint4 *kb = sk[(r + 1) & 3] + lane, *vb = sv[r & 3] + lane;
+        half8_t ph[2], pl[2], v[4], k[2];
+        float pa, pb;
+        auto exps = [&](int j) {   // elements 2 j, 2 j + 1
+            pa = __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * j], ck, -moff));
+            pb = __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * j + 1], ck, -moff));
+        };
+        auto split = [&](int j) {   // hi and lo of p' vs, each rounded once from the exact product
+            lsum += pa;
+            lsum += pb;
+            half2_t hi, lo;
+            hi.x = (_Float16)__builtin_fmaf(pa, vs, 0.0f);
+            hi.y = (_Float16)__builtin_fmaf(pb, vs, 0.0f);
+            lo.x = (_Float16)__builtin_fmaf(pa, vs, -(float)hi.x);
+            lo.y = (_Float16)__builtin_fmaf(pb, vs, -(float)hi.y);
+            ph[j >> 2][2 * (j & 3)] = hi.x;
+            ph[j >> 2][2 * (j & 3) + 1] = hi.y;
+            pl[j >> 2][2 * (j & 3)] = lo.x;
+            pl[j >> 2][2 * (j & 3) + 1] = lo.y;
+        };
+#pragma unroll
+        for (int i = 0; i < 16; ++i) sn[i] = 0.0f;
+        k[0] = __builtin_bit_cast(half8_t, kb[0]);
+        k[1] = __builtin_bit_cast(half8_t, kb[64]);
+        SLOT();
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            sn = __builtin_amdgcn_mfma_f32_32x32x16_f16(k[i & 1], qh[i], sn, 0, 0, 0);
+            if (i < 6) exps(i);
+            SLOT();
+            sn = __builtin_amdgcn_mfma_f32_32x32x16_f16(k[i & 1], ql[i], sn, 0, 0, 0);
+            if (i < 6) split(i);
+            if (i < 6) k[i & 1] = __builtin_bit_cast(half8_t, kb[(i + 2) * 64]);
+            else
+                for (int d = 2 * (i - 6); d < 2 * (i - 5); ++d) v[d] = __builtin_bit_cast(half8_t, vb[d * 128]);
+            SLOT();
+        }
+#pragma unroll
+        for (int d = 0; d < 4; ++d) {
+            o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[d], ph[0], o[d], 0, 0, 0);
+            if (d & 1) split(6 + (d >> 1));
+            else exps(6 + (d >> 1));
+            SLOT();
+        }
+#pragma unroll
+        for (int d = 0; d < 4; ++d) {
+            o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[d], pl[0], o[d], 0, 0, 0);
+            v[d] = __builtin_bit_cast(half8_t, vb[d * 128 + 64]);
+            if (d == 1) stage0();
+            SLOT();
+        }
+#pragma unroll
+        for (int d = 0; d < 4; ++d) {
+            o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[d], ph[1], o[d], 0, 0, 0);
+            if (d == 1) stage1();
+            SLOT();
+        }
+#pragma unroll
+        for (int d = 0; d < 4; ++d) {
+            o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[d], pl[1], o[d], 0, 0, 0);
+            smax = d == 0 ? top(sn, 0) : fmaxf(smax, top(sn, 4 * d));
+            SLOT();
+        }
+#undef SLOT
+    };
+    auto stage_k = [&](int r) { return [&, r] { stage(sk[(r + 3) & 3], ck4[0]); }; };
+    auto stage_k1 = [&](int r) { return [&, r] { stage(sk[r & 3], ck4[1]); }; };
+    auto stage_v = [&](int r) { return [&, r] { stage(sv[(r + 2) & 3], cv4[0]); }; };
+    auto stage_v1 = [&](int r) { return [&, r] { stage(sv[(r + 3) & 3], cv4[1]); }; };
+    // The two waves of a SIMD take turns at priority, a pair of blocks each (their
+    // slots differ in the lowest bit as a rule): by age alone one runs at its
+    // full speed, 1.35 us a block, and the other, at half of it, finishes late.
+    uint32_t hwid;
+    asm volatile("s_getreg_b32 %0, hwreg(HW_REG_HW_ID)" : "=s"(hwid));
+    int b = b0;
+    for (; b + 1 < wb; b += 2) {
+        const int r = b - b0;
+        if (((r >> 1) ^ hwid) & 1) __builtin_amdgcn_s_setprio(1);
+        else __builtin_amdgcn_s_setprio(0);
+        clear_v(b + 2, cv4[0]);
+        clear_v(b + 3, cv4[1]);
+        block(b, r, s0, s1, stage_k(r), stage_k1(r));
+        block(b + 1, r + 1, s1, s0, stage_v(r), stage_v1(r));
+        fetch_pair(b + 2);
+        lds_barrier();
+    }
+    for (; b < b1; b += 2) {   // a last block alone, and what only other waves see
+        const int r = b - b0;
+        clear_v(b + 2, cv4[0]);
+        clear_v(b + 3, cv4[1]);
+        auto none = [] {};
+        if (b < wb) block(b, r, s0, s1, none, none);
+        stage_k(r)();
+        stage_k1(r)();
+        stage_v(r)();
+        stage_v1(r)();
+        fetch_pair(b + 2);
+        lds_barrier();
     }
     lsum += __shfl_xor(lsum, 32, 64);
-    if (!live) return;
-    // lane's dims: 32 d + 8 k + 4 h + 0..3
-    const float moff = ref.off() - kPreBase, f = 1.0f / ref.r;
-    const bool direct = a.splits == 1;
-    float *dst;
+    // the lane's row again (not held in registers over the loop)
+    const int elane = lane + opaque_zero(), eh = elane >> 5, erow = r0 + wave * 32 + (elane & 31);
+    if (erow >= a.rows) return;
+    // (a wave may see nothing of a run that others see)
+    const float M = b0 * kKv8Block < wseen ? ref.off() - kPreBase : -__builtin_inff();
+    const bool direct = blocks <= a.per;   // the row tile's only run
+    float *dst, f = 1.0f / ref.r;          // o in l's units
     if (direct) {
-        dst = a.out + ((size_t)tok * a.H + head) * kKv8Hd;
-        if (a.weights && h == 0)
-            a.lse[(size_t)kvh * pre_rows32(a.rows) + row].x = moff + __builtin_amdgcn_logf(lsum);
+        dst = a.out + ((size_t)(erow / a.G) * a.H + kvh * a.G + erow % a.G) * kKv8Hd;
+        f /= lsum;
+        if (a.weights && eh == 0)
+            a.lse[(size_t)kvh * pre_rows32(a.rows) + erow].x = M + __builtin_amdgcn_logf(lsum);
     } else {
-        const size_t p = ((size_t)split * a.Hkv + kvh) * a.rows + row;
-        dst = a.o + p * kKv8Hd;
-        // (a wave may see nothing of a split that others see)
-        if (h == 0) a.ml[p] = make_float2(t0 * kPreTile < wseen ? moff : -__builtin_inff(), lsum);
+        const size_t part = ((size_t)split * a.Hkv + kvh) * a.rows + erow;
+        dst = a.o + part * kKv8Hd;
+        if (eh == 0) a.ml[part] = make_float2(M, lsum);
     }
+    // lane's dims: 32 d + 8 k + 4 h + 0..3
 #pragma unroll
     for (int d = 0; d < 4; ++d)
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            float4 v = make_float4(o[d][4 * k] * f, o[d][4 * k + 1] * f, o[d][4 * k + 2] * f,
-                                   o[d][4 * k + 3] * f);
-            if (direct) v = make_float4(v.x / lsum, v.y / lsum, v.z / lsum, v.w / lsum);
-            *(float4 *)(dst + 32 * d + 8 * k + 4 * h) = v;
-        }
+        for (int k = 0; k < 4; ++k)
+            *(float4 *)(dst + 32 * d + 8 * k + 4 * eh) =
+                make_float4(o[d][4 * k] * f, o[d][4 * k + 1] * f, o[d][4 * k + 2] * f, o[d][4 * k + 3] * f);
 }
 
-// Joins a row's splits: 32 threads a row, 4 dims each.
+// Joins a row's runs: 32 threads a row, 4 dims each; bound by the parts' bytes.
 __global__ __launch_bounds__(256) void kv8_prefill_join_kernel(Kv8PrefillArgs a) {
     const int row = blockIdx.x * 8 + (threadIdx.x >> 5), kvh = blockIdx.y, d = (threadIdx.x & 31) * 4;
     if (row >= a.rows) return;
     const int tok = row / a.G, head = kvh * a.G + row % a.G;
-    // splits that the row's workgroup had tiles in
-    const int lastrow = min((row / kPreRows + 1) * kPreRows, a.rows) - 1;
-    const int tiles = (a.pos0 + lastrow / a.G + kPreTile) / kPreTile;
-    const int ns = (tiles + a.per - 1) / a.per;
+    const int lastrow = min((row / kPreRows + 1) * kPreRows, a.rows) - 1;   // of the row's tile
+    const int ns = (kv8_blocks(a.pos0 + lastrow / a.G + 1) + a.per - 1) / a.per;
+    if (ns == 1) return;   // written by its only run
     const size_t step = (size_t)a.Hkv * a.rows, r = (size_t)kvh * a.rows + row;
-    float M = -__builtin_inff();
-    for (int s = 0; s < ns; ++s) M = fmaxf(M, a.ml[r + s * step].x);
-    float lt = 0.0f;
+    float M = -__builtin_inff(), lt = 0.0f;
     float4 t = make_float4(0, 0, 0, 0);
-    for (int s = 0; s < ns; ++s) {
-        const float2 p = a.ml[r + s * step];
-        const float4 v = *(const float4 *)(a.o + (r + s * step) * kKv8Hd + d);
-        const float f = __builtin_amdgcn_exp2f(p.x - M);
-        lt = __builtin_fmaf(p.y, f, lt);
-        t.x = __builtin_fmaf(v.x, f, t.x);
-        t.y = __builtin_fmaf(v.y, f, t.y);
-        t.z = __builtin_fmaf(v.z, f, t.z);
-        t.w = __builtin_fmaf(v.w, f, t.w);
+    constexpr int kB = 8;   // parts in flight
+    for (int i0 = 0; i0 < ns; i0 += kB) {
+        float2 p[kB];
+        float4 v[kB];
+#pragma unroll
+        for (int i = 0; i < kB; ++i) {
+            p[i] = make_float2(-__builtin_inff(), 0.0f);
+            if (i0 + i < ns) {   // (uniform: the workgroup's rows are of one tile)
+                const size_t at = r + (i0 + i) * step;
+                p[i] = a.ml[at];
+                v[i] = *(const float4 *)(a.o + at * kKv8Hd + d);
+            }
+        }
+        float m = M;
+#pragma unroll
+        for (int i = 0; i < kB; ++i) m = fmaxf(m, p[i].x);
+        const float f0 = m == M ? 1.0f : __builtin_amdgcn_exp2f(M - m);
+        M = m;
+        lt *= f0;
+        t = make_float4(t.x * f0, t.y * f0, t.z * f0, t.w * f0);
+#pragma unroll
+        for (int i = 0; i < kB; ++i) {
+            if (i0 + i >= ns) break;
+            const float f = __builtin_amdgcn_exp2f(p[i].x - M);
+            lt = __builtin_fmaf(p[i].y, f, lt);
+            t.x = __builtin_fmaf(v[i].x, f, t.x);
+            t.y = __builtin_fmaf(v[i].y, f, t.y);
+            t.z = __builtin_fmaf(v[i].z, f, t.z);
+            t.w = __builtin_fmaf(v[i].w, f, t.w);
+        }
     }
     *(float4 *)(a.out + ((size_t)tok * a.H + head) * kKv8Hd + d) =
         make_float4(t.x / lt, t.y / lt, t.z / lt, t.w / lt);
@@ -666,14 +839,31 @@ __global__ __launch_bounds__(256) void kv8_prefill_join_kernel(Kv8PrefillArgs a)
 }
 
 // A block's weight from the rows' softmax sums: the scores again, K in
-// registers (two blocks a wave), q's operands streamed.  Sums are in a fixed
-// order: rows of a lane, then lanes, then row splits.
+// registers (two blocks a wave, eight a workgroup), groups of 32 rows of q
+// (as MFMA operands, from the attention's first runs) through LDS, the next
+// group on its way meanwhile.  A group's exponentials alternate with the next
+// one's score products, which bound it (32 MFMAs of 32 cycles a wave and
+// group).  Sums are in a fixed order: rows of a lane, then lanes, then row splits.
+constexpr int kWtWaves = 4;
+constexpr int kWtBlocks = 2 * kWtWaves;
+constexpr int kWtGroup = 16 * 64;   // uint4 of a group's operands
 template <int FMT>
-__global__ __launch_bounds__(256) void kv8_weights_kernel(Kv8PrefillArgs a) {
+__global__ __launch_bounds__(64 * kWtWaves, 2) void kv8_weights_kernel(Kv8PrefillArgs a) {
+    __shared__ uint4 sq[2][kWtGroup];
     const int lane = threadIdx.x & 63, kvh = blockIdx.y, h = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-    const int nblk = kv8_blocks(a.pos0 + a.n), b0 = (blockIdx.x * 4 + wave) * 2;
-    if (b0 >= nblk) return;
+    const int nblk = kv8_blocks(a.pos0 + a.n), wg0 = blockIdx.x * kWtBlocks, b0 = wg0 + wave * 2;
+    const int r32 = pre_rows32(a.rows), groups = r32 / 32;
+    const int per = (groups + a.rsplits - 1) / a.rsplits;
+    // rows before the workgroup's first block see nothing of it
+    const int g0 = max(max(0, wg0 * kKv8Block - a.pos0) * a.G / 32, (int)blockIdx.z * per);
+    const int g1 = min(groups, (int)(blockIdx.z + 1) * per);
+    const uint4 *qf = a.qf + ((size_t)kvh * groups * 16 + 4 * wave) * 64 + lane;
+    auto fetch = [&](int g, int buf) {   // four of the group's operands each
+#pragma unroll
+        for (int i = 0; i < 4; ++i) lds_dma16(qf + (size_t)g * kWtGroup + i * 64, &sq[buf][(4 * wave + i) * 64]);
+    };
+    if (g0 < g1) fetch(g0, 0);
     const Kv8Layout l = kv8_layout(a.Hkv, a.nb);
     const float2 *sc = (const float2 *)(a.cache + l.scales) + (size_t)kvh * a.nb;
     half8_t kf[2][8];
@@ -690,45 +880,98 @@ __global__ __launch_bounds__(256) void kv8_weights_kernel(Kv8PrefillArgs a) {
         }
         ks[b] = sc[blk].x;
     }
-    const int r32 = pre_rows32(a.rows), groups = r32 / 32;
-    const int per = (groups + a.rsplits - 1) / a.rsplits;
-    // rows before the block see nothing of it
-    const int first = max(0, b0 * kKv8Block - a.pos0) * a.G / 32;
-    const int g1 = min(groups, (int)(blockIdx.z + 1) * per);
-    for (int g = max(first, (int)blockIdx.z * per); g < g1; ++g) {
-        const uint4 *f = a.qf + ((size_t)kvh * groups + g) * (8 * 2 * 64) + lane;
-        const int row = 32 * g + (lane & 31);
-        const float2 ls = a.lse[(size_t)kvh * r32 + row];
-        f32x16 s[2];
+    f32x16 s0[2], s1[2];   // scores of the group before, and of this one
+    float2 l0 = make_float2(__builtin_inff(), 0), l1;   // before the first: weighs nothing
+    // Group g's products into s, the group before's exponentials from t into acc.
+    auto group = [&](int g, int buf, f32x16 *s, f32x16 *t, const float2 &lt) {
+        const float c0 = ks[0] * lt.y, c1 = ks[1] * lt.y;
+        float p0 = 0.0f, p1 = 0.0f;
 #pragma unroll
         for (int b = 0; b < 2; ++b)
 #pragma unroll
             for (int i = 0; i < 16; ++i) s[b][i] = 0.0f;
+        const uint4 *q = sq[buf] + lane;
+        half8_t f[2] = {__builtin_bit_cast(half8_t, q[0]), __builtin_bit_cast(half8_t, q[64])};
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-            const half8_t q = __builtin_bit_cast(half8_t, f[i * 64]);
-            s[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[0][i >> 1], q, s[0], 0, 0, 0);
-            s[1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[1][i >> 1], q, s[1], 0, 0, 0);
+            s[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[0][i >> 1], f[i & 1], s[0], 0, 0, 0);
+            p0 += __builtin_amdgcn_exp2f(__builtin_fmaf(t[0][i], c0, -lt.x));
+            __builtin_amdgcn_sched_barrier(0);
+            s[1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[1][i >> 1], f[i & 1], s[1], 0, 0, 0);
+            p1 += __builtin_amdgcn_exp2f(__builtin_fmaf(t[1][i], c1, -lt.x));
+            if (i < 14) f[i & 1] = __builtin_bit_cast(half8_t, q[(i + 2) * 64]);
+            __builtin_amdgcn_sched_barrier(0);
         }
-        // positions that the row sees, from the lane's first one on
-        const int left = row < a.rows ? a.pos0 + row / a.G + 1 - b0 * kKv8Block - 4 * h : -1000;
+        asm volatile("" : "+v"(p0), "+v"(p1));   // (the sums stay in this basic block)
+        acc[0] += p0;
+        acc[1] += p1;
+        // rows that do not see all of the wave's positions (uniform test)
+        const int seen = a.pos0 + min(32 * g, a.rows - 1) / a.G + 1 - b0 * kKv8Block;
+        if (seen < 2 * kKv8Block) {
+            const int left = a.pos0 + min(32 * g + (lane & 31), a.rows - 1) / a.G + 1 - b0 * kKv8Block -
+                             4 * h + opaque_zero();
+#pragma unroll
+            for (int b = 0; b < 2; ++b)
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    s[b][i] = 32 * b + (i & 3) + 8 * (i >> 2) < left ? s[b][i] : -__builtin_inff();
+        }
+    };
+    // (hidden scores are -inf: scales of 0, of zero blocks, made positive)
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+        ks[b] = ks[b] < 1.2e-38f ? 1.2e-38f : ks[b];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            s0[b][i] = 0.0f;
+            s1[b][i] = 0.0f;
+        }
+    }
+    const float2 *lse = a.lse + (size_t)kvh * r32 + (lane & 31);
+    float2 ln = g0 < g1 ? lse[32 * g0] : make_float2(0, 0);
+    for (int g = g0; g < g1; g += 2) {
+        wait_vmcnt<0>();
+        lds_barrier();
+        l1 = ln;
+        if (g + 1 < g1) {
+            fetch(g + 1, 1);
+            ln = lse[32 * (g + 1)];
+        }
+        group(g, 0, s1, s0, l0);
+        if (g + 1 >= g1) {
+            l0 = l1;
+            s0[0] = s1[0];
+            s0[1] = s1[1];
+            break;
+        }
+        wait_vmcnt<0>();
+        lds_barrier();
+        l0 = ln;
+        if (g + 2 < g1) {
+            fetch(g + 2, 0);
+            ln = lse[32 * (g + 2)];
+        }
+        group(g + 1, 1, s0, s1, l1);
+    }
+    if (g0 < g1) {   // the last group's
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
-            const float ck = ks[b] * ls.y;
-            float ps = 0.0f;
+            float p = 0.0f;
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][i], ck, -ls.x));
-                ps += 32 * b + (i & 3) + 8 * (i >> 2) < left ? p : 0.0f;
-            }
-            acc[b] += ps;
+            for (int i = 0; i < 16; ++i) p += __builtin_amdgcn_exp2f(__builtin_fmaf(s0[b][i], ks[b] * l0.y, -l0.x));
+            acc[b] += p;
         }
     }
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
         acc[b] = wave_sum(acc[b]);
-        if (lane == 0 && b0 + b < nblk)
-            a.part[((size_t)blockIdx.z * a.Hkv + kvh) * nblk + b0 + b] = acc[b];
+        if (lane == 0 && b0 + b < nblk) {
+            if (a.rsplits > 1)
+                a.part[((size_t)blockIdx.z * a.Hkv + kvh) * nblk + b0 + b] = acc[b];
+            else
+                ((float *)(a.cache + l.weights))[(size_t)kvh * a.nb + b0 + b] += acc[b];
+        }
     }
 }
 
@@ -744,6 +987,7 @@ __global__ __launch_bounds__(256) void kv8_weights_add_kernel(Kv8PrefillArgs a) 
 // The launch shapes of a prefill call and its workspace.
 struct PrefillPlan {
     int rows, rtiles, splits, per, rsplits;
+    int64_t wgs;
     size_t ml, o, lse, qf, part, bytes;
 };
 static PrefillPlan prefill_plan(int n, int pos0, int H, int Hkv, bool weights) {
@@ -751,33 +995,49 @@ static PrefillPlan prefill_plan(int n, int pos0, int H, int Hkv, bool weights) {
     const int G = H / Hkv, total = pos0 + n, nblk = kv8_blocks(total);
     p.rows = n * G;
     p.rtiles = (p.rows + kPreRows - 1) / kPreRows;
-    const int tiles = (total + kPreTile - 1) / kPreTile;
-    // two workgroups per CU are resident; splits of at least four tiles
-    const int64_t wgs = (int64_t)p.rtiles * Hkv, target = 2 * (int64_t)device_cus();
-    int64_t s = (target + wgs - 1) / wgs;
-    if (s > (tiles + 3) / 4) s = (tiles + 3) / 4;
-    if (s < 1) s = 1;
-    p.per = (int)((tiles + s - 1) / s);
-    p.splits = (tiles + p.per - 1) / p.per;
-    size_t at = 0;
+    // Two workgroups per CU are resident: the shortest runs, of at least eight
+    // blocks, whose workgroups (row tiles that see less have fewer) all are;
+    // a longest run is what the launch takes.
+    const int most = kv8_blocks(total);
+    auto count = [&](int per) {
+        int64_t wgs = 0;
+        for (int r = 0; r < p.rtiles; ++r) {
+            const int last = (r + 1) * kPreRows < p.rows ? (r + 1) * kPreRows : p.rows;
+            wgs += (kv8_blocks(pos0 + (last - 1) / G + 1) + per - 1) / per;
+        }
+        return wgs * Hkv;
+    };
+    int lo = 8, hi = most;   // runs of `most` blocks are no split at all
+    if ((int64_t)p.rtiles * Hkv > 2 * device_cus()) lo = hi;
+    while (lo < hi) {
+        const int mid = lo + (hi - lo) / 2;
+        if (count(mid) <= 2 * device_cus()) hi = mid;
+        else lo = mid + 1;
+    }
+    p.per = hi < 8 ? 8 : hi;
+    p.splits = (most + p.per - 1) / p.per;
+    p.wgs = p.splits == 1 ? (int64_t)p.rtiles * Hkv : count(p.per);
+    size_t at = kArrivals * 4;
     auto take = [&](size_t b) {
         const size_t o = at;
         at += kv8_align(b);
         return o;
     };
     if (p.splits > 1) {
-        p.ml = take((size_t)p.splits * Hkv * p.rows * 8);
-        p.o = take((size_t)p.splits * Hkv * p.rows * kKv8Hd * 4);
+        const size_t parts = (size_t)p.splits * Hkv * p.rows;
+        p.ml = take(parts * 8);
+        p.o = take(parts * kKv8Hd * 4);
     }
     if (weights) {
         const size_t r32 = pre_rows32(p.rows);
         p.lse = take(Hkv * r32 * 8);
         p.qf = take(Hkv * r32 * kKv8Hd * 4);
-        const int64_t w = (int64_t)((nblk + 7) / 8) * Hkv, groups = r32 / 32;
-        int64_t rs = (4 * (int64_t)device_cus() + w - 1) / w;
-        if (rs > (groups + 3) / 4) rs = (groups + 3) / 4;
+        // row splits (of at least eight groups) while two workgroups per CU have room
+        const int64_t w = (int64_t)((nblk + kWtBlocks - 1) / kWtBlocks) * Hkv, groups = r32 / 32;
+        int64_t rs = 2 * (int64_t)device_cus() / w;
+        if (rs > groups / 8) rs = groups / 8;
         p.rsplits = (int)(rs < 1 ? 1 : rs);
-        p.part = take((size_t)p.rsplits * Hkv * nblk * 4);
+        if (p.rsplits > 1) p.part = take((size_t)p.rsplits * Hkv * nblk * 4);
     }
     p.bytes = at;
     return p;
@@ -809,16 +1069,16 @@ extern "C" int oxb_attn_decode_kv8(const float *q, void *cache, size_t cache_str
     OXB_REQUIRE(q && out && (((uintptr_t)q | (uintptr_t)out) & 15) == 0,
                 "attention: q or out is NULL or not 16-byte aligned");
     OXB_REQUIRE(pos && pos_stride >= 0, "attention: pos is NULL or its stride %d", pos_stride);
-    const int nb = kv8_blocks(max_seq), G = H / Hkv, HC = (G + kDecRows - 1) / kDecRows;
+    const int nb = kv8_blocks(max_seq);
     const DecodeWs w = decode_ws(batch, H, Hkv, nb);
     OXB_REQUIRE(ws && ((uintptr_t)ws & 255) == 0 && ws_bytes >= w.bytes,
                 "attention: workspace is NULL, not 256-byte aligned or %zu bytes < %zu", ws_bytes, w.bytes);
-    Kv8DecodeArgs a{q, (uint8_t *)cache, cache_stride, pos, pos_stride, H, Hkv, G, HC, max_seq, nb,
-                    decode_splits(batch, Hkv, HC, nb), add_weights != 0, out,
-                    (float2 *)((char *)ws + w.ml), (float *)((char *)ws + w.o),
-                    (float2 *)((char *)ws + w.bw)};
+    char *wp = (char *)ws;
+    const Kv8DecodeArgs a{q, (uint8_t *)cache, cache_stride, pos, pos_stride, H, Hkv, H / Hkv, max_seq, nb,
+                          decode_splits(batch, Hkv, nb), out, (int *)wp, (uint64_t *)(wp + w.ml),
+                          (uint64_t *)(wp + w.o), (uint64_t *)(wp + w.bw)};
     hipStream_t s = (hipStream_t)stream;
-    const dim3 grid(a.splits, Hkv * HC, batch), th(kDecThreads);
+    const dim3 grid(a.splits, Hkv, batch), th(kDecThreads);
     if (fmt == OXB_KV8_INT8) {
         if (add_weights)
             hipLaunchKernelGGL((kv8_decode_kernel<OXB_KV8_INT8, true>), grid, th, 0, s, a);
@@ -831,11 +1091,6 @@ extern "C" int oxb_attn_decode_kv8(const float *q, void *cache, size_t cache_str
             hipLaunchKernelGGL((kv8_decode_kernel<OXB_KV8_E4M3, false>), grid, th, 0, s, a);
     }
     OXB_CHECK_HIP(hipGetLastError());
-    if (a.splits > 1 || add_weights) {
-        const int chunks = add_weights ? Hkv * ((nb + kJoinThreads - 1) / kJoinThreads) : 0;
-        hipLaunchKernelGGL(kv8_decode_join_kernel, dim3(H + chunks, batch), dim3(kJoinThreads), 0, s, a);
-        OXB_CHECK_HIP(hipGetLastError());
-    }
     return 0;
 }
 
@@ -858,22 +1113,19 @@ extern "C" int oxb_attn_prefill_kv8(const float *q, void *cache, int fmt, int n_
                 "prefill attention: bad range");
     OXB_REQUIRE((int64_t)n_tok * (H / Hkv) <= (1 << 30), "prefill attention: %d tokens", n_tok);
     const PrefillPlan p = prefill_plan(n_tok, pos0, H, Hkv, add_weights != 0);
-    OXB_REQUIRE(p.bytes == 0 || (ws && ((uintptr_t)ws & 255) == 0 && ws_bytes >= p.bytes),
+    OXB_REQUIRE(ws && ((uintptr_t)ws & 255) == 0 && ws_bytes >= p.bytes,
                 "attention: workspace is NULL, not 256-byte aligned or %zu bytes < %zu", ws_bytes, p.bytes);
     char *w = (char *)ws;
     Kv8PrefillArgs a{q, (uint8_t *)cache, n_tok, pos0, H, Hkv, H / Hkv, kv8_blocks(max_seq), p.rows,
-                     p.splits, p.per, add_weights != 0, out, (float2 *)(w + p.ml), (float *)(w + p.o),
+                     p.rtiles, p.splits, p.per, add_weights != 0, out, (float2 *)(w + p.ml), (float *)(w + p.o),
                      (float2 *)(w + p.lse), (uint4 *)(w + p.qf), (float *)(w + p.part), p.rsplits};
     hipStream_t s = (hipStream_t)stream;
-    const dim3 grid(p.rtiles, Hkv, p.splits), th(kPreThreads);
-    const size_t lds = 2 * kPreTileBytes;
-    if (fmt == OXB_KV8_INT8) {
-        if (allow_dynamic_lds((const void *)kv8_prefill_kernel<OXB_KV8_INT8>)) return -1;
-        hipLaunchKernelGGL(kv8_prefill_kernel<OXB_KV8_INT8>, grid, th, lds, s, a);
-    } else {
-        if (allow_dynamic_lds((const void *)kv8_prefill_kernel<OXB_KV8_E4M3>)) return -1;
-        hipLaunchKernelGGL(kv8_prefill_kernel<OXB_KV8_E4M3>, grid, th, lds, s, a);
-    }
+    OXB_REQUIRE(p.wgs < (1 << 30), "prefill attention: %d tokens", n_tok);
+    const dim3 grid((unsigned)p.wgs), th(kPreThreads);
+    if (fmt == OXB_KV8_INT8)
+        hipLaunchKernelGGL(kv8_prefill_kernel<OXB_KV8_INT8>, grid, th, 0, s, a);
+    else
+        hipLaunchKernelGGL(kv8_prefill_kernel<OXB_KV8_E4M3>, grid, th, 0, s, a);
     OXB_CHECK_HIP(hipGetLastError());
     if (p.splits > 1) {
         hipLaunchKernelGGL(kv8_prefill_join_kernel, dim3((p.rows + 7) / 8, Hkv), dim3(256), 0, s, a);
@@ -881,14 +1133,16 @@ extern "C" int oxb_attn_prefill_kv8(const float *q, void *cache, int fmt, int n_
     }
     if (add_weights) {
         const int nblk = kv8_blocks(pos0 + n_tok);
-        const dim3 wg((nblk + 7) / 8, Hkv, p.rsplits);
+        const dim3 wg((nblk + kWtBlocks - 1) / kWtBlocks, Hkv, p.rsplits);
         if (fmt == OXB_KV8_INT8)
             hipLaunchKernelGGL(kv8_weights_kernel<OXB_KV8_INT8>, wg, dim3(256), 0, s, a);
         else
             hipLaunchKernelGGL(kv8_weights_kernel<OXB_KV8_E4M3>, wg, dim3(256), 0, s, a);
         OXB_CHECK_HIP(hipGetLastError());
-        hipLaunchKernelGGL(kv8_weights_add_kernel, dim3((nblk + 255) / 256, Hkv), dim3(256), 0, s, a);
-        OXB_CHECK_HIP(hipGetLastError());
+        if (p.rsplits > 1) {
+            hipLaunchKernelGGL(kv8_weights_add_kernel, dim3((nblk + 255) / 256, Hkv), dim3(256), 0, s, a);
+            OXB_CHECK_HIP(hipGetLastError());
+        }
     }
     return 0;
 }

@@ -39,14 +39,6 @@ __global__ __launch_bounds__(kLrThreads) void logit_rules_kernel(RulesArgs a) {
     __shared__ int last[kLrChunk];   // 1 + the last bias entry of the id
     const int r = blockIdx.y, base = blockIdx.x * kLrChunk, tid = threadIdx.x;
     const int n = min(kLrChunk, a.V - base);
-    const float *lg = a.logits + (size_t)r * a.stride + base;
-    float x[kLrPer];
-#pragma unroll
-    for (int u = 0; u < kLrPer; ++u) {
-        x[u] = lg[min(tid + u * kLrThreads, n - 1)];
-        cnt[tid + u * kLrThreads] = 0;
-        last[tid + u * kLrThreads] = 0;
-    }
     // ranges of this row, kept inside the lists whatever the offsets say
     int h0 = 0, h1 = 0, b0 = 0, b1 = 0;
     if (a.pen && a.n_hist > 0) {
@@ -57,36 +49,60 @@ __global__ __launch_bounds__(kLrThreads) void logit_rules_kernel(RulesArgs a) {
         b0 = min(max(a.bias_off[r], 0), a.n_bias);
         b1 = min(a.bias_off[r + 1], a.n_bias);
     }
-    lds_barrier();
-    for (int j = h0 + tid; j < h1; j += kLrThreads) {
-        const unsigned i = (unsigned)a.hist[j] - (unsigned)base;
-        if (i < (unsigned)n) atomicAdd(&cnt[i], 1);
+    // every load that depends on nothing goes out at once
+    const float *lg = a.logits + (size_t)r * a.stride + base;
+    const uint32_t *mask = a.mask ? a.mask + (size_t)r * a.mask_stride : nullptr;
+    float x[kLrPer];
+    uint32_t mw[kLrPer];
+#pragma unroll
+    for (int u = 0; u < kLrPer; ++u) {
+        const int i = min(tid + u * kLrThreads, n - 1);
+        x[u] = lg[i];
+        mw[u] = mask ? mask[(base + i) >> 5] : 0xffffffffu;
     }
-    for (int j = b0 + tid; j < b1; j += kLrThreads) {
-        const unsigned i = (unsigned)a.bias_ids[j] - (unsigned)base;
-        if (i < (unsigned)n) atomicMax(&last[i], j + 1);
-    }
-    lds_barrier();
     float rep = 1.0f, freq = 0.0f, pres = 0.0f;
     if (a.pen) {
         rep = a.pen[3 * r];
         freq = a.pen[3 * r + 1];
         pres = a.pen[3 * r + 2];
     }
-    const uint32_t *mask = a.mask ? a.mask + (size_t)r * a.mask_stride : nullptr;
+    const bool lists = h0 < h1 || b0 < b1;   // uniform
+    if (lists) {
+#pragma unroll
+        for (int u = 0; u < kLrPer; ++u) {
+            cnt[tid + u * kLrThreads] = 0;
+            last[tid + u * kLrThreads] = 0;
+        }
+        lds_barrier();
+        for (int j0 = h0 + tid; j0 < h1; j0 += kLrPer * kLrThreads) {
+            int id[kLrPer];
+#pragma unroll
+            for (int u = 0; u < kLrPer; ++u) id[u] = a.hist[min(j0 + u * kLrThreads, h1 - 1)];
+#pragma unroll
+            for (int u = 0; u < kLrPer; ++u) {
+                const unsigned i = (unsigned)id[u] - (unsigned)base;
+                if (j0 + u * kLrThreads < h1 && i < (unsigned)n) atomicAdd(&cnt[i], 1);
+            }
+        }
+        for (int j = b0 + tid; j < b1; j += kLrThreads) {
+            const unsigned i = (unsigned)a.bias_ids[j] - (unsigned)base;
+            if (i < (unsigned)n) atomicMax(&last[i], j + 1);
+        }
+        lds_barrier();
+    }
     float *out = a.out + (size_t)r * a.out_stride + base;
 #pragma unroll
     for (int u = 0; u < kLrPer; ++u) {
         const int i = tid + u * kLrThreads;
         if (i >= n) continue;
         float y = x[u];
-        const int c = cnt[i], b = last[i];
+        const int c = lists ? cnt[i] : 0, b = lists ? last[i] : 0;
         if (c > 0) {
             y = y > 0.0f ? y / rep : y * rep;
             y = y - (freq * (float)c + pres);
         }
         if (b > 0) y = y + a.bias[b - 1];
-        if (mask && !(mask[(base + i) >> 5] >> ((base + i) & 31) & 1)) y = -__builtin_inff();
+        if (!(mw[u] >> ((base + i) & 31) & 1)) y = -__builtin_inff();
         out[i] = y;
     }
 }

@@ -312,7 +312,7 @@ class Kv8Cache:
         dq, dp = DeviceArray.from_host(q), DeviceArray.from_host(np.ascontiguousarray(pos, np.int32))
         out = DeviceArray(q.shape, np.float32)
         n = lib().oxb_attn_decode_kv8_ws_bytes(self.batch, H, self.Hkv, self.hd, self.max_seq)
-        ws = DeviceArray((max(n, 16),), np.uint8)
+        ws = DeviceArray((max(n, 16),), np.uint8, zero=True)
         check(lib().oxb_attn_decode_kv8(dq.ptr, self.data.ptr, self.stride, self.fmt, dp.ptr, 1, self.batch,
                                         H, self.Hkv, self.hd, self.max_seq, int(add_weights), out.ptr,
                                         ws.ptr, n, None), "attn_decode_kv8")
@@ -325,7 +325,7 @@ class Kv8Cache:
         n, H = q.shape[0], q.shape[1] // self.hd
         dq, out = DeviceArray.from_host(q), DeviceArray(q.shape, np.float32)
         b = lib().oxb_attn_prefill_kv8_ws_bytes(n, pos0, H, self.Hkv, self.hd, int(add_weights))
-        ws = DeviceArray((max(b, 16),), np.uint8)
+        ws = DeviceArray((max(b, 16),), np.uint8, zero=True)
         check(lib().oxb_attn_prefill_kv8(dq.ptr, self.data.offset(slot * self.stride), self.fmt, n, pos0, H,
                                          self.Hkv, self.hd, self.max_seq, int(add_weights), out.ptr, ws.ptr,
                                          b, None), "attn_prefill_kv8")

@@ -332,8 +332,11 @@ int oxb_kv8_read(const void *cache, size_t cache_stride, int fmt, int batch, int
  * add_weights, the softmax weights of each block's positions, summed over the
  * KV head's query heads, are added to the block's weight.  The result does not
  * depend on timing.  ws: a device workspace of oxb_attn_decode_kv8_ws_bytes
- * bytes, 256-byte aligned, any contents; calls that share one must not run
- * concurrently.  Replaces nn/attention.rs:109-118 over this cache. */
+ * bytes, 256-byte aligned; its first 4 KB are arrival counters that must be
+ * zero before its first use (a zero-filled allocation) and that every call
+ * leaves zero, so one of the largest size serves calls of any shapes in turn.
+ * Calls that share one must not run concurrently.  Replaces
+ * nn/attention.rs:109-118 over this cache. */
 size_t oxb_attn_decode_kv8_ws_bytes(int batch, int H, int Hkv, int hd, int max_seq);
 int oxb_attn_decode_kv8(const float *q, void *cache, size_t cache_stride, int fmt, const int *pos,
                         int pos_stride, int batch, int H, int Hkv, int hd, int max_seq,
@@ -341,8 +344,8 @@ int oxb_attn_decode_kv8(const float *q, void *cache, size_t cache_stride, int fm
 
 /* Causal prefill attention over one sequence's 8-bit cache: query i (q, out:
  * [n_tok][H*128]) attends over positions 0..pos0 + i, which the cache holds
- * already (append first).  Arithmetic, weights and workspace as above; the
- * workspace may be 0 bytes and NULL for some shapes. */
+ * already (append first).  Arithmetic, weights and workspace as above (one
+ * workspace may serve both). */
 size_t oxb_attn_prefill_kv8_ws_bytes(int n_tok, int pos0, int H, int Hkv, int hd, int add_weights);
 int oxb_attn_prefill_kv8(const float *q, void *cache, int fmt, int n_tok, int pos0, int H, int Hkv,
                          int hd, int max_seq, int add_weights, float *out, void *ws,

@@ -318,7 +318,7 @@ def test_prefill_leaves_rows_behind_the_last():
     q = ops.DeviceArray.from_host(rng.standard_normal((45, 8 * HD)).astype(np.float32))
     out = ops.DeviceArray.from_host(np.full((64, 8 * HD), 7.0, np.float32))
     n = L.oxb_attn_prefill_kv8_ws_bytes(40, 5, 8, 2, HD, 0)
-    ws = ops.DeviceArray((max(n, 16),), np.uint8)
+    ws = ops.DeviceArray((max(n, 16),), np.uint8, zero=True)
     before = c.data.download()
     ops.check(L.oxb_attn_prefill_kv8(q.ptr, c.data.ptr, 0, 40, 5, 8, 2, HD, 64, 0, out.ptr, ws.ptr, n, None))
     ops.sync()
@@ -536,7 +536,7 @@ def test_captured_step_replays():
     dq, out = (ops.DeviceArray((B, H * HD), np.float32) for _ in "qo")
     dp = ops.DeviceArray((B,), np.int32)
     n = L.oxb_attn_decode_kv8_ws_bytes(B, H, hkv, HD, ms)
-    ws = ops.DeviceArray((n,), np.uint8)
+    ws = ops.DeviceArray((n,), np.uint8, zero=True)
     ops.sync()
     ops.check(L.oxb_stream_begin_capture(st))
     ops.check(L.oxb_kv8_append(c.data.ptr, c.stride, fmt, B, hkv, HD, ms, dk.ptr, dv.ptr, hkv * HD, HD, 0,
