@@ -23,6 +23,7 @@
 namespace oxb {
 
 constexpr int kKvThreads = 256;
+typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
 
 struct Kv8AppendArgs {
     uint8_t *cache;
@@ -49,12 +50,18 @@ __device__ inline void kv8_span(const Kv8AppendArgs &a, int z, int &p0, int &cnt
     cnt = min(c, a.max_seq - p0);
 }
 
-// One workgroup per (block, K or V, head, sequence).  Each thread holds 8 dims
-// of two rows.  Latency bound for one row (a block's rows come from L2), and by
-// the codes' and rows' bytes for a prompt.
+// One workgroup per (block, K or V, head, sequence).  A thread holds 4 dims of 4
+// consecutive positions, so that it has the 4 bytes that a V row keeps together
+// (and 4 of a K row).  Latency bound for one row (a block's rows come from L2),
+// by the rows' and codes' bytes for a prompt: the quotient is two products and
+// its own remainder's correction,
+//   y = t (1/a),  y' = y + (t - y a) (1/a),  t = top x (exact),
+// off by 2^-24 of itself at most and exact where the quotient is an f32 number,
+// ties among them: the same codes as the f32 division's, in a third of its
+// instructions.
 template <int FMT>
 __global__ __launch_bounds__(kKvThreads) void kv8_append_kernel(Kv8AppendArgs a) {
-    __shared__ uint4 vt[kKv8Half / 16];   // V codes, [dim][byte]
+    __shared__ uint32_t vt[kKv8Hd * 9];   // V codes, [dim][9 dwords]: 8, and one against bank conflicts
     __shared__ int red[4];
     const int z = blockIdx.z, h = blockIdx.y, isv = blockIdx.x & 1;
     int p0, cnt;
@@ -67,25 +74,24 @@ __global__ __launch_bounds__(kKvThreads) void kv8_append_kernel(Kv8AppendArgs a)
     uint16_t *tail = (uint16_t *)(seq + l.tails) + ((size_t)h * 2 + isv) * kKv8Half;
     const uint16_t *src = (isv ? a.v : a.k) + (size_t)z * a.src_stride + (size_t)h * a.src_head;
     const int row0 = a.src_at_pos ? 0 : p0;          // source row = position - row0
-    const int tid = threadIdx.x, d = (tid & 15) * 8;
+    const int tid = threadIdx.x, d = (tid & 31) * 4, t0 = (tid >> 5) * 4;
 
-    u32x4_t x[2];
+    u32x2_t x[4];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const int t = (tid >> 4) + 16 * i, p = b * kKv8Block + t;
-        x[i] = u32x4_t{0, 0, 0, 0};
+    for (int i = 0; i < 4; ++i) {
+        const int t = t0 + i, p = b * kKv8Block + t;
+        x[i] = u32x2_t{0, 0};
         if (p < p0)
-            x[i] = *(const u32x4_t *)(tail + t * kKv8Hd + d);
+            x[i] = *(const u32x2_t *)(tail + t * kKv8Hd + d);
         else if (p < end)
-            x[i] = *(const u32x4_t *)(src + (size_t)(p - row0) * kKv8Hd + d);
+            x[i] = *(const u32x2_t *)(src + (size_t)(p - row0) * kKv8Hd + d);
     }
     // |x| as the f16's low 15 bits: ordered like the values, 0x7c00 and up not finite
     int m = 0;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-            m = max(m, max((int)(x[i][j] & 0x7fff), (int)(x[i][j] >> 16 & 0x7fff)));
+    for (int i = 0; i < 4; ++i) {
+        m = max(m, max((int)(x[i].x & 0x7fff), (int)(x[i].x >> 16 & 0x7fff)));
+        m = max(m, max((int)(x[i].y & 0x7fff), (int)(x[i].y >> 16 & 0x7fff)));
     }
 #pragma unroll
     for (int s = 32; s > 0; s >>= 1) m = max(m, __shfl_xor(m, s, 64));
@@ -95,50 +101,52 @@ __global__ __launch_bounds__(kKvThreads) void kv8_append_kernel(Kv8AppendArgs a)
     constexpr float kTop = FMT == OXB_KV8_INT8 ? 127.0f : 448.0f;
     const bool finite = m < 0x7c00;
     const float amax = finite ? __half2float(__ushort_as_half((unsigned short)m)) : 1.0f;
-    const float div = amax > 0.0f ? amax : 1.0f;
-    uint2 c[2];
+    const float div = amax > 0.0f ? amax : 1.0f, rdiv = 1.0f / div;
+    uint32_t c[4];   // 4 dims of a position
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        uint32_t o[2];
+    for (int i = 0; i < 4; ++i) {
+        float r[4];
 #pragma unroll
-        for (int g = 0; g < 2; ++g) {
-            float r[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const uint32_t bits = x[i][2 * g + (j >> 1)] >> (16 * (j & 1)) & 0xffff;
-                const float v = finite ? __half2float(__ushort_as_half((unsigned short)bits)) : 0.0f;
-                r[j] = v * kTop / div;
-            }
-            if constexpr (FMT == OXB_KV8_INT8) {
-                o[g] = 0;
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    o[g] |= (uint32_t)((int)rintf(r[j]) + 128) << (8 * j);
-            } else {
-                int q = __builtin_amdgcn_cvt_pk_fp8_f32(r[0], r[1], 0, false);
-                o[g] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(r[2], r[3], q, true);
-            }
+        for (int j = 0; j < 4; ++j) {
+            const uint32_t bits = (j < 2 ? x[i].x : x[i].y) >> (16 * (j & 1)) & 0xffff;
+            const float t = finite ? __half2float(__ushort_as_half((unsigned short)bits)) * kTop : 0.0f;
+            const float y = t * rdiv;
+            r[j] = __builtin_fmaf(__builtin_fmaf(-y, div, t), rdiv, y);
+            if constexpr (FMT == OXB_KV8_E4M3) r[j] = __builtin_copysignf(r[j], t);   // -0 stays
         }
-        c[i] = make_uint2(o[0], o[1]);
+        if constexpr (FMT == OXB_KV8_INT8) {
+            // 2^23 + 2^22 + 128: the sum's rounding is the quotient's to a whole
+            // number, and its low byte the code's
+            uint32_t w[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) w[j] = __float_as_uint(r[j] + 12583040.0f);
+            const uint32_t lo = __builtin_amdgcn_perm(w[1], w[0], 0x0c0c0400u);
+            const uint32_t hi = __builtin_amdgcn_perm(w[3], w[2], 0x0c0c0400u);
+            c[i] = lo | hi << 16;
+        } else {
+            const int q = __builtin_amdgcn_cvt_pk_fp8_f32(r[0], r[1], 0, false);
+            c[i] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(r[2], r[3], q, true);
+        }
     }
     const size_t blk = (size_t)h * a.nb + b;
     uint8_t *codes = seq + blk * kKv8Codes;
     if (isv) {
-        uint8_t *vb = (uint8_t *)vt;
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int at = kv8_v_byte((tid >> 4) + 16 * i);
-            const uint32_t w[2] = {c[i].x, c[i].y};
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-                vb[(d + j) * kKv8Block + at] = (uint8_t)(w[j >> 2] >> (8 * (j & 3)));
-        }
+        // bytes to positions: dword j holds dim d + j of positions t0 .. t0 + 3
+        const uint32_t l0 = __builtin_amdgcn_perm(c[1], c[0], 0x05010400u);   // c0.0 c1.0 c0.1 c1.1
+        const uint32_t l1 = __builtin_amdgcn_perm(c[3], c[2], 0x05010400u);
+        const uint32_t h0 = __builtin_amdgcn_perm(c[1], c[0], 0x07030602u);   // c0.2 c1.2 c0.3 c1.3
+        const uint32_t h1 = __builtin_amdgcn_perm(c[3], c[2], 0x07030602u);
+        uint32_t *at = vt + d * 9 + kv8_v_byte(t0) / 4;
+        at[0] = __builtin_amdgcn_perm(l1, l0, 0x05040100u);
+        at[9] = __builtin_amdgcn_perm(l1, l0, 0x07060302u);
+        at[18] = __builtin_amdgcn_perm(h1, h0, 0x05040100u);
+        at[27] = __builtin_amdgcn_perm(h1, h0, 0x07060302u);
         __syncthreads();
-        ((uint4 *)(codes + kKv8Half))[tid] = vt[tid];
+        const uint32_t *w = vt + (tid >> 1) * 9 + (tid & 1) * 4;
+        ((uint4 *)(codes + kKv8Half))[tid] = make_uint4(w[0], w[1], w[2], w[3]);
     } else {
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
-            *(uint2 *)(codes + ((tid >> 4) + 16 * i) * kKv8Hd + d) = c[i];
+        for (int i = 0; i < 4; ++i) *(uint32_t *)(codes + (t0 + i) * kKv8Hd + d) = c[i];
     }
     if (tid == 0) {
         ((float *)(seq + l.scales))[2 * blk + isv] = finite ? amax / kTop : __builtin_nanf("");
@@ -151,12 +159,12 @@ __global__ __launch_bounds__(kKvThreads) void kv8_append_kernel(Kv8AppendArgs a)
     if (b == first && end % kKv8Block) {
         __syncthreads();
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int t = (tid >> 4) + 16 * i, p = last * kKv8Block + t;
+        for (int i = 0; i < 4; ++i) {
+            const int t = t0 + i, p = last * kKv8Block + t;
             if (p >= p0 && p < end) {
-                u32x4_t y = x[i];
-                if (last != first) y = *(const u32x4_t *)(src + (size_t)(p - row0) * kKv8Hd + d);
-                *(u32x4_t *)(tail + t * kKv8Hd + d) = y;
+                u32x2_t y = x[i];
+                if (last != first) y = *(const u32x2_t *)(src + (size_t)(p - row0) * kKv8Hd + d);
+                *(u32x2_t *)(tail + t * kKv8Hd + d) = y;
             }
         }
     }
@@ -174,10 +182,11 @@ struct Kv8ReadArgs {
 };
 
 // One workgroup per (block, K or V, head, sequence): its positions among the
-// asked ones as f32 rows.  Bound by the rows' bytes.
+// asked ones as f32 rows, 4 dims of 4 positions a thread as in the append.
+// Bound by the rows' bytes.
 template <int FMT>
 __global__ __launch_bounds__(kKvThreads) void kv8_read_kernel(Kv8ReadArgs a) {
-    __shared__ uint4 vt[kKv8Half / 16];
+    __shared__ uint32_t vt[kKv8Hd * 9];
     const int z = blockIdx.z, h = blockIdx.y, isv = blockIdx.x & 1, tid = threadIdx.x;
     const int64_t p0 = (int64_t)(a.pos ? a.pos[(size_t)z * a.pos_stride] : 0) + a.pos0;
     int64_t limit = a.max_seq;
@@ -190,38 +199,41 @@ __global__ __launch_bounds__(kKvThreads) void kv8_read_kernel(Kv8ReadArgs a) {
     const size_t blk = (size_t)h * a.nb + (there ? (int)b : 0);
     const uint8_t *codes = seq + blk * kKv8Codes + (isv ? kKv8Half : 0);
     const float scale = there ? ((const float *)(seq + l.scales))[2 * blk + isv] : 0.0f;
-    const int d = (tid & 15) * 8;
-    if (there && isv) vt[tid] = ((const uint4 *)codes)[tid];
-    __syncthreads();
+    const int d = (tid & 31) * 4, t0 = (tid >> 5) * 4;
+    uint32_t c[4] = {0, 0, 0, 0};
+    if (there && isv) {
+        const uint4 v = ((const uint4 *)codes)[tid];
+        uint32_t *w = vt + (tid >> 1) * 9 + (tid & 1) * 4;
+        w[0] = v.x;
+        w[1] = v.y;
+        w[2] = v.z;
+        w[3] = v.w;
+        __syncthreads();   // (uniform)
+        const uint32_t *at = vt + d * 9 + kv8_v_byte(t0) / 4;
+        const uint32_t l0 = __builtin_amdgcn_perm(at[9], at[0], 0x05010400u);
+        const uint32_t l1 = __builtin_amdgcn_perm(at[27], at[18], 0x05010400u);
+        const uint32_t h0 = __builtin_amdgcn_perm(at[9], at[0], 0x07030602u);
+        const uint32_t h1 = __builtin_amdgcn_perm(at[27], at[18], 0x07030602u);
+        c[0] = __builtin_amdgcn_perm(l1, l0, 0x05040100u);
+        c[1] = __builtin_amdgcn_perm(l1, l0, 0x07060302u);
+        c[2] = __builtin_amdgcn_perm(h1, h0, 0x05040100u);
+        c[3] = __builtin_amdgcn_perm(h1, h0, 0x07060302u);
+    } else if (there) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) c[i] = *(const uint32_t *)(codes + (t0 + i) * kKv8Hd + d);
+    }
     float *out = (isv ? a.v : a.k) + ((size_t)z * a.Hkv + h) * (size_t)a.n * kKv8Hd;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const int t = (tid >> 4) + 16 * i;
-        const int64_t p = b * kKv8Block + t;
+    for (int i = 0; i < 4; ++i) {
+        const int64_t p = b * kKv8Block + t0 + i;
         if (p < p0 || p >= p0 + a.n) continue;
-        float4 lo = make_float4(0, 0, 0, 0), hi = lo;
+        float4 v = make_float4(0, 0, 0, 0);
         if (p >= 0 && p < limit) {
-            uint2 w;
-            if (isv) {
-                const uint8_t *vb = (const uint8_t *)vt + kv8_v_byte(t);
-                w = make_uint2(0, 0);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    w.x |= (uint32_t)vb[(d + j) * kKv8Block] << (8 * j);
-                    w.y |= (uint32_t)vb[(d + 4 + j) * kKv8Block] << (8 * j);
-                }
-            } else {
-                w = *(const uint2 *)(codes + t * kKv8Hd + d);
-            }
-            const half8_t v = kv8_unpack8<FMT>(w.x, w.y);
-            lo = make_float4((float)v[0] * scale, (float)v[1] * scale, (float)v[2] * scale,
-                             (float)v[3] * scale);
-            hi = make_float4((float)v[4] * scale, (float)v[5] * scale, (float)v[6] * scale,
-                             (float)v[7] * scale);
+            half2_t x, y;
+            kv8_unpack4<FMT>(c[i], x, y);
+            v = make_float4((float)x.x * scale, (float)x.y * scale, (float)y.x * scale, (float)y.y * scale);
         }
-        float4 *row = (float4 *)(out + (size_t)(p - p0) * kKv8Hd + d);
-        row[0] = lo;
-        row[1] = hi;
+        *(float4 *)(out + (size_t)(p - p0) * kKv8Hd + d) = v;
     }
 }
 
@@ -326,10 +338,13 @@ __global__ __launch_bounds__(kEvThreads) void kv8_select_kernel(Kv8EvictArgs a) 
     }
 }
 
-constexpr int kMvCols = 32;                        // workgroups per head: 256-byte columns of a block
-constexpr int kMvLanes = kKv8Codes / kMvCols / 16; // 16-byte lanes of a column
-constexpr int kMvRows = kKvThreads / kMvLanes;     // blocks per pass
-constexpr int kMvUnroll = 4;                       // passes in flight
+// A workgroup moves a 256-byte column of a head's kept blocks, 16 blocks a pass
+// and 4 passes in flight.  (1 KB columns in a quarter of the workgroups: 24.0 us
+// against 22.7 for 32 sequences of 32 blocks.)
+constexpr int kMvCols = 32;
+constexpr int kMvLanes = kKv8Codes / kMvCols / 16;   // 16-byte lanes of a column
+constexpr int kMvRows = kKvThreads / kMvLanes;       // blocks per pass
+constexpr int kMvUnroll = 4;
 
 __global__ __launch_bounds__(kKvThreads) void kv8_move_kernel(Kv8EvictArgs a) {
     const int col = blockIdx.x, h = blockIdx.y, z = blockIdx.z, tid = threadIdx.x;
@@ -347,20 +362,21 @@ __global__ __launch_bounds__(kKvThreads) void kv8_move_kernel(Kv8EvictArgs a) {
         int from[kMvUnroll];
 #pragma unroll
         for (int u = 0; u < kMvUnroll; ++u)   // (clamped; not written past the kept ones)
-            from[u] = list[min(j0 + u * kMvRows + tid / kMvLanes, kept - 1)];
+            if (j0 + u * kMvRows < kept) from[u] = list[min(j0 + u * kMvRows + tid / kMvLanes, kept - 1)];
 #pragma unroll
-        for (int u = 0; u < kMvUnroll; ++u) v[u] = *(const u32x4_t *)(src + (size_t)from[u] * kKv8Codes);
-        __syncthreads();   // the group is read before any of it is overwritten
+        for (int u = 0; u < kMvUnroll; ++u)
+            if (j0 + u * kMvRows < kept) v[u] = *(const u32x4_t *)(src + (size_t)from[u] * kKv8Codes);
+        if (inplace) __syncthreads();   // the group is read before any of it is overwritten
 #pragma unroll
         for (int u = 0; u < kMvUnroll; ++u) {
             const int j = j0 + u * kMvRows + tid / kMvLanes;
             if (j < kept && !(inplace && from[u] == j)) *(u32x4_t *)(dst + (size_t)j * kKv8Codes) = v[u];
         }
     }
-    if (!inplace) {   // the unfinished block's f16 rows: 512 B of 16 KB each
+    if (!inplace) {   // the unfinished block's f16 rows, 16 KB over the columns
         const Kv8Layout ls = kv8_layout(a.Hkv, a.nb), ld = kv8_layout(a.Hkv, a.dst_nb);
-        const size_t t = (size_t)h * 2 * kKv8Half * 2 + (size_t)col * 512 + tid * 16;
-        if (tid < 32) *(uint4 *)(dseq + ld.tails + t) = *(const uint4 *)(seq + ls.tails + t);
+        const size_t t = (size_t)h * 2 * kKv8Half * 2 + (size_t)col * (16384 / kMvCols) + tid * 16;
+        if (tid < 1024 / kMvCols) *(uint4 *)(dseq + ld.tails + t) = *(const uint4 *)(seq + ls.tails + t);
     }
     if (col == 0 && h == 0 && tid == 0) a.len_out[(size_t)z * a.len_out_stride] = a.head[2 * zh + 1];
 }

@@ -362,49 +362,70 @@ __global__ __launch_bounds__(kDecThreads) void kv8_decode_kernel(Kv8DecodeArgs a
     if (!s_last) return;
     for (int hc = 0; hc < a.G; hc += kDecRows) {
         const int g0 = kvh * a.G + hc, ng = min(kDecRows, a.G - hc);
-        if (orow < ng) {   // 32 lanes a row: lane i holds every 32nd run's factor
-            const size_t row = (size_t)z * a.H + g0 + orow;
+        // 32 lanes a head; the lanes that fewer than 8 heads leave take every
+        // second, fourth or eighth run of one
+        const int np = ng > 4 ? 8 : ng > 2 ? 4 : ng, step = kDecRows / np, jr = orow % np;
+        if (jr < ng) {
+            const size_t row = (size_t)z * a.H + g0 + jr;
             const uint64_t *ml = a.ml + row * a.splits, *op = a.o + row * a.splits * 64 + (od >> 1);
-            const int i = tid & 31;
-            float M = -__builtin_inff();
-            for (int s = i; s < runs; s += 32) M = fmaxf(M, kv8_get(ml + s).x);
-#pragma unroll
-            for (int s = 16; s > 0; s >>= 1) M = fmaxf(M, __shfl_xor(M, s, 64));
-            float lt = 0.0f;
+            float M = -__builtin_inff(), lt = 0.0f;
             float4 t = make_float4(0, 0, 0, 0);
-            for (int s0 = 0; s0 < runs; s0 += 32) {
-                float f = 0.0f, lf = 0.0f;
-                if (s0 + i < runs) {
-                    const float2 p = kv8_get(ml + s0 + i);
-                    f = __builtin_amdgcn_exp2f(p.x - M);
-                    lf = p.y * f;
+            constexpr int kB = 16;   // runs in flight
+            for (int s0 = orow / np; s0 < runs; s0 += kB * step) {
+                float2 p[kB], lo[kB], hi[kB];
+#pragma unroll
+                for (int j = 0; j < kB; ++j) {
+                    p[j] = make_float2(-__builtin_inff(), 0.0f);
+                    lo[j] = hi[j] = make_float2(0, 0);
+                    const int s = s0 + j * step;
+                    if (s < runs) {
+                        p[j] = kv8_get(ml + s);
+                        lo[j] = kv8_get(op + (size_t)s * 64);
+                        hi[j] = kv8_get(op + (size_t)s * 64 + 1);
+                    }
                 }
-                const int n = min(32, runs - s0);
-                for (int j0 = 0; j0 < n; j0 += 8) {
-                    float2 lo[8], hi[8];
+                float m = M;
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) {   // (clamped; its factor is 0)
-                        const uint64_t *p = op + (size_t)min(s0 + j0 + j, runs - 1) * 64;
-                        lo[j] = kv8_get(p);
-                        hi[j] = kv8_get(p + 1);
-                    }
+                for (int j = 0; j < kB; ++j) m = fmaxf(m, p[j].x);
+                const float f0 = m == M ? 1.0f : __builtin_amdgcn_exp2f(M - m);
+                M = m;
+                lt *= f0;
+                t = make_float4(t.x * f0, t.y * f0, t.z * f0, t.w * f0);
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        if (j0 + j >= n) break;
-                        const float fj = __shfl(f, (j0 + j) | (lane & 32), 64);
-                        lt += __shfl(lf, (j0 + j) | (lane & 32), 64);
-                        t.x = __builtin_fmaf(lo[j].x, fj, t.x);
-                        t.y = __builtin_fmaf(lo[j].y, fj, t.y);
-                        t.z = __builtin_fmaf(hi[j].x, fj, t.z);
-                        t.w = __builtin_fmaf(hi[j].y, fj, t.w);
-                    }
+                for (int j = 0; j < kB; ++j) {
+                    if (s0 + j * step >= runs) break;
+                    const float f = __builtin_amdgcn_exp2f(p[j].x - M);
+                    lt = __builtin_fmaf(p[j].y, f, lt);
+                    t.x = __builtin_fmaf(lo[j].x, f, t.x);
+                    t.y = __builtin_fmaf(lo[j].y, f, t.y);
+                    t.z = __builtin_fmaf(hi[j].x, f, t.z);
+                    t.w = __builtin_fmaf(hi[j].y, f, t.w);
                 }
             }
-            *(float4 *)(a.out + row * kKv8Hd + od) = make_float4(t.x / lt, t.y / lt, t.z / lt, t.w / lt);
+            so[0][orow][od >> 2] = t;
+            if (od == 0) sml[0][orow] = make_float2(M, lt);
+        }
+        lds_barrier();
+        if (orow < ng) {
+            float M = -__builtin_inff(), lt = 0.0f;
+            float4 t = make_float4(0, 0, 0, 0);
+            for (int i = orow; i < kDecRows; i += np) M = fmaxf(M, sml[0][i].x);
+            for (int i = orow; i < kDecRows; i += np) {
+                const float2 p = sml[0][i];
+                const float f = __builtin_amdgcn_exp2f(p.x - M);
+                const float4 v = so[0][i][od >> 2];
+                lt = __builtin_fmaf(p.y, f, lt);
+                t.x = __builtin_fmaf(v.x, f, t.x);
+                t.y = __builtin_fmaf(v.y, f, t.y);
+                t.z = __builtin_fmaf(v.z, f, t.z);
+                t.w = __builtin_fmaf(v.w, f, t.w);
+            }
+            *(float4 *)(a.out + ((size_t)z * a.H + g0 + orow) * kKv8Hd + od) =
+                make_float4(t.x / lt, t.y / lt, t.z / lt, t.w / lt);
             if (od == 0) stot[orow] = make_float2(M, lt);
         }
+        lds_barrier();
         if constexpr (WEIGHTS) {
-            lds_barrier();
             kv8_add_weights(a, z, kvh, g0, ng, nblk, stot);
             lds_barrier();
         }

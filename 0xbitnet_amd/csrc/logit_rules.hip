@@ -49,7 +49,16 @@ __global__ __launch_bounds__(kLrThreads) void logit_rules_kernel(RulesArgs a) {
         b0 = min(max(a.bias_off[r], 0), a.n_bias);
         b1 = min(a.bias_off[r + 1], a.n_bias);
     }
-    // every load that depends on nothing goes out at once
+    const bool lists = h0 < h1 || b0 < b1;   // uniform
+    // The lists' first ids are asked for before the logits: loads return in
+    // order, and their counting runs while the logits come.
+    int id[kLrPer], bid = -1;
+#pragma unroll
+    for (int u = 0; u < kLrPer; ++u) {
+        const int j = h0 + tid + u * kLrThreads;
+        id[u] = j < h1 ? a.hist[j] : -1;
+    }
+    if (b0 + tid < b1) bid = a.bias_ids[b0 + tid];
     const float *lg = a.logits + (size_t)r * a.stride + base;
     const uint32_t *mask = a.mask ? a.mask + (size_t)r * a.mask_stride : nullptr;
     float x[kLrPer];
@@ -66,7 +75,6 @@ __global__ __launch_bounds__(kLrThreads) void logit_rules_kernel(RulesArgs a) {
         freq = a.pen[3 * r + 1];
         pres = a.pen[3 * r + 2];
     }
-    const bool lists = h0 < h1 || b0 < b1;   // uniform
     if (lists) {
 #pragma unroll
         for (int u = 0; u < kLrPer; ++u) {
@@ -74,20 +82,19 @@ __global__ __launch_bounds__(kLrThreads) void logit_rules_kernel(RulesArgs a) {
             last[tid + u * kLrThreads] = 0;
         }
         lds_barrier();
-        for (int j0 = h0 + tid; j0 < h1; j0 += kLrPer * kLrThreads) {
-            int id[kLrPer];
-#pragma unroll
-            for (int u = 0; u < kLrPer; ++u) id[u] = a.hist[min(j0 + u * kLrThreads, h1 - 1)];
-#pragma unroll
-            for (int u = 0; u < kLrPer; ++u) {
-                const unsigned i = (unsigned)id[u] - (unsigned)base;
-                if (j0 + u * kLrThreads < h1 && i < (unsigned)n) atomicAdd(&cnt[i], 1);
-            }
-        }
-        for (int j = b0 + tid; j < b1; j += kLrThreads) {
-            const unsigned i = (unsigned)a.bias_ids[j] - (unsigned)base;
+        auto count = [&](int v) {
+            const unsigned i = (unsigned)v - (unsigned)base;
+            if (i < (unsigned)n) atomicAdd(&cnt[i], 1);
+        };
+        auto entry = [&](int v, int j) {
+            const unsigned i = (unsigned)v - (unsigned)base;
             if (i < (unsigned)n) atomicMax(&last[i], j + 1);
-        }
+        };
+#pragma unroll
+        for (int u = 0; u < kLrPer; ++u) count(id[u]);
+        for (int j = h0 + kLrPer * kLrThreads + tid; j < h1; j += kLrThreads) count(a.hist[j]);
+        entry(bid, b0 + tid);
+        for (int j = b0 + kLrThreads + tid; j < b1; j += kLrThreads) entry(a.bias_ids[j], j);
         lds_barrier();
     }
     float *out = a.out + (size_t)r * a.out_stride + base;
