@@ -23,6 +23,8 @@
 // 2^(x - m2) vs V is then o / (l r), r = 2^(m - m2).
 #include "kv8.h"
 
+#include <algorithm>
+
 namespace oxb {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
@@ -472,8 +474,9 @@ static DecodeWs decode_ws(int batch, int H, int Hkv, int nb) {
 // alternates them 349, the MFMAs alone 261; two waves per SIMD).  K runs a
 // block ahead of V; rings of four blocks of each leave one barrier per two
 // blocks.
-// Row tiles see different lengths and finish apart; where they alone leave CUs
-// idle, their runs are split and a second launch joins the parts.
+// Row tiles see different lengths; where they alone leave CUs idle or finish
+// far apart, the launch cuts them into runs (prefill_plan), and a second launch
+// joins the parts.
 constexpr int kPreWaves = 4;
 constexpr int kPreThreads = 64 * kPreWaves;
 constexpr int kPreRows = 32 * kPreWaves;
@@ -484,7 +487,7 @@ constexpr float kPreBase = 6.0f;             // p' <= 2^(6 + kStep)
 struct Kv8PrefillArgs {
     const float *q;
     uint8_t *cache;
-    int n, pos0, H, Hkv, G, nb, rows, rtiles, splits, per, weights;
+    int n, pos0, H, Hkv, G, nb, rows, rtiles, planned, per, weights;
     float *out;
     float2 *ml;     // [splits][Hkv][rows] a row's reference and sum
     float *o;       // [splits][Hkv][rows][128]
@@ -495,31 +498,37 @@ struct Kv8PrefillArgs {
 };
 
 __host__ __device__ inline int pre_rows32(int rows) { return (rows + 31) & ~31; }
-// The first row tile that sees a block of run `split`: its last row's token is at
-// position 32 per split at least.
-__device__ __forceinline__ int pre_first_tile(const Kv8PrefillArgs &a, int split) {
-    const int64_t tok = (int64_t)split * a.per * kKv8Block - a.pos0;
-    return tok <= 0 ? 0 : (int)min(tok * a.G / kPreRows, (int64_t)a.rtiles);
+// A row tile's blocks in even runs.
+__host__ __device__ inline int pre_run_start(int blocks, int runs, int i) {
+    return (int)((int64_t)blocks * i / runs);
 }
+// The order in which runs are started: row tile | run << 16.  By value with the
+// launch, so that a captured graph keeps it.
+constexpr int kPreOrder = 512;
+struct Kv8PrefillOrder {
+    uint32_t run[kPreOrder];
+};
 
 template <int FMT>
-__global__ __launch_bounds__(kPreThreads, 2) void kv8_prefill_kernel(Kv8PrefillArgs a) {
+__global__ __launch_bounds__(kPreThreads, 2) void kv8_prefill_kernel(Kv8PrefillArgs a, const Kv8PrefillOrder order) {
     // rings of K [8][64] and V operands [4 dims][2][64]: block b of the run in slot b % 4
     __shared__ uint4 sk[kPreRing][kPreOps], sv[kPreRing][kPreOps];
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    // The grid holds the workgroups that have work and no others: run 0 of every
-    // row tile, then run 1 of those that have one, .., each from the last row
-    // tile (the longest rows) on, the KV heads side by side.
+    // workgroups take the plan's runs in its order, the KV heads side by side
     const int kvh = blockIdx.x % a.Hkv;
-    int at = blockIdx.x / a.Hkv, split = 0;
-    for (int n; at >= (n = a.rtiles - pre_first_tile(a, split)); at -= n) ++split;
-    const int rtile = a.rtiles - 1 - at;
+    int rtile = a.rtiles - 1 - (int)(blockIdx.x / a.Hkv), split = 0;
+    if (a.planned) {
+        const uint32_t e = order.run[blockIdx.x / a.Hkv];
+        rtile = e & 0xffff;
+        split = e >> 16;
+    }
     const int r0 = rtile * kPreRows, row = r0 + wave * 32 + (lane & 31), h = lane >> 5;
     const int total = a.pos0 + a.n;
     const int lastrow = min(r0 + kPreRows, a.rows) - 1;
     const int blocks = kv8_blocks(a.pos0 + lastrow / a.G + 1);   // that the tile's last row sees
-    const int b0 = split * a.per, b1 = min(blocks, b0 + a.per);
+    const int runs = a.planned ? (blocks + a.per - 1) / a.per : 1;
+    const int b0 = pre_run_start(blocks, runs, split), b1 = pre_run_start(blocks, runs, split + 1);
     const int tok = min(row, a.rows - 1) / a.G, head = kvh * a.G + min(row, a.rows - 1) % a.G;
     const int qpos = a.pos0 + tok;
 
@@ -790,7 +799,7 @@ __global__ __launch_bounds__(kPreThreads, 2) void kv8_prefill_kernel(Kv8PrefillA
     if (erow >= a.rows) return;
     // (a wave may see nothing of a run that others see)
     const float M = b0 * kKv8Block < wseen ? ref.off() - kPreBase : -__builtin_inff();
-    const bool direct = blocks <= a.per;   // the row tile's only run
+    const bool direct = runs == 1;
     float *dst, f = 1.0f / ref.r;          // o in l's units
     if (direct) {
         dst = a.out + ((size_t)(erow / a.G) * a.H + kvh * a.G + erow % a.G) * kKv8Hd;
@@ -817,7 +826,7 @@ __global__ __launch_bounds__(256) void kv8_prefill_join_kernel(Kv8PrefillArgs a)
     if (row >= a.rows) return;
     const int tok = row / a.G, head = kvh * a.G + row % a.G;
     const int lastrow = min((row / kPreRows + 1) * kPreRows, a.rows) - 1;   // of the row's tile
-    const int ns = (kv8_blocks(a.pos0 + lastrow / a.G + 1) + a.per - 1) / a.per;
+    const int ns = (kv8_blocks(a.pos0 + lastrow / a.G + 1) + a.per - 1) / a.per;   // runs
     if (ns == 1) return;   // written by its only run
     const size_t step = (size_t)a.Hkv * a.rows, r = (size_t)kvh * a.rows + row;
     float M = -__builtin_inff(), lt = 0.0f;
@@ -1007,7 +1016,7 @@ __global__ __launch_bounds__(256) void kv8_weights_add_kernel(Kv8PrefillArgs a) 
 
 // The launch shapes of a prefill call and its workspace.
 struct PrefillPlan {
-    int rows, rtiles, splits, per, rsplits;
+    int rows, rtiles, runs, splits, per, rsplits;
     int64_t wgs;
     size_t ml, o, lse, qf, part, bytes;
 };
@@ -1016,28 +1025,30 @@ static PrefillPlan prefill_plan(int n, int pos0, int H, int Hkv, bool weights) {
     const int G = H / Hkv, total = pos0 + n, nblk = kv8_blocks(total);
     p.rows = n * G;
     p.rtiles = (p.rows + kPreRows - 1) / kPreRows;
-    // Two workgroups per CU are resident: the shortest runs, of at least eight
-    // blocks, whose workgroups (row tiles that see less have fewer) all are;
-    // a longest run is what the launch takes.
-    const int most = kv8_blocks(total);
+    // Two workgroups per CU are resident, and a row tile's blocks may be cut into
+    // even runs of `per` at most: the least per, of eight at least, whose runs all
+    // are resident at once.  (2048 tokens: 56 us; 850 workgroups of the same
+    // work in two rounds 69, as beginning and ending a run takes about 9 us.)
+    const int slots = 2 * device_cus() / Hkv, most = kv8_blocks(total);
     auto count = [&](int per) {
-        int64_t wgs = 0;
+        int64_t n = 0;
         for (int r = 0; r < p.rtiles; ++r) {
             const int last = (r + 1) * kPreRows < p.rows ? (r + 1) * kPreRows : p.rows;
-            wgs += (kv8_blocks(pos0 + (last - 1) / G + 1) + per - 1) / per;
+            n += (kv8_blocks(pos0 + (last - 1) / G + 1) + per - 1) / per;
         }
-        return wgs * Hkv;
+        return n;
     };
-    int lo = 8, hi = most;   // runs of `most` blocks are no split at all
-    if ((int64_t)p.rtiles * Hkv > 2 * device_cus()) lo = hi;
+    int lo = 8, hi = most;   // runs of `most` blocks are no cut at all
+    if (p.rtiles > slots) lo = hi;
     while (lo < hi) {
         const int mid = lo + (hi - lo) / 2;
-        if (count(mid) <= 2 * device_cus()) hi = mid;
+        if (count(mid) <= slots) hi = mid;
         else lo = mid + 1;
     }
-    p.per = hi < 8 ? 8 : hi;
+    p.per = hi;
+    p.runs = hi == most ? p.rtiles : (int)count(hi);
     p.splits = (most + p.per - 1) / p.per;
-    p.wgs = p.splits == 1 ? (int64_t)p.rtiles * Hkv : count(p.per);
+    p.wgs = (int64_t)p.runs * Hkv;
     size_t at = kArrivals * 4;
     auto take = [&](size_t b) {
         const size_t o = at;
@@ -1062,6 +1073,26 @@ static PrefillPlan prefill_plan(int n, int pos0, int H, int Hkv, bool weights) {
     }
     p.bytes = at;
     return p;
+}
+
+// The plan's runs, the longest first; of those that run at once, the second half
+// the other way round: a CU gets the longest and the shortest.
+static void prefill_order(const PrefillPlan &p, int pos0, int G, int Hkv, Kv8PrefillOrder &o) {
+    struct Run {
+        int len;
+        uint32_t id;
+    } run[kPreOrder];
+    int n = 0;
+    for (int r = 0; r < p.rtiles; ++r) {
+        const int last = (r + 1) * kPreRows < p.rows ? (r + 1) * kPreRows : p.rows;
+        const int b = kv8_blocks(pos0 + (last - 1) / G + 1), k = (b + p.per - 1) / p.per;
+        for (int i = 0; i < k; ++i)
+            run[n++] = {pre_run_start(b, k, i + 1) - pre_run_start(b, k, i), (uint32_t)r | (uint32_t)i << 16};
+    }
+    std::sort(run, run + n, [](const Run &x, const Run &y) { return x.len != y.len ? x.len > y.len : x.id > y.id; });
+    const int half = device_cus() / Hkv, two = 2 * half < n ? 2 * half : n;
+    if (half < two) std::reverse(run + half, run + two);
+    for (int i = 0; i < n; ++i) o.run[i] = run[i].id;
 }
 
 static int heads_check(int H, int Hkv) {
@@ -1138,15 +1169,17 @@ extern "C" int oxb_attn_prefill_kv8(const float *q, void *cache, int fmt, int n_
                 "attention: workspace is NULL, not 256-byte aligned or %zu bytes < %zu", ws_bytes, p.bytes);
     char *w = (char *)ws;
     Kv8PrefillArgs a{q, (uint8_t *)cache, n_tok, pos0, H, Hkv, H / Hkv, kv8_blocks(max_seq), p.rows,
-                     p.rtiles, p.splits, p.per, add_weights != 0, out, (float2 *)(w + p.ml), (float *)(w + p.o),
+                     p.rtiles, p.rtiles <= kPreOrder, p.per, add_weights != 0, out, (float2 *)(w + p.ml), (float *)(w + p.o),
                      (float2 *)(w + p.lse), (uint4 *)(w + p.qf), (float *)(w + p.part), p.rsplits};
     hipStream_t s = (hipStream_t)stream;
     OXB_REQUIRE(p.wgs < (1 << 30), "prefill attention: %d tokens", n_tok);
     const dim3 grid((unsigned)p.wgs), th(kPreThreads);
+    Kv8PrefillOrder order;
+    if (a.planned) prefill_order(p, pos0, a.G, Hkv, order);
     if (fmt == OXB_KV8_INT8)
-        hipLaunchKernelGGL(kv8_prefill_kernel<OXB_KV8_INT8>, grid, th, 0, s, a);
+        hipLaunchKernelGGL(kv8_prefill_kernel<OXB_KV8_INT8>, grid, th, 0, s, a, order);
     else
-        hipLaunchKernelGGL(kv8_prefill_kernel<OXB_KV8_E4M3>, grid, th, 0, s, a);
+        hipLaunchKernelGGL(kv8_prefill_kernel<OXB_KV8_E4M3>, grid, th, 0, s, a, order);
     OXB_CHECK_HIP(hipGetLastError());
     if (p.splits > 1) {
         hipLaunchKernelGGL(kv8_prefill_join_kernel, dim3((p.rows + 7) / 8, Hkv), dim3(256), 0, s, a);
