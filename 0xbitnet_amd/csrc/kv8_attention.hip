@@ -1172,7 +1172,7 @@ extern "C" int oxb_attn_prefill_kv8(const float *q, void *cache, int fmt, int n_
                      p.rtiles, p.rtiles <= kPreOrder, p.per, add_weights != 0, out, (float2 *)(w + p.ml), (float *)(w + p.o),
                      (float2 *)(w + p.lse), (uint4 *)(w + p.qf), (float *)(w + p.part), p.rsplits};
     hipStream_t s = (hipStream_t)stream;
-    OXB_REQUIRE(p.wgs < (1 << 30), "prefill attention: %d tokens", n_tok);
+    OXB_REQUIRE(p.wgs < (1 << 24), "prefill attention: %d tokens of %d heads", n_tok, H);
     const dim3 grid((unsigned)p.wgs), th(kPreThreads);
     Kv8PrefillOrder order;
     if (a.planned) prefill_order(p, pos0, a.G, Hkv, order);

@@ -7,7 +7,7 @@ import zlib
 import numpy as np
 import pytest
 
-from helpers import ops, pkg
+from helpers import ops, synth, ternary
 import kv8_reference as ref
 
 pytestmark = pytest.mark.gpu
@@ -221,9 +221,11 @@ def test_decode_long_many_splits(fmt):
     c, K, V = filled(rng, [n, 3], 1, n + 20, fmt)
     q = rng.standard_normal((2, 4 * HD)).astype(np.float32) * 2
     got = c.attn_decode(q, [n - 1, 2])
+    assert np.array_equal(bits(c.attn_decode(q, [n - 1, 2], True)), bits(got))
     for z, m in enumerate((n, 3)):
-        want, tol, _, _ = ref.attend_rows(q[z:z + 1], K[z], V[z], 1, m - 1)
+        want, tol, w, wtol = ref.attend_rows(q[z:z + 1], K[z], V[z], 1, m - 1)
         check_rows(got[z:z + 1], want, tol, z)
+        check_rows(c.weights()[z, :, :(m + 31) // 32], w[:, :(m + 31) // 32], wtol[:, :(m + 31) // 32], z)
 
 
 @pytest.mark.parametrize("fmt", FMTS)
@@ -309,6 +311,33 @@ def test_prefill_matches_reference(fmt, H, hkv, n, pos0, max_seq):
     bound = max(ref.rms_bound(q[i, h * HD:(h + 1) * HD], K[1][h // (H // hkv)])
                 for i in range(n) for h in range(H))
     assert rel(got, want) <= bound
+
+
+@pytest.mark.parametrize("H,hkv,n,pos0", [
+    (8, 1, 2500, 700),       # row tiles cut into runs of different number
+    (16, 1, 4200, 0),        # more row tiles than a plan orders
+    (20, 5, 700, 3000)])
+def test_prefill_long(H, hkv, n, pos0):
+    """Long prompts, some of their rows against the reference."""
+    fmt = n % 2
+    rng = rng_of("long prefill", H, n)
+    c, K, V = filled(rng, [pos0 + n], hkv, pos0 + n, fmt)
+    q = rng.standard_normal((n, H * HD)).astype(np.float32)
+    got = c.attn_prefill(q, pos0)
+    for i in sorted({0, 1, 31, 32, n // 3, n // 2, n - 33, n - 1} | set(rng.integers(0, n, 8).tolist())):
+        want, tol, _, _ = ref.attend_rows(q[i:i + 1], K[0], V[0], hkv, pos0 + i)
+        check_rows(got[i:i + 1], want, tol, i)
+
+
+@pytest.mark.parametrize("H,hkv,n,pos0", [(8, 1, 600, 200), (4, 2, 900, 0)])
+def test_prefill_weights_long(H, hkv, n, pos0):
+    """Weights over many rows (split over workgroups) against all rows' own."""
+    rng = rng_of("long weights", H, n)
+    c, K, V = filled(rng, [pos0 + n], hkv, pos0 + n, 0)
+    q = rng.standard_normal((n, H * HD)).astype(np.float32)
+    c.attn_prefill(q, pos0, add_weights=True)
+    _, _, want, tol = ref.attend_rows(q, K[0], V[0], hkv, pos0)
+    check_rows(c.weights()[0], want, tol)
 
 
 def test_prefill_leaves_rows_behind_the_last():
@@ -521,6 +550,77 @@ def test_a_serving_run():
                 check_rows(got_w[z, h, :m], w[z][h], wt[z][h] + 1e-30)
 
 
+def test_behind_the_projections():
+    """As a layer uses them: the q|k|v projections leave rotated f16 rows in a scratch
+    cache, the append takes them at their position, attention follows; after a cut
+    the tokens' own positions go on through a rope table shifted by the dropped
+    rows."""
+    L = ops.lib()
+    for fmt in FMTS:
+        rng = rng_of("layer", fmt)
+        D, H, hkv, ms, n = 512, 8, 2, 256, 150
+        Dq, Dkv = H * HD, hkv * HD
+        N = Dq + 2 * Dkv
+        Wt = ops.upload_ternary(synth.i2s_pack(ternary(rng, N, D)), D)
+        g = ops.DeviceArray.from_host(rng.uniform(0.5, 1.5, D).astype(np.float32))
+        wsc = ops.DeviceArray.from_host(rng.uniform(0.01, 0.02, N).astype(np.float32))
+        table = np.empty((ms, HD // 2, 2), np.float32)
+        ops.check(L.oxb_rope_table(table.ctypes.data, ms, HD, 500000.0))
+        rope = ops.DeviceArray.from_host(table)
+        kc, vc, k2, v2 = (ops.DeviceArray((hkv, ms, HD), np.uint16, zero=True) for _ in range(4))
+        c = new_cache(1, hkv, ms, fmt)
+        # the prompt
+        x = ops.DeviceArray.from_host(rng.standard_normal((n, D)).astype(np.float32))
+        pad = (n + 63) // 64 * 64
+        Xt, sc, sm = (ops.DeviceArray((pad * D,), np.int8, zero=True), ops.DeviceArray((pad,), np.float32),
+                      ops.DeviceArray((pad,), np.int32))
+        q = ops.DeviceArray((n, Dq), np.float32)
+        ops.quantize_rows_tiled(x, g, 1e-5, n, D, Xt, sc, sm)
+        ops.check(L.oxb_gemm_qkv(Wt.ptr, Xt.ptr, sc.ptr, sm.ptr, wsc.ptr, Dq, Dkv, HD, D, n, 0, q.ptr, kc.ptr,
+                                 vc.ptr, ms, rope.ptr, None))
+        ops.check(L.oxb_kv8_append(c.data.ptr, c.stride, fmt, 1, hkv, HD, ms, kc.ptr, vc.ptr, 0, ms * HD, 1, None, 0,
+                                   0, n, None, None))
+        ops.sync()
+        k, v = ([h[:n] for h in a.download().view(np.float16)] for a in (kc, vc))
+        got = c.attn_prefill(q.download(), 0, add_weights=True)
+        K, V = (np.stack([ref.values(h, fmt) for h in a]) for a in (k, v))
+        want, tol, _, _ = ref.attend_rows(q.download(), K, V, hkv, 0)
+        check_rows(got, want, tol)
+        # a token a step; a cut before the fourth
+        pos, dropped = n, 0
+        dp, dt = ops.DeviceArray((1,), np.int32), ops.DeviceArray((1,), np.int32)
+        q1, q2 = ops.DeviceArray((Dq,), np.float32), ops.DeviceArray((Dq,), np.float32)
+        for step in range(8):
+            if step == 3:
+                w = c.weights()[0]
+                new = int(c.evict([pos], 3, 1, 1)[0])
+                for h in range(hkv):
+                    keep = ref.kept_blocks(w[h], (pos + 31) // 32, 3, 1, 1)
+                    at = np.concatenate([np.arange(32 * b, min(32 * b + 32, pos)) for b in keep])
+                    k[h], v[h] = k[h][at], v[h][at]
+                dropped, pos = pos - new, new
+                assert dropped == 64
+            x1 = ops.DeviceArray.from_host(rng.standard_normal(D).astype(np.float32))
+            dp.upload(np.array([pos], np.int32))
+            dt.upload(np.array([pos + dropped], np.int32))
+            for qq, kk, vv, tab, p in ((q1, kc, vc, rope.offset(dropped * HD * 4), dp), (q2, k2, v2, rope.ptr, dt)):
+                ops.check(L.oxb_bitlinear_qkv(Wt.ptr, x1.ptr, g.ptr, 1e-5, wsc.ptr, Dq, Dkv, HD, D, qq.ptr, kk.ptr,
+                                              vv.ptr, ms, tab, p.ptr, None))
+            ops.check(L.oxb_kv8_append(c.data.ptr, c.stride, fmt, 1, hkv, HD, ms, kc.ptr, vc.ptr, 0, ms * HD, 1,
+                                       dp.ptr, 0, 0, 1, None, None))
+            ops.sync()
+            assert np.array_equal(bits(q1.download()), bits(q2.download()))
+            ka, va = (a.download().view(np.float16)[:, pos] for a in (kc, vc))
+            assert np.array_equal(ka.view(np.uint16), k2.download()[:, pos + dropped])
+            k, v = ([np.concatenate([h, r[None]]) for h, r in zip(a, b)] for a, b in ((k, ka), (v, va)))
+            qh = q1.download()[None]
+            got = c.attn_decode(qh, [pos], True)
+            K, V = (np.stack([ref.values(h, fmt) for h in a]) for a in (k, v))
+            want, tol, _, _ = ref.attend_rows(qh, K, V, hkv, pos)
+            check_rows(got, want, tol, step)
+            pos += 1
+
+
 def test_captured_step_replays():
     """Append and decode attention in one graph, replayed with new rows and positions
     and eager work between the replays, on a stream of its own."""
@@ -563,6 +663,105 @@ def test_captured_step_replays():
         assert np.array_equal(bits(c.weights()[z, :, :m[z]]), bits(e.weights()[z, :, :m[z]]))
     ops.check(L.oxb_graph_destroy(g))
     ops.check(L.oxb_stream_destroy(st))
+
+
+def test_offsets_past_32_bits():
+    """A cache of which the last head's blocks and the second sequence lie past 4 GB."""
+    hkv, ms, B, n = 17, 1 << 20, 2, 70
+    rng = rng_of("4 GB")
+    c = ops.Kv8Cache(B, hkv, ms, 1)
+    assert c.stride > 1 << 32 and 16 * (ms // 32) * 8192 >= 1 << 32
+    k, v = rows(rng, B, hkv, n)
+    c.append(k, v, [0, 0])
+    gk, gv = c.read([0, 0], n)
+    K, V = [held(x, n, 1) for x in k], [held(x, n, 1) for x in v]
+    for z in range(B):
+        assert np.array_equal(bits(gk[z]), bits(K[z])) and np.array_equal(bits(gv[z]), bits(V[z]))
+    q = rng.standard_normal((B, 2 * hkv * HD)).astype(np.float32)
+    got = c.attn_decode(q, [n - 1, n - 2], True)
+    qp = rng.standard_normal((5, 2 * hkv * HD)).astype(np.float32)
+    gp = c.attn_prefill(qp, n - 5, slot=1, add_weights=True)
+    for z in range(B):
+        want, tol, _, _ = ref.attend_rows(q[z:z + 1], K[z], V[z], hkv, n - 1 - z)
+        check_rows(got[z:z + 1], want, tol, z)
+    want, tol, _, _ = ref.attend_rows(qp, K[1], V[1], hkv, n - 5)
+    check_rows(gp, want, tol)
+    new = c.evict([n, n], 2, 1, 1)
+    assert new.tolist() == [n - 32] * 2
+    gk, gv = c.read([0, 0], n - 32)
+    at = np.r_[0:32, 64:n]
+    for z in range(B):
+        assert np.array_equal(bits(gk[z]), bits(K[z][:, at])) and np.array_equal(bits(gv[z]), bits(V[z][:, at]))
+
+
+def test_one_workspace_for_calls_of_any_shape():
+    """Decode and prefill calls of different shapes in turn on one workspace: each as
+    on one of its own."""
+    L, rng = ops.lib(), rng_of("ws")
+    shapes = [(1, 8, 2, 3000), (3, 20, 5, 200), (1, 4, 4, 40), (2, 16, 1, 1500)]
+    need = 0
+    for b, H, hkv, n in shapes:
+        need = max(need, L.oxb_attn_decode_kv8_ws_bytes(b, H, hkv, HD, n),
+                   L.oxb_attn_prefill_kv8_ws_bytes(70, n - 70 if n > 70 else 0, H, hkv, HD, 1))
+    ws = ops.DeviceArray((need,), np.uint8, zero=True)
+    made = []
+    for b, H, hkv, n in shapes:
+        c, _, _ = filled(rng, [n] * b, hkv, n, 0)
+        m = min(70, n)
+        made.append((b, H, hkv, n, m, c, rng.standard_normal((b, H * HD)).astype(np.float32),
+                     rng.standard_normal((m, H * HD)).astype(np.float32)))
+    for _ in range(2):
+        for b, H, hkv, n, m, c, q, qp in made:
+            dq, dqp = ops.DeviceArray.from_host(q), ops.DeviceArray.from_host(qp)
+            out, outp = ops.DeviceArray(q.shape, np.float32), ops.DeviceArray(qp.shape, np.float32)
+            pos = ops.DeviceArray.from_host(np.full(b, n - 1, np.int32))
+            ops.check(L.oxb_attn_decode_kv8(dq.ptr, c.data.ptr, c.stride, 0, pos.ptr, 1, b, H, hkv, HD, n, 0,
+                                            out.ptr, ws.ptr, need, None))
+            ops.check(L.oxb_attn_prefill_kv8(dqp.ptr, c.data.ptr, 0, m, n - m, H, hkv, HD, n, 1, outp.ptr,
+                                             ws.ptr, need, None))
+            ops.sync()
+            assert np.array_equal(bits(out.download()), bits(c.attn_decode(q, [n - 1] * b)))
+            assert np.array_equal(bits(outp.download()), bits(c.attn_prefill(qp, n - m)))
+
+
+def test_two_streams_at_once():
+    """Two sequences of calls on streams, caches and workspaces of their own, queued
+    without waiting for either."""
+    L, rng = ops.lib(), rng_of("streams")
+    hkv, H, B, ms, steps = 2, 8, 2, 512, 12
+    side = []
+    for i in range(2):
+        c, e = new_cache(B, hkv, ms, i), new_cache(B, hkv, ms, i)
+        k, v = rows(rng, B, hkv, 300 + steps)
+        for x in (c, e):
+            x.append(k[:, :, :300], v[:, :, :300], [0, 0], [300, 180])
+        q = rng.standard_normal((steps, B, H * HD)).astype(np.float32)
+        pos = np.array([[300 + s, 180 + s] for s in range(steps)], np.int32)
+        n = L.oxb_attn_decode_kv8_ws_bytes(B, H, hkv, HD, ms)
+        side.append(dict(c=c, e=e, k=k, v=v, q=q, pos=pos, n=n, st=L.oxb_stream_create(),
+                         ws=ops.DeviceArray((n,), np.uint8, zero=True), dq=ops.DeviceArray.from_host(q),
+                         dk=ops.DeviceArray.from_host(k.view(np.uint16)), dv=ops.DeviceArray.from_host(v.view(np.uint16)),
+                         dp=ops.DeviceArray.from_host(pos), out=ops.DeviceArray(q.shape, np.float32)))
+    ops.sync()
+    row = HD * 2
+    for s in range(steps):
+        for d in side:
+            c, n_src = d["c"], (300 + steps) * HD
+            ops.check(L.oxb_kv8_append(c.data.ptr, c.stride, c.fmt, B, hkv, HD, ms, d["dk"].offset((300 + s) * row),
+                                       d["dv"].offset((300 + s) * row), hkv * n_src, n_src, 0, d["dp"].offset(8 * s), 1, 0,
+                                       1, None, d["st"]))
+            ops.check(L.oxb_attn_decode_kv8(d["dq"].offset(4 * s * B * H * HD), c.data.ptr, c.stride, c.fmt,
+                                            d["dp"].offset(8 * s), 1, B, H, hkv, HD, ms, 1,
+                                            d["out"].offset(4 * s * B * H * HD), d["ws"].ptr, d["n"], d["st"]))
+    for d in side:
+        ops.check(L.oxb_stream_sync(d["st"]))
+    for d in side:
+        got = d["out"].download()
+        for s in range(steps):
+            d["e"].append(d["k"][:, :, 300 + s:301 + s], d["v"][:, :, 300 + s:301 + s], d["pos"][s])
+            assert np.array_equal(bits(got[s]), bits(d["e"].attn_decode(d["q"][s], d["pos"][s], True))), s
+        assert np.array_equal(bits(d["c"].weights()[:, :, :6]), bits(d["e"].weights()[:, :, :6]))
+        ops.check(L.oxb_stream_destroy(d["st"]))
 
 
 # ---------------------------------------------------------------------------
