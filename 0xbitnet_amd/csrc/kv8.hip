@@ -20,6 +20,8 @@
 #include "kv8.h"
 #include "radix_select.h"
 
+#include <algorithm>
+
 namespace oxb {
 
 constexpr int kKvThreads = 256;
@@ -443,6 +445,7 @@ extern "C" int oxb_kv8_read(const void *cache, size_t cache_stride, int fmt, int
 
 extern "C" size_t oxb_kv8_evict_ws_bytes(int batch, int Hkv, int max_seq, int budget) {
     if (batch < 1 || Hkv < 1 || max_seq < 1 || max_seq > OXB_KV8_MAX_SEQ || budget < 1) return 0;
+    budget = std::min(budget, kv8_blocks(max_seq));   // no more are kept
     return kv8_align((size_t)batch * Hkv * budget * 4) + kv8_align((size_t)batch * Hkv * 8);
 }
 
@@ -476,6 +479,7 @@ extern "C" int oxb_kv8_evict(const void *cache, size_t cache_stride, int max_seq
                     ws_bytes >= oxb_kv8_evict_ws_bytes(batch, Hkv, max_seq, budget),
                 "kv8 evict: workspace is NULL, unaligned or %zu bytes < %zu", ws_bytes,
                 oxb_kv8_evict_ws_bytes(batch, Hkv, max_seq, budget));
+    budget = std::min(budget, nb);   // (then nothing is dropped)
     Kv8EvictArgs a{(const uint8_t *)cache, (uint8_t *)dst, cache_stride, dst_stride, Hkv, max_seq, nb,
                    dnb, len, len_stride, len_out, len_out_stride, budget, sink, recent, (int *)ws,
                    (int *)((char *)ws + kv8_align((size_t)batch * Hkv * budget * 4))};

@@ -160,6 +160,13 @@ __global__ __launch_bounds__(kDecThreads) void kv8_decode_kernel(Kv8DecodeArgs a
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int z = blockIdx.z, kvh = blockIdx.y, split = blockIdx.x;
+    const int orow = tid >> 5, od = (tid & 31) * 4;         // the row and dims a thread joins
+    auto load_q = [&](int hc) {
+        float4 v = make_float4(0, 0, 0, 0);
+        if (hc + orow < a.G) v = *(const float4 *)(a.q + ((size_t)z * a.H + kvh * a.G + hc + orow) * kKv8Hd + od);
+        return v;
+    };
+    float4 qv = load_q(0);   // with pos, before the cache's loads: loads return in order
     const int64_t p1 = (int64_t)a.pos[(size_t)z * a.pos_stride] + 1;
     const int len = (int)(p1 < 0 ? 0 : p1 > a.max_seq ? a.max_seq : p1), nblk = kv8_blocks(len);
     // blocks of a run: an even share, at least one per wave
@@ -195,15 +202,13 @@ __global__ __launch_bounds__(kDecThreads) void kv8_decode_kernel(Kv8DecodeArgs a
         x.s = sc[b];
         return x;
     };
-    const int orow = tid >> 5, od = (tid & 31) * 4;         // the row and dims a thread joins
 
     for (int hc = 0; hc < a.G; hc += kDecRows) {
         const int g0 = kvh * a.G + hc, ng = min(kDecRows, a.G - hc);
         // the first block is on its way while q is made ready
         Blk cur = load(min(b0 + wave, b1 - 1));
         {   // q rows: scaled, split, and their score units
-            float4 v = make_float4(0, 0, 0, 0);
-            if (orow < ng) v = *(const float4 *)(a.q + ((size_t)z * a.H + g0 + orow) * kKv8Hd + od);
+            const float4 v = qv;
             float m = fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w)));
 #pragma unroll
             for (int s = 16; s > 0; s >>= 1) m = fmaxf(m, __shfl_xor(m, s, 64));
@@ -350,6 +355,7 @@ __global__ __launch_bounds__(kDecThreads) void kv8_decode_kernel(Kv8DecodeArgs a
             if (od == 0) kv8_put(a.ml + part, M, lt);
         }
         lds_barrier();   // LDS is free for the next heads
+        qv = load_q(hc + kDecRows);
     }
     if (runs == 1) return;
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -1029,7 +1035,7 @@ static PrefillPlan prefill_plan(int n, int pos0, int H, int Hkv, bool weights) {
     // even runs of `per` at most: the least per, of eight at least, whose runs all
     // are resident at once.  (2048 tokens: 56 us; 850 workgroups of the same
     // work in two rounds 69, as beginning and ending a run takes about 9 us.)
-    const int slots = 2 * device_cus() / Hkv, most = kv8_blocks(total);
+    const int slots = std::min(2 * device_cus() / Hkv, kPreOrder), most = kv8_blocks(total);
     auto count = [&](int per) {
         int64_t n = 0;
         for (int r = 0; r < p.rtiles; ++r) {

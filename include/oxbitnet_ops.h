@@ -308,9 +308,9 @@ size_t oxb_kv8_bytes(int Hkv, int hd, int max_seq);
  * where the q|k|v projections leave them (a f16 cache [Hkv][max_seq][128] that
  * all layers may share as scratch).  p is the position after the last one
  * appended, or less within that position's block (its later rows are dropped),
- * or the start of any block (a multiple of 32).  The cache's content depends on the rows alone, not on how
- * they were split over calls.  Positions past max_seq are dropped; p < 0 skips
- * the sequence. */
+ * or the start of any block (a multiple of 32).  The cache's content depends on
+ * the rows alone, not on how they were split over calls.  Positions past max_seq
+ * are dropped; p < 0 skips the sequence. */
 int oxb_kv8_append(void *cache, size_t cache_stride, int fmt, int batch, int Hkv, int hd,
                    int max_seq, const uint16_t *k, const uint16_t *v, size_t src_stride,
                    size_t src_head_stride, int src_at_pos, const int *pos, int pos_stride, int pos0,
@@ -410,8 +410,8 @@ int oxb_sample_device(const float *logits, int V, float temperature, size_t top_
  * penalties: [n_rows][3] repeat, frequency, presence (NULL: none, the history
  * is not read).  mask may be NULL.  The offsets have n_rows + 1 entries;
  * n_history, n_bias are the lists' entries, which bound what the offsets may
- * reach; ids outside 0..V-1 are ignored.  Penalties extend rs/sampling.rs:14-24; biases and masks have no
- * counterpart in the reference. */
+ * reach; ids outside 0..V-1 are ignored.  Penalties extend rs/sampling.rs:14-24;
+ * biases and masks have no counterpart in the reference. */
 int oxb_logits_rules(const float *logits, size_t stride, int n_rows, int V, const float *penalties,
                      const int32_t *history, const int *history_off, int n_history,
                      const int32_t *bias_ids, const float *bias, const int *bias_off, int n_bias,

@@ -441,6 +441,21 @@ def test_evict_keeps_the_heaviest_blocks(inplace, lens, max_seq, budget, sink, r
             assert np.array_equal(bits(got_w[z, h, :len(keep)]), bits(w[z, h, keep]))
 
 
+def test_evict_with_room_for_all():
+    """A budget past every block, sink and recent past the sequence's: nothing changes."""
+    rng = rng_of("room")
+    lens, ms = [100, 33, 0], 100
+    c = new_cache(3, 2, ms, ops.KV8_INT8)
+    k, v = (rng.standard_normal((3, 2, ms, HD)).astype(np.float16) for _ in "kv")
+    c.append(k, v, [0] * 3, lens)
+    want, wt = c.read([0] * 3, ms, lens), c.weights()
+    assert c.evict(lens, (1 << 31) - 1, 40, 1 << 30).tolist() == lens
+    for a, b in zip(c.read([0] * 3, ms, lens), want):
+        assert np.array_equal(a, b)
+    for z, n in enumerate(lens):
+        assert np.array_equal(c.weights()[z][:, :(n + 31) // 32], wt[z][:, :(n + 31) // 32])
+
+
 @pytest.mark.parametrize("inplace", [True, False])
 def test_evict_then_append_and_attend(inplace):
     """The unfinished block goes on growing after a cut: rows, scales, attention."""

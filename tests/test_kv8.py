@@ -163,3 +163,10 @@ def test_reference_e4m3():
         d = np.abs(codes - v)
         near = np.flatnonzero(d == d.min())
         assert r == codes[near[near % 2 == 0][0] if len(near) > 1 else near[0]]
+
+
+def test_evict_workspace_is_of_the_cache_at_most():
+    """A budget past the cache's blocks keeps all of them and asks for no more memory."""
+    b = L().oxb_kv8_evict_ws_bytes
+    assert b(3, 5, 100, 4) == 256 + 256
+    assert b(3, 5, 100, (1 << 31) - 1) == b(3, 5, 100, 4)
