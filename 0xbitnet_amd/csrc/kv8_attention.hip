@@ -661,10 +661,13 @@ __global__ __launch_bounds__(kPreThreads, 2) void kv8_prefill_kernel(Kv8PrefillA
     lds_barrier();   // the first K slot is free
     const int wb = min(b1, kv8_blocks(wseen));   // blocks that some row of the wave sees
     float2 sb = sc[b0];
-    auto top = [&](const f32x16 &s, int i) {   // of four scores
-        return fmaxf(fmaxf(s[i], s[i + 1]), fmaxf(s[i + 2], s[i + 3]));
+    // the running maximum with four more scores (in v_max3's form)
+    auto top = [&](float m, const f32x16 &s, int i) {
+        m = fmaxf(fmaxf(s[i], s[i + 1]), m);
+        return fmaxf(fmaxf(s[i + 2], s[i + 3]), m);
     };
-    float smax = fmaxf(fmaxf(top(s0, 0), top(s0, 4)), fmaxf(top(s0, 8), top(s0, 12)));
+    constexpr float kNone = -__builtin_inff();
+    float smax = top(top(top(top(kNone, s0, 0), s0, 4), s0, 8), s0, 12);
     // Block b, its scores in s and their maximum in smax; the next one's go to sn.
     // r: b's place in the run; stage0, stage1: what is unpacked under it.
     auto block = [&](int b, int r, f32x16 &s, f32x16 &sn, auto stage0, auto stage1) {
@@ -682,7 +685,7 @@ __global__ __launch_bounds__(kPreThreads, 2) void kv8_prefill_kernel(Kv8PrefillA
                 ck = 1.2e-38f;
                 vs = 0.0f;
             }
-            smax = fmaxf(fmaxf(top(s, 0), top(s, 4)), fmaxf(top(s, 8), top(s, 12)));
+            smax = top(top(top(top(kNone, s, 0), s, 4), s, 8), s, 12);
         }
         const float mx = smax * ck;
         const float mx2 = mx + kv8_scale_exp(vs);
@@ -713,6 +716,7 @@ __global__ __launch_bounds__(kPreThreads, 2) void kv8_prefill_kernel(Kv8PrefillA
             half2_t hi, lo;
             hi.x = (_Float16)__builtin_fmaf(pa, vs, 0.0f);
             hi.y = (_Float16)__builtin_fmaf(pb, vs, 0.0f);
+            asm("" : "+v"(hi));   // (one register for both, or the products are formed twice)
             lo.x = (_Float16)__builtin_fmaf(pa, vs, -(float)hi.x);
             lo.y = (_Float16)__builtin_fmaf(pb, vs, -(float)hi.y);
             ph[j >> 2][2 * (j & 3)] = hi.x;
@@ -760,7 +764,7 @@ __global__ __launch_bounds__(kPreThreads, 2) void kv8_prefill_kernel(Kv8PrefillA
 #pragma unroll
         for (int d = 0; d < 4; ++d) {
             o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[d], pl[1], o[d], 0, 0, 0);
-            smax = d == 0 ? top(sn, 0) : fmaxf(smax, top(sn, 4 * d));
+            smax = top(d == 0 ? kNone : smax, sn, 4 * d);
             SLOT();
         }
 #undef SLOT
