@@ -517,8 +517,11 @@ struct Kv8PrefillOrder {
 
 template <int FMT>
 __global__ __launch_bounds__(kPreThreads, 2) void kv8_prefill_kernel(Kv8PrefillArgs a, const Kv8PrefillOrder order) {
-    // rings of K [8][64] and V operands [4 dims][2][64]: block b of the run in slot b % 4
-    __shared__ uint4 sk[kPreRing][kPreOps], sv[kPreRing][kPreOps];
+    // rings of K [8][64] and V operands [4 dims][2][64]: block b of the run in slot
+    // b % 4; the rows of q before
+    __shared__ uint4 lds[2][kPreRing][kPreOps];
+    static_assert(sizeof lds == sizeof(float) * kPreRows * kKv8Hd, "q rows fill the rings");
+    auto &sk = lds[0], &sv = lds[1];
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     // workgroups take the plan's runs in its order, the KV heads side by side
@@ -568,6 +571,18 @@ __global__ __launch_bounds__(kPreThreads, 2) void kv8_prefill_kernel(Kv8PrefillA
         c.z &= mk[2];
         c.w &= mk[3];
     };
+    // q first, through the rings' LDS, 16 KB a wave: two of its rows a load, row r's
+    // 16-byte piece c at c ^ r, so that the rows' reads of one piece meet no bank
+    // twice (a lane loading its own row, 64 pieces of 32 rows at a time: 101 tokens
+    // 11.0 us against 10.5, 300 behind 500 22.9 against 22.6)
+    uint4 *sq = &lds[0][0][0] + 1024 * wave;
+    const uint32_t qrow = (uint32_t)tok * a.H + head;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        const uint32_t ra = __builtin_amdgcn_readlane(qrow, 2 * i), rb = __builtin_amdgcn_readlane(qrow, 2 * i + 1);
+        const int c = (lane & 31) ^ (2 * i + h);
+        lds_dma16(a.q + (size_t)(h ? rb : ra) * kKv8Hd + 4 * c, sq + 64 * i);
+    }
     ck4[0] = fetch(b0, koff);
     ck4[1] = fetch(b0 + 1, koff);
     cv4[0] = fetch(b0, voff);
@@ -578,32 +593,39 @@ __global__ __launch_bounds__(kPreThreads, 2) void kv8_prefill_kernel(Kv8PrefillA
     half8_t qh[8], ql[8];
     float qs;
     {
-        const float *q = a.q + ((size_t)tok * a.H + head) * kKv8Hd + 16 * h;
         float m = 0.0f;
         float v[64];
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 #pragma unroll
-        for (int c = 0; c < 4; ++c)
+        for (int i = 0; i < 16; ++i) {
+            const int p = (8 * (i >> 2) + 4 * h + (i & 3)) ^ (lane & 31);
+            const float4 f = __builtin_bit_cast(float4, sq[32 * (lane & 31) + p]);
+            v[4 * i] = f.x;
+            v[4 * i + 1] = f.y;
+            v[4 * i + 2] = f.z;
+            v[4 * i + 3] = f.w;
+        }
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const float4 f = *(const float4 *)(q + 32 * c + 4 * j);
-                v[16 * c + 4 * j] = f.x;
-                v[16 * c + 4 * j + 1] = f.y;
-                v[16 * c + 4 * j + 2] = f.z;
-                v[16 * c + 4 * j + 3] = f.w;
-            }
-#pragma unroll
-        for (int i = 0; i < 64; ++i) m = fmaxf(m, fabsf(v[i]));
+        for (int i = 0; i < 64; i += 2) m = fmaxf(fmaxf(fabsf(v[i]), fabsf(v[i + 1])), m);
         m = fmaxf(m, __shfl_xor(m, 32, 64));
-        const int e = kv8_row_exp(m);
+        const int e = max(kv8_row_exp(m), -127);   // (a row below 2^-113 stays below 2^kQExp)
+        const float up = ldexpf(1.0f, -e);
         qs = ldexpf(kScoreUnit, e);
 #pragma unroll
         for (int s = 0; s < 8; ++s)
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const float x = ldexpf(v[8 * s + j], -e);
-                const _Float16 hi = (_Float16)x;
-                qh[s][j] = hi;
-                ql[s][j] = (_Float16)(x - (float)hi);
+            for (int j = 0; j < 8; j += 2) {
+                const float x = v[8 * s + j], y = v[8 * s + j + 1];
+                half2_t hi, lo;
+                hi.x = (_Float16)__builtin_fmaf(x, up, 0.0f);
+                hi.y = (_Float16)__builtin_fmaf(y, up, 0.0f);
+                asm("" : "+v"(hi));
+                lo.x = (_Float16)__builtin_fmaf(x, up, -(float)hi.x);
+                lo.y = (_Float16)__builtin_fmaf(y, up, -(float)hi.y);
+                qh[s][j] = hi.x;
+                qh[s][j + 1] = hi.y;
+                ql[s][j] = lo.x;
+                ql[s][j + 1] = lo.y;
             }
     }
     if (a.weights && split == 0) {
@@ -633,6 +655,7 @@ __global__ __launch_bounds__(kPreThreads, 2) void kv8_prefill_kernel(Kv8PrefillA
     const int wseen = a.pos0 + min(r0 + wave * 32 + 31, a.rows - 1) / a.G + 1;   // the wave's last row
     const int wfull = a.pos0 + min(r0 + wave * 32, a.rows - 1) / a.G + 1;        // its first row
 
+    lds_barrier();   // every wave has its q
     clear_v(b0, cv4[0]);
     clear_v(b0 + 1, cv4[1]);
     stage(sk[0], ck4[0]);

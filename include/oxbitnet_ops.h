@@ -327,7 +327,8 @@ int oxb_kv8_read(const void *cache, size_t cache_stride, int fmt, int batch, int
  * q + z*H*128 attends over positions 0..pos[z*pos_stride] (device, at most
  * max_seq - 1; below 0: the output is zeros), any H that is a multiple of Hkv,
  * any length.  f32 in and out: codes are exact in f16, q and the softmax
- * weights go through f16 MFMA as two parts each, sums are f32; not the
+ * weights go through f16 MFMA as two parts each, sums are f32 (22 bits of each
+ * weight, and none below about 2^-30 of the row's largest p max|V|); not the
  * reference's summation order (oxb_attn_decode keeps that).  With
  * add_weights, the softmax weights of each block's positions, summed over the
  * KV head's query heads, are added to the block's weight.  The result does not

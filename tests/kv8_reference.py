@@ -54,6 +54,17 @@ def attend(q, k, v):
     return p @ v, p, rel * (p @ np.abs(v)) + 1e-37, rel
 
 
+def parts_floor(v):
+    """What attend()'s bound leaves out where a position that takes nearly all of the
+    weight has the value 0 in some dim, so that weights far below 2^-22 make up
+    the whole output there: the two f16 parts of x = 2^6 2^(s - m2) vs hold it to
+    2^-25 (f16's smallest step is 2^-24), so an output's numerator is off by at
+    most n 2^-25 top (top: the largest code).  The denominator is at least 2^6
+    2^(s_max - m2), and m2 <= s_max + e, 2^e <= 2 vs_max: the output is off by at
+    most n 2^-25 top 2 vs_max 2^-6 = n 2^-30 max|v|."""
+    return len(v) * 2.0 ** -30 * float(np.abs(v).max(initial=0))
+
+
 def rms_bound(q, k):
     """A bound on the outputs' relative error in the 2-norm: roundings of a score's
     128 products fall either way, so they add as sqrt(128) u, with q's split

@@ -242,6 +242,24 @@ def test_decode_scales_of_q(fmt, qscale):
     check_rows(got, want, tol)
 
 
+@pytest.mark.parametrize("qscale", [1e-42, 1e-36, 1e-30, 40.0, 3e4])
+def test_prefill_scales_of_q(qscale):
+    """As above, rows of subnormal numbers and of zeros among them."""
+    for fmt in FMTS:
+        rng = rng_of("qp", fmt, qscale)
+        c, K, V = filled(rng, [300], 2, 300, fmt)
+        q = (rng.standard_normal((150, 8 * HD)) * qscale).astype(np.float32)
+        q[7] = 0
+        q[60] = np.float32(1e-45)
+        q[100, :HD] = 1.5
+        want, tol, w, wtol = ref.attend_rows(q, K[0], V[0], 2, 150)
+        tol = tol + max(ref.parts_floor(v) for v in V[0])
+        got = c.attn_prefill(q, 150, add_weights=True)
+        assert np.isfinite(got).all() and np.abs(got).max() <= np.abs(V[0]).max() * 1.0001
+        check_rows(got, want, tol)
+        check_rows(c.weights()[0, :, :10], w[:, :10], wtol[:, :10])
+
+
 def test_decode_values_of_very_different_blocks():
     """A block of large values that no weight goes to leaves the small ones exact."""
     for fmt in FMTS:
