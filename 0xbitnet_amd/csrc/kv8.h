@@ -59,6 +59,7 @@ inline int kv8_check(const void *cache, size_t stride, int fmt, int batch, int H
 #ifdef __HIPCC__
 namespace oxb {
 
+typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
 typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
 typedef _Float16 half8_t __attribute__((ext_vector_type(8)));
 

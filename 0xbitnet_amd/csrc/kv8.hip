@@ -25,7 +25,6 @@
 namespace oxb {
 
 constexpr int kKvThreads = 256;
-typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
 
 struct Kv8AppendArgs {
     uint8_t *cache;

@@ -493,17 +493,14 @@ constexpr float kPreBase = 6.0f;             // p' <= 2^(6 + kStep)
 struct Kv8PrefillArgs {
     const float *q;
     uint8_t *cache;
-    int n, pos0, H, Hkv, G, nb, rows, rtiles, planned, per, weights;
+    int n, pos0, H, Hkv, G, nb, rows, rtiles, planned, per, nblk;
     float *out;
     float2 *ml;     // [splits][Hkv][rows] a row's reference and sum
     float *o;       // [splits][Hkv][rows][128]
-    float2 *lse;    // [Hkv][rows32] log2 of the row's softmax sum, its score unit
-    uint4 *qf;      // [Hkv][rows32 / 32][8][2][64] q as MFMA operands
-    float *part;    // [row splits][Hkv][blocks of the call] weights
-    int rsplits;
+    float *lse;     // [Hkv][rows] log2 of the row's softmax sum, or NULL: no weights
+    float2 *bw;     // [Hkv][nblk][rtiles * 128] a block's sum of p' in a row, its reference
 };
 
-__host__ __device__ inline int pre_rows32(int rows) { return (rows + 31) & ~31; }
 // A row tile's blocks in even runs.
 __host__ __device__ inline int pre_run_start(int blocks, int runs, int i) {
     return (int)((int64_t)blocks * i / runs);
@@ -515,7 +512,7 @@ struct Kv8PrefillOrder {
     uint32_t run[kPreOrder];
 };
 
-template <int FMT>
+template <int FMT, bool WEIGHTS>
 __global__ __launch_bounds__(kPreThreads, 2) void kv8_prefill_kernel(Kv8PrefillArgs a, const Kv8PrefillOrder order) {
     // rings of K [8][64] and V operands [4 dims][2][64]: block b of the run in slot
     // b % 4; the rows of q before
@@ -628,22 +625,9 @@ __global__ __launch_bounds__(kPreThreads, 2) void kv8_prefill_kernel(Kv8PrefillA
                 ql[s][j + 1] = lo.y;
             }
     }
-    if (a.weights && split == 0) {
-        const int r32 = pre_rows32(a.rows);
-        if (r0 + wave * 32 < r32) {
-            uint4 *f = a.qf + (((size_t)kvh * r32 + r0 + wave * 32) / 32) * (8 * 2 * 64) + lane;
-#pragma unroll
-            for (int s = 0; s < 8; ++s) {
-                f[(2 * s) * 64] = __builtin_bit_cast(uint4, qh[s]);
-                f[(2 * s + 1) * 64] = __builtin_bit_cast(uint4, ql[s]);
-            }
-            if (h == 0) {
-                float2 *ls = a.lse + (size_t)kvh * r32 + row;
-                ls->y = qs;
-                if (row >= a.rows) ls->x = __builtin_inff();   // weighs nothing
-            }
-        }
-    }
+    // where the row's sums of the blocks go: the first half's lanes and the second's
+    // store the same
+    const int wrows = a.rtiles * kPreRows, woff = row * 8;
 
     f32x16 o[4];
 #pragma unroll
@@ -728,14 +712,15 @@ __global__ __launch_bounds__(kPreThreads, 2) void kv8_prefill_kernel(Kv8PrefillA
 #define SLOT() __builtin_amdgcn_sched_barrier(0)
         const uint4 *kb = sk[(r + 1) & 3] + lane, *vb = sv[r & 3] + lane;
         half8_t ph[2], pl[2], v[4], k[2];
-        float pa, pb;
+        float pa, pb, ps = 0.0f;
         auto exps = [&](int j) {   // elements 2 j, 2 j + 1
             pa = __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * j], ck, -moff));
             pb = __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * j + 1], ck, -moff));
         };
         auto split = [&](int j) {   // hi and lo of p' vs, each rounded once from the exact product
-            lsum += pa;
-            lsum += pb;
+            ps += pa;
+            ps += pb;
+            asm volatile("" : "+v"(ps));   // (here, not all sums at the end)
             half2_t hi, lo;
             hi.x = (_Float16)__builtin_fmaf(pa, vs, 0.0f);
             hi.y = (_Float16)__builtin_fmaf(pb, vs, 0.0f);
@@ -788,9 +773,18 @@ __global__ __launch_bounds__(kPreThreads, 2) void kv8_prefill_kernel(Kv8PrefillA
         for (int d = 0; d < 4; ++d) {
             o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[d], pl[1], o[d], 0, 0, 0);
             smax = top(d == 0 ? kNone : smax, sn, 4 * d);
+            if constexpr (WEIGHTS)
+                if (d == 1) {
+                    const auto w = __builtin_amdgcn_permlane32_swap(__float_as_uint(ps), __float_as_uint(ps), false, false);
+                    const u32x2_t v = {__float_as_uint(__uint_as_float(w[0]) + __uint_as_float(w[1])), __float_as_uint(moff)};
+                    const __amdgpu_buffer_rsrc_t wr = __builtin_amdgcn_make_buffer_rsrc(
+                        a.bw + ((size_t)kvh * a.nblk + b) * wrows, 0, wrows * 8, 0x00027000);
+                    __builtin_amdgcn_raw_buffer_store_b64(v, wr, woff, 0, 0);
+                }
             SLOT();
         }
 #undef SLOT
+        lsum += ps;
     };
     auto stage_k = [&](int r) { return [&, r] { stage(sk[(r + 3) & 3], ck4[0]); }; };
     auto stage_k1 = [&](int r) { return [&, r] { stage(sk[r & 3], ck4[1]); }; };
@@ -837,8 +831,7 @@ __global__ __launch_bounds__(kPreThreads, 2) void kv8_prefill_kernel(Kv8PrefillA
     if (direct) {
         dst = a.out + ((size_t)(erow / a.G) * a.H + kvh * a.G + erow % a.G) * kKv8Hd;
         f /= lsum;
-        if (a.weights && eh == 0)
-            a.lse[(size_t)kvh * pre_rows32(a.rows) + erow].x = M + __builtin_amdgcn_logf(lsum);
+        if (WEIGHTS && eh == 0) a.lse[(size_t)kvh * a.rows + erow] = M + __builtin_amdgcn_logf(lsum);
     } else {
         const size_t part = ((size_t)split * a.Hkv + kvh) * a.rows + erow;
         dst = a.o + part * kKv8Hd;
@@ -897,165 +890,50 @@ __global__ __launch_bounds__(256) void kv8_prefill_join_kernel(Kv8PrefillArgs a)
     }
     *(float4 *)(a.out + ((size_t)tok * a.H + head) * kKv8Hd + d) =
         make_float4(t.x / lt, t.y / lt, t.z / lt, t.w / lt);
-    if (a.weights && d == 0)
-        a.lse[(size_t)kvh * pre_rows32(a.rows) + row].x = M + __builtin_amdgcn_logf(lt);
+    if (a.lse && d == 0) a.lse[r] = M + __builtin_amdgcn_logf(lt);
 }
 
-// A block's weight from the rows' softmax sums: the scores again, K in
-// registers (two blocks a wave, eight a workgroup), groups of 32 rows of q
-// (as MFMA operands, from the attention's first runs) through LDS, the next
-// group on its way meanwhile.  A group's exponentials alternate with the next
-// one's score products, which bound it (32 MFMAs of 32 cycles a wave and
-// group).  Sums are in a fixed order: rows of a lane, then lanes, then row splits.
-constexpr int kWtWaves = 4;
-constexpr int kWtBlocks = 2 * kWtWaves;
-constexpr int kWtGroup = 16 * 64;   // uint4 of a group's operands
-template <int FMT>
-__global__ __launch_bounds__(64 * kWtWaves, 2) void kv8_weights_kernel(Kv8PrefillArgs a) {
-    __shared__ uint4 sq[2][kWtGroup];
-    const int lane = threadIdx.x & 63, kvh = blockIdx.y, h = lane >> 5;
-    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-    const int nblk = kv8_blocks(a.pos0 + a.n), wg0 = blockIdx.x * kWtBlocks, b0 = wg0 + wave * 2;
-    const int r32 = pre_rows32(a.rows), groups = r32 / 32;
-    const int per = (groups + a.rsplits - 1) / a.rsplits;
-    // rows before the workgroup's first block see nothing of it
-    const int g0 = max(max(0, wg0 * kKv8Block - a.pos0) * a.G / 32, (int)blockIdx.z * per);
-    const int g1 = min(groups, (int)(blockIdx.z + 1) * per);
-    const uint4 *qf = a.qf + ((size_t)kvh * groups * 16 + 4 * wave) * 64 + lane;
-    auto fetch = [&](int g, int buf) {   // four of the group's operands each
-#pragma unroll
-        for (int i = 0; i < 4; ++i) lds_dma16(qf + (size_t)g * kWtGroup + i * 64, &sq[buf][(4 * wave + i) * 64]);
-    };
-    if (g0 < g1) fetch(g0, 0);
-    const Kv8Layout l = kv8_layout(a.Hkv, a.nb);
-    const float2 *sc = (const float2 *)(a.cache + l.scales) + (size_t)kvh * a.nb;
-    half8_t kf[2][8];
-    float ks[2], acc[2] = {0.0f, 0.0f};
-#pragma unroll
-    for (int b = 0; b < 2; ++b) {
-        const int blk = min(b0 + b, nblk - 1);
-        const uint8_t *p = a.cache + ((size_t)kvh * a.nb + blk) * kKv8Codes + (lane & 31) * kKv8Hd + 16 * h;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const uint4 c = *(const uint4 *)(p + 32 * i);
-            kf[b][2 * i] = kv8_unpack8<FMT>(c.x, c.y);
-            kf[b][2 * i + 1] = kv8_unpack8<FMT>(c.z, c.w);
-        }
-        ks[b] = sc[blk].x;
-    }
-    f32x16 s0[2], s1[2];   // scores of the group before, and of this one
-    float2 l0 = make_float2(__builtin_inff(), 0), l1;   // before the first: weighs nothing
-    // Group g's products into s, the group before's exponentials from t into acc.
-    auto group = [&](int g, int buf, f32x16 *s, f32x16 *t, const float2 &lt) {
-        const float c0 = ks[0] * lt.y, c1 = ks[1] * lt.y;
-        float p0 = 0.0f, p1 = 0.0f;
-#pragma unroll
-        for (int b = 0; b < 2; ++b)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) s[b][i] = 0.0f;
-        const uint4 *q = sq[buf] + lane;
-        half8_t f[2] = {__builtin_bit_cast(half8_t, q[0]), __builtin_bit_cast(half8_t, q[64])};
-        __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            s[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[0][i >> 1], f[i & 1], s[0], 0, 0, 0);
-            p0 += __builtin_amdgcn_exp2f(__builtin_fmaf(t[0][i], c0, -lt.x));
-            __builtin_amdgcn_sched_barrier(0);
-            s[1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[1][i >> 1], f[i & 1], s[1], 0, 0, 0);
-            p1 += __builtin_amdgcn_exp2f(__builtin_fmaf(t[1][i], c1, -lt.x));
-            if (i < 14) f[i & 1] = __builtin_bit_cast(half8_t, q[(i + 2) * 64]);
-            __builtin_amdgcn_sched_barrier(0);
-        }
-        asm volatile("" : "+v"(p0), "+v"(p1));   // (the sums stay in this basic block)
-        acc[0] += p0;
-        acc[1] += p1;
-        // rows that do not see all of the wave's positions (uniform test)
-        const int seen = a.pos0 + min(32 * g, a.rows - 1) / a.G + 1 - b0 * kKv8Block;
-        if (seen < 2 * kKv8Block) {
-            const int left = a.pos0 + min(32 * g + (lane & 31), a.rows - 1) / a.G + 1 - b0 * kKv8Block -
-                             4 * h + opaque_zero();
-#pragma unroll
-            for (int b = 0; b < 2; ++b)
-#pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    s[b][i] = 32 * b + (i & 3) + 8 * (i >> 2) < left ? s[b][i] : -__builtin_inff();
-        }
-    };
-    // (hidden scores are -inf: scales of 0, of zero blocks, made positive)
-#pragma unroll
-    for (int b = 0; b < 2; ++b) {
-        ks[b] = ks[b] < 1.2e-38f ? 1.2e-38f : ks[b];
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            s0[b][i] = 0.0f;
-            s1[b][i] = 0.0f;
-        }
-    }
-    const float2 *lse = a.lse + (size_t)kvh * r32 + (lane & 31);
-    float2 ln = g0 < g1 ? lse[32 * g0] : make_float2(0, 0);
-    for (int g = g0; g < g1; g += 2) {
-        wait_vmcnt<0>();
-        lds_barrier();
-        l1 = ln;
-        if (g + 1 < g1) {
-            fetch(g + 1, 1);
-            ln = lse[32 * (g + 1)];
-        }
-        group(g, 0, s1, s0, l0);
-        if (g + 1 >= g1) {
-            l0 = l1;
-            s0[0] = s1[0];
-            s0[1] = s1[1];
-            break;
-        }
-        wait_vmcnt<0>();
-        lds_barrier();
-        l0 = ln;
-        if (g + 2 < g1) {
-            fetch(g + 2, 0);
-            ln = lse[32 * (g + 2)];
-        }
-        group(g + 1, 1, s0, s1, l1);
-    }
-    if (g0 < g1) {   // the last group's
-#pragma unroll
-        for (int b = 0; b < 2; ++b) {
-            float p = 0.0f;
-#pragma unroll
-            for (int i = 0; i < 16; ++i) p += __builtin_amdgcn_exp2f(__builtin_fmaf(s0[b][i], ks[b] * l0.y, -l0.x));
-            acc[b] += p;
-        }
-    }
-#pragma unroll
-    for (int b = 0; b < 2; ++b) {
-        acc[b] = wave_sum(acc[b]);
-        if (lane == 0 && b0 + b < nblk) {
-            if (a.rsplits > 1)
-                a.part[((size_t)blockIdx.z * a.Hkv + kvh) * nblk + b0 + b] = acc[b];
-            else
-                ((float *)(a.cache + l.weights))[(size_t)kvh * a.nb + b0 + b] += acc[b];
-        }
-    }
-}
-
-__global__ __launch_bounds__(256) void kv8_weights_add_kernel(Kv8PrefillArgs a) {
-    const int b = blockIdx.x * 256 + threadIdx.x, kvh = blockIdx.y;
-    const int nblk = kv8_blocks(a.pos0 + a.n);
-    if (b >= nblk) return;
+// A block's weight: its sums of p' over the rows that see it, which the
+// attention has left, in the units of their softmax sums, known only now.  A
+// workgroup a block, in a fixed order; bound by the sums' bytes.
+__global__ __launch_bounds__(256) void kv8_prefill_weights_kernel(Kv8PrefillArgs a) {
+    __shared__ float red[4];
+    const int b = blockIdx.x, kvh = blockIdx.y, tid = threadIdx.x;
+    const int first = max(0, b * kKv8Block - a.pos0) * a.G;
+    const float2 *bw = a.bw + ((size_t)kvh * a.nblk + b) * a.rtiles * kPreRows;
+    const float *lse = a.lse + (size_t)kvh * a.rows;
     float s = 0.0f;
-    for (int i = 0; i < a.rsplits; ++i) s += a.part[((size_t)i * a.Hkv + kvh) * nblk + b];
-    ((float *)(a.cache + kv8_layout(a.Hkv, a.nb).weights))[(size_t)kvh * a.nb + b] += s;
+    constexpr int kB = 4;   // rows in flight
+    for (int r0 = first + tid; r0 < a.rows; r0 += kB * 256) {
+        float2 p[kB];
+        float x[kB];
+#pragma unroll
+        for (int i = 0; i < kB; ++i) {
+            const int r = min(r0 + i * 256, a.rows - 1);
+            p[i] = bw[r];
+            x[i] = lse[r];
+        }
+#pragma unroll
+        for (int i = 0; i < kB; ++i)
+            if (r0 + i * 256 < a.rows) s += p[i].x * __builtin_amdgcn_exp2f(p[i].y - x[i]);
+    }
+    s = wave_sum(s);
+    if ((tid & 63) == 0) red[tid >> 6] = s;
+    __syncthreads();
+    if (tid == 0)
+        ((float *)(a.cache + kv8_layout(a.Hkv, a.nb).weights))[(size_t)kvh * a.nb + b] +=
+            (red[0] + red[1]) + (red[2] + red[3]);
 }
 
 // The launch shapes of a prefill call and its workspace.
 struct PrefillPlan {
-    int rows, rtiles, runs, splits, per, rsplits;
+    int rows, rtiles, runs, splits, per;
     int64_t wgs;
-    size_t ml, o, lse, qf, part, bytes;
+    size_t ml, o, lse, bw, bytes;
 };
 static PrefillPlan prefill_plan(int n, int pos0, int H, int Hkv, bool weights) {
     PrefillPlan p{};
-    const int G = H / Hkv, total = pos0 + n, nblk = kv8_blocks(total);
+    const int G = H / Hkv, total = pos0 + n;
     p.rows = n * G;
     p.rtiles = (p.rows + kPreRows - 1) / kPreRows;
     // Two workgroups per CU are resident, and a row tile's blocks may be cut into
@@ -1094,18 +972,20 @@ static PrefillPlan prefill_plan(int n, int pos0, int H, int Hkv, bool weights) {
         p.o = take(parts * kKv8Hd * 4);
     }
     if (weights) {
-        const size_t r32 = pre_rows32(p.rows);
-        p.lse = take(Hkv * r32 * 8);
-        p.qf = take(Hkv * r32 * kKv8Hd * 4);
-        // row splits (of at least eight groups) while two workgroups per CU have room
-        const int64_t w = (int64_t)((nblk + kWtBlocks - 1) / kWtBlocks) * Hkv, groups = r32 / 32;
-        int64_t rs = 2 * (int64_t)device_cus() / w;
-        if (rs > groups / 8) rs = groups / 8;
-        p.rsplits = (int)(rs < 1 ? 1 : rs);
-        if (p.rsplits > 1) p.part = take((size_t)p.rsplits * Hkv * nblk * 4);
+        p.lse = take((size_t)Hkv * p.rows * 4);
+        p.bw = take((size_t)Hkv * most * p.rtiles * kPreRows * 8);
     }
     p.bytes = at;
     return p;
+}
+
+// Tokens of a launch: all, but with weights, whose sums take 8 bytes per row and
+// block, as many as keep those under 256 MB.
+static int prefill_step(int n, int pos0, int H, int Hkv, bool weights) {
+    if (!weights) return n;
+    const int64_t token = (int64_t)8 * H * kv8_blocks(pos0 + n);
+    const int64_t most = std::max<int64_t>(1, (256 << 20) / token), calls = (n + most - 1) / most;
+    return (int)((n + calls - 1) / calls);
 }
 
 // The plan's runs, the longest first; of those that run at once, the second half
@@ -1126,6 +1006,49 @@ static void prefill_order(const PrefillPlan &p, int pos0, int G, int Hkv, Kv8Pre
     const int half = device_cus() / Hkv, two = 2 * half < n ? 2 * half : n;
     if (half < two) std::reverse(run + half, run + two);
     for (int i = 0; i < n; ++i) o.run[i] = run[i].id;
+}
+
+static size_t prefill_bytes(int n, int pos0, int H, int Hkv, bool weights) {
+    const int step = prefill_step(n, pos0, H, Hkv, weights);
+    size_t b = 0;
+    for (int i = 0; i < n; i += step)
+        b = std::max(b, prefill_plan(std::min(step, n - i), pos0 + i, H, Hkv, weights).bytes);
+    return b;
+}
+
+// Tokens pos0 .. pos0 + n - 1 of a call.
+static int prefill_launch(const float *q, void *cache, int fmt, int n, int pos0, int H, int Hkv,
+                          int max_seq, bool weights, float *out, char *w, hipStream_t s) {
+    const PrefillPlan p = prefill_plan(n, pos0, H, Hkv, weights);
+    OXB_REQUIRE(p.wgs < (1 << 24), "prefill attention: %d tokens of %d heads", n, H);
+    const int nblk = kv8_blocks(pos0 + n);
+    const Kv8PrefillArgs a{q, (uint8_t *)cache, n, pos0, H, Hkv, H / Hkv, kv8_blocks(max_seq), p.rows, p.rtiles,
+                           p.rtiles <= kPreOrder, p.per, nblk, out, (float2 *)(w + p.ml), (float *)(w + p.o),
+                           weights ? (float *)(w + p.lse) : nullptr, (float2 *)(w + p.bw)};
+    const dim3 grid((unsigned)p.wgs), th(kPreThreads);
+    Kv8PrefillOrder order;
+    if (a.planned) prefill_order(p, pos0, a.G, Hkv, order);
+    if (fmt == OXB_KV8_INT8) {
+        if (weights)
+            hipLaunchKernelGGL((kv8_prefill_kernel<OXB_KV8_INT8, true>), grid, th, 0, s, a, order);
+        else
+            hipLaunchKernelGGL((kv8_prefill_kernel<OXB_KV8_INT8, false>), grid, th, 0, s, a, order);
+    } else {
+        if (weights)
+            hipLaunchKernelGGL((kv8_prefill_kernel<OXB_KV8_E4M3, true>), grid, th, 0, s, a, order);
+        else
+            hipLaunchKernelGGL((kv8_prefill_kernel<OXB_KV8_E4M3, false>), grid, th, 0, s, a, order);
+    }
+    OXB_CHECK_HIP(hipGetLastError());
+    if (p.splits > 1) {
+        hipLaunchKernelGGL(kv8_prefill_join_kernel, dim3((p.rows + 7) / 8, Hkv), dim3(256), 0, s, a);
+        OXB_CHECK_HIP(hipGetLastError());
+    }
+    if (weights) {
+        hipLaunchKernelGGL(kv8_prefill_weights_kernel, dim3(nblk, Hkv), dim3(256), 0, s, a);
+        OXB_CHECK_HIP(hipGetLastError());
+    }
+    return 0;
 }
 
 static int heads_check(int H, int Hkv) {
@@ -1184,7 +1107,7 @@ extern "C" size_t oxb_attn_prefill_kv8_ws_bytes(int n_tok, int pos0, int H, int 
     if (n_tok < 1 || pos0 < 0 || pos0 > OXB_KV8_MAX_SEQ - n_tok || Hkv < 1 || H < 1 || H % Hkv ||
         H > 65535 || hd != kKv8Hd || (int64_t)n_tok * (H / Hkv) > (1 << 30))
         return 0;
-    return prefill_plan(n_tok, pos0, H, Hkv, add_weights != 0).bytes;
+    return prefill_bytes(n_tok, pos0, H, Hkv, add_weights != 0);
 }
 
 extern "C" int oxb_attn_prefill_kv8(const float *q, void *cache, int fmt, int n_tok, int pos0, int H,
@@ -1197,39 +1120,13 @@ extern "C" int oxb_attn_prefill_kv8(const float *q, void *cache, int fmt, int n_
     OXB_REQUIRE(n_tok >= 1 && pos0 >= 0 && n_tok <= max_seq && pos0 <= max_seq - n_tok,
                 "prefill attention: bad range");
     OXB_REQUIRE((int64_t)n_tok * (H / Hkv) <= (1 << 30), "prefill attention: %d tokens", n_tok);
-    const PrefillPlan p = prefill_plan(n_tok, pos0, H, Hkv, add_weights != 0);
-    OXB_REQUIRE(ws && ((uintptr_t)ws & 255) == 0 && ws_bytes >= p.bytes,
-                "attention: workspace is NULL, not 256-byte aligned or %zu bytes < %zu", ws_bytes, p.bytes);
-    char *w = (char *)ws;
-    Kv8PrefillArgs a{q, (uint8_t *)cache, n_tok, pos0, H, Hkv, H / Hkv, kv8_blocks(max_seq), p.rows,
-                     p.rtiles, p.rtiles <= kPreOrder, p.per, add_weights != 0, out, (float2 *)(w + p.ml), (float *)(w + p.o),
-                     (float2 *)(w + p.lse), (uint4 *)(w + p.qf), (float *)(w + p.part), p.rsplits};
-    hipStream_t s = (hipStream_t)stream;
-    OXB_REQUIRE(p.wgs < (1 << 24), "prefill attention: %d tokens of %d heads", n_tok, H);
-    const dim3 grid((unsigned)p.wgs), th(kPreThreads);
-    Kv8PrefillOrder order;
-    if (a.planned) prefill_order(p, pos0, a.G, Hkv, order);
-    if (fmt == OXB_KV8_INT8)
-        hipLaunchKernelGGL(kv8_prefill_kernel<OXB_KV8_INT8>, grid, th, 0, s, a, order);
-    else
-        hipLaunchKernelGGL(kv8_prefill_kernel<OXB_KV8_E4M3>, grid, th, 0, s, a, order);
-    OXB_CHECK_HIP(hipGetLastError());
-    if (p.splits > 1) {
-        hipLaunchKernelGGL(kv8_prefill_join_kernel, dim3((p.rows + 7) / 8, Hkv), dim3(256), 0, s, a);
-        OXB_CHECK_HIP(hipGetLastError());
-    }
-    if (add_weights) {
-        const int nblk = kv8_blocks(pos0 + n_tok);
-        const dim3 wg((nblk + kWtBlocks - 1) / kWtBlocks, Hkv, p.rsplits);
-        if (fmt == OXB_KV8_INT8)
-            hipLaunchKernelGGL(kv8_weights_kernel<OXB_KV8_INT8>, wg, dim3(256), 0, s, a);
-        else
-            hipLaunchKernelGGL(kv8_weights_kernel<OXB_KV8_E4M3>, wg, dim3(256), 0, s, a);
-        OXB_CHECK_HIP(hipGetLastError());
-        if (p.rsplits > 1) {
-            hipLaunchKernelGGL(kv8_weights_add_kernel, dim3((nblk + 255) / 256, Hkv), dim3(256), 0, s, a);
-            OXB_CHECK_HIP(hipGetLastError());
-        }
-    }
+    const size_t bytes = prefill_bytes(n_tok, pos0, H, Hkv, add_weights != 0);
+    OXB_REQUIRE(ws && ((uintptr_t)ws & 255) == 0 && ws_bytes >= bytes,
+                "attention: workspace is NULL, not 256-byte aligned or %zu bytes < %zu", ws_bytes, bytes);
+    const int step = prefill_step(n_tok, pos0, H, Hkv, add_weights != 0);
+    for (int i = 0; i < n_tok; i += step)
+        if (prefill_launch(q + (size_t)i * H * hd, cache, fmt, std::min(step, n_tok - i), pos0 + i, H, Hkv,
+                           max_seq, add_weights != 0, out + (size_t)i * H * hd, (char *)ws, (hipStream_t)stream))
+            return -1;
     return 0;
 }

@@ -358,6 +358,31 @@ def test_prefill_weights_long(H, hkv, n, pos0):
     check_rows(c.weights()[0], want, tol)
 
 
+def test_prefill_weights_in_several_launches():
+    """Rows times blocks past what a launch's sums may take: outputs of rows on both
+    sides of where the call is cut, weights against those of three calls, and each
+    row's weights add up to 1."""
+    rng = rng_of("cut")
+    H, n, pos0 = 8, 600, 261000       # 8200 blocks: 8 heads' sums of 511 tokens fill 256 MB
+    total = pos0 + n
+    c, K, V = filled(rng, [total], 1, total, 0)
+    q = rng.standard_normal((n, H * HD)).astype(np.float32)
+    got = c.attn_prefill(q, pos0, add_weights=True)
+    w = c.weights()[0].astype(np.float64)
+    for i in (0, 299, 300, 511, n - 1):
+        want, tol, _, _ = ref.attend_rows(q[i:i + 1], K[0], V[0], 1, pos0 + i)
+        check_rows(got[i:i + 1], want, tol, i)
+    for i in range(0, n, 200):
+        c.attn_prefill(q[i:i + 200], pos0 + i, add_weights=True)
+    parts = c.weights()[0] - w
+    # attend()'s bound on a weight, S by Cauchy-Schwarz; the sums as in attend_rows,
+    # and the two subtracted ones' roundings
+    S = np.linalg.norm(q.reshape(-1, HD), axis=1).max() * np.linalg.norm(K[0][0], axis=1).max() / np.sqrt(HD)
+    rel_w = 2 * (140 * ref.U * S + 8 * ref.U) + (total / 32 + 64 + 4 + n * H + 64) * ref.U
+    check_rows(parts, w, 3 * rel_w * w + 1e-37)
+    assert abs(w.sum() - n * H) <= rel_w * n * H
+
+
 def test_prefill_leaves_rows_behind_the_last():
     rng = rng_of("behind")
     L = ops.lib()

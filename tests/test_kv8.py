@@ -170,3 +170,12 @@ def test_evict_workspace_is_of_the_cache_at_most():
     b = L().oxb_kv8_evict_ws_bytes
     assert b(3, 5, 100, 4) == 256 + 256
     assert b(3, 5, 100, (1 << 31) - 1) == b(3, 5, 100, 4)
+
+
+def test_prefill_workspace_with_weights_stays_bounded():
+    """8 bytes per row and block, 256 MB at most (and the parts of two launches' rows
+    at a time beside them)."""
+    b = L().oxb_attn_prefill_kv8_ws_bytes
+    assert b(101, 0, 20, 5, 128, 1) - b(101, 0, 20, 5, 128, 0) == (20 * 101 * 4 + 255) // 256 * 256 + 5 * 4 * 512 * 8
+    for n, pos0, H, hkv in ((8192, 0, 20, 5), (100000, 0, 20, 5), (600, 261000, 8, 1), (1, (1 << 24) - 1, 64, 1)):
+        assert b(n, pos0, H, hkv, 128, 1) <= b(n, pos0, H, hkv, 128, 0) + (600 << 20), (n, pos0)
