@@ -266,6 +266,11 @@ def attn_prefill(q: np.ndarray, kcache: np.ndarray, vcache: np.ndarray, n_tok: i
 KV8_INT8, KV8_E4M3, KV8_BLOCK = 0, 1, 32   # include/oxbitnet_ops.h OXB_KV8_*
 
 
+def _require(ok, what: str) -> None:
+    if not ok:
+        raise ValueError(what)
+
+
 class Kv8Cache:
     """A batch's 8-bit KV cache (oxb_kv8_*, oxb_attn_*_kv8): numpy rows in, numpy out."""
 
@@ -276,13 +281,27 @@ class Kv8Cache:
             raise NativeError(f"no 8-bit cache of {Hkv} heads of {hd}, {max_seq} positions")
         self.data = DeviceArray((batch, self.stride), np.uint8)
 
+    def _per_seq(self, x, what: str) -> np.ndarray:
+        x = np.ascontiguousarray(x, np.int32)
+        _require(x.shape == (self.batch,), f"{what}: {x.shape} for {self.batch} sequences")
+        return x
+
+    def _heads(self, q: np.ndarray) -> int:
+        _require(q.shape[1] % (self.hd * self.Hkv) == 0 and q.shape[1] > 0,
+                 f"q rows of {q.shape[1]} for {self.Hkv} KV heads of {self.hd}")
+        return q.shape[1] // self.hd
+
     def append(self, k: np.ndarray, v: np.ndarray, pos, counts=None, stream=None) -> None:
         """f16 rows [batch][Hkv][n][128] at each sequence's position."""
         k, v = (np.ascontiguousarray(x, np.float16) for x in (k, v))
+        _require(k.ndim == 4 and k.shape == v.shape == (self.batch, self.Hkv, k.shape[2], self.hd),
+                 f"k {k.shape} and v {v.shape} for [{self.batch}][{self.Hkv}][n][{self.hd}]")
         n = k.shape[2]
+        pos = self._per_seq(pos, "pos")
+        counts = self._per_seq(counts, "counts") if counts is not None else None
         dk, dv = (DeviceArray.from_host(x.view(np.uint16)) for x in (k, v))
-        dp = DeviceArray.from_host(np.ascontiguousarray(pos, np.int32))
-        dc = DeviceArray.from_host(np.ascontiguousarray(counts, np.int32)) if counts is not None else None
+        dp = DeviceArray.from_host(pos)
+        dc = DeviceArray.from_host(counts) if counts is not None else None
         check(lib().oxb_kv8_append(self.data.ptr, self.stride, self.fmt, self.batch, self.Hkv, self.hd,
                                    self.max_seq, dk.ptr, dv.ptr, self.Hkv * n * self.hd, n * self.hd, 0,
                                    dp.ptr, 1, 0, n, _p(dc), stream), "kv8_append")
@@ -290,8 +309,10 @@ class Kv8Cache:
 
     def read(self, pos, n: int, length=None):
         """The values of n positions from each sequence's pos on: k, v f32 [batch][Hkv][n][128]."""
-        dp = DeviceArray.from_host(np.ascontiguousarray(pos, np.int32))
-        dl = DeviceArray.from_host(np.ascontiguousarray(length, np.int32)) if length is not None else None
+        pos = self._per_seq(pos, "pos")
+        length = self._per_seq(length, "length") if length is not None else None
+        dp = DeviceArray.from_host(pos)
+        dl = DeviceArray.from_host(length) if length is not None else None
         k, v = (DeviceArray((self.batch, self.Hkv, n, self.hd), np.float32) for _ in "kv")
         check(lib().oxb_kv8_read(self.data.ptr, self.stride, self.fmt, self.batch, self.Hkv, self.hd,
                                  self.max_seq, dp.ptr, 1, 0, n, _p(dl), 1, k.ptr, v.ptr, None), "kv8_read")
@@ -308,8 +329,8 @@ class Kv8Cache:
     def attn_decode(self, q: np.ndarray, pos, add_weights: bool = False) -> np.ndarray:
         """q f32 [batch][H*128]; sequence z attends over pos[z] + 1 positions."""
         q = np.ascontiguousarray(q, np.float32).reshape(self.batch, -1)
-        H = q.shape[1] // self.hd
-        dq, dp = DeviceArray.from_host(q), DeviceArray.from_host(np.ascontiguousarray(pos, np.int32))
+        H, pos = self._heads(q), self._per_seq(pos, "pos")
+        dq, dp = DeviceArray.from_host(q), DeviceArray.from_host(pos)
         out = DeviceArray(q.shape, np.float32)
         n = lib().oxb_attn_decode_kv8_ws_bytes(self.batch, H, self.Hkv, self.hd, self.max_seq)
         ws = DeviceArray((max(n, 16),), np.uint8, zero=True)
@@ -322,7 +343,8 @@ class Kv8Cache:
     def attn_prefill(self, q: np.ndarray, pos0: int, slot: int = 0, add_weights: bool = False) -> np.ndarray:
         """q f32 [n][H*128] of sequence `slot` at positions pos0.., causal."""
         q = np.ascontiguousarray(np.atleast_2d(q), np.float32)
-        n, H = q.shape[0], q.shape[1] // self.hd
+        _require(0 <= slot < self.batch, f"sequence {slot} of {self.batch}")
+        n, H = q.shape[0], self._heads(q)
         dq, out = DeviceArray.from_host(q), DeviceArray(q.shape, np.float32)
         b = lib().oxb_attn_prefill_kv8_ws_bytes(n, pos0, H, self.Hkv, self.hd, int(add_weights))
         ws = DeviceArray((max(b, 16),), np.uint8, zero=True)
@@ -335,7 +357,9 @@ class Kv8Cache:
     def evict(self, length, budget: int, sink: int = 1, recent: int = 1, dst: "Kv8Cache | None" = None):
         """Cut to `budget` blocks, in place or into dst; returns the new lengths."""
         dst = dst or self
-        dl = DeviceArray.from_host(np.ascontiguousarray(length, np.int32))
+        _require((dst.batch, dst.Hkv, dst.hd, dst.fmt) == (self.batch, self.Hkv, self.hd, self.fmt),
+                 "dst is a cache of another shape or format")
+        dl = DeviceArray.from_host(self._per_seq(length, "length"))
         n = lib().oxb_kv8_evict_ws_bytes(self.batch, self.Hkv, self.max_seq, budget)
         ws = DeviceArray((max(n, 16),), np.uint8)
         check(lib().oxb_kv8_evict(self.data.ptr, self.stride, self.max_seq, dst.data.ptr, dst.stride,
@@ -353,21 +377,23 @@ def logits_rules(logits: np.ndarray, penalties=None, history=None, bias=None, ma
     n, V = x.shape
 
     def csr(lists, dtype):
+        _require(len(lists) == n, f"{len(lists)} lists for {n} rows")
         off = np.concatenate([[0], np.cumsum([len(r) for r in lists])]).astype(np.int32)
         flat = np.concatenate([np.asarray(r, dtype).reshape(-1) for r in lists]).astype(dtype)
         return flat, off
 
-    up = lambda a: DeviceArray.from_host(np.ascontiguousarray(a)) if a is not None and a.size else None  # noqa: E731
-    dx = DeviceArray.from_host(x)
-    dpen = up(np.asarray(penalties, np.float32).reshape(n, 3)) if penalties is not None else None
+    pen = np.asarray(penalties, np.float32).reshape(n, 3) if penalties is not None else None
     h, ho = csr(history, np.int32) if history is not None else (np.empty(0, np.int32), None)
     bi, bo = csr([[i for i, _ in r] for r in bias], np.int32) if bias is not None else (np.empty(0, np.int32), None)
     bv = csr([[b for _, b in r] for r in bias], np.float32)[0] if bias is not None else None
-    dh, dho, dbi, dbo, dbv = up(h), up(ho), up(bi), up(bo), up(bv)
-    dm, words = None, 0
+    words = 0
     if mask is not None:
         mask = np.ascontiguousarray(mask, np.uint32)
-        dm, words = up(mask), mask.shape[1] if mask.ndim == 2 else 0
+        _require(mask.shape[-1] >= (V + 31) // 32 and mask.shape[:-1] in ((), (n,)),
+                 f"mask {mask.shape} for {n} rows of {V}")
+        words = mask.shape[1] if mask.ndim == 2 else 0
+    up = lambda a: DeviceArray.from_host(a) if a is not None and a.size else None  # noqa: E731
+    dx, dpen, dh, dho, dbi, dbo, dbv, dm = (up(a) for a in (x, pen, h, ho, bi, bo, bv, mask))
     out = DeviceArray((n, V), np.float32)
     check(lib().oxb_logits_rules(dx.ptr, V, n, V, _p(dpen), _p(dh), _p(dho), h.size, _p(dbi), _p(dbv),
                                  _p(dbo), bi.size, _p(dm), words, out.ptr, V, None), "logits_rules")

@@ -346,7 +346,8 @@ int oxb_attn_decode_kv8(const float *q, void *cache, size_t cache_stride, int fm
 /* Causal prefill attention over one sequence's 8-bit cache: query i (q, out:
  * [n_tok][H*128]) attends over positions 0..pos0 + i, which the cache holds
  * already (append first).  Arithmetic, weights and workspace as above (one
- * workspace may serve both). */
+ * workspace may serve both); with add_weights it holds a sum per row and block
+ * too, of as many tokens at a time as fit in 256 MB. */
 size_t oxb_attn_prefill_kv8_ws_bytes(int n_tok, int pos0, int H, int Hkv, int hd, int add_weights);
 int oxb_attn_prefill_kv8(const float *q, void *cache, int fmt, int n_tok, int pos0, int H, int Hkv,
                          int hd, int max_seq, int add_weights, float *out, void *ws,

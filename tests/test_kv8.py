@@ -179,3 +179,26 @@ def test_prefill_workspace_with_weights_stays_bounded():
     assert b(101, 0, 20, 5, 128, 1) - b(101, 0, 20, 5, 128, 0) == (20 * 101 * 4 + 255) // 256 * 256 + 5 * 4 * 512 * 8
     for n, pos0, H, hkv in ((8192, 0, 20, 5), (100000, 0, 20, 5), (600, 261000, 8, 1), (1, (1 << 24) - 1, 64, 1)):
         assert b(n, pos0, H, hkv, 128, 1) <= b(n, pos0, H, hkv, 128, 0) + (600 << 20), (n, pos0)
+
+
+def test_python_arguments_of_other_shapes_are_refused():
+    """Before anything is uploaded: the kernels take the arrays' sizes on trust."""
+    c = ops.Kv8Cache.__new__(ops.Kv8Cache)
+    c.batch, c.Hkv, c.max_seq, c.fmt, c.hd, c.stride = 2, 2, 64, ops.KV8_INT8, 128, 0
+    d = ops.Kv8Cache.__new__(ops.Kv8Cache)
+    d.batch, d.Hkv, d.max_seq, d.fmt, d.hd, d.stride = 2, 2, 64, ops.KV8_E4M3, 128, 0
+    kv = np.zeros((2, 2, 3, 128), np.float16)
+    q = np.zeros((2, 512), np.float32)
+    x = np.zeros((2, 70), np.float32)
+    for call in (lambda: c.append(kv[:1], kv, [0, 0]), lambda: c.append(kv, kv[:, :, :2], [0, 0]),
+                 lambda: c.append(kv[..., :64], kv[..., :64], [0, 0]), lambda: c.append(kv, kv, [0]),
+                 lambda: c.append(kv, kv, [0, 0], [1]), lambda: c.read([0], 3), lambda: c.read([0, 0], 3, [4]),
+                 lambda: c.attn_decode(q, [5]), lambda: c.attn_decode(q[:, :200], [5, 5]),
+                 lambda: c.attn_decode(q[:, :384], [5, 5]), lambda: c.attn_prefill(q, 0, slot=2),
+                 lambda: c.attn_prefill(q[:, :100], 0), lambda: c.evict([1], 2), lambda: c.evict([1, 1], 2, dst=d),
+                 lambda: ops.logits_rules(x, history=[[1]]), lambda: ops.logits_rules(x, bias=[[(1, 0.5)]]),
+                 lambda: ops.logits_rules(x, mask=np.zeros((2, 2), np.uint32)),
+                 lambda: ops.logits_rules(x, mask=np.zeros((1, 3), np.uint32)),
+                 lambda: ops.logits_rules(x, penalties=np.ones((1, 3)))):
+        with pytest.raises(ValueError):
+            call()
