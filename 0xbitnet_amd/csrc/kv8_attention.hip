@@ -94,7 +94,7 @@ __device__ __forceinline__ int kv8_row_exp(float a) {
 //   own eight p' -- no exchange between lanes.
 // Bound by the cache's bytes; a wave keeps its next block's 8 KB in flight
 // under the current one's arithmetic (32 sequences of up to 2304 positions, H 20
-// over 5, with weights: 22.6 us; 33.4 without, 25.0 with two ahead).  A
+// over 5, with weights: 22.2 us; 33.4 without, 25.0 with two ahead).  A
 // sequence's runs meet in the workspace: each stores its part and counts in,
 // and the last one joins them in order, so the sum does not depend on which is
 // last.  Those 32 read 73 MB, 3.2 TB/s, of which about 8 us are no bytes' time:
@@ -111,7 +111,7 @@ struct Kv8DecodeArgs {
     uint8_t *cache;
     size_t stride;
     const int *pos;
-    int pos_stride, H, Hkv, G, max_seq, nb, splits;
+    int pos_stride, H, Hkv, G, max_seq, nb, splits, many, least;
     float *out;
     int *cnt;        // [batch * Hkv] zero between calls
     uint64_t *ml;    // [batch][H][splits] reference and sum (two floats)
@@ -163,7 +163,7 @@ __global__ __launch_bounds__(kDecThreads) void kv8_decode_kernel(Kv8DecodeArgs a
     __shared__ int s_last;
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int z = blockIdx.z, kvh = blockIdx.y, split = blockIdx.x;
+    const int kvh = blockIdx.x, z = a.many ? blockIdx.y : blockIdx.z, split = a.many ? blockIdx.z : blockIdx.y;
     const int orow = tid >> 5, od = (tid & 31) * 4;         // the row and dims a thread joins
     auto load_q = [&](int hc) {
         float4 v = make_float4(0, 0, 0, 0);
@@ -173,8 +173,9 @@ __global__ __launch_bounds__(kDecThreads) void kv8_decode_kernel(Kv8DecodeArgs a
     float4 qv = load_q(0);   // with pos, before the cache's loads: loads return in order
     const int64_t p1 = (int64_t)a.pos[(size_t)z * a.pos_stride] + 1;
     const int len = (int)(p1 < 0 ? 0 : p1 > a.max_seq ? a.max_seq : p1), nblk = kv8_blocks(len);
-    // blocks of a run: an even share, at least one per wave
-    const int per = max(kDecWaves, (nblk + a.splits - 1) / a.splits), runs = (nblk + per - 1) / per;
+    // blocks of a run: an even share of `least` or more, or all of a short sequence
+    const int share = max(a.least, (nblk + a.splits - 1) / a.splits);
+    const int per = nblk <= 2 * a.least ? max(nblk, 1) : share, runs = (nblk + per - 1) / per;
     const int b0 = split * per, b1 = min(nblk, b0 + per);
     if (b0 >= b1) {
         if (split == 0)
@@ -445,7 +446,7 @@ __global__ __launch_bounds__(kDecThreads) void kv8_decode_kernel(Kv8DecodeArgs a
 }
 
 // Runs per KV head and sequence: two workgroups per CU over the launch (what
-// the registers let reside; the 32 sequences above: 22.6 us, with one per CU
+// the registers let reside; the 32 sequences above: 22.2 us, with one per CU
 // 28.6, with four 28.4), none with fewer blocks than waves.
 static int decode_splits(int batch, int Hkv, int nb) {
     const int64_t rows = (int64_t)batch * Hkv, most = (nb + kDecWaves - 1) / kDecWaves;
@@ -453,6 +454,17 @@ static int decode_splits(int batch, int Hkv, int nb) {
     if (s > most) s = most;
     return (int)(s < 1 || rows > kArrivals ? 1 : s);
 }
+
+// Many rows (sequence and KV head) fill a good part of the CUs by themselves.  Then
+// a run has 8 blocks at least (else 4), and twice as many are not cut: the
+// hand-over and the join take 3-5 us, a workgroup's next four blocks 1.  H 20
+// over 5, with runs of 4 and of 8: 8 sequences of up to 600 positions 8.2, 8.9
+// us; 16 of 640 9.4, 8.7; 32 of 512 11.2, 8.2.  And a sequence's second runs,
+// which it may not have, are started after all first ones, so that those are on
+// all XCDs alike (16 of 640: 8.7 against 10.9 with a sequence's runs side by
+// side); of few rows each has its runs side by side (4 of 100001: 75 us against
+// 82 the other way).
+static bool decode_many(int batch, int Hkv) { return (int64_t)batch * Hkv >= 64; }
 
 struct DecodeWs {
     size_t ml, o, bw, bytes;
@@ -1096,11 +1108,12 @@ extern "C" int oxb_attn_decode_kv8(const float *q, void *cache, size_t cache_str
     OXB_REQUIRE(ws && ((uintptr_t)ws & 255) == 0 && ws_bytes >= w.bytes,
                 "attention: workspace is NULL, not 256-byte aligned or %zu bytes < %zu", ws_bytes, w.bytes);
     char *wp = (char *)ws;
+    const bool many = decode_many(batch, Hkv);
     const Kv8DecodeArgs a{q, (uint8_t *)cache, cache_stride, pos, pos_stride, H, Hkv, H / Hkv, max_seq, nb,
-                          decode_splits(batch, Hkv, nb), out, (int *)wp, (uint64_t *)(wp + w.ml),
-                          (uint64_t *)(wp + w.o), (uint64_t *)(wp + w.bw)};
+                          decode_splits(batch, Hkv, nb), many, many ? 2 * kDecWaves : kDecWaves, out,
+                          (int *)wp, (uint64_t *)(wp + w.ml), (uint64_t *)(wp + w.o), (uint64_t *)(wp + w.bw)};
     hipStream_t s = (hipStream_t)stream;
-    const dim3 grid(a.splits, Hkv, batch), th(kDecThreads);
+    const dim3 grid(Hkv, a.many ? batch : a.splits, a.many ? a.splits : batch), th(kDecThreads);
     if (fmt == OXB_KV8_INT8) {
         if (add_weights)
             hipLaunchKernelGGL((kv8_decode_kernel<OXB_KV8_INT8, true>), grid, th, 0, s, a);

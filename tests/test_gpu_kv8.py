@@ -228,6 +228,27 @@ def test_decode_long_many_splits(fmt):
         check_rows(c.weights()[z, :, :(m + 31) // 32], w[:, :(m + 31) // 32], wtol[:, :(m + 31) // 32], z)
 
 
+@pytest.mark.parametrize("batch,H,hkv", [(13, 10, 5), (12, 10, 5), (3, 64, 32), (40, 5, 5)])
+def test_decode_rows_of_many_lengths(batch, H, hkv):
+    """Around 64 rows (sequence and KV head) the runs' least length changes: sequences
+    of one run, of several and of none side by side, with their weights."""
+    fmt = batch % 2
+    rng = rng_of("lengths", batch, H)
+    lens = [0, 1, 127, 128, 129, 255, 256, 257, 300, 511, 512, 513, 700]
+    lens = (lens * 4)[:batch] if batch > 3 else [513, 0, 257]
+    c, K, V = filled(rng, lens, hkv, 700, fmt)
+    q = rng.standard_normal((batch, H * HD)).astype(np.float32)
+    got = c.attn_decode(q, [n - 1 for n in lens], True)
+    for z, n in enumerate(lens):
+        if n == 0:
+            assert not got[z].any()
+            continue
+        want, tol, w, wtol = ref.attend_rows(q[z:z + 1], K[z], V[z], hkv, n - 1)
+        check_rows(got[z:z + 1], want, tol, z)
+        nb = (n + 31) // 32
+        check_rows(c.weights()[z, :, :nb], w[:, :nb], wtol[:, :nb], z)
+
+
 @pytest.mark.parametrize("fmt", FMTS)
 @pytest.mark.parametrize("qscale", [1e-30, 1e-3, 40.0, 3e4])
 def test_decode_scales_of_q(fmt, qscale):
