@@ -744,6 +744,51 @@ def test_captured_step_replays():
     ops.check(L.oxb_stream_destroy(st))
 
 
+def test_captured_prefill_evict_and_rules():
+    """A prompt's attention in several runs with weights, a cut into another cache and
+    logit rules in one graph, replayed with new inputs and eager work between."""
+    L, rng = ops.lib(), rng_of("graph2")
+    hkv, H, n, pos0, fmt, V = 2, 8, 150, 900, 1, 5003
+    total = n + pos0
+    st = L.oxb_stream_create()
+    c, K, Vv = filled(rng, [total], hkv, total, fmt)
+    e, d, ed = new_cache(1, hkv, total, fmt), new_cache(1, hkv, 10 * 32, fmt), new_cache(1, hkv, 10 * 32, fmt)
+    start = c.data.download()
+    dq, out = (ops.DeviceArray((n, H * HD), np.float32) for _ in "qo")
+    dl, dn = ops.DeviceArray.from_host(np.array([total], np.int32)), ops.DeviceArray((1,), np.int32)
+    lg, ro = ops.DeviceArray((2, V), np.float32), ops.DeviceArray((2, V), np.float32)
+    pen = ops.DeviceArray.from_host(np.array([[1.2, 0.1, 0.3], [1, 0, 0.5]], np.float32))
+    hist, hoff = ops.DeviceArray((64,), np.int32), ops.DeviceArray.from_host(np.array([0, 40, 64], np.int32))
+    wsn = L.oxb_attn_prefill_kv8_ws_bytes(n, pos0, H, hkv, HD, 1)
+    evn = L.oxb_kv8_evict_ws_bytes(1, hkv, total, 10)
+    ws, ew = ops.DeviceArray((wsn,), np.uint8, zero=True), ops.DeviceArray((evn,), np.uint8)
+    ops.sync()
+    ops.check(L.oxb_stream_begin_capture(st))
+    ops.check(L.oxb_attn_prefill_kv8(dq.ptr, c.data.ptr, fmt, n, pos0, H, hkv, HD, total, 1, out.ptr, ws.ptr, wsn, st))
+    ops.check(L.oxb_kv8_evict(c.data.ptr, c.stride, total, d.data.ptr, d.stride, 320, dl.ptr, 1, dn.ptr, 1, 1, hkv, HD,
+                              10, 1, 2, ew.ptr, evn, st))
+    ops.check(L.oxb_logits_rules(lg.ptr, V, 2, V, pen.ptr, hist.ptr, hoff.ptr, 64, None, None, None, 0, None, 0,
+                                 ro.ptr, V, st))
+    g = L.oxb_stream_end_capture(st)
+    assert g
+    for step in range(4):
+        q = rng.standard_normal((n, H * HD)).astype(np.float32)
+        x, ids = rng.standard_normal((2, V)).astype(np.float32), rng.integers(0, 50, 64).astype(np.int32)
+        for a, b in ((c.data, start), (e.data, start), (dq, q), (lg, x), (hist, ids)):
+            a.upload(b)
+        ops.check(L.oxb_graph_launch(g, st))
+        ops.check(L.oxb_stream_sync(st))
+        assert np.array_equal(bits(out.download()), bits(e.attn_prefill(q, pos0, add_weights=True))), step
+        assert np.array_equal(bits(c.weights()), bits(e.weights()))
+        assert dn.download()[0] == e.evict([total], 10, 1, 2, ed)[0]
+        for a, b in zip(d.read([0], 320, dn.download()), ed.read([0], 320, dn.download())):
+            assert np.array_equal(bits(a), bits(b)), step
+        want = ops.logits_rules(x, [[1.2, 0.1, 0.3], [1, 0, 0.5]], [ids[:40], ids[40:]])
+        assert np.array_equal(bits(ro.download()), bits(want)), step
+    ops.check(L.oxb_graph_destroy(g))
+    ops.check(L.oxb_stream_destroy(st))
+
+
 def test_offsets_past_32_bits():
     """A cache of which the last head's blocks and the second sequence lie past 4 GB."""
     hkv, ms, B, n = 17, 1 << 20, 2, 70
