@@ -74,6 +74,12 @@ def rms_bound(q, k):
     return 2 * 16 * U * (S + 1)
 
 
+def check_rows(got, want, tol, what=""):
+    """Every value within its bound; a NaN on any side is within none."""
+    ok = np.abs(np.asarray(got, np.float64) - want) <= tol
+    assert ok.all(), (what, int((~ok).sum()), float(np.max(np.abs(got - want) / tol)))
+
+
 def attend_rows(q, K, V, Hkv, first):
     """Queries q [n][H*128] at positions first.. over one sequence's K, V
     [Hkv][S][128]: out, error bounds, block weights [Hkv][blocks], their bounds."""
