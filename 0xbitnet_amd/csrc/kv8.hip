@@ -17,6 +17,8 @@
 // in f16 beside the codes (the tail, 16 KB per KV head), and each append
 // quantizes the whole block again from them, so the cache depends on the rows
 // alone, not on how they were split over calls, and no value is rounded twice.
+// The tail keeps a completed block's rows too, until the next block's first ones
+// take their place: rows may be taken back within it.
 #include "kv8.h"
 #include "radix_select.h"
 
@@ -157,8 +159,8 @@ __global__ __launch_bounds__(kKvThreads) void kv8_append_kernel(Kv8AppendArgs a)
     // the last block's new rows join the tail, written by the workgroup that
     // has read the tail (of the first block), so that no other one reads it
     // while it changes
-    const int last = end / kKv8Block;
-    if (b == first && end % kKv8Block) {
+    const int last = (end - 1) / kKv8Block;
+    if (b == first) {
         __syncthreads();
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -380,7 +382,7 @@ __global__ __launch_bounds__(kKvThreads) void kv8_move_kernel(Kv8EvictArgs a) {
             if (j < kept && !(inplace && from[u] == j)) *(u32x4_t *)(dst + (size_t)j * kKv8Codes) = v[u];
         }
     }
-    if (!inplace) {   // the unfinished block's f16 rows, 16 KB over the columns
+    if (!inplace) {   // the newest block's f16 rows, 16 KB over the columns
         const Kv8Layout ls = kv8_layout(a.Hkv, a.nb), ld = kv8_layout(a.Hkv, a.dst_nb);
         const size_t t = (size_t)h * 2 * kKv8Half * 2 + (size_t)col * (16384 / kMvCols) + tid * 16;
         if (tid < 1024 / kMvCols) *(uint4 *)(dseq + ld.tails + t) = *(const uint4 *)(seq + ls.tails + t);

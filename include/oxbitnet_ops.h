@@ -295,8 +295,8 @@ int oxb_attn_prefill(const float *q, const uint16_t *kcache, const uint16_t *vca
  *   scales  [Hkv][nb][2] f32: K, V
  *   weights [Hkv][nb] f32: accumulated attention weight (see the attention
  *           calls), 0 when the block is begun
- *   tails   [Hkv][2][32][128] f16: the K and V rows of the unfinished block,
- *           from which the block is quantized again as it grows
+ *   tails   [Hkv][2][32][128] f16: the K and V rows of the newest block, from
+ *           which the block is quantized again as it grows
  * No counterpart in the reference (nn/attention.rs:23-48: f32 rows). */
 size_t oxb_kv8_bytes(int Hkv, int hd, int max_seq);
 
@@ -307,10 +307,12 @@ size_t oxb_kv8_bytes(int Hkv, int hd, int max_seq);
  * 16-byte aligned rows), r = i, or p + i with src_at_pos, which takes rows
  * where the q|k|v projections leave them (a f16 cache [Hkv][max_seq][128] that
  * all layers may share as scratch).  p is the position after the last one
- * appended, or less within that position's block (its later rows are dropped),
- * or the start of any block (a multiple of 32).  The cache's content depends on
- * the rows alone, not on how they were split over calls.  Positions past max_seq
- * are dropped; p < 0 skips the sequence. */
+ * appended, or any position of the last one's block (that block's later rows are
+ * dropped), or the start of any block (a multiple of 32).  Nothing checks this:
+ * the tail holds the newest block's rows only, and an append inside an earlier
+ * block quantizes that one from them.  The cache's content depends on the rows
+ * alone, not on how they were split over calls.  Positions past max_seq are
+ * dropped; p < 0 skips the sequence. */
 int oxb_kv8_append(void *cache, size_t cache_stride, int fmt, int batch, int Hkv, int hd,
                    int max_seq, const uint16_t *k, const uint16_t *v, size_t src_stride,
                    size_t src_head_stride, int src_at_pos, const int *pos, int pos_stride, int pos0,
