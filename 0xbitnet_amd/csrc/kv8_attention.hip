@@ -951,6 +951,12 @@ __global__ __launch_bounds__(256) void kv8_prefill_weights_kernel(Kv8PrefillArgs
             (red[0] + red[1]) + (red[2] + red[3]);
 }
 
+// Workgroups of a KV head that are resident at once, two per CU, as far as a plan
+// orders them; the least blocks of a run; bytes of a launch's sums of weights.
+static int prefill_slots(int Hkv) { return std::min(2 * device_cus() / Hkv, kPreOrder); }
+constexpr int kPreLeast = 8;
+constexpr int64_t kPreSums = 256 << 20;
+
 // The launch shapes of a prefill call and its workspace.
 struct PrefillPlan {
     int rows, rtiles, runs, splits, per;
@@ -962,11 +968,10 @@ static PrefillPlan prefill_plan(int n, int pos0, int H, int Hkv, bool weights) {
     const int G = H / Hkv, total = pos0 + n;
     p.rows = n * G;
     p.rtiles = (p.rows + kPreRows - 1) / kPreRows;
-    // Two workgroups per CU are resident, and a row tile's blocks may be cut into
-    // even runs of `per` at most: the least per, of eight at least, whose runs all
-    // are resident at once.  (2048 tokens: 56 us; 850 workgroups of the same
+    // A row tile's blocks may be cut into even runs of `per` at most: the least per,
+    // of kPreLeast at least, whose runs all are resident at once.  (2048 tokens: 56 us; 850 workgroups of the same
     // work in two rounds 69, as beginning and ending a run takes about 9 us.)
-    const int slots = std::min(2 * device_cus() / Hkv, kPreOrder), most = kv8_blocks(total);
+    const int slots = prefill_slots(Hkv), most = kv8_blocks(total);
     auto count = [&](int per) {
         int64_t n = 0;
         for (int r = 0; r < p.rtiles; ++r) {
@@ -975,7 +980,7 @@ static PrefillPlan prefill_plan(int n, int pos0, int H, int Hkv, bool weights) {
         }
         return n;
     };
-    int lo = 8, hi = most;   // runs of `most` blocks are no cut at all
+    int lo = kPreLeast, hi = most;   // runs of `most` blocks are no cut at all
     if (p.rtiles > slots) lo = hi;
     while (lo < hi) {
         const int mid = lo + (hi - lo) / 2;
@@ -1006,11 +1011,11 @@ static PrefillPlan prefill_plan(int n, int pos0, int H, int Hkv, bool weights) {
 }
 
 // Tokens of a launch: all, but with weights, whose sums take 8 bytes per row and
-// block, as many as keep those under 256 MB.
+// block, as many as keep those under kPreSums.
 static int prefill_step(int n, int pos0, int H, int Hkv, bool weights) {
     if (!weights) return n;
     const int64_t token = (int64_t)8 * H * kv8_blocks(pos0 + n);
-    const int64_t most = std::max<int64_t>(1, (256 << 20) / token), calls = (n + most - 1) / most;
+    const int64_t most = std::max<int64_t>(1, kPreSums / token), calls = (n + most - 1) / most;
     return (int)((n + calls - 1) / calls);
 }
 
@@ -1034,18 +1039,36 @@ static void prefill_order(const PrefillPlan &p, int pos0, int G, int Hkv, Kv8Pre
     for (int i = 0; i < n; ++i) o.run[i] = run[i].id;
 }
 
+// What prefill_plan asks for at most over all calls of up to n tokens that end at
+// pos0 + n or before, so that a workspace of the largest call serves every smaller one.
+// Parts: a cut launch has at most `slots` runs, of eight blocks at least, and a row
+// tile that sees more blocks than another has no fewer of them.  With T tokens
+// visible to the last row and r tiles, the tiles' blocks add up to r T / 64 or more,
+// so r T / (32 per) <= 2 slots, and splits r < 2 slots + r <= 3 slots.
+// Sums of the weights: a launch's stay under 256 MB (or are one token's), but for the
+// last tile's rounding to kPreRows rows.
 static size_t prefill_bytes(int n, int pos0, int H, int Hkv, bool weights) {
-    const int step = prefill_step(n, pos0, H, Hkv, weights);
-    size_t b = 0;
-    for (int i = 0; i < n; i += step)
-        b = std::max(b, prefill_plan(std::min(step, n - i), pos0 + i, H, Hkv, weights).bytes);
-    return b;
+    const int64_t rows = (int64_t)n * (H / Hkv), most = kv8_blocks(pos0 + n), slots = prefill_slots(Hkv);
+    size_t at = kArrivals * 4;
+    if (most > kPreLeast && slots > 1) {
+        const int64_t uncut = std::min<int64_t>(rows, slots * kPreRows);
+        const size_t parts = Hkv * std::min((most + kPreLeast - 1) / kPreLeast * uncut, 3 * slots * kPreRows);
+        at += kv8_align(parts * 8) + kv8_align(parts * kKv8Hd * 4);
+    }
+    if (weights) {
+        const int64_t pad = (rows + kPreRows - 1) / kPreRows * kPreRows, token = 8 * H * most;
+        const int64_t launch = std::max<int64_t>(kPreSums, token) + 8 * (kPreRows - 1) * Hkv * most;
+        at += kv8_align((size_t)Hkv * rows * 4) + kv8_align(std::min(8 * Hkv * most * pad, launch));
+    }
+    return at;
 }
 
 // Tokens pos0 .. pos0 + n - 1 of a call.
 static int prefill_launch(const float *q, void *cache, int fmt, int n, int pos0, int H, int Hkv,
-                          int max_seq, bool weights, float *out, char *w, hipStream_t s) {
+                          int max_seq, bool weights, float *out, char *w, size_t ws_bytes, hipStream_t s) {
     const PrefillPlan p = prefill_plan(n, pos0, H, Hkv, weights);
+    OXB_REQUIRE(p.bytes <= ws_bytes, "prefill attention: a launch of %zu bytes of workspace, %zu there", p.bytes,
+                ws_bytes);
     OXB_REQUIRE(p.wgs < (1 << 24), "prefill attention: %d tokens of %d heads", n, H);
     const int nblk = kv8_blocks(pos0 + n);
     const Kv8PrefillArgs a{q, (uint8_t *)cache, n, pos0, H, Hkv, H / Hkv, kv8_blocks(max_seq), p.rows, p.rtiles,
@@ -1153,7 +1176,7 @@ extern "C" int oxb_attn_prefill_kv8(const float *q, void *cache, int fmt, int n_
     const int step = prefill_step(n_tok, pos0, H, Hkv, add_weights != 0);
     for (int i = 0; i < n_tok; i += step)
         if (prefill_launch(q + (size_t)i * H * hd, cache, fmt, std::min(step, n_tok - i), pos0 + i, H, Hkv,
-                           max_seq, add_weights != 0, out + (size_t)i * H * hd, (char *)ws, (hipStream_t)stream))
+                           max_seq, add_weights != 0, out + (size_t)i * H * hd, (char *)ws, ws_bytes, (hipStream_t)stream))
             return -1;
     return 0;
 }

@@ -349,7 +349,9 @@ int oxb_attn_decode_kv8(const float *q, void *cache, size_t cache_stride, int fm
  * [n_tok][H*128]) attends over positions 0..pos0 + i, which the cache holds
  * already (append first).  Arithmetic, weights and workspace as above (one
  * workspace may serve both); with add_weights it holds a sum per row and block
- * too, of as many tokens at a time as fit in 256 MB. */
+ * too, of as many tokens at a time as fit in 256 MB.  The workspace's size grows
+ * with n_tok, pos0 and add_weights: one for (n, p) serves every call of up to n
+ * tokens that ends at position n + p or before. */
 size_t oxb_attn_prefill_kv8_ws_bytes(int n_tok, int pos0, int H, int Hkv, int hd, int add_weights);
 int oxb_attn_prefill_kv8(const float *q, void *cache, int fmt, int n_tok, int pos0, int H, int Hkv,
                          int hd, int max_seq, int add_weights, float *out, void *ws,
