@@ -466,11 +466,15 @@ static int decode_splits(int batch, int Hkv, int nb) {
 // 82 the other way).
 static bool decode_many(int batch, int Hkv) { return (int64_t)batch * Hkv >= 64; }
 
+// Parts are as many as a batch of up to this size leaves at most, whatever its own
+// cut: fewer sequences have more runs each (51 of 5 KV heads two, 52 one), and a
+// workspace of the largest batch serves every smaller one.
 struct DecodeWs {
     size_t ml, o, bw, bytes;
 };
 static DecodeWs decode_ws(int batch, int H, int Hkv, int nb) {
-    const size_t parts = (size_t)batch * H * decode_splits(batch, Hkv, nb);
+    const int64_t rows = (int64_t)batch * Hkv, most = (nb + kDecWaves - 1) / kDecWaves;
+    const size_t parts = H / Hkv * std::max(rows, std::min<int64_t>(2 * device_cus(), rows * most));
     DecodeWs w;
     w.ml = kArrivals * 4;
     w.o = w.ml + kv8_align(parts * 8);

@@ -74,3 +74,25 @@ def test_prefill_workspace_of_the_largest_call_serves_all(H, hkv, weights):
             assert size(m, p, H, hkv, 128, weights) <= big, (n, pos0, m, p)
             assert prefill_need(m, p, H, hkv, weights) <= size(m, p, H, hkv, 128, weights), (m, p)
             assert size(m, p, H, hkv, 128, 0) <= big
+
+
+def decode_need(batch, H, hkv, max_seq, cus=256):
+    """What a decode call lays out: two workgroups per CU over the rows (sequence and KV
+    head) as runs, each of four blocks or more; past 1024 rows no cuts."""
+    nb, rows, al = -(-max_seq // 32), batch * hkv, lambda b: -(-b // 256) * 256
+    splits = 1 if rows > 1024 else max(1, min(2 * cus // rows, -(-nb // 4)))
+    return 4096 + al(batch * H * splits * 8) + al(batch * H * splits * 512) + al(batch * H * nb * 8)
+
+
+@pytest.mark.parametrize("H,hkv", HEADS)
+def test_decode_workspace_of_the_largest_batch_serves_all(H, hkv):
+    """52 sequences of 5 KV heads have one run each, 51 have two: a workspace for the
+    larger batch and longer cache holds the smaller ones'."""
+    size = L().oxb_attn_decode_kv8_ws_bytes
+    for batch, max_seq in ((1, 1), (52, 2304), (64, 4096), (33, 700), (205, 130), (300, 40), (1025, 500)):
+        big = size(batch, H, hkv, 128, max_seq)
+        for b in sorted({1, 2, 3, 51, 52, 102, batch // 2 + 1, batch - 1, batch}):
+            for ms in {1, 33, 129, 700, max_seq - 1, max_seq}:
+                if 1 <= b <= batch and 1 <= ms <= max_seq:
+                    n = size(b, H, hkv, 128, ms)
+                    assert decode_need(b, H, hkv, ms) <= n <= big, (batch, max_seq, b, ms)
