@@ -41,15 +41,16 @@ __global__ __launch_bounds__(kLrThreads) void logit_rules_kernel(RulesArgs a) {
     __shared__ int last[kLrChunk];   // 1 + the last bias entry of the id
     const int r = blockIdx.y, base = blockIdx.x * kLrChunk, tid = threadIdx.x;
     const int n = min(kLrChunk, a.V - base);
-    // ranges of this row, kept inside the lists whatever the offsets say
-    int h0 = 0, h1 = 0, b0 = 0, b1 = 0;
+    // ranges of this row, kept inside the lists whatever the offsets say; unsigned, as
+    // a thread's places run past the end of a list, which may be 2^31 - 1 long
+    uint32_t h0 = 0, h1 = 0, b0 = 0, b1 = 0;
     if (a.pen && a.n_hist > 0) {
         h0 = min(max(a.hist_off[r], 0), a.n_hist);
-        h1 = min(a.hist_off[r + 1], a.n_hist);
+        h1 = min(max(a.hist_off[r + 1], 0), a.n_hist);
     }
     if (a.n_bias > 0) {
         b0 = min(max(a.bias_off[r], 0), a.n_bias);
-        b1 = min(a.bias_off[r + 1], a.n_bias);
+        b1 = min(max(a.bias_off[r + 1], 0), a.n_bias);
     }
     const bool lists = h0 < h1 || b0 < b1;   // uniform
     // The lists' first ids are asked for before the logits: loads return in
@@ -57,7 +58,7 @@ __global__ __launch_bounds__(kLrThreads) void logit_rules_kernel(RulesArgs a) {
     int id[kLrPer], bid = -1;
 #pragma unroll
     for (int u = 0; u < kLrPer; ++u) {
-        const int j = h0 + tid + u * kLrThreads;
+        const uint32_t j = h0 + tid + u * kLrThreads;
         id[u] = j < h1 ? a.hist[j] : -1;
     }
     if (b0 + tid < b1) bid = a.bias_ids[b0 + tid];
@@ -88,15 +89,15 @@ __global__ __launch_bounds__(kLrThreads) void logit_rules_kernel(RulesArgs a) {
             const unsigned i = (unsigned)v - (unsigned)base;
             if (i < (unsigned)n) atomicAdd(&cnt[i], 1);
         };
-        auto entry = [&](int v, int j) {
+        auto entry = [&](int v, uint32_t j) {
             const unsigned i = (unsigned)v - (unsigned)base;
-            if (i < (unsigned)n) atomicMax(&last[i], j + 1);
+            if (i < (unsigned)n) atomicMax(&last[i], (int)j + 1);
         };
 #pragma unroll
         for (int u = 0; u < kLrPer; ++u) count(id[u]);
-        for (int j = h0 + kLrPer * kLrThreads + tid; j < h1; j += kLrThreads) count(a.hist[j]);
+        for (uint32_t j = h0 + kLrPer * kLrThreads + tid; j < h1; j += kLrThreads) count(a.hist[j]);
         entry(bid, b0 + tid);
-        for (int j = b0 + kLrThreads + tid; j < b1; j += kLrThreads) entry(a.bias_ids[j], j);
+        for (uint32_t j = b0 + kLrThreads + tid; j < b1; j += kLrThreads) entry(a.bias_ids[j], j);
         lds_barrier();
     }
     float *out = a.out + (size_t)r * a.out_stride + base;
