@@ -521,9 +521,21 @@ struct Kv8PrefillArgs {
     float *out;
     float2 *ml;     // [splits][Hkv][rows] a row's reference and sum
     float *o;       // [splits][Hkv][rows][128]
-    float *lse;     // [Hkv][rows] log2 of the row's softmax sum, or NULL: no weights
+    float *rsum;    // [Hkv][rows] 1 / the row's softmax sum, or NULL: no weights
     float2 *bw;     // [Hkv][nblk][rtiles * 128] a block's sum of p' in a row, its reference
 };
+
+// A row's final reference and softmax sum, for its blocks' weights: the sum's
+// reciprocal, and the reference in the pair of the row's first block, whose own sum
+// is brought to it.  (One f32 logarithm of both in their place has steps of 2^-20
+// from 16 on, and the instruction's error leans to one side: the weights of 333
+// tokens behind 20011 were 5.9e-7 from the 64-bit ones; this way 6e-8, as f32
+// torch, in the same time.)
+__device__ __forceinline__ void kv8_row_total(const Kv8PrefillArgs &a, int kvh, int row, float M, float l) {
+    a.rsum[(size_t)kvh * a.rows + row] = 1.0f / l;
+    float2 *p = a.bw + (size_t)kvh * a.nblk * a.rtiles * kPreRows + row;
+    *p = make_float2(p->x * __builtin_amdgcn_exp2f(p->y - M), M);
+}
 
 // A row tile's blocks in even runs.
 __host__ __device__ inline int pre_run_start(int blocks, int runs, int i) {
@@ -857,7 +869,7 @@ __global__ __launch_bounds__(kPreThreads, 2) void kv8_prefill_kernel(Kv8PrefillA
     if (direct) {
         dst = a.out + ((size_t)(erow / a.G) * a.H + kvh * a.G + erow % a.G) * kKv8Hd;
         f /= lsum;
-        if (WEIGHTS && eh == 0) a.lse[(size_t)kvh * a.rows + erow] = M + __builtin_amdgcn_logf(lsum);
+        if (WEIGHTS && eh == 0) kv8_row_total(a, kvh, erow, M, lsum);
     } else {
         const size_t part = ((size_t)split * a.Hkv + kvh) * a.rows + erow;
         dst = a.o + part * kKv8Hd;
@@ -918,7 +930,7 @@ __global__ __launch_bounds__(256) void kv8_prefill_join_kernel(Kv8PrefillArgs a)
     }
     *(float4 *)(a.out + ((size_t)tok * a.H + head) * kKv8Hd + d) =
         make_float4(t.x / lt, t.y / lt, t.z / lt, t.w / lt);
-    if (a.lse && d == 0) a.lse[r] = M + __builtin_amdgcn_logf(lt);
+    if (a.rsum && d == 0) kv8_row_total(a, kvh, row, M, lt);
 }
 
 // A block's weight: its sums of p' over the rows that see it, which the
@@ -931,21 +943,23 @@ __global__ __launch_bounds__(256) void kv8_prefill_weights_kernel(Kv8PrefillArgs
     const int b = blockIdx.x, kvh = blockIdx.y, tid = threadIdx.x;
     const int first = max(0, b * kKv8Block - a.pos0) * a.G;
     const float2 *bw = a.bw + ((size_t)kvh * a.nblk + b) * a.rtiles * kPreRows;
-    const float *lse = a.lse + (size_t)kvh * a.rows;
+    const float2 *total = a.bw + (size_t)kvh * a.nblk * a.rtiles * kPreRows;   // the first block's: .y
+    const float *rsum = a.rsum + (size_t)kvh * a.rows;
     float s = 0.0f;
     constexpr int kB = 4;   // rows in flight
     for (int r0 = first + tid; r0 < a.rows; r0 += kB * 256) {
         float2 p[kB];
-        float x[kB];
+        float m[kB], f[kB];
 #pragma unroll
         for (int i = 0; i < kB; ++i) {
             const int r = min(r0 + i * 256, a.rows - 1);
             p[i] = bw[r];
-            x[i] = lse[r];
+            m[i] = total[r].y;
+            f[i] = rsum[r];
         }
 #pragma unroll
         for (int i = 0; i < kB; ++i)
-            if (r0 + i * 256 < a.rows) s += p[i].x * __builtin_amdgcn_exp2f(p[i].y - x[i]);
+            if (r0 + i * 256 < a.rows) s += p[i].x * __builtin_amdgcn_exp2f(p[i].y - m[i]) * f[i];
     }
     s = wave_sum(s);
     if ((tid & 63) == 0) red[tid >> 6] = s;
@@ -965,7 +979,7 @@ constexpr int64_t kPreSums = 256 << 20;
 struct PrefillPlan {
     int rows, rtiles, runs, splits, per;
     int64_t wgs;
-    size_t ml, o, lse, bw, bytes;
+    size_t ml, o, rsum, bw, bytes;
 };
 static PrefillPlan prefill_plan(int n, int pos0, int H, int Hkv, bool weights) {
     PrefillPlan p{};
@@ -1007,7 +1021,7 @@ static PrefillPlan prefill_plan(int n, int pos0, int H, int Hkv, bool weights) {
         p.o = take(parts * kKv8Hd * 4);
     }
     if (weights) {
-        p.lse = take((size_t)Hkv * p.rows * 4);
+        p.rsum = take((size_t)Hkv * p.rows * 4);
         p.bw = take((size_t)Hkv * most * p.rtiles * kPreRows * 8);
     }
     p.bytes = at;
@@ -1077,7 +1091,7 @@ static int prefill_launch(const float *q, void *cache, int fmt, int n, int pos0,
     const int nblk = kv8_blocks(pos0 + n);
     const Kv8PrefillArgs a{q, (uint8_t *)cache, n, pos0, H, Hkv, H / Hkv, kv8_blocks(max_seq), p.rows, p.rtiles,
                            p.rtiles <= kPreOrder, p.per, nblk, out, (float2 *)(w + p.ml), (float *)(w + p.o),
-                           weights ? (float *)(w + p.lse) : nullptr, (float2 *)(w + p.bw)};
+                           weights ? (float *)(w + p.rsum) : nullptr, (float2 *)(w + p.bw)};
     const dim3 grid((unsigned)p.wgs), th(kPreThreads);
     Kv8PrefillOrder order;
     if (a.planned) prefill_order(p, pos0, a.G, Hkv, order);
