@@ -537,7 +537,13 @@ __device__ __forceinline__ void kv8_row_total(const Kv8PrefillArgs &a, int kvh, 
     *p = make_float2(p->x * __builtin_amdgcn_exp2f(p->y - M), M);
 }
 
-// A row tile's blocks in even runs.
+// A row tile's blocks in even runs, of `per` blocks at most and cut as few times as
+// that takes: the last of k + 1 has (k per + 1) / (k + 1) blocks or more, (per + 1) / 2
+// at least, rounded up.  The tile's rows end in at most kPreRows / 32 + 1 blocks, so
+// with runs of kPreLeast or more each row sees some position of each run, and its
+// reference is a score's.
+constexpr int kPreLeast = 8;
+static_assert((kPreLeast + 2) / 2 >= kPreRows / kKv8Block + 1, "a row sees nothing of its tile's last run");
 __host__ __device__ inline int pre_run_start(int blocks, int runs, int i) {
     return (int)((int64_t)blocks * i / runs);
 }
@@ -862,8 +868,7 @@ __global__ __launch_bounds__(kPreThreads, 2) void kv8_prefill_kernel(Kv8PrefillA
     // the lane's row again (not held in registers over the loop)
     const int elane = lane + opaque_zero(), eh = elane >> 5, erow = r0 + wave * 32 + (elane & 31);
     if (erow >= a.rows) return;
-    // (a wave may see nothing of a run that others see)
-    const float M = b0 * kKv8Block < wseen ? ref.off() - kPreBase : -__builtin_inff();
+    const float M = ref.off() - kPreBase;
     const bool direct = runs == 1;
     float *dst, f = 1.0f / ref.r;          // o in l's units
     if (direct) {
@@ -970,9 +975,8 @@ __global__ __launch_bounds__(256) void kv8_prefill_weights_kernel(Kv8PrefillArgs
 }
 
 // Workgroups of a KV head that are resident at once, two per CU, as far as a plan
-// orders them; the least blocks of a run; bytes of a launch's sums of weights.
+// orders them; bytes of a launch's sums of weights.
 static int prefill_slots(int Hkv) { return std::min(2 * device_cus() / Hkv, kPreOrder); }
-constexpr int kPreLeast = 8;
 constexpr int64_t kPreSums = 256 << 20;
 
 // The launch shapes of a prefill call and its workspace.
