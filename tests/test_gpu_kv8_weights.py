@@ -41,3 +41,15 @@ def test_prefill_weights_of_even_rows(fmt, n, pos0, G):
     rows = n * G
     adds = (rows + 255) // 256 + 9 if rows > 1 else 0
     ref.check_rows(c.weights()[0, 0, :nb], want, (2 + adds) * ref.U * want, (n, pos0))
+
+
+def test_prefill_weights_of_more_tiles_than_a_plan_orders():
+    """525 row tiles in one launch with weights: keys of 0, as above."""
+    n, G = 4200, 16
+    c = new_cache(1, 1, n, 0)
+    c.append(np.zeros((1, 1, n, HD), np.float16), np.ones((1, 1, n, HD), np.float16), [0])
+    out = c.attn_prefill(rng_of("tiles").standard_normal((n, G * HD)).astype(np.float32), 0, add_weights=True)
+    want = even(n, 0, G, (n + 31) // 32)
+    ref.check_rows(c.weights()[0, 0], want, (2 + (n * G + 255) // 256 + 9) * ref.U * want)
+    # values of 1: 127 times the f32 nearest 1 / 127, within 2 u of it; attend()'s bound at S = 0
+    ref.check_rows(out, np.ones(out.shape), np.full(out.shape, (2 + 16 + n / 32 + 64 + 4) * ref.U))
