@@ -62,7 +62,9 @@ __device__ inline void kv8_span(const Kv8AppendArgs &a, int z, int &p0, int &cnt
 // off by 2^-24 of itself at most and exact where the quotient is an f32 number,
 // ties among them: the same codes as the f32 division's, in a third of its
 // instructions.  One row: 3.8 us.  Four prompts of up to 2048 rows, 5 heads (16 MB
-// in, 8 out): 9.1 us, 2.7 TB/s; 13.9 with divisions and V's bytes stored one by one.
+// in, 8 out): 8.5-9.1 us, 2.7-2.9 TB/s; 13.9 with divisions and V's bytes stored one
+// by one.  Short of the copy's rate as nothing of another block is in flight while a
+// workgroup waits for its rows, their maximum and its two barriers.
 template <int FMT>
 __global__ __launch_bounds__(kKvThreads) void kv8_append_kernel(Kv8AppendArgs a) {
     __shared__ uint32_t vt[kKv8Hd * 9];   // V codes, [dim][9 dwords]: 8, and one against bank conflicts
@@ -348,8 +350,9 @@ __global__ __launch_bounds__(kEvThreads) void kv8_select_kernel(Kv8EvictArgs a) 
 // A workgroup moves a 256-byte column of a head's kept blocks, 16 blocks a pass
 // and 4 passes in flight.  Bound by the codes' bytes, and by the list's and the
 // codes' loads one behind the other: 32 sequences of 5 heads and 32 kept blocks
-// (89 MB in all) 22.8 us, 3.9 TB/s; with 1 KB columns in a quarter of the
-// workgroups 24.0.
+// (89 MB in all) 22.7 us, 3.9 TB/s; with 1 KB columns in a quarter of the
+// workgroups 24.0.  The same cut in place, behind a copy that has left the codes in
+// the caches: 13.5 us, and the blocks that stay where they are not written.
 constexpr int kMvCols = 32;
 constexpr int kMvLanes = kKv8Codes / kMvCols / 16;   // 16-byte lanes of a column
 constexpr int kMvRows = kKvThreads / kMvLanes;       // blocks per pass

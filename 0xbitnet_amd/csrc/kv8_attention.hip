@@ -94,12 +94,12 @@ __device__ __forceinline__ int kv8_row_exp(float a) {
 //   own eight p' -- no exchange between lanes.
 // Bound by the cache's bytes; a wave keeps its next block's 8 KB in flight
 // under the current one's arithmetic (32 sequences of up to 2304 positions, H 20
-// over 5, with weights: 22.2 us; 33.4 without, 25.0 with two ahead).  A
+// over 5, with weights: 22.2 us; 33.4 with no block in flight, 25.0 with two).  A
 // sequence's runs meet in the workspace: each stores its part and counts in,
 // and the last one joins them in order, so the sum does not depend on which is
 // last.  Those 32 read 73 MB, 3.2 TB/s, of which about 8 us are no bytes' time:
 // the position, the first block, the hand-over, the join (one sequence of 2304
-// alone: 8.6 us).  Four sequences of up to 100001: 77 us, 415 MB, 5.4 TB/s.
+// alone: 8.9 us).  Four sequences of up to 100001: 77 us, 415 MB, 5.4 TB/s.
 constexpr int kDecWaves = 4;
 constexpr int kDecThreads = 64 * kDecWaves;
 constexpr int kDecRows = 8;            // query heads of a pass
@@ -447,7 +447,11 @@ __global__ __launch_bounds__(kDecThreads) void kv8_decode_kernel(Kv8DecodeArgs a
 
 // Runs per KV head and sequence: two workgroups per CU over the launch (what
 // the registers let reside; the 32 sequences above: 22.2 us, with one per CU
-// 28.6, with four 28.4), none with fewer blocks than waves.
+// 28.6, with four 28.4), none with fewer blocks than waves.  The division is
+// rounded down and knows no lengths.  51 sequences of up to 2304 have two runs
+// each and take 28.0 us; 52 have one, half of the places stay empty, and they take
+// 35.3 (64: 40.1, 96: 45.8).  A long sequence among many short ones gets their few
+// runs: 100000 positions beside 63 of 500, H 64 over 8, 770 us (alone 50).
 static int decode_splits(int batch, int Hkv, int nb) {
     const int64_t rows = (int64_t)batch * Hkv, most = (nb + kDecWaves - 1) / kDecWaves;
     int64_t s = 2 * (int64_t)device_cus() / rows;
@@ -459,11 +463,12 @@ static int decode_splits(int batch, int Hkv, int nb) {
 // a run has 8 blocks at least (else 4), and twice as many are not cut: the
 // hand-over and the join take 3-5 us, a workgroup's next four blocks 1.  H 20
 // over 5, with runs of 4 and of 8: 8 sequences of up to 600 positions 8.2, 8.9
-// us; 16 of 640 9.4, 8.7; 32 of 512 11.2, 8.2.  And a sequence's second runs,
+// us; 16 of 640 9.4, 8.8; 32 of 512 11.2, 8.5; just past the uncut lengths it
+// loses, 32 of 700 by 3%, 48 of 600 with weights by 4%.  And a sequence's second runs,
 // which it may not have, are started after all first ones, so that those are on
-// all XCDs alike (16 of 640: 8.7 against 10.9 with a sequence's runs side by
+// all XCDs alike (16 of 640: 8.8 against 10.9 with a sequence's runs side by
 // side); of few rows each has its runs side by side (4 of 100001: 75 us against
-// 82 the other way).
+// 82 the other way, on one box).
 static bool decode_many(int batch, int Hkv) { return (int64_t)batch * Hkv >= 64; }
 
 // Parts are as many as a batch of up to this size leaves at most, whatever its own
@@ -500,13 +505,17 @@ static DecodeWs decode_ws(int batch, int H, int Hkv, int nb) {
 // issues 16 MFMAs and then 128 VALU instructions takes 395 ns, one that
 // alternates them 349, the MFMAs alone 261; two waves per SIMD).  K runs a
 // block ahead of V; rings of four blocks of each leave one barrier per two
-// blocks.  8192 tokens, H 20 over 5: 596 us, 1150 TFLOP/s of MFMA work (a large
+// blocks.  8192 tokens, H 20 over 5: 612 us, 1124 TFLOP/s of MFMA work (a large
 // f16 product of the library: 1330); 2048 tokens 54 us and 9 for the join; 333
-// behind 20011 137 us and 8.  The MFMAs are busy for two thirds of a wave's time
+// behind 20011 137-153 us and 9.  The MFMAs are busy for two thirds of a wave's time
 // and the clock falls under them, so what saves VALU instructions saves time.
 // Row tiles see different lengths; where they alone leave CUs idle or finish
 // far apart, the launch cuts them into runs (prefill_plan), and a second launch
-// joins the parts.
+// joins the parts.  More tiles than resident workgroups are not cut at all: behind
+// a long context, where all are equally long, a few too many cost a second round
+// (3264 tokens behind 20000, 510 workgroups: 1221 us; 3300, 520: 1781; 4096: 1950).
+// From position 0 the lengths differ and the last ones are short (3264 tokens 125
+// us, 3300 127).
 constexpr int kPreWaves = 4;
 constexpr int kPreThreads = 64 * kPreWaves;
 constexpr int kPreRows = 32 * kPreWaves;
@@ -941,8 +950,8 @@ __global__ __launch_bounds__(256) void kv8_prefill_join_kernel(Kv8PrefillArgs a)
 // A block's weight: its sums of p' over the rows that see it, which the
 // attention has left, in the units of their softmax sums, known only now.  A
 // workgroup a block, in a fixed order; bound by the sums' bytes (333 tokens
-// behind 20011, H 20: 36 MB in 8.2 us; the scores a second time, K in registers
-// and q through LDS: 72).
+// behind 20011, H 20: 35 MB in 9.4-10.8 us; the scores a second time, K in
+// registers and q through LDS: 72).
 __global__ __launch_bounds__(256) void kv8_prefill_weights_kernel(Kv8PrefillArgs a) {
     __shared__ float red[4];
     const int b = blockIdx.x, kvh = blockIdx.y, tid = threadIdx.x;
