@@ -61,7 +61,7 @@ __device__ inline void kv8_span(const Kv8AppendArgs &a, int z, int &p0, int &cnt
 //   y = t (1/a),  y' = y + (t - y a) (1/a),  t = top x (exact),
 // off by 2^-24 of itself at most and exact where the quotient is an f32 number,
 // ties among them: the same codes as the f32 division's, in a third of its
-// instructions.  One row: 3.8 us.  Four prompts of up to 2048 rows, 5 heads (16 MB
+// instructions.  One row: 3.4 us.  Four prompts of up to 2048 rows, 5 heads (16 MB
 // in, 8 out): 8.5-9.1 us, 2.7-2.9 TB/s; 13.9 with divisions and V's bytes stored one
 // by one.  Short of the copy's rate as nothing of another block is in flight while a
 // workgroup waits for its rows, their maximum and its two barriers.

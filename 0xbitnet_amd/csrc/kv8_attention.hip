@@ -1000,8 +1000,9 @@ static PrefillPlan prefill_plan(int n, int pos0, int H, int Hkv, bool weights) {
     p.rows = n * G;
     p.rtiles = (p.rows + kPreRows - 1) / kPreRows;
     // A row tile's blocks may be cut into even runs of `per` at most: the least per,
-    // of kPreLeast at least, whose runs all are resident at once.  (2048 tokens: 56 us; 850 workgroups of the same
-    // work in two rounds 69, as beginning and ending a run takes about 9 us.)
+    // of kPreLeast at least, whose runs all are resident at once.  (2048 tokens: 56
+    // us; 850 workgroups of the same work in two rounds 69, as beginning and ending a
+    // run takes about 9 us.)
     const int slots = prefill_slots(Hkv), most = kv8_blocks(total);
     auto count = [&](int per) {
         int64_t n = 0;
@@ -1072,12 +1073,12 @@ static void prefill_order(const PrefillPlan &p, int pos0, int G, int Hkv, Kv8Pre
 
 // What prefill_plan asks for at most over all calls of up to n tokens that end at
 // pos0 + n or before, so that a workspace of the largest call serves every smaller one.
-// Parts: a cut launch has at most `slots` runs, of eight blocks at least, and a row
-// tile that sees more blocks than another has no fewer of them.  With T tokens
-// visible to the last row and r tiles, the tiles' blocks add up to r T / 64 or more,
-// so r T / (32 per) <= 2 slots, and splits r < 2 slots + r <= 3 slots.
-// Sums of the weights: a launch's stay under 256 MB (or are one token's), but for the
-// last tile's rounding to kPreRows rows.
+// Parts are splits times rows.  A cut launch has `slots` runs at most, of up to per
+// blocks, per >= kPreLeast.  With T tokens visible to the last of r tiles, the tiles
+// see r T / 64 blocks or more between them, as what they see rises evenly; so r T /
+// (64 per) <= slots, and with splits < T / (32 per) + 1, splits r < 2 slots + r <= 3
+// slots.  Sums of the weights: a launch's stay under kPreSums (or are one token's), but
+// for the last tile's rounding to kPreRows rows.
 static size_t prefill_bytes(int n, int pos0, int H, int Hkv, bool weights) {
     const int64_t rows = (int64_t)n * (H / Hkv), most = kv8_blocks(pos0 + n), slots = prefill_slots(Hkv);
     size_t at = kArrivals * 4;

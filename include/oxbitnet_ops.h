@@ -340,8 +340,7 @@ int oxb_kv8_read(const void *cache, size_t cache_stride, int fmt, int batch, int
  * leaves zero, so one of the largest size serves calls of any shapes in turn.
  * The size grows with batch and max_seq: one for the largest serves every
  * smaller batch and cache of these heads.  Calls that share one must not run
- * concurrently.  Replaces
- * nn/attention.rs:109-118 over this cache. */
+ * concurrently.  Replaces nn/attention.rs:109-118 over this cache. */
 size_t oxb_attn_decode_kv8_ws_bytes(int batch, int H, int Hkv, int hd, int max_seq);
 int oxb_attn_decode_kv8(const float *q, void *cache, size_t cache_stride, int fmt, const int *pos,
                         int pos_stride, int batch, int H, int Hkv, int hd, int max_seq,

@@ -3,7 +3,6 @@ completed the block."""
 import numpy as np
 import pytest
 
-from helpers import ops
 import kv8_reference as ref
 from test_gpu_kv8 import FMTS, HD, bits, held, new_cache, rng_of, rows, set_weights
 

@@ -2,7 +2,6 @@
 import numpy as np
 import pytest
 
-from helpers import ops
 import kv8_reference as ref
 from test_gpu_kv8 import FMTS, HD, new_cache, rng_of
 
