@@ -1,4 +1,4 @@
-"""The 8-bit cache's tests that judge values by their bounds alone, with a check that
+"""The 8-bit cache's tests that compare values by their bounds alone, with a check that
 takes no NaN: caches start as NaN wherever nothing has been written, so stale codes,
 scales and weights that reach a result show up as one."""
 import pytest
