@@ -127,6 +127,16 @@ SIGNATURES = {
     "oxb_kv8_evict_ws_bytes": (sz, [i32, i32, i32, i32]),
     "oxb_kv8_evict": (C.c_int, [vp, sz, i32, vp, sz, i32, vp, i32, vp, i32, i32, i32, i32, i32, i32,
                                 i32, vp, sz, vp]),
+    "oxb_paged_bytes": (sz, [i32, i32, i32, i32]),
+    "oxb_paged_update": (C.c_int, [i32, i32, vp, vp, vp, i32, vp, i32, vp, vp, vp, vp, vp, vp, vp, i32,
+                                   vp]),
+    "oxb_paged_append": (C.c_int, [vp, i32, i32, i32, i32, vp, vp, sz, sz, vp, vp, i32, vp]),
+    "oxb_attn_decode_paged_ws_bytes": (sz, [i32, i32, i32, i32]),
+    "oxb_attn_decode_paged": (C.c_int, [vp, i32, vp, i32, i32, vp, i32, vp, i32, i32, i32, i32, vp, vp,
+                                        sz, vp]),
+    "oxb_attn_prefill_paged_ws_bytes": (sz, [i32, i32, i32, i32, i32]),
+    "oxb_attn_prefill_paged": (C.c_int, [vp, i32, vp, i32, i32, vp, i32, vp, vp, i32, i32, i32, i32, i32,
+                                         vp, vp, sz, vp]),
     "oxb_logits_rules": (C.c_int, [vp, sz, i32, i32, vp, vp, vp, i32, vp, vp, vp, i32, vp, sz, vp,
                                    sz, vp]),
     "oxb_embedding": (C.c_int, [vp, i32, i32, vp, i32, vp, vp, vp]),

@@ -54,6 +54,17 @@ extern "C" {
 #define OXB_KV8_BLOCK 32
 #define OXB_KV8_MAX_SEQ (1 << 24)
 
+/* Types of activations (q, out) in calls that take one. */
+#define OXB_F32 0
+#define OXB_F16 1
+
+/* The paged KV cache (oxb_paged_*): positions of its layout unit, the largest
+ * page, the longest sequence and the largest batch. */
+#define OXB_PAGED_UNIT 32
+#define OXB_PAGED_MAX_PAGE 4096
+#define OXB_PAGED_MAX_SEQ (1 << 24)
+#define OXB_PAGED_MAX_BATCH 4096
+
 /* ---- errors, device memory, streams, events (plumbing) ----------------- */
 const char *oxb_last_error(void);
 void *oxb_device_malloc(size_t bytes);
@@ -376,6 +387,91 @@ int oxb_kv8_evict(const void *cache, size_t cache_stride, int max_seq, void *dst
                   int dst_max_seq, const int *len, int len_stride, int *len_out, int len_out_stride,
                   int batch, int Hkv, int hd, int budget, int sink, int recent, void *ws,
                   size_t ws_bytes, void *stream);
+
+/* ---- paged KV cache ---------------------------------------------------------- */
+/* f16 K and V in pages of one pool that all sequences of a server share.  A page
+ * holds page_size positions (a power of two, OXB_PAGED_UNIT to OXB_PAGED_MAX_PAGE)
+ * of every KV head; a sequence is a row of a block table, int32 page ids, of which
+ * the first ceil(len / page_size) are in use.  A layer's pool is one allocation of
+ * oxb_paged_bytes bytes, 256-byte aligned, which needs no clearing; tables, lengths
+ * and slots serve all layers.  All calls are plain launches on the caller's stream
+ * and may be captured; arrays are device memory.
+ *   pool  [n_pages][Hkv][page_size / 32] units of 8192 f16: 4096 K elements,
+ *         position t, dim d at ((d / 8) * 32 + t) * 8 + d % 8, then 4096 V
+ *         elements, at ((t / 8) * 128 + d) * 8 + t % 8 (t counted in the unit): the
+ *         operands of the attention's matrix products as they lie
+ * No counterpart in the reference (one buffer per layer, nn/attention.rs:23-48). */
+size_t oxb_paged_bytes(int n_pages, int page_size, int Hkv, int hd);
+
+/* A step's bookkeeping: sequence z of len[z] positions is to grow by delta[z] tokens
+ * (> 0), keep its length (0) or lose its last -delta[z] positions (all of them and
+ * more end it).  Pages that hold no position any more go back to the free list, a
+ * stack of *n_free ids in free_pages[free_cap], and growing sequences take theirs:
+ * what is given back in this call first, its last page first, then from the list's
+ * end.  Sequences are served in order.  Growth is granted whole or not at all: not
+ * where it passes table_stride pages or its tokens the packed buffer of n_max, and,
+ * from the first sequence whose pages are not there, to none that needs a page.
+ *   len_out[z]   the new length (as before where growth is not granted; may be len)
+ *   n_free_out   ids on the free list (may be n_free)
+ *   cu[batch+1]  where the tokens of each sequence begin among the packed ones (the
+ *                sums of the growths wanted, granted or not, n_max at most)
+ *   granted[z]   tokens granted (NULL: not written)
+ *   slots[n_max] a packed token's slot, page * page_size + offset; -1 where growth is
+ *                not granted and behind the last token (NULL: not written)
+ *   pos[n_max]   its position in the sequence, or -1 (NULL: not written)
+ * Table entries of new pages and ids pushed on the list are written, others stay.
+ * Outputs other than len_out and n_free_out lie apart from the inputs.  Pages in two
+ * rows of the table are not counted: they would be given back twice. */
+int oxb_paged_update(int page_size, int batch, const int *len, const int *delta, int *table,
+                     int table_stride, int *free_pages, int free_cap, const int *n_free, int *len_out,
+                     int *n_free_out, int *cu, int *granted, int *slots, int *pos, int n_max,
+                     void *stream);
+
+/* Rows of n_tok packed tokens into the slots of slots[n_tok], which are distinct; a
+ * slot outside the pool (-1) skips its token.  Token t's row of head h is
+ * k + t*tok_stride + h*head_stride (f16; strides in elements, multiples of 8,
+ * 16-byte aligned rows), or, with src_pos, src_pos[t]*128 elements further: the row
+ * where the q|k|v projections leave a position in a f16 cache [Hkv][max_seq][128]
+ * that serves as scratch (src_pos is then oxb_paged_update's pos; below 0: skipped). */
+int oxb_paged_append(void *pages, int n_pages, int page_size, int Hkv, int hd, const uint16_t *k,
+                     const uint16_t *v, size_t tok_stride, size_t head_stride, const int *src_pos,
+                     const int *slots, int n_tok, void *stream);
+
+/* Decode attention over the pages for a batch: sequence z's query q + z*H*128 attends
+ * over positions 0..len[z]-1 (append first; 0 or less: the output is zeros; more than
+ * the table's row holds: what it holds), any H that is a multiple of Hkv.  Positions
+ * of a page id outside 0..n_pages-1 are not there.  What lies behind the length, and
+ * in other pages, may hold anything; a visible Inf or NaN makes what it reaches NaN
+ * or Inf.
+ *   OXB_F32  q and out f32: q and the softmax weights go through f16 MFMA as two
+ *            parts each, sums are f32 (22 bits of each value)
+ *   OXB_F16  q and out f16, the same sums, rounded once
+ * The result does not depend on timing.  ws: a device workspace of
+ * oxb_attn_decode_paged_ws_bytes bytes, 256-byte aligned; its first 4 KB are arrival
+ * counters that must be zero before its first use (a zero-filled allocation) and that
+ * every call leaves zero, so one serves calls of any batch and lengths in turn (the
+ * size depends on H / Hkv alone).  Calls that share one must not run concurrently.
+ * Replaces nn/attention.rs:109-118 over this cache. */
+size_t oxb_attn_decode_paged_ws_bytes(int batch, int H, int Hkv, int hd);
+int oxb_attn_decode_paged(const void *q, int dtype, const void *pages, int n_pages, int page_size,
+                          const int *table, int table_stride, const int *len, int batch, int H,
+                          int Hkv, int hd, void *out, void *ws, size_t ws_bytes, void *stream);
+
+/* Causal attention of packed tokens: sequence z's are cu[z] .. cu[z+1]-1 of q and out
+ * ([n_tok][H*128]), the newest of its len[z] positions, which the pages hold already;
+ * the i-th of n attends over positions 0 .. len[z] - n + i (none: zeros).  Whole
+ * prompts, later parts of prompts and drafts of a few tokens go in one call.  cu
+ * ascends (oxb_paged_update's); rows before cu[0] and from cu[batch] on are left as
+ * they were.  Types, pages and what is not there as above; with OXB_F16 the softmax
+ * weights are f16.  ws: oxb_attn_prefill_paged_ws_bytes bytes, 256-byte aligned, any
+ * contents (one workspace may serve decode too, whose counters this call leaves
+ * alone); the size grows with n_tok and batch.  Calls that share one must not run
+ * concurrently. */
+size_t oxb_attn_prefill_paged_ws_bytes(int n_tok, int batch, int H, int Hkv, int hd);
+int oxb_attn_prefill_paged(const void *q, int dtype, const void *pages, int n_pages, int page_size,
+                           const int *table, int table_stride, const int *cu, const int *len,
+                           int n_tok, int batch, int H, int Hkv, int hd, void *out, void *ws,
+                           size_t ws_bytes, void *stream);
 
 /* ---- sampling ---------------------------------------------------------------- */
 /* One draw of rs/sampling.rs:4-80 over logits[V] (modified in place):
