@@ -369,6 +369,100 @@ class Kv8Cache:
         return dl.download()
 
 
+F32, F16 = 0, 1   # include/oxbitnet_ops.h OXB_F32, OXB_F16
+PAGED_UNIT = 32   # OXB_PAGED_UNIT
+
+
+class PagedCache:
+    """A batch's f16 KV cache in pages of one pool (oxb_paged_*, oxb_attn_*_paged):
+    numpy rows in, numpy out."""
+
+    def __init__(self, batch: int, Hkv: int, n_pages: int, page_size: int, table_pages: int, hd: int = 128):
+        self.batch, self.Hkv, self.n_pages, self.page_size, self.hd = batch, Hkv, n_pages, page_size, hd
+        n = lib().oxb_paged_bytes(n_pages, page_size, Hkv, hd)
+        if not n:
+            raise NativeError(f"no pool of {n_pages} pages of {page_size} positions, {Hkv} heads of {hd}")
+        self.pool = DeviceArray((n // 2,), np.uint16)
+        self.table = DeviceArray.from_host(np.full((batch, table_pages), -1, np.int32))
+        self.free = DeviceArray.from_host(np.arange(n_pages, dtype=np.int32)[::-1])
+        self.n_free = DeviceArray.from_host(np.array([n_pages], np.int32))
+        self.len = DeviceArray((batch,), np.int32, zero=True)
+        self._ws = {}
+
+    def _workspace(self, n: int) -> tuple:
+        _require(n > 0, "no workspace for this shape")
+        if n not in self._ws:
+            self._ws[n] = DeviceArray((n,), np.uint8, zero=True)
+        return self._ws[n].ptr, n
+
+    def step(self, delta, n_max: int | None = None) -> dict:
+        """Grow, keep or shrink each sequence: granted tokens, and the packed tokens'
+        starts (cu), slots and positions."""
+        delta = np.ascontiguousarray(delta, np.int32)
+        _require(delta.shape == (self.batch,), f"delta {delta.shape} for {self.batch} sequences")
+        n = int(np.maximum(delta, 0).sum()) if n_max is None else n_max
+        dd = DeviceArray.from_host(delta)
+        cu, granted = DeviceArray((self.batch + 1,), np.int32), DeviceArray((self.batch,), np.int32)
+        slots, pos = (DeviceArray((n,), np.int32) for _ in "sp")
+        check(lib().oxb_paged_update(self.page_size, self.batch, self.len.ptr, dd.ptr, self.table.ptr,
+                                     self.table.shape[1], self.free.ptr, self.n_pages, self.n_free.ptr, self.len.ptr,
+                                     self.n_free.ptr, cu.ptr, granted.ptr, slots.ptr, pos.ptr, n, None),
+              "paged_update")
+        sync()
+        return {"cu": cu.download(), "granted": granted.download(), "slots": slots.download(),
+                "pos": pos.download()}
+
+    def append(self, k: np.ndarray, v: np.ndarray, slots) -> None:
+        """f16 rows [n][Hkv][128] of packed tokens into their slots."""
+        k, v = (np.ascontiguousarray(x, np.float16) for x in (k, v))
+        slots = np.ascontiguousarray(slots, np.int32)
+        _require(k.shape == v.shape == (slots.size, self.Hkv, self.hd) and slots.ndim == 1,
+                 f"k {k.shape} and v {v.shape} for [{slots.size}][{self.Hkv}][{self.hd}]")
+        if not slots.size:
+            return
+        dk, dv = (DeviceArray.from_host(x.view(np.uint16)) for x in (k, v))
+        ds = DeviceArray.from_host(slots)
+        check(lib().oxb_paged_append(self.pool.ptr, self.n_pages, self.page_size, self.Hkv, self.hd, dk.ptr, dv.ptr,
+                                     self.Hkv * self.hd, self.hd, None, ds.ptr, slots.size, None), "paged_append")
+        sync()
+
+    def _q(self, q: np.ndarray) -> tuple:
+        q = np.ascontiguousarray(q)
+        _require(q.dtype in (np.float32, np.float16) and q.ndim == 2, f"q is {q.dtype} {q.shape}")
+        _require(q.shape[1] % (self.hd * self.Hkv) == 0 and q.shape[1] > 0,
+                 f"q rows of {q.shape[1]} for {self.Hkv} KV heads of {self.hd}")
+        return q, F32 if q.dtype == np.float32 else F16, q.shape[1] // self.hd
+
+    def attn_decode(self, q: np.ndarray) -> np.ndarray:
+        """q f32 or f16 [batch][H*128]; each sequence attends over all it holds."""
+        q, dtype, H = self._q(q)
+        _require(q.shape[0] == self.batch, f"{q.shape[0]} queries for {self.batch} sequences")
+        dq, out = DeviceArray.from_host(q), DeviceArray(q.shape, q.dtype)
+        ws = self._workspace(lib().oxb_attn_decode_paged_ws_bytes(self.batch, H, self.Hkv, self.hd))
+        check(lib().oxb_attn_decode_paged(dq.ptr, dtype, self.pool.ptr, self.n_pages, self.page_size, self.table.ptr,
+                                          self.table.shape[1], self.len.ptr, self.batch, H, self.Hkv, self.hd,
+                                          out.ptr, *ws, None), "attn_decode_paged")
+        sync()
+        return out.download()
+
+    def attn_prefill(self, q: np.ndarray, cu, out: np.ndarray | None = None) -> np.ndarray:
+        """q f32 or f16 [n][H*128] packed, sequence z's newest tokens at cu[z]..cu[z+1]-1,
+        causal; out: what the rows of no sequence hold before (and after)."""
+        q, dtype, H = self._q(q)
+        cu = np.ascontiguousarray(cu, np.int32)
+        _require(cu.shape == (self.batch + 1,), f"cu {cu.shape} for {self.batch} sequences")
+        dq, dc = DeviceArray.from_host(q), DeviceArray.from_host(cu)
+        do = DeviceArray.from_host(np.zeros_like(q) if out is None else np.ascontiguousarray(out, q.dtype))
+        _require(do.shape == q.shape, f"out {do.shape} for {q.shape}")
+        ws = self._workspace(lib().oxb_attn_prefill_paged_ws_bytes(q.shape[0], self.batch, H, self.Hkv, self.hd))
+        check(lib().oxb_attn_prefill_paged(dq.ptr, dtype, self.pool.ptr, self.n_pages, self.page_size,
+                                           self.table.ptr, self.table.shape[1], dc.ptr, self.len.ptr, q.shape[0],
+                                           self.batch, H, self.Hkv, self.hd, do.ptr, *ws, None),
+              "attn_prefill_paged")
+        sync()
+        return do.download()
+
+
 def logits_rules(logits: np.ndarray, penalties=None, history=None, bias=None, mask=None) -> np.ndarray:
     """Rules on logits [n][V] (oxb_logits_rules).  penalties: [n][3] repeat, frequency,
     presence; history: a list of ids per row; bias: a list of (id, value) per row;

@@ -417,9 +417,11 @@ size_t oxb_paged_bytes(int n_pages, int page_size, int Hkv, int hd);
  *                sums of the growths wanted, granted or not, n_max at most)
  *   granted[z]   tokens granted (NULL: not written)
  *   slots[n_max] a packed token's slot, page * page_size + offset; -1 where growth is
- *                not granted and behind the last token (NULL: not written)
+ *                not granted, where the page id is below 0 or the slot past 31 bits, and
+ *                behind the last token (NULL: not written)
  *   pos[n_max]   its position in the sequence, or -1 (NULL: not written)
- * Table entries of new pages and ids pushed on the list are written, others stay.
+ * Table entries of new pages and ids pushed on the list are written, others stay; ids
+ * past free_cap are lost.
  * Outputs other than len_out and n_free_out lie apart from the inputs.  Pages in two
  * rows of the table are not counted: they would be given back twice. */
 int oxb_paged_update(int page_size, int batch, const int *len, const int *delta, int *table,

@@ -1,0 +1,709 @@
+"""The paged KV cache (bookkeeping, append, decode and packed prefill attention) on the
+GPU against numpy in 64 bits.  Pools start filled with 0xffff, NaN in every element
+that nothing has been written to."""
+import zlib
+
+import numpy as np
+import pytest
+
+from helpers import ops, synth, ternary
+import paged_reference as ref
+
+pytestmark = pytest.mark.gpu
+HD = 128
+
+
+def rng_of(*key):
+    return np.random.default_rng(zlib.crc32(repr(key).encode()))
+
+
+def rows(rng, n, hkv):
+    k = rng.standard_normal((n, hkv, HD)) * np.exp(0.4 * rng.standard_normal((1, hkv, HD)))
+    return k.astype(np.float16), rng.standard_normal((n, hkv, HD)).astype(np.float16)
+
+
+def new_cache(batch, hkv, n_pages, page, table_pages):
+    c = ops.PagedCache(batch, hkv, n_pages, page, table_pages)
+    c.pool.upload(np.full(c.pool.shape, 0xffff, np.uint16))
+    return c
+
+
+def shuffle(c, rng):
+    """The free list in a random order."""
+    c.free.upload(rng.permutation(c.n_pages).astype(np.int32))
+
+
+def filled(rng, lens, hkv, page, spare=2, table_pages=None):
+    """A cache holding lens[z] rows, and the rows: K, V [z][n][Hkv][128]."""
+    need = sum(ref.pages(n, page) for n in lens)
+    c = new_cache(len(lens), hkv, need + spare, page, table_pages or max(1, ref.pages(max(lens), page)))
+    shuffle(c, rng)
+    s = c.step(lens)
+    assert s["granted"].tolist() == list(lens)
+    k, v = rows(rng, int(sum(lens)), hkv)
+    c.append(k, v, s["slots"])
+    at = s["cu"]
+    return c, [k[at[z]:at[z + 1]] for z in range(len(lens))], [v[at[z]:at[z + 1]] for z in range(len(lens))]
+
+
+def expect(q, K, V, hkv, first, f16=False, parts=2):
+    """Rows q [n][H*128] at positions first.. of one sequence: outputs and bounds."""
+    n, H = q.shape[0], q.shape[1] // HD
+    G = H // hkv
+    out, tol = np.zeros(q.shape), np.zeros(q.shape)
+    seen = np.clip(first + 1 + np.arange(n), 0, len(K))
+    for h in range(H):
+        at = slice(h * HD, (h + 1) * HD)
+        out[:, at], tol[:, at] = ref.attend(q[:, at], K[:, h // G], V[:, h // G], seen, f16, parts)
+    return out, tol
+
+
+def bits(a):
+    return np.ascontiguousarray(a).view(np.uint32 if a.dtype.itemsize == 4 else np.uint16)
+
+
+# ---------------------------------------------------------------------------
+# bookkeeping
+# ---------------------------------------------------------------------------
+def run_update(page, length, delta, table, free, n_free, n_max, optional=True):
+    L = ops.lib()
+    B, W = np.shape(table)
+    up = lambda x: ops.DeviceArray.from_host(np.asarray(x, np.int32).reshape(-1))  # noqa: E731
+    dl, dd, dt, df, dn = up(length), up(delta), up(table), up(free), up([n_free])
+    cu, gr, sl, ps = (ops.DeviceArray.from_host(np.full(n, 12345, np.int32)) for n in (B + 1, B, n_max + 1, n_max + 1))
+    o = lambda x: x.ptr if optional else None  # noqa: E731
+    ops.check(L.oxb_paged_update(page, B, dl.ptr, dd.ptr, dt.ptr, W, df.ptr, len(free), dn.ptr, dl.ptr, dn.ptr, cu.ptr,
+                                 o(gr), o(sl), o(ps), n_max, None))
+    ops.sync()
+    s, p = sl.download(), ps.download()
+    assert s[n_max] == p[n_max] == 12345
+    return (dl.download().tolist(), dt.download().reshape(B, W), df.download(), int(dn.download()[0]),
+            cu.download().tolist(), gr.download().tolist(), s[:n_max], p[:n_max])
+
+
+def same_update(*args):
+    got, want = run_update(*args), ref.update(*args)
+    for i, (a, b) in enumerate(zip(got, want)):
+        assert np.array_equal(a, b), i
+
+
+def random_state(rng, page, B, W, most):
+    length = [int(x) for x in rng.integers(0, most + 1, B)]
+    need = sum(ref.pages(n, page) for n in length)
+    order = rng.permutation(need + 4 * B).astype(np.int32)
+    table, at = np.full((B, W), -1, np.int32), 0
+    for z, n in enumerate(length):
+        m = ref.pages(n, page)
+        table[z, :m] = order[at:at + m]
+        at += m
+    free = np.full(len(order), -7, np.int32)
+    free[:len(order) - at] = order[at:]
+    return length, table, free, len(order) - at
+
+
+@pytest.mark.parametrize("page", [32, 64, 4096])
+@pytest.mark.parametrize("B,most,grow", [(1, 0, 1), (1, 100, 40), (3, 200, 1), (64, 300, 1), (65, 90, 33),
+                                         (200, 500, 60), (1025, 70, 5)])
+def test_update_matches_reference(page, B, most, grow):
+    rng = rng_of("update", page, B, most, grow)
+    for kind in range(3):
+        W = ref.pages(most + grow, page) + (0 if kind == 2 else 1)
+        length, table, free, n_free = random_state(rng, page, B, W, most)
+        delta = rng.integers(-grow, grow + 1, B)
+        delta[rng.random(B) < 0.1] = -10 ** 9
+        total = int(np.maximum(delta, 0).sum())
+        if kind == 1:                      # too few pages, and a buffer that does not hold all tokens
+            n_free = min(n_free, B // 3)
+            total = total * 2 // 3
+        same_update(page, length, delta.tolist(), table, free, n_free, total)
+
+
+def test_update_of_many_tokens():
+    """Several workgroups, lengths in place: 40 prompts of 130000 tokens."""
+    rng = rng_of("many")
+    B, page = 40, 32
+    length, table, free, n_free = random_state(rng, page, B, 400, 6000)
+    delta = rng.integers(2000, 5000, B)
+    delta[::7] = -length[0]
+    free = np.concatenate([free, np.arange(len(free), len(free) + 5000, dtype=np.int32)])
+    free[:n_free + 5000] = rng.permutation(np.concatenate([free[:n_free], free[-5000:]]))
+    same_update(page, length, delta.tolist(), table, free, n_free + 5000, int(np.maximum(delta, 0).sum()) + 77)
+
+
+def test_update_at_its_limits():
+    """Sums past 32 bits, lengths outside the table, pages that are none, empty lists."""
+    I = 2 ** 31 - 1
+    same_update(32, [0, 40, 5], [I, 1, I], [[1, 2], [3, 4], [5, 6]], [9, 8], 2, 10)
+    same_update(32, [-5, 100, 64], [1, 1, -1], [[1, 2], [3, 4], [5, 6]], [9, 8], 2, 10)
+    same_update(32, [0, 0], [1, 0], [[-1], [-1]], [-3], 1, 4)              # a page id below 0: no slot
+    same_update(32, [0, 0], [1, 1], [[-1], [-1]], [2], 0, 4)               # nothing free
+    same_update(32, [0, 0], [1, 1], [[-1], [-1]], [2], -4, 4)
+    same_update(32, [0, 0], [1, 1], [[-1], [-1]], [2], 100, 4)             # a count past the list
+    same_update(32, [33, 31], [-33, 3], [[4, 5], [6, -1]], [7], 1, 3)      # one list slot for three ids: dropped
+    same_update(32, [1] * 4096, [I] * 4096, [[1]] * 4096, [2], 1, 8)
+    same_update(32, [1] * 4096, [-2 ** 31] * 4096, [[z] for z in range(4096)], [2] * 5000, 5, 0)
+    got = run_update(32, [31, 0], [2, 3], [[1, -1], [-1, -1]], [3, 4, 5], 3, 5, optional=False)
+    assert got[0] == [33, 3] and got[1].tolist() == [[1, 5], [4, -1]] and got[3] == 1 and got[4] == [0, 2, 5]
+
+
+def test_update_of_steps_in_a_row():
+    """A hundred steps of a random batch: no page in two places, none lost."""
+    rng = rng_of("steps")
+    B, page, n_pages = 24, 32, 150
+    c = ops.PagedCache(B, 1, n_pages, page, 12)
+    shuffle(c, rng)
+    t, f, n, length = c.table.download(), c.free.download(), n_pages, [0] * B
+    for step in range(100):
+        delta = rng.choice([1, 1, 1, 0, -3, 70, -400, 33], B)
+        want = ref.update(page, length, delta, t, f, n, 600)
+        got = c.step(delta, 600)
+        length, t, f, n = want[:4]
+        assert c.len.download().tolist() == length and int(c.n_free.download()[0]) == n, step
+        assert np.array_equal(c.table.download(), t) and np.array_equal(c.free.download(), f)
+        for name, x in zip(("cu", "granted", "slots", "pos"), want[4:]):
+            assert np.array_equal(got[name], x), (step, name)
+        held = [int(x) for z in range(B) for x in t[z, :ref.pages(length[z], page)]] + f[:n].tolist()
+        assert sorted(held) == list(range(n_pages))
+
+
+# ---------------------------------------------------------------------------
+# append
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("page", [32, 128])
+@pytest.mark.parametrize("hkv,lens", [(1, [1]), (5, [31, 0, 33]), (3, [100, 7, 64, 250]), (2, [1] * 40)])
+def test_append_places_every_element(page, hkv, lens):
+    rng = rng_of("append", page, hkv, lens)
+    c = new_cache(len(lens), hkv, sum(ref.pages(n, page) for n in lens) + 40, page, 8)
+    shuffle(c, rng)
+    want = np.full(c.pool.shape, 0xffff, np.uint16).view(np.float16)
+    for delta in (lens, [5] * len(lens), [-2] * len(lens), [1] * len(lens), [3] * len(lens)):
+        s = c.step(delta, max(1, int(np.maximum(delta, 0).sum())) + 9)
+        n = len(s["slots"])
+        k, v = rows(rng, n, hkv)
+        c.append(k, v, s["slots"])
+        ref.place(want, page, hkv, s["slots"], k, v)
+        assert np.array_equal(c.pool.download(), want.view(np.uint16)), delta
+
+
+def test_append_slots_in_any_order():
+    """Slots that jump, run backwards and lie outside the pool; subnormals, Inf and NaN
+    as they are."""
+    rng = rng_of("slots")
+    page, hkv, n_pages = 64, 2, 6
+    c = new_cache(1, hkv, n_pages, page, 4)
+    total = n_pages * page
+    slots = np.concatenate([rng.permutation(total)[:90], [-1, total, 2 ** 31 - 1, -2 ** 31],
+                            np.full(3, -1)]).astype(np.int32)
+    k, v = rows(rng, len(slots), hkv)
+    k[3, 0, :4] = [np.inf, -np.inf, np.nan, 6e-8]
+    v[5, 1, 7] = np.nan
+    c.append(k, v, slots)
+    want = np.full(c.pool.shape, 0xffff, np.uint16).view(np.float16)
+    ref.place(want, page, hkv, [s if 0 <= s < total else -1 for s in slots], k, v)
+    assert np.array_equal(c.pool.download(), want.view(np.uint16))
+    back = np.arange(total - 1, -1, -1, dtype=np.int32)
+    k, v = rows(rng, total, hkv)
+    c.append(k, v, back)
+    ref.place(want, page, hkv, back, k, v)
+    assert np.array_equal(c.pool.download(), want.view(np.uint16))
+
+
+def test_append_takes_rows_at_their_position():
+    """Rows in a f16 cache [Hkv][max_seq][128] per sequence, where the projections leave
+    them, and rows inside a wider buffer."""
+    L, rng = ops.lib(), rng_of("at")
+    hkv, ms, page, B = 3, 80, 32, 2
+    k, v = rng.standard_normal((2, B, hkv, ms, HD)).astype(np.float16)
+    dk, dv = (ops.DeviceArray.from_host(x.view(np.uint16)) for x in (k, v))
+    slots = np.array([70, 5], np.int32)
+    pos = np.array([79, 11], np.int32)
+    c = new_cache(1, hkv, 4, page, 4)
+    ds, dp = ops.DeviceArray.from_host(slots), ops.DeviceArray.from_host(pos)
+    ops.check(L.oxb_paged_append(c.pool.ptr, 4, page, hkv, HD, dk.ptr, dv.ptr, hkv * ms * HD, ms * HD, dp.ptr, ds.ptr,
+                                 2, None))
+    want = np.full(c.pool.shape, 0xffff, np.uint16).view(np.float16)
+    at = np.arange(B)
+    ref.place(want, page, hkv, slots, k[at, :, pos], v[at, :, pos])
+    ops.sync()
+    assert np.array_equal(c.pool.download(), want.view(np.uint16))
+    # a position below 0 is skipped; rows of [n][Hkv][2][128], K and V side by side
+    dp.upload(np.array([-1, 3], np.int32))
+    ds.upload(np.array([1, 2], np.int32))
+    ops.check(L.oxb_paged_append(c.pool.ptr, 4, page, hkv, HD, dk.ptr, dv.ptr, hkv * ms * HD, ms * HD, dp.ptr, ds.ptr,
+                                 2, None))
+    ref.place(want, page, hkv, [-1, 2], k[at, :, [0, 3]], v[at, :, [0, 3]])
+    both = rng.standard_normal((40, hkv, 2, HD)).astype(np.float16)
+    db = ops.DeviceArray.from_host(both.view(np.uint16))
+    wide = np.arange(60, 100, dtype=np.int32)
+    dw = ops.DeviceArray.from_host(wide)
+    ops.check(L.oxb_paged_append(c.pool.ptr, 4, page, hkv, HD, db.ptr, db.offset(2 * HD), hkv * 2 * HD, 2 * HD, None,
+                                 dw.ptr, 40, None))
+    ref.place(want, page, hkv, wide, both[:, :, 0], both[:, :, 1])
+    ops.sync()
+    assert np.array_equal(c.pool.download(), want.view(np.uint16))
+
+
+# ---------------------------------------------------------------------------
+# decode attention
+# ---------------------------------------------------------------------------
+DECODE = [  # H, Hkv, lengths, page
+    (4, 4, [1], 32),
+    (20, 5, [1, 2, 31, 32, 33], 32),
+    (6, 2, [64, 65, 0, 127, 129], 64),
+    (32, 2, [100, 7], 128),                     # 16 heads a KV head: two groups
+    (9, 1, [300, 257], 256),                    # nine: a full group and one more
+    (20, 5, [1000], 32),
+    (15, 5, [2000, 1, 0, 0, 700, 33], 64),
+    (8, 8, [500, 0, 1, 33, 320, 499, 64, 2], 32),
+]
+
+
+@pytest.mark.parametrize("dtype", [np.float32, np.float16])
+@pytest.mark.parametrize("H,hkv,lens,page", DECODE)
+def test_decode_matches_reference(dtype, H, hkv, lens, page):
+    rng = rng_of("decode", H, hkv, lens, page)
+    c, K, V = filled(rng, lens, hkv, page)
+    q = rng.standard_normal((len(lens), H * HD)).astype(dtype)
+    got = c.attn_decode(q)
+    assert got.dtype == dtype
+    for z, n in enumerate(lens):
+        want, tol = expect(q[z:z + 1], K[z], V[z], hkv, n - 1, dtype == np.float16)
+        ref.check_rows(got[z:z + 1], want, tol, z)
+        if n == 0:
+            assert not got[z].any()
+    assert np.array_equal(bits(got), bits(c.attn_decode(q)))      # the counters were left zero
+
+
+@pytest.mark.parametrize("batch,H,hkv,longest", [(1, 4, 1, 20011), (70, 4, 2, 900), (200, 3, 3, 80), (130, 8, 8, 70),
+                                                 (3, 20, 5, 5000)])
+def test_decode_batches(batch, H, hkv, longest):
+    """Many runs of one sequence, more sequences than lanes, than resident workgroups."""
+    rng = rng_of("batches", batch, H, hkv)
+    lens = [longest] + [int(x) for x in rng.integers(0, longest // 2, batch - 1)]
+    c, K, V = filled(rng, lens, hkv, 32, table_pages=ref.pages(longest, 32) + 5)
+    q = rng.standard_normal((batch, H * HD)).astype(np.float32)
+    got = c.attn_decode(q)
+    for z, n in enumerate(lens):
+        want, tol = expect(q[z:z + 1], K[z], V[z], hkv, n - 1)
+        ref.check_rows(got[z:z + 1], want, tol, z)
+    z = 0
+    want, _ = expect(q[:1], K[0], V[0], hkv, longest - 1)
+    ref.close_in_norm(got[:1], want, q[0].reshape(H, HD), K[0][:, 0], longest)
+
+
+@pytest.mark.parametrize("qscale", [0.0, 1e-38, 1e-30, 1e-4, 30.0, 1e4])
+def test_scales_of_q(qscale):
+    """Rows of q from subnormals to scores in the thousands, in both calls."""
+    rng = rng_of("qscale", qscale)
+    lens, hkv, H = [150, 40], 2, 4
+    c, K, V = filled(rng, lens, hkv, 32)
+    q = (rng.standard_normal((60, H * HD)) * qscale).astype(np.float32)
+    q[0, :HD] *= np.float32(1e-3)
+    got = c.attn_decode(q[:2])
+    for z, n in enumerate(lens):
+        want, tol = expect(q[z:z + 1], K[z], V[z], hkv, n - 1)
+        ref.check_rows(got[z:z + 1], want, tol, z)
+    got = c.attn_prefill(q, [0, 37, 60])
+    for z, (a, b) in enumerate(((0, 37), (37, 60))):
+        want, tol = expect(q[a:b], K[z], V[z], hkv, lens[z] - (b - a))
+        ref.check_rows(got[a:b], want, tol, z)
+
+
+def test_scores_far_apart():
+    """One position takes nearly all of a row's weight, early or late, and f16's largest
+    values: the reference rises late, or the first run holds it."""
+    rng = rng_of("apart")
+    for at in (0, 5, 200, 399):
+        c, K, V = filled(rng, [400], 1, 64)
+        k, v = K[0].copy(), V[0].copy()
+        q = rng.standard_normal((1, 2 * HD)).astype(np.float32)
+        k[at, 0] = (8 * q[0, :HD]).astype(np.float16)
+        v[at] = 65504
+        s = ref.slots_of(c.table.download()[0], 400, 64)
+        c.append(k, v, s)
+        want, tol = expect(q, k, v, 1, 399)
+        ref.check_rows(c.attn_decode(q), want, tol, at)
+        q2 = np.repeat(q, 50, 0)
+        want, tol = expect(q2, k, v, 1, 350)
+        ref.check_rows(c.attn_prefill(q2, [0, 50]), want, tol, at)
+
+
+# ---------------------------------------------------------------------------
+# prefill attention
+# ---------------------------------------------------------------------------
+PREFILL = [  # H, Hkv, (new, past) of each sequence, page
+    (4, 4, [(1, 0)], 32),
+    (20, 5, [(101, 0)], 32),
+    (20, 5, [(33, 0), (0, 0), (1, 0), (64, 0), (7, 0)], 64),
+    (8, 2, [(40, 100), (1, 300), (0, 50), (129, 31)], 32),
+    (9, 1, [(50, 77), (15, 0)], 256),
+    (15, 5, [(70, 5), (3, 900)], 64),
+    (32, 2, [(20, 12), (9, 0)], 128),
+    (3, 3, [(300, 0), (1, 1)], 32),
+    (6, 1, [(5, 2000)], 64),
+]
+
+
+def packed(spec):
+    new = [a for a, _ in spec]
+    return new, [a + b for a, b in spec], np.concatenate([[0], np.cumsum(new)]).astype(np.int32)
+
+
+@pytest.mark.parametrize("dtype", [np.float32, np.float16])
+@pytest.mark.parametrize("H,hkv,spec,page", PREFILL)
+def test_prefill_matches_reference(dtype, H, hkv, spec, page):
+    rng = rng_of("prefill", H, hkv, spec, page)
+    new, lens, cu = packed(spec)
+    c, K, V = filled(rng, lens, hkv, page)
+    n = int(cu[-1])
+    q = rng.standard_normal((n + 21, H * HD)).astype(dtype)        # rows of no sequence behind the last
+    before = rng.standard_normal(q.shape).astype(dtype)
+    got = c.attn_prefill(q, cu, before)
+    f16 = dtype == np.float16
+    for z, m in enumerate(new):
+        at = slice(cu[z], cu[z + 1])
+        want, tol = expect(q[at], K[z], V[z], hkv, lens[z] - m, f16, 1 if f16 else 2)
+        ref.check_rows(got[at], want, tol, z)
+    assert np.array_equal(bits(got[n:]), bits(before[n:]))
+    assert np.array_equal(bits(got), bits(c.attn_prefill(q, cu, before)))
+
+
+@pytest.mark.parametrize("dtype", [np.float32, np.float16])
+@pytest.mark.parametrize("H,hkv,spec,page", [
+    (4, 1, [(5, 20000)], 32),                                   # one short tile, many runs
+    (4, 2, [(700, 0), (90, 3000), (2, 1), (33, 64)], 32),       # cut and uncut tiles
+    (8, 8, [(1500, 0), (400, 1200)], 128),                      # more tiles than resident workgroups
+    (2, 2, [(9, 700)] * 80, 64),                                # drafts of more sequences than lanes
+])
+def test_prefill_larger(dtype, H, hkv, spec, page):
+    rng = rng_of("larger", H, hkv, page)
+    new, lens, cu = packed(spec)
+    c, K, V = filled(rng, lens, hkv, page)
+    q = rng.standard_normal((int(cu[-1]), H * HD)).astype(dtype)
+    got = c.attn_prefill(q, cu)
+    f16 = dtype == np.float16
+    for z, m in enumerate(new):
+        at = slice(cu[z], cu[z + 1])
+        want, tol = expect(q[at], K[z], V[z], hkv, lens[z] - m, f16, 1 if f16 else 2)
+        ref.check_rows(got[at], want, tol, z)
+        ref.close_in_norm(got[at], want, q[at].reshape(-1, HD)[:200], K[z][:, 0], lens[z], f16)
+
+
+def test_prefill_rows_with_nothing_to_see():
+    """More tokens than positions (the first rows see nothing), empty sequences between
+    them, cu that begins past 0."""
+    rng = rng_of("nothing")
+    H, hkv = 4, 2
+    lens = [3, 0, 40, 1]
+    c, K, V = filled(rng, lens, hkv, 32)
+    cu = np.array([4, 44, 50, 50, 60], np.int32)
+    q = rng.standard_normal((64, H * HD)).astype(np.float32)
+    before = np.full(q.shape, 7, np.float32)
+    got = c.attn_prefill(q, cu, before)
+    assert (got[:4] == 7).all() and (got[60:] == 7).all()
+    for z, n in enumerate(lens):
+        a, b = cu[z], cu[z + 1]
+        want, tol = expect(q[a:b], K[z], V[z], hkv, n - (b - a))
+        ref.check_rows(got[a:b], want, tol, z)
+        assert not got[a:max(a, b - n)].any()
+
+
+def test_cu_outside_the_buffer():
+    """Values that do not ascend or lie outside 0..n_tok: whatever comes of them stays
+    inside, and sequences with good ones are right."""
+    rng = rng_of("cu")
+    c, K, V = filled(rng, [30, 30, 30], 1, 32)
+    q = rng.standard_normal((40, HD)).astype(np.float32)
+    c.attn_prefill(q, [0, 2 ** 31 - 1, -5, 10 ** 6])
+    c.attn_prefill(q, [30, 20, 10, 0])
+    got = c.attn_prefill(q, [0, 20, 20, 2 ** 31 - 1])
+    for z, a, b in ((0, 0, 20), (2, 20, 40)):
+        want, tol = expect(q[a:b], K[z], V[z], 1, 30 - (b - a))
+        ref.check_rows(got[a:b], want, tol, z)
+
+
+# ---------------------------------------------------------------------------
+# what is not seen
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("bad", [np.inf, -np.inf, np.nan])
+def test_later_tokens_have_no_part(bad):
+    """An Inf or NaN in a later token's K or V reaches no earlier row, and what sees it
+    is not finite."""
+    rng = rng_of("later", str(bad))
+    H, hkv, n = 4, 2, 150
+    for at in (0, 31, 32, 77, 149):
+        c, K, V = filled(rng, [n], hkv, 32)
+        q = rng.standard_normal((n, H * HD)).astype(np.float32)
+        clean, tol = expect(q, K[0], V[0], hkv, 0)
+        for which in "kv":
+            k, v = K[0].copy(), V[0].copy()
+            (k if which == "k" else v)[at, 1, 9] = bad
+            c.append(k, v, ref.slots_of(c.table.download()[0], n, 32))
+            for x, t in ((q, 1.0), (q.astype(np.float16), None)):
+                got = c.attn_prefill(x, [0, n]).astype(np.float64)
+                hit = np.zeros(got.shape, bool)
+                hit[at:, 2 * HD:] = True                          # the second KV head's query heads
+                if which == "v":
+                    hit &= np.arange(H * HD) % HD == 9
+                    assert not np.isfinite(got[hit]).any(), (at, which)
+                if t is None:
+                    clean16, tol16 = expect(x, K[0], V[0], hkv, 0, True, 1)
+                    ref.check_rows(got[~hit], clean16[~hit], tol16[~hit], (at, which))
+                else:
+                    ref.check_rows(got[~hit], clean[~hit], tol[~hit], (at, which))
+
+
+@pytest.mark.parametrize("dtype", [np.float32, np.float16])
+def test_pages_that_are_none(dtype):
+    """Positions of a page id outside the pool are not there, in the middle of a
+    sequence, at its end or all of it."""
+    rng = rng_of("none")
+    H, hkv, page, n = 4, 2, 32, 300
+    c, K, V = filled(rng, [n, n, n], hkv, page)
+    t = c.table.download()
+    t[0, [2, 3, 9]] = [-1, c.n_pages, 2 ** 31 - 1]
+    t[1] = -2 ** 31
+    t[2, 0] = c.n_pages
+    c.table.upload(t)
+    q = rng.standard_normal((3, H * HD)).astype(dtype)
+    f16 = dtype == np.float16
+    got = c.attn_decode(q)
+    p = np.arange(n)
+    there = [np.isin(p // page, [2, 3, 9], invert=True), p < 0, p >= page]
+    for z in range(3):
+        k, v = K[z][there[z]], V[z][there[z]]
+        want, tol = expect(q[z:z + 1], k, v, hkv, len(k) - 1, f16)
+        ref.check_rows(got[z:z + 1], want, tol, z)
+    assert not got[1].any()
+    m = 290
+    q = rng.standard_normal((3 * m, H * HD)).astype(dtype)
+    got = c.attn_prefill(q, [0, m, 2 * m, 3 * m])
+    for z in range(3):
+        for i in range(m):
+            seen = there[z] & (p <= n - m + i)
+            r = z * m + i
+            if i % 7 == 0 or i > m - 3:
+                want, tol = expect(q[r:r + 1], K[z][seen], V[z][seen], hkv, seen.sum() - 1, f16, 1 if f16 else 2)
+                ref.check_rows(got[r:r + 1], want, tol, (z, i))
+    assert not got[m:2 * m].any()
+
+
+def test_lengths_outside_the_table():
+    """A length past the table's row is the row's, one below 0 is 0."""
+    rng = rng_of("outside")
+    c, K, V = filled(rng, [128, 64], 2, 64, table_pages=2)
+    q = rng.standard_normal((2, 4 * HD)).astype(np.float32)
+    for lens, n in (([10 ** 9, -3], [128, 0]), ([2 ** 31 - 1, -2 ** 31], [128, 0])):
+        c.len.upload(np.array(lens, np.int32))
+        got, pre = c.attn_decode(q), c.attn_prefill(q, [0, 1, 2])
+        for z in range(2):
+            want, tol = expect(q[z:z + 1], K[z], V[z], 2, n[z] - 1)
+            ref.check_rows(got[z:z + 1], want, tol, z)
+            ref.check_rows(pre[z:z + 1], want, tol, z)
+
+
+# ---------------------------------------------------------------------------
+# together, captured, large
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("n_pages", [30, 12])
+def test_a_serving_run(n_pages):
+    """Prompts packed, chats that join, end, take drafts back and, with few pages, stall:
+    table, cache and attention against the reference at every step."""
+    rng = rng_of("serve")
+    B, H, hkv, page = 5, 8, 2, 32
+    c = new_cache(B, hkv, n_pages, page, 12)
+    shuffle(c, rng)
+    K, V = ([np.zeros((0, hkv, HD), np.float16) for _ in range(B)] for _ in "kv")
+    stalled = 0
+    for step in range(25):
+        delta = [int(rng.choice([1, 1, 1, 4, 60, 0, -2, -1000])) if K[z].shape[0] else int(rng.integers(0, 120))
+                 for z in range(B)]
+        total = max(1, sum(max(d, 0) for d in delta))
+        s = c.step(delta, total + 3)
+        k, v = rows(rng, total + 3, hkv)
+        c.append(k, v, s["slots"])
+        lens = c.len.download()
+        for z in range(B):
+            if s["granted"][z]:
+                at = slice(s["cu"][z], s["cu"][z] + s["granted"][z])
+                K[z], V[z] = np.concatenate([K[z], k[at]]), np.concatenate([V[z], v[at]])
+            elif delta[z] < 0:
+                m = max(0, len(K[z]) + delta[z])
+                K[z], V[z] = K[z][:m], V[z][:m]
+            elif delta[z] > 0:
+                stalled += 1
+            assert lens[z] == len(K[z])
+        q = rng.standard_normal((total + 3, H * HD)).astype(np.float32)
+        got = c.attn_prefill(q, s["cu"])
+        for z in range(B):
+            if s["granted"][z]:
+                at = slice(s["cu"][z], s["cu"][z + 1])
+                want, tol = expect(q[at], K[z], V[z], hkv, lens[z] - s["granted"][z])
+                ref.check_rows(got[at], want, tol, (step, z))
+        got = c.attn_decode(q[:1].repeat(B, 0))
+        for z in range(B):
+            want, tol = expect(q[:1], K[z], V[z], hkv, lens[z] - 1)
+            ref.check_rows(got[z:z + 1], want, tol, (step, z))
+    assert stalled or n_pages > 12
+
+
+def test_behind_the_projections():
+    """As a layer uses them: a prompt's q|k|v projections leave rotated f16 rows in a
+    scratch cache, the append takes them at their positions, attention follows; then
+    a token a step, two sequences."""
+    L, rng = ops.lib(), rng_of("layer")
+    D, H, hkv, ms, page, B = 512, 8, 2, 128, 32, 2
+    Dq, Dkv = H * HD, hkv * HD
+    N = Dq + 2 * Dkv
+    Wt = ops.upload_ternary(synth.i2s_pack(ternary(rng, N, D)), D)
+    g = ops.DeviceArray.from_host(rng.uniform(0.5, 1.5, D).astype(np.float32))
+    wsc = ops.DeviceArray.from_host(rng.uniform(0.01, 0.02, N).astype(np.float32))
+    table = np.empty((ms, HD // 2, 2), np.float32)
+    ops.check(L.oxb_rope_table(table.ctypes.data, ms, HD, 500000.0))
+    rope = ops.DeviceArray.from_host(table)
+    kc, vc = (ops.DeviceArray((B, hkv, ms, HD), np.uint16, zero=True) for _ in "kv")
+    seq = hkv * ms * HD
+    c = new_cache(B, hkv, 10, page, 4)
+    K, V = [None] * B, [None] * B
+
+    def take(z, n):
+        for store, dev in ((K, kc), (V, vc)):
+            store[z] = np.ascontiguousarray(dev.download().view(np.float16)[z, :, :n].swapaxes(0, 1))
+
+    def append(s, tok_stride, sel=slice(None)):
+        slots, pos = (ops.DeviceArray.from_host(np.ascontiguousarray(s[x][sel])) for x in ("slots", "pos"))
+        return slots, pos
+
+    for z, n in enumerate((70, 45)):               # each prompt's rows from its own scratch
+        s = c.step([n if i == z else 0 for i in range(B)])
+        slots, pos = append(s, 0)
+        x = ops.DeviceArray.from_host(rng.standard_normal((n, D)).astype(np.float32))
+        pad = (n + 63) // 64 * 64
+        Xt, sc, sm = (ops.DeviceArray((pad * D,), np.int8, zero=True), ops.DeviceArray((pad,), np.float32),
+                      ops.DeviceArray((pad,), np.int32))
+        q = ops.DeviceArray((n, Dq), np.float32)
+        ops.quantize_rows_tiled(x, g, 1e-5, n, D, Xt, sc, sm)
+        ops.check(L.oxb_gemm_qkv(Wt.ptr, Xt.ptr, sc.ptr, sm.ptr, wsc.ptr, Dq, Dkv, HD, D, n, 0, q.ptr,
+                                 kc.offset(2 * z * seq), vc.offset(2 * z * seq), ms, rope.ptr, None))
+        ops.check(L.oxb_paged_append(c.pool.ptr, c.n_pages, page, hkv, HD, kc.offset(2 * z * seq),
+                                     vc.offset(2 * z * seq), 0, ms * HD, pos.ptr, slots.ptr, n, None))
+        ops.sync()
+        take(z, n)
+        got = c.attn_prefill(q.download(), s["cu"])
+        want, tol = expect(q.download(), K[z], V[z], hkv, 0)
+        ref.check_rows(got, want, tol, z)
+    q = ops.DeviceArray((B, Dq), np.float32)
+    for step in range(6):
+        before = c.len.download()
+        dp = ops.DeviceArray.from_host(before)
+        s = c.step([1] * B)
+        assert np.array_equal(s["pos"], before)
+        slots, pos = append(s, seq)
+        for z in range(B):
+            x1 = ops.DeviceArray.from_host(rng.standard_normal(D).astype(np.float32))
+            ops.check(L.oxb_bitlinear_qkv(Wt.ptr, x1.ptr, g.ptr, 1e-5, wsc.ptr, Dq, Dkv, HD, D, q.offset(4 * z * Dq),
+                                          kc.offset(2 * z * seq), vc.offset(2 * z * seq), ms, rope.ptr,
+                                          dp.offset(4 * z), None))
+        ops.check(L.oxb_paged_append(c.pool.ptr, c.n_pages, page, hkv, HD, kc.ptr, vc.ptr, seq, ms * HD, pos.ptr,
+                                     slots.ptr, B, None))
+        ops.sync()
+        got = c.attn_decode(q.download())
+        for z in range(B):
+            take(z, before[z] + 1)
+            want, tol = expect(q.download()[z:z + 1], K[z], V[z], hkv, before[z])
+            ref.check_rows(got[z:z + 1], want, tol, (step, z))
+
+
+def test_captured_step_replays():
+    """Bookkeeping, append and both attentions in one graph on a stream of its own,
+    replayed with other growths, rows and eager work between: each replay gives the
+    bits of the eager calls."""
+    L, rng = ops.lib(), rng_of("graph")
+    B, H, hkv, page, n_pages, W, n = 4, 8, 2, 32, 40, 8, 64
+    st = L.oxb_stream_create()
+    c, e = new_cache(B, hkv, n_pages, page, W), new_cache(B, hkv, n_pages, page, W)
+    dk, dv = (ops.DeviceArray((n, hkv, HD), np.uint16) for _ in "kv")
+    dq, out, one = (ops.DeviceArray(s, np.float32, zero=True) for s in ((n, H * HD), (n, H * HD), (B, H * HD)))
+    dd, cu, slots = (ops.DeviceArray((m,), np.int32) for m in (B, B + 1, n))
+    nd, np_ = L.oxb_attn_decode_paged_ws_bytes(B, H, hkv, HD), L.oxb_attn_prefill_paged_ws_bytes(n, B, H, hkv, HD)
+    ws = ops.DeviceArray((max(nd, np_),), np.uint8, zero=True)    # one workspace for both
+    ops.sync()
+    ops.check(L.oxb_stream_begin_capture(st))
+    ops.check(L.oxb_paged_update(page, B, c.len.ptr, dd.ptr, c.table.ptr, W, c.free.ptr, n_pages, c.n_free.ptr,
+                                 c.len.ptr, c.n_free.ptr, cu.ptr, None, slots.ptr, None, n, st))
+    ops.check(L.oxb_paged_append(c.pool.ptr, n_pages, page, hkv, HD, dk.ptr, dv.ptr, hkv * HD, HD, None, slots.ptr, n, st))
+    ops.check(L.oxb_attn_prefill_paged(dq.ptr, 0, c.pool.ptr, n_pages, page, c.table.ptr, W, cu.ptr, c.len.ptr, n, B, H,
+                                       hkv, HD, out.ptr, ws.ptr, max(nd, np_), st))
+    ops.check(L.oxb_attn_decode_paged(dq.ptr, 0, c.pool.ptr, n_pages, page, c.table.ptr, W, c.len.ptr, B, H, hkv, HD,
+                                      one.ptr, ws.ptr, max(nd, np_), st))
+    g = L.oxb_stream_end_capture(st)
+    assert g
+    for delta in ([30, 0, 20, 1], [1, 1, 1, 1], [40, 1, -5, 2], [1, 33, 1, 0], [-100, 9, 1, 1], [50, 1, 1, 1]):
+        k, v = rows(rng, n, hkv)
+        q = rng.standard_normal((n, H * HD)).astype(np.float32)
+        for d, x in ((dk, k.view(np.uint16)), (dv, v.view(np.uint16)), (dq, q), (dd, np.array(delta, np.int32))):
+            d.upload(x)
+        ops.check(L.oxb_graph_launch(g, st))
+        ops.check(L.oxb_stream_sync(st))
+        s = e.step(delta, n)
+        e.append(k, v, s["slots"])
+        m = s["cu"][-1]
+        assert np.array_equal(slots.download(), s["slots"]) and np.array_equal(cu.download(), s["cu"])
+        assert np.array_equal(c.table.download(), e.table.download())
+        assert np.array_equal(bits(out.download()[:m]), bits(e.attn_prefill(q, s["cu"])[:m])), delta
+        assert np.array_equal(bits(one.download()), bits(e.attn_decode(q[:B]))), delta
+        assert np.array_equal(c.pool.download(), e.pool.download())
+    ops.check(L.oxb_graph_destroy(g))
+    ops.check(L.oxb_stream_destroy(st))
+
+
+def test_two_streams_at_once():
+    """Two pools, two workspaces, two streams: each call's bits are those of the call
+    alone."""
+    L, rng = ops.lib(), rng_of("streams")
+    H, hkv, page = 8, 2, 32
+    side = []
+    for i in range(2):
+        lens = [700 - 300 * i, 64, 5]
+        c, _, _ = filled(rng, lens, hkv, page)
+        q = rng.standard_normal((60, H * HD)).astype(np.float32)
+        cu = np.array([0, 50, 58, 60], np.int32)
+        n = L.oxb_attn_prefill_paged_ws_bytes(60, 3, H, hkv, HD)
+        n = max(n, L.oxb_attn_decode_paged_ws_bytes(3, H, hkv, HD))
+        side.append((c, ops.DeviceArray.from_host(q), ops.DeviceArray.from_host(cu),
+                     ops.DeviceArray((60, H * HD), np.float32, zero=True), ops.DeviceArray((3, H * HD), np.float32),
+                     ops.DeviceArray((n,), np.uint8, zero=True), n, L.oxb_stream_create(),
+                     c.attn_prefill(q, cu), c.attn_decode(q[:3])))
+    for _ in range(10):
+        for c, dq, dc, out, one, ws, n, st, _, _ in side:
+            ops.check(L.oxb_attn_prefill_paged(dq.ptr, 0, c.pool.ptr, c.n_pages, page, c.table.ptr, c.table.shape[1],
+                                               dc.ptr, c.len.ptr, 60, 3, H, hkv, HD, out.ptr, ws.ptr, n, st))
+            ops.check(L.oxb_attn_decode_paged(dq.ptr, 0, c.pool.ptr, c.n_pages, page, c.table.ptr, c.table.shape[1],
+                                              c.len.ptr, 3, H, hkv, HD, one.ptr, ws.ptr, n, st))
+    for c, dq, dc, out, one, ws, n, st, pre, dec in side:
+        ops.check(L.oxb_stream_sync(st))
+        assert np.array_equal(bits(out.download()), bits(pre)) and np.array_equal(bits(one.download()), bits(dec))
+        ops.check(L.oxb_stream_destroy(st))
+
+
+def test_offsets_past_32_bits():
+    """A pool of 9 GB whose used pages are its last: element offsets past 2^32."""
+    rng = rng_of("far")
+    H, hkv, page = 8, 8, 4096
+    n_pages = 550
+    c = ops.PagedCache(2, hkv, n_pages, page, 2)
+    assert c.pool.nbytes > 2 * 2 ** 32        # 550 pages of 16 MB: 9.2e9 bytes
+    c.free.upload(np.arange(n_pages, dtype=np.int32))          # the last page first
+    s = c.step([5000, 90])
+    assert int(s["slots"].max()) * hkv * 2 * HD > 2 ** 32
+    k, v = rows(rng, 5090, hkv)
+    c.append(k, v, s["slots"])
+    K, V = (k[:5000], k[5000:]), (v[:5000], v[5000:])
+    q = rng.standard_normal((60, H * HD)).astype(np.float32)
+    got = c.attn_decode(q[:2])
+    pre = c.attn_prefill(q, [0, 20, 60])
+    for z, n, a, b in ((0, 5000, 0, 20), (1, 90, 20, 60)):
+        want, tol = expect(q[z:z + 1], K[z], V[z], hkv, n - 1)
+        ref.check_rows(got[z:z + 1], want, tol, z)
+        want, tol = expect(q[a:b], K[z], V[z], hkv, n - (b - a))
+        ref.check_rows(pre[a:b], want, tol, z)
