@@ -508,12 +508,14 @@ constexpr int kPreOps = kPgHalf * 2 / 16;    // 16-byte operands of a unit's K (
 constexpr int kPreLeast = 8;                 // units of a run
 constexpr int kPreSlots = 512;               // resident workgroups, at most
 constexpr int kPlanThreads = 1024;
+constexpr int64_t kPreMost = 1 << 27;        // rows of a call: 2^20 tiles, 1024 times which is in 32 bits
 constexpr size_t kPreHead = kDecParts * 4;   // decode's counters, in a workspace of both, then the counts
 
 // A run: a tile's units u0 .. u1, and a cut tile: its parts.
 struct PgRun {
     int tile, u0, u1, part;   // part -1: the tile's only run
     int cu, nq, past, z;
+    int tok, unused[3];       // the token of the tile's first row
 };
 struct PgCut {
     int tile, part, runs, cu, nq, unused[3];
@@ -524,6 +526,7 @@ struct PgPrefillArgs {
     const _Float16 *pages;
     const int *table, *cu, *len;
     int n_pages, page_log, table_stride, batch, n_tok, H, Hkv, G, most, slots, half, rows;
+    float inv_G;
     void *out;
     int *counts;    // runs, cut tiles
     PgRun *runs;    // [most]
@@ -532,43 +535,55 @@ struct PgPrefillArgs {
     float *o;       // [slots][Hkv][rows][128]
 };
 
+// Latency is all that counts here: lengths are loaded once and kept in LDS, a sum over
+// the workgroup takes one barrier, and the search for `per` starts between the bounds
+// that the units' sum gives (sum ceil(n / per) lies between sum n / per and that plus
+// the tiles), so that one round of candidates decides as a rule.
 __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PgPrefillArgs a) {
-    __shared__ uint32_t upto[kPgBatch];         // tiles of the sequences up to z
+    constexpr int kWaves = kPlanThreads / 64;
+    __shared__ int s_cu[kPgBatch], s_nq[kPgBatch], s_past[kPgBatch];
+    __shared__ uint32_t upto[kPgBatch];                 // tiles of the sequences up to z
     __shared__ int cost[kPreSlots], first[kPreSlots];   // of a tile that may be cut: units, runs up to it
-    __shared__ uint32_t wsum[kPlanThreads / 64], hist[kPlanThreads];
-    __shared__ int fit[kPlanThreads / 64], s_max, s_cuts;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, B = a.batch;
+    __shared__ int hist[kPlanThreads];
+    __shared__ uint32_t wsum[5][kWaves];
+    __shared__ int wmax[kWaves], fit[2][kWaves];
+    const int tid = threadIdx.x, lane = tid & 63, B = a.batch;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int64_t cap = (int64_t)a.table_stride << a.page_log;
-    auto scan = [&](uint32_t v) {   // inclusive, over the workgroup; saturates
-#pragma unroll
-        for (int s = 1; s < 64; s <<= 1) {
-            const uint32_t x = __shfl_up(v, s, 64);
-            if (lane >= s) v = min(v + x, 1u << 30);
-        }
-        if (lane == 63) wsum[wave] = v;
+    // Inclusive sum over the threads; `all` is the whole one.  `to` is free again after
+    // the next barrier but one.
+    auto scan = [&](int v, uint32_t *to, int &all) {
+        v = wave_iscan(v);
+        if (lane == 63) to[wave] = v;
         __syncthreads();
-        for (int w = 0; w < wave; ++w) v = min(v + wsum[w], 1u << 30);
-        __syncthreads();
-        return v;
+        const int w = wave_iscan(lane < kWaves ? (int)to[lane] : 0);
+        all = __builtin_amdgcn_readlane(w, kWaves - 1);
+        return v + (wave ? __builtin_amdgcn_readlane(w, wave - 1) : 0);
     };
-    auto start = [&](int z) { return min(max(a.cu[z], 0), a.n_tok); };
-    auto tokens = [&](int z) { return max(start(z + 1) - start(z), 0); };
-    auto tiles_of = [&](int z) { return (uint32_t)(((int64_t)tokens(z) * a.G + kPreRows - 1) / kPreRows); };
-    if (tid == 0) s_max = s_cuts = 0;
-    uint32_t base = 0;
-    for (int c = 0; c < B; c += kPlanThreads) {   // (uniform)
+    hist[tid] = 0;
+    int nt = 0;   // (cut off at what a cu that ascends has at most)
+    for (int c = 0, i = 0; c < B; c += kPlanThreads, i ^= 1) {   // (uniform)
         const int z = c + tid;
-        const uint32_t v = min(base + scan(z < B ? tiles_of(z) : 0), 1u << 30);
-        if (z < B) upto[z] = v;
-        __syncthreads();
-        base = upto[min(c + kPlanThreads, B) - 1];
+        int tiles = 0;
+        if (z < B) {
+            const int c0 = min(max(a.cu[z], 0), a.n_tok), c1 = min(max(a.cu[z + 1], 0), a.n_tok);
+            const int nq = max(c1 - c0, 0);
+            s_cu[z] = c0;
+            s_nq[z] = nq;
+            s_past[z] = (int)(min(max((int64_t)a.len[z], (int64_t)0), cap) - nq);
+            tiles = (nq * a.G + kPreRows - 1) / kPreRows;
+        }
+        int all;
+        const int v = scan(tiles, wsum[i], all);
+        if (z < B) upto[z] = nt + v;
+        nt = min(nt + all, a.most);
     }
-    const int nt = (int)min(base, (uint32_t)a.most);   // (more: cu does not ascend)
-    // tile t: sequence, index, units that its last row sees
+    __syncthreads();
+    const bool cut = nt <= a.slots;
     struct Tile {
-        int z, i, nq, past, units;
+        int z, i, units;
     };
-    auto tile = [&](int t) {
+    auto tile = [&](int t) {   // sequence, index in it, units that its last row sees
         int lo = 0, hi = B - 1;
         while (lo < hi) {
             const int mid = (lo + hi) >> 1;
@@ -578,58 +593,60 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PgPrefillArgs 
         Tile r;
         r.z = lo;
         r.i = t - (lo ? (int)upto[lo - 1] : 0);
-        r.nq = tokens(lo);
-        const int64_t held = min(max((int64_t)a.len[lo], (int64_t)0), cap);
-        r.past = (int)(held - r.nq);
-        const int64_t last = min((int64_t)(r.i + 1) * kPreRows, (int64_t)r.nq * a.G) - 1;
-        r.units = pg_units(max((int64_t)r.past + last / a.G + 1, (int64_t)0));
+        const int last = min((r.i + 1) * kPreRows, s_nq[lo] * a.G) - 1;
+        r.units = pg_units(max(s_past[lo] + last / a.G + 1, 0));
         return r;
     };
-    int mx = 0;
-    const bool cut = nt <= a.slots;
-    for (int t = tid; t < nt; t += kPlanThreads) {
-        const int u = tile(t).units;
-        if (cut) cost[t] = u;
-        mx = max(mx, u);
+    Tile own{0, 0, 0};   // of a tile a thread, where they may be cut
+    int mx = 0, sum = 0;
+    if (cut) {
+        if (tid < nt) {
+            own = tile(tid);
+            cost[tid] = mx = sum = own.units;
+        }
+    } else {
+        for (int t = tid; t < nt; t += kPlanThreads) mx = max(mx, tile(t).units);
     }
-    if (mx) atomicMax(&s_max, mx);
-    __syncthreads();
-    // the least run length whose runs all are resident: 16 candidates at a time, one a wave
-    int per = max(s_max, 1), lo = kPreLeast, hi = per;
-    while (cut && lo < hi) {
-        const int step = (hi - lo + kPlanThreads / 64 - 1) / (kPlanThreads / 64), c = min(hi, lo + wave * step);
-        int n = 0;
-        for (int t = lane; t < nt; t += 64) n += max(1, (cost[t] + c - 1) / c);
-        n = wave_isum_dpp(n);
-        if (lane == 0) fit[wave] = n <= a.slots;
-        __syncthreads();
-        int w = 0;
-        while (w < kPlanThreads / 64 && !fit[w]) ++w;
-        const int l = lo;
-        if (w < kPlanThreads / 64) hi = min(hi, l + w * step);
-        if (w > 0) lo = min(hi, l + (w - 1) * step + 1);
+#pragma unroll
+    for (int s = 32; s > 0; s >>= 1) mx = max(mx, __shfl_xor(mx, s, 64));
+    if (lane == 0) wmax[wave] = mx;
+    scan(sum, wsum[2], sum);
+    mx = lane < kWaves ? wmax[lane] : 0;
+#pragma unroll
+    for (int s = 32; s > 0; s >>= 1) mx = max(mx, __shfl_xor(mx, s, 64));
+    int per = max(mx, 1), total = nt, cuts = 0;
+    if (cut) {
+        // the least run length whose runs all are resident: a candidate a wave
+        int lo = max(kPreLeast, nt ? sum / a.slots : 0), hi = per;
+        if (nt < a.slots) hi = min(hi, max(lo, (sum + a.slots - nt - 1) / (a.slots - nt)));
+        for (int i = 0; lo < hi; i ^= 1) {
+            const int step = (hi - lo + kWaves - 1) / kWaves, c = min(hi, lo + wave * step);
+            int n = 0;
+            for (int t = lane; t < nt; t += 64) n += max(1, (cost[t] + c - 1) / c);
+            n = wave_isum_dpp(n);
+            if (lane == 0) fit[i][wave] = n <= a.slots;
+            __syncthreads();
+            const uint64_t ok = __ballot(lane < kWaves && fit[i][lane & (kWaves - 1)]);
+            const int w = ok ? __builtin_ctzll(ok) : kWaves, l = lo;
+            if (w < kWaves) hi = min(hi, l + w * step);
+            if (w > 0) lo = min(hi, l + (w - 1) * step + 1);
+        }
+        per = max(hi, 1);
+        // runs of the tiles up to each, and cut tiles above bit 16
+        const int k = tid < nt ? max(1, (own.units + per - 1) / per) : 0;
+        const int v = scan(k | (k > 1 ? 1 << 16 : 0), wsum[3], total);
+        cuts = total >> 16;
+        total &= 0xffff;
+        if (tid < nt) first[tid] = v & 0xffff;
+        if (k > 1) a.cuts[(v >> 16) - 1] = PgCut{own.i, (v & 0xffff) - k, k, s_cu[own.z], s_nq[own.z], {0, 0, 0}};
         __syncthreads();
     }
-    if (cut) per = hi;
-    int total = nt;
-    if (cut) {   // runs of the tiles up to each (slots <= threads)
-        const int k = tid < nt ? max(1, (cost[tid] + per - 1) / per) : 0;
-        const uint32_t v = scan(k);
-        if (tid < nt) first[tid] = v;
-        __syncthreads();
-        total = nt ? first[nt - 1] : 0;
+    if (tid == 0) {
+        a.counts[0] = total;
+        a.counts[1] = cuts;
     }
-    hist[tid] = 0;
-    __syncthreads();
-    struct Run {
-        Tile t;
-        int id, k, i, u0, u1;
-    };
     auto run = [&](int j) {
-        Run r;
-        r.id = j;
-        r.k = 1;
-        r.i = 0;
+        int k = 1, i = 0, t = j;
         if (cut) {
             int l = 0, h = nt - 1;
             while (l < h) {
@@ -638,39 +655,36 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PgPrefillArgs 
                 else l = mid + 1;
             }
             const int before = l ? first[l - 1] : 0;
-            r.id = l;
-            r.k = first[l] - before;
-            r.i = j - before;
+            t = l;
+            k = first[l] - before;
+            i = j - before;
         }
-        r.t = tile(r.id);
-        r.u0 = (int)((int64_t)r.t.units * r.i / r.k);
-        r.u1 = (int)((int64_t)r.t.units * (r.i + 1) / r.k);
-        return r;
+        const Tile r = tile(t);
+        // (units < 2^20, runs <= 512)
+        return PgRun{r.i, r.units * i / k, r.units * (i + 1) / k, k > 1 ? j : -1, s_cu[r.z], s_nq[r.z], s_past[r.z],
+                     r.z, r.i * kPreRows / a.G, {0, 0, 0}};
     };
     // the longest first, to a thousandth of the longest
-    auto bucket = [&](const Run &r) {
-        return (int)((int64_t)(per - min(per, r.u1 - r.u0)) * (kPlanThreads - 1) / per);
-    };
-    for (int j = tid; j < total; j += kPlanThreads) atomicAdd(&hist[bucket(run(j))], 1u);
-    __syncthreads();
-    const uint32_t mine = hist[tid], v = scan(mine);
-    hist[tid] = v - mine;
-    __syncthreads();
+    const float scale = (float)(kPlanThreads - 1) / (float)per;
+    auto bucket = [&](const PgRun &r) { return (int)((float)(per - min(per, r.u1 - r.u0)) * scale); };
     const int two = min(2 * a.half, total);
-    for (int j = tid; j < total; j += kPlanThreads) {
-        const Run r = run(j);
-        int at = (int)atomicAdd(&hist[bucket(r)], 1u);
+    auto put = [&](const PgRun &r) {
+        int at = atomicAdd(&hist[bucket(r)], 1);
         // of those that run at once, the second half the other way round: a CU gets
         // the longest and the shortest
         if (at >= a.half && at < two) at = a.half + two - 1 - at;
-        a.runs[at] = PgRun{r.t.i, r.u0, r.u1, r.k > 1 ? j : -1, start(r.t.z), r.t.nq, r.t.past, r.t.z};
-        if (r.k > 1 && r.i == 0) a.cuts[atomicAdd(&s_cuts, 1)] = PgCut{r.t.i, j, r.k, start(r.t.z), r.t.nq, {0, 0, 0}};
-    }
+        a.runs[at] = r;
+    };
+    PgRun mine{};
+    if (tid < total) mine = run(tid);
+    for (int j = tid; j < total; j += kPlanThreads) atomicAdd(&hist[bucket(j == tid ? mine : run(j))], 1);
     __syncthreads();
-    if (tid == 0) {
-        a.counts[0] = total;
-        a.counts[1] = s_cuts;
-    }
+    const int h = hist[tid];
+    int all;
+    const int v = scan(h, wsum[4], all);
+    hist[tid] = v - h;
+    __syncthreads();
+    for (int j = tid; j < total; j += kPlanThreads) put(j == tid ? mine : run(j));
 }
 
 // 16 bytes of each lane from base + off to LDS at m0 + 16 * lane (as lds_dma16, with a
@@ -684,106 +698,155 @@ __device__ __forceinline__ void pg_dma16(const void *base, uint32_t off, uint32_
         : "memory");
 }
 
+// What all lanes read and no kernel in flight writes: by scalar loads.
+template <typename R>
+__device__ __forceinline__ R pg_uniform(const R *p) {
+    static_assert(sizeof(R) % 4 == 0, "whole words");
+    struct Words {
+        int w[sizeof(R) / 4];
+    } r;
+    const auto *c = (const __attribute__((address_space(4))) int *)p;
+#pragma unroll
+    for (unsigned i = 0; i < sizeof(R) / 4; ++i) r.w[i] = c[i];
+    return __builtin_bit_cast(R, r);
+}
+
+// A row's 16-byte pieces lie in LDS exchanged by the row's number, so that neither a
+// piece of all rows nor a row's pieces meet in a bank.
+template <int PIECES>
+__device__ __forceinline__ int pg_piece(int row, int c) { return row * PIECES + (c ^ (row & (PIECES - 1))); }
+
 template <typename T>
 __global__ __launch_bounds__(kPreThreads, 2) void paged_prefill_kernel(PgPrefillArgs a) {
     constexpr int PARTS = std::is_same<T, float>::value ? 2 : 1;
-    // rings of K [8][64] and V operands [4 dims][2][64]: unit u of the run in slot u % 4
-    __shared__ uint4 lds[2][kPreRing][kPreOps];
-    auto &sk = lds[0], &sv = lds[1];
+    // rings of K [8][64] and V operands [4 dims][2][64]: unit u of the run in slot u % 4.
+    // The rows of q lie in V's ring and in K's behind its first slot before, those of
+    // the output in all of them after.
+    __shared__ uint4 lds[2 * kPreRing + PARTS - 1][kPreOps];
+    uint4(*sk)[kPreOps] = lds, (*sv)[kPreOps] = lds + kPreRing + PARTS - 1;
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int kvh = blockIdx.x % a.Hkv, item = blockIdx.x / a.Hkv;
-    if (item >= a.counts[0]) return;
-    const PgRun run = a.runs[item];
-    const int rows = run.nq * a.G, r0 = run.tile * kPreRows, row = r0 + wave * 32 + (lane & 31), h = lane >> 5;
-    const int b0 = run.u0, b1 = run.u1;
+    // (the record with the count; past it, whatever is there)
+    const PgRun run = pg_uniform(a.runs + item);
+    if (item >= pg_uniform(a.counts)) return;
+    const int r0 = run.tile * kPreRows, rows = min(kPreRows, run.nq * a.G - r0);   // of the tile
+    const int b0 = run.u0, b1 = run.u1, h = lane >> 5;
+    // x / G for x below 2^22: x + 1/2 is 1 / 2G or more from every multiple of G, the
+    // product 2^-23 of it off at most
+    const int rest = r0 - run.tok * a.G;
+    auto tok_of = [&](int r) { return (int)(((float)(rest + r) + 0.5f) * a.inv_G); };   // from run.tok on
+    T *out = (T *)a.out + ((size_t)(run.cu + run.tok) * a.H + kvh * a.G) * kPgHd;
+    const T *q = (const T *)a.q + ((size_t)(run.cu + run.tok) * a.H + kvh * a.G) * kPgHd;
+    const int wrow = wave * 32, row = wrow + (lane & 31);   // of the tile
+    const int tok = tok_of(min(row, rows - 1));
+    const int qrow = tok * a.H + rest + min(row, rows - 1) - tok * a.G;   // its row from q on
     if (b0 >= b1) {   // the tile sees nothing
-        for (int i = tid; i < min(kPreRows, rows - r0) * kPgHd; i += kPreThreads) {
-            const int r = r0 + i / kPgHd;
-            ((T *)a.out)[((size_t)(run.cu + r / a.G) * a.H + kvh * a.G + r % a.G) * kPgHd + i % kPgHd] = (T)0.0f;
+        for (int r = 0; r < 32; ++r) {
+            const int at = __builtin_amdgcn_readlane(qrow, r);
+            if (wrow + r < rows)
+                for (int i = lane; i < kPgHd; i += 64) out[(size_t)at * kPgHd + i] = (T)0.0f;
         }
         return;
     }
-    const int tok = min(row, rows - 1) / a.G, head = kvh * a.G + min(row, rows - 1) % a.G;
-    const int qpos = run.past + tok;
+    const int past = run.past + run.tok, qpos = past + tok;
     // positions that the wave's last and first rows see (none: no row at all)
-    const bool some = r0 + wave * 32 < rows;
-    const int wseen = some ? run.past + min(r0 + wave * 32 + 31, rows - 1) / a.G + 1 : 0;
-    const int wfull = run.past + min(r0 + wave * 32, rows - 1) / a.G + 1;
+    const bool some = wrow < rows;
+    const int wseen = some ? past + tok_of(min(wrow + 31, rows - 1)) + 1 : 0;
+    const int wfull = past + tok_of(min(wrow, rows - 1)) + 1;
     const int wb = max(b0, min(b1, pg_units(max(wseen, 0))));
 
-    // (the constant space: looked up by scalar loads, which wait for no others)
-    const auto *table = (const __attribute__((address_space(4))) int *)(a.table + (size_t)run.z * a.table_stride);
+    // Pages by lanes: of the run's first units, and of 64 from unit b0 + 3 on, which is
+    // the first that the loop brings.
+    const int *table = a.table + (size_t)run.z * a.table_stride;
+    auto load_ids = [&](int u) { return table[min(u + lane, b1 - 1) >> (a.page_log - 5)]; };
     const int in_page = (1 << (a.page_log - 5)) - 1;
+    const int ids0 = load_ids(b0);
+    int ids = load_ids(b0 + 3);
     uint32_t gone = 0;   // bit u % 32: unit u's page is none
-    auto unit = [&](int u) {
-        const int c = min(u, b1 - 1);
-        int id = __builtin_amdgcn_readfirstlane(table[c >> (a.page_log - 5)]);
+    auto unit = [&](int id, int u) {
         const uint32_t bit = 1u << (u & 31);
         gone &= ~bit;
         if ((unsigned)id >= (unsigned)a.n_pages) {
             gone |= bit;
             id = 0;
         }
-        return a.pages + paged_unit(id, kvh, c & in_page, a.Hkv, a.page_log);
+        return a.pages + paged_unit(id, kvh, min(u, b1 - 1) & in_page, a.Hkv, a.page_log);
     };
     // a wave brings 32 dims of K and of V of each unit: operands 2 wave, 2 wave + 1.
     // MFMA row i holds position i with bits 2 and 3 exchanged.
     const int kpos = (lane & 19) | ((lane & 4) << 1) | ((lane & 8) >> 1);
     const uint32_t koff = 2 * paged_k_elem(kpos, 8 * (4 * wave + h));
     const uint32_t voff = 2 * paged_v_elem(8 * h, 32 * wave + (lane & 31));
-    const uint32_t lds0 = (uint32_t)(size_t)(__attribute__((address_space(3))) void *)&lds[0][0][0] + 2048 * wave;
+    const uint32_t lds0 = (uint32_t)(size_t)(__attribute__((address_space(3))) void *)&lds[0][0] + 2048 * wave;
     auto bring_k = [&](const _Float16 *p, int r) {
         const uint32_t to = lds0 + (r & 3) * kPreOps * 16;
         pg_dma16(p, koff, to);
         pg_dma16(p, koff + 2 * kPgUnit * 16, to + 1024);
     };
     auto bring_v = [&](const _Float16 *p, int r) {
-        const uint32_t to = lds0 + (kPreRing + (r & 3)) * kPreOps * 16;
+        const uint32_t to = lds0 + (kPreRing + PARTS - 1 + (r & 3)) * kPreOps * 16;
         pg_dma16(p, voff, to);
         pg_dma16(p, voff + 2 * kPgHd * 16, to + 1024);
     };
-    const _Float16 *u0 = unit(b0), *u1 = unit(b0 + 1), *u2 = unit(b0 + 2);
-    bring_k(u0, 0);
-    bring_k(u1, 1);
-    bring_k(u2, 2);
-    bring_v(u0, 0);
-    bring_v(u1, 1);
 
-    // q: dims 16 s + 8 h + j are operand s
+    // q through LDS, 256 bytes of each row at a time (a lane loading its own row's
+    // pieces meets 32 rows with each load), to operand s: dims 16 s + 8 h + j of row
+    // lane % 32
     half8_t qh[8], ql[8];
     float qs = kPgScore;
-    {
-        const T *q = (const T *)a.q + ((size_t)(run.cu + tok) * a.H + head) * kPgHd + 8 * h;
-        if constexpr (PARTS == 1) {
+    const _Float16 *u0 = unit(__builtin_amdgcn_readlane(ids0, 0), b0);
+    const _Float16 *u1 = unit(__builtin_amdgcn_readlane(ids0, 1), b0 + 1);
+    const _Float16 *u2 = unit(__builtin_amdgcn_readlane(ids0, 2), b0 + 2);
+    bring_k(u0, 0);
+    uint4 *sq[2] = {&sv[0][0] + 512 * wave, &sk[1][0] + 512 * wave};
 #pragma unroll
-            for (int s = 0; s < 8; ++s) qh[s] = *(const half8_t *)(q + 16 * s);
-        } else {
-            float v[64];
-            float m = 0.0f;
+    for (int i = 0; i < 8; ++i) {
+        const int r = 4 * i + (lane >> 4), c = (lane & 15) ^ (r & 15);
+        const uint32_t off = __shfl(qrow, r, 64) * (uint32_t)(kPgHd * sizeof(T)) + 16 * c;
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const float4 f = *(const float4 *)(q + 16 * (i >> 1) + 4 * (i & 1));
-                v[4 * i] = f.x;
-                v[4 * i + 1] = f.y;
-                v[4 * i + 2] = f.z;
-                v[4 * i + 3] = f.w;
-            }
+        for (int p = 0; p < PARTS; ++p)
+            pg_dma16(q, off + 256 * p, lds0 - 2048 * wave + (uint32_t)((char *)(sq[p] + 64 * i) - (char *)&lds[0][0]));
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    if constexpr (PARTS == 1) {
 #pragma unroll
-            for (int i = 0; i < 64; i += 2) m = fmaxf(fmaxf(fabsf(v[i]), fabsf(v[i + 1])), m);
-            m = fmaxf(m, __shfl_xor(m, 32, 64));
-            const int e = max(pg_row_exp(m), -127);   // (a row below 2^-113 stays below 2^kPgQExp)
-            const float up = ldexpf(1.0f, -e);
-            qs = ldexpf(kPgScore, e);
+        for (int s = 0; s < 8; ++s)
+            qh[s] = __builtin_bit_cast(half8_t, sq[0][pg_piece<16>(lane & 31, 2 * s + h)]);
+    } else {
+        float v[64];
+        float m = 0.0f;
 #pragma unroll
-            for (int s = 0; s < 8; ++s)
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const float x = v[8 * s + j] * up;
-                    qh[s][j] = (_Float16)x;
-                    ql[s][j] = (_Float16)(x - (float)qh[s][j]);
-                }
+        for (int i = 0; i < 16; ++i) {
+            const float4 f = __builtin_bit_cast(float4, sq[i >> 3][pg_piece<16>(lane & 31, 4 * (i >> 1 & 3) + 2 * h + (i & 1))]);
+            v[4 * i] = f.x;
+            v[4 * i + 1] = f.y;
+            v[4 * i + 2] = f.z;
+            v[4 * i + 3] = f.w;
         }
+#pragma unroll
+        for (int i = 0; i < 64; i += 2) m = fmaxf(fmaxf(fabsf(v[i]), fabsf(v[i + 1])), m);
+        m = fmaxf(m, __shfl_xor(m, 32, 64));
+        const int e = max(pg_row_exp(m), -127);   // (a row below 2^-113 stays below 2^kPgQExp)
+        const float up = ldexpf(1.0f, -e);
+        qs = ldexpf(kPgScore, e);
+        // each part rounded once from the exact product
+#pragma unroll
+        for (int s = 0; s < 8; ++s)
+#pragma unroll
+            for (int j = 0; j < 8; j += 2) {
+                const float x = v[8 * s + j], y = v[8 * s + j + 1];
+                half2_t hi, lo;
+                hi.x = (_Float16)__builtin_fmaf(x, up, 0.0f);
+                hi.y = (_Float16)__builtin_fmaf(y, up, 0.0f);
+                asm("" : "+v"(hi));
+                lo.x = (_Float16)__builtin_fmaf(x, up, -(float)hi.x);
+                lo.y = (_Float16)__builtin_fmaf(y, up, -(float)hi.y);
+                qh[s][j] = hi.x;
+                qh[s][j + 1] = hi.y;
+                ql[s][j] = lo.x;
+                ql[s][j + 1] = lo.y;
+            }
     }
     f32x16 o[4];
 #pragma unroll
@@ -793,8 +856,11 @@ __global__ __launch_bounds__(kPreThreads, 2) void paged_prefill_kernel(PgPrefill
     PgRef ref;
     float lsum = 0.0f;
 
-    wait_vmcnt<0>();
-    lds_barrier();
+    lds_barrier();   // the first K is there, and every wave has its q
+    bring_k(u1, 1);
+    bring_k(u2, 2);
+    bring_v(u0, 0);
+    bring_v(u1, 1);
     f32x16 s0, s1;
 #pragma unroll
     for (int i = 0; i < 16; ++i) s0[i] = 0.0f;
@@ -804,13 +870,14 @@ __global__ __launch_bounds__(kPreThreads, 2) void paged_prefill_kernel(PgPrefill
         s0 = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, qh[i], s0, 0, 0, 0);
         if constexpr (PARTS == 2) s0 = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, ql[i], s0, 0, 0, 0);
     }
-    lds_barrier();   // the first K slot is free
     // the running maximum with four more scores (in v_max3's form)
     auto top = [&](float m, const f32x16 &s, int i) {
         m = fmaxf(fmaxf(s[i], s[i + 1]), m);
         return fmaxf(fmaxf(s[i + 2], s[i + 3]), m);
     };
     float smax = top(top(top(top(kPgNone, s0, 0), s0, 4), s0, 8), s0, 12);
+    wait_vmcnt<0>();
+    lds_barrier();   // the others are there, and the first K slot is free
     // Unit b, its scores in s and their maximum in smax; the next one's go to sn.
     // r: b's place in the run; SOME: some rows may not see all of it.
     auto block = [&](auto SOME, int b, int r, f32x16 &s, f32x16 &sn) {
@@ -840,7 +907,8 @@ __global__ __launch_bounds__(kPreThreads, 2) void paged_prefill_kernel(PgPrefill
         const uint4 *kb = sk[(r + 1) & 3] + lane, *vb = sv[r & 3] + lane;
         half8_t ph[2], pl[2], v[4], k[2];
         float pa, pb, ps = 0.0f;
-        uint32_t odd = 0;   // V that is not finite has been taken out
+        uint32_t found = 0;   // bits 15 and 31: V that is not finite
+        bool wild = false;
         auto exps = [&](int j) {   // elements 2 j, 2 j + 1
             pa = __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * j], qs, -moff));
             pb = __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * j + 1], qs, -moff));
@@ -863,21 +931,30 @@ __global__ __launch_bounds__(kPreThreads, 2) void paged_prefill_kernel(PgPrefill
                 pl[j >> 2][2 * (j & 3) + 1] = lo.y;
             }
         };
+        auto look = [&](int i) {   // at operand i of V
+            const uint4 x = vb[64 * i];
+            auto word = [&](uint32_t w) { found |= (w & 0x7c007c00u) + 0x04000400u; };
+            word(x.x);
+            word(x.y);
+            word(x.z);
+            word(x.w);
+        };
+        // (of a unit with V that is not finite, only what the wave's last row sees and
+        // is finite)
         auto get_v = [&](int d, int m) {
             uint4 x = vb[d * 128 + 64 * m];
             if constexpr (some_hidden) {
-                // seen by the wave's last row
-                const int left = (there ? wseen - p0 - 8 * h : 0) - 16 * m + opaque_zero();
-                auto word = [&](uint32_t &w, int j) {
-                    w &= pg_first2(left - 2 * j);
-                    const uint32_t wild = pg_wild2(w);
-                    odd |= wild;
-                    w &= ~(wild * 0xffffu);
-                };
-                word(x.x, 0);
-                word(x.y, 1);
-                word(x.z, 2);
-                word(x.w, 3);
+                if (wild) {   // uniform
+                    const int left = (there ? wseen - p0 - 8 * h : 0) - 16 * m + opaque_zero();
+                    auto word = [&](uint32_t &w, int j) {
+                        w &= pg_first2(left - 2 * j);
+                        w &= ~(pg_wild2(w) * 0xffffu);
+                    };
+                    word(x.x, 0);
+                    word(x.y, 1);
+                    word(x.z, 2);
+                    word(x.w, 3);
+                }
             }
             return __builtin_bit_cast(half8_t, x);
         };
@@ -890,11 +967,14 @@ __global__ __launch_bounds__(kPreThreads, 2) void paged_prefill_kernel(PgPrefill
         for (int i = 0; i < 8; ++i) {
             sn = __builtin_amdgcn_mfma_f32_32x32x16_f16(k[i & 1], qh[i], sn, 0, 0, 0);
             if (i < 6) exps(i);
+            if (some_hidden && i < 4) look(2 * i);
             if constexpr (PARTS == 2) {
                 SLOT();
                 sn = __builtin_amdgcn_mfma_f32_32x32x16_f16(k[i & 1], ql[i], sn, 0, 0, 0);
             }
+            if (some_hidden && i < 4) look(2 * i + 1);
             if (i < 6) split(i);
+            if (some_hidden && i == 5) wild = __any(found & 0x80008000u);
             if (i < 6) k[i & 1] = __builtin_bit_cast(half8_t, kb[(i + 2) * 64]);
             else
                 for (int d = 2 * (i - 6); d < 2 * (i - 5); ++d) v[d] = get_v(d, 0);
@@ -929,7 +1009,7 @@ __global__ __launch_bounds__(kPreThreads, 2) void paged_prefill_kernel(PgPrefill
 #undef SLOT
         lsum += ps;
         if constexpr (some_hidden) {
-            if (__any(odd)) {   // a dim of a row that sees such a V is NaN
+            if (wild) {   // a dim of a row that sees such a V is NaN
                 const int seen = there ? wseen - p0 - 8 * h : 0, sees = there ? qpos + 1 - p0 - 8 * h : 0;
                 for (int d = 0; d < 4; ++d) {
                     f32x16 n;
@@ -963,20 +1043,20 @@ __global__ __launch_bounds__(kPreThreads, 2) void paged_prefill_kernel(PgPrefill
     // full speed and the other, at half of it, finishes late.
     uint32_t hwid;
     asm volatile("s_getreg_b32 %0, hwreg(HW_REG_HW_ID)" : "=s"(hwid));
-    // pages of the pair after next's units are looked up a pair ahead
-    const _Float16 *u3 = unit(b0 + 3), *u4 = unit(b0 + 4);
     // K of b + 3, b + 4 and V of b + 2, b + 3 come under the pair b, b + 1
     auto bring = [&](int b) {
         const int r = b - b0;
+        if (((r >> 1) ^ hwid) & 1) __builtin_amdgcn_s_setprio(1);
+        else __builtin_amdgcn_s_setprio(0);
+        if (b + 2 >= b1) return;   // uniform
+        const _Float16 *u3 = unit(__builtin_amdgcn_readlane(ids, r & 63), b + 3);
+        const _Float16 *u4 = unit(__builtin_amdgcn_readlane(ids, (r & 63) + 1), b + 4);
         bring_k(u3, r + 3);
         bring_k(u4, r + 4);
         bring_v(u2, r + 2);
         bring_v(u3, r + 3);
         u2 = u4;
-        u3 = unit(b + 5);
-        u4 = unit(b + 6);
-        if (((r >> 1) ^ hwid) & 1) __builtin_amdgcn_s_setprio(1);
-        else __builtin_amdgcn_s_setprio(0);
+        if ((r & 63) == 62) ids = load_ids(b + 5);   // (waited for with the pair)
     };
     // pairs that every row of the wave sees whole, then the rest of the run (with
     // one loop of both, the registers do not suffice)
@@ -999,28 +1079,43 @@ __global__ __launch_bounds__(kPreThreads, 2) void paged_prefill_kernel(PgPrefill
         lds_barrier();
     }
     lsum += __shfl_xor(lsum, 32, 64);
-    // the lane's row again (not held in registers over the loop)
-    const int elane = lane + opaque_zero(), eh = elane >> 5, erow = r0 + wave * 32 + (elane & 31);
-    if (erow >= rows) return;
-    // lane's dims: 32 d + 8 k + 4 h + 0..3
-    if (run.part < 0) {
-        T *dst = (T *)a.out + ((size_t)(run.cu + erow / a.G) * a.H + kvh * a.G + erow % a.G) * kPgHd;
-        const float f = lsum == 0.0f ? 0.0f : 1.0f / lsum;
+    if (!some) return;
+    // The rows of the output whole, through LDS: a lane's dims are 32 d + 8 k + 4 h + 0..3
+    // of its row.  (Stored from there, 16 or 32 bytes a row with each store: twice the
+    // time.)
+    const bool direct = run.part < 0;
+    const float f = !direct ? 1.0f : lsum == 0.0f ? 0.0f : 1.0f / lsum;
+    uint4 *so = &lds[0][0] + 1024 * wave;
+    const int er = lane & 31;
+    if (direct && PARTS == 1) {
 #pragma unroll
         for (int d = 0; d < 4; ++d)
 #pragma unroll
             for (int k = 0; k < 4; ++k)
-                pg_store4(dst + 32 * d + 8 * k + 4 * eh, o[d][4 * k] * f, o[d][4 * k + 1] * f, o[d][4 * k + 2] * f,
-                          o[d][4 * k + 3] * f);
-    } else {
-        const size_t at = ((size_t)run.part * a.Hkv + kvh) * a.rows + (erow - r0);
-        if (eh == 0) a.ml[at] = make_float2(ref.part(), lsum);
+                pg_store4((_Float16 *)&so[pg_piece<16>(er, 4 * d + k)] + 4 * h, o[d][4 * k] * f, o[d][4 * k + 1] * f,
+                          o[d][4 * k + 2] * f, o[d][4 * k + 3] * f);
 #pragma unroll
-        for (int d = 0; d < 4; ++d)
+        for (int i = 0; i < 8; ++i) {
+            const int r = 4 * i + (lane >> 4), at = __shfl(qrow, r, 64);
+            const uint4 x = so[pg_piece<16>(r, lane & 15)];
+            if (wrow + r < rows) *(uint4 *)(out + (size_t)at * kPgHd + 8 * (lane & 15)) = x;
+        }
+        return;
+    }
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-                pg_store4(a.o + at * kPgHd + 32 * d + 8 * k + 4 * eh, o[d][4 * k], o[d][4 * k + 1], o[d][4 * k + 2],
-                          o[d][4 * k + 3]);
+    for (int d = 0; d < 4; ++d)
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            pg_store4((float *)&so[pg_piece<32>(er, 8 * d + 2 * k + h)], o[d][4 * k] * f, o[d][4 * k + 1] * f,
+                      o[d][4 * k + 2] * f, o[d][4 * k + 3] * f);
+    const size_t first = ((size_t)run.part * a.Hkv + kvh) * a.rows + wrow;   // (of a part)
+    if (!direct && h == 0 && row < rows) a.ml[first + er] = make_float2(ref.part(), lsum);
+    float *dst = direct ? (float *)out : a.o + first * kPgHd;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        const int r = 2 * i + h, at = direct ? __shfl(qrow, r, 64) : r;
+        const uint4 x = so[pg_piece<32>(r, lane & 31)];
+        if (wrow + r < rows) *(uint4 *)(dst + (size_t)at * kPgHd + 4 * (lane & 31)) = x;
     }
 }
 
@@ -1028,8 +1123,8 @@ __global__ __launch_bounds__(kPreThreads, 2) void paged_prefill_kernel(PgPrefill
 template <typename T>
 __global__ __launch_bounds__(256) void paged_join_kernel(PgPrefillArgs a) {
     const int c = blockIdx.x / (kPreRows / 8), kvh = blockIdx.y, d = (threadIdx.x & 31) * 4;
-    if (c >= a.counts[1]) return;
-    const PgCut t = a.cuts[c];
+    const PgCut t = pg_uniform(a.cuts + c);   // (with the count; past it, whatever is there)
+    if (c >= pg_uniform(a.counts + 1)) return;
     const int lrow = blockIdx.x % (kPreRows / 8) * 8 + (threadIdx.x >> 5), row = t.tile * kPreRows + lrow;
     if (row >= t.nq * a.G) return;
     const size_t step = (size_t)a.Hkv * a.rows, r = ((size_t)t.part * a.Hkv + kvh) * a.rows + lrow;
@@ -1146,7 +1241,7 @@ extern "C" int oxb_attn_decode_paged(const void *q, int dtype, const void *pages
 
 extern "C" size_t oxb_attn_prefill_paged_ws_bytes(int n_tok, int batch, int H, int Hkv, int hd) {
     if (n_tok < 1 || batch < 1 || batch > kPgBatch || Hkv < 1 || Hkv > 4096 || H < 1 || H % Hkv || H > 65535 ||
-        hd != kPgHd || (int64_t)n_tok * (H / Hkv) > (1 << 30))
+        hd != kPgHd || (int64_t)n_tok * (H / Hkv) > kPreMost)
         return 0;
     return prefill_plan(n_tok, batch, H / Hkv, Hkv).bytes;
 }
@@ -1161,14 +1256,14 @@ extern "C" int oxb_attn_prefill_paged(const void *q, int dtype, const void *page
         return -1;
     OXB_REQUIRE(cu && len, "prefill attention: cu or len is NULL");
     const int G = H / Hkv;
-    OXB_REQUIRE(n_tok >= 1 && (int64_t)n_tok * G <= (1 << 30), "prefill attention: %d tokens", n_tok);
+    OXB_REQUIRE(n_tok >= 1 && (int64_t)n_tok * G <= kPreMost, "prefill attention: %d tokens", n_tok);
     const PrefillPlan p = prefill_plan(n_tok, batch, G, Hkv);
     OXB_REQUIRE(p.items * Hkv < (1 << 24), "prefill attention: %d tokens of %d heads", n_tok, H);
     OXB_REQUIRE(ws && ((uintptr_t)ws & 255) == 0 && ws_bytes >= p.bytes,
                 "attention: workspace is NULL, not 256-byte aligned or %zu bytes < %zu", ws_bytes, p.bytes);
     char *w = (char *)ws;
     const PgPrefillArgs a{q, (const _Float16 *)pages, table, cu, len, n_pages, paged_log(page_size), table_stride,
-                          batch, n_tok, H, Hkv, G, p.most, p.slots, p.half, p.rows, out, (int *)(w + kPreHead),
+                          batch, n_tok, H, Hkv, G, p.most, p.slots, p.half, p.rows, 1.0f / G, out, (int *)(w + kPreHead),
                           (PgRun *)(w + p.runs), (PgCut *)(w + p.cuts), (float2 *)(w + p.ml), (float *)(w + p.o)};
     hipStream_t s = (hipStream_t)stream;
     hipLaunchKernelGGL(paged_plan_kernel, dim3(1), dim3(kPlanThreads), 0, s, a);

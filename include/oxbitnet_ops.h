@@ -467,7 +467,7 @@ int oxb_attn_decode_paged(const void *q, int dtype, const void *pages, int n_pag
  * they were.  Types, pages and what is not there as above; with OXB_F16 the softmax
  * weights are f16.  ws: oxb_attn_prefill_paged_ws_bytes bytes, 256-byte aligned, any
  * contents (one workspace may serve decode too, whose counters this call leaves
- * alone); the size grows with n_tok and batch.  Calls that share one must not run
+ * alone); the size grows with n_tok and batch.  n_tok * H / Hkv is 2^27 at most.  Calls that share one must not run
  * concurrently. */
 size_t oxb_attn_prefill_paged_ws_bytes(int n_tok, int batch, int H, int Hkv, int hd);
 int oxb_attn_prefill_paged(const void *q, int dtype, const void *pages, int n_pages, int page_size,
