@@ -76,6 +76,10 @@ __device__ __forceinline__ float pg_ror8(float v) {   // lane i of 16 takes lane
     return __int_as_float(__builtin_amdgcn_update_dpp(i, i, 0x128, 0xf, 0xf, false));
 }
 
+// x / d for x below 2^21, with inv within 2^-23 of 1 / d: x + 1/2 is 1 / 2d or more from
+// every multiple of d, the product less than that off.
+__device__ __forceinline__ int pg_div(int x, float inv) { return (int)(((float)x + 0.5f) * inv); }
+
 __device__ __forceinline__ int pg_units(int64_t positions) { return (int)((positions + kPgUnit - 1) >> 5); }
 
 // Sums over the lanes up to this one.
@@ -507,6 +511,7 @@ constexpr int kPreRing = 4;
 constexpr int kPreOps = kPgHalf * 2 / 16;    // 16-byte operands of a unit's K (or V)
 constexpr int kPreLeast = 8;                 // units of a run
 constexpr int kPreSlots = 512;               // resident workgroups, at most
+constexpr int kPreOrder = kPreSlots;         // (a multiple of 8)
 constexpr int kPlanThreads = 1024;
 constexpr int64_t kPreMost = 1 << 27;        // rows of a call: 2^20 tiles, 1024 times which is in 32 bits
 constexpr size_t kPreHead = kDecParts * 4;   // decode's counters, in a workspace of both, then the counts
@@ -515,7 +520,7 @@ constexpr size_t kPreHead = kDecParts * 4;   // decode's counters, in a workspac
 struct PgRun {
     int tile, u0, u1, part;   // part -1: the tile's only run
     int cu, nq, past, z;
-    int tok, unused[3];       // the token of the tile's first row
+    int tok, head, unused[2]; // the token of the tile's first row; the KV head, -1 where there is no run
 };
 struct PgCut {
     int tile, part, runs, cu, nq, unused[3];
@@ -525,11 +530,11 @@ struct PgPrefillArgs {
     const void *q;
     const _Float16 *pages;
     const int *table, *cu, *len;
-    int n_pages, page_log, table_stride, batch, n_tok, H, Hkv, G, most, slots, half, rows;
+    int n_pages, page_log, table_stride, batch, n_tok, H, Hkv, G, most, slots, cus, rows;
     float inv_G;
     void *out;
-    int *counts;    // runs, cut tiles
-    PgRun *runs;    // [most]
+    int *counts;    // runs, cut tiles, whether tiles may be cut (then a record a workgroup)
+    PgRun *runs;    // [most], or [kPreOrder] in the order of the workgroups
     PgCut *cuts;    // [slots / 2 or most]
     float2 *ml;     // [slots][Hkv][rows] a row's reference and sum
     float *o;       // [slots][Hkv][rows][128]
@@ -544,6 +549,7 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PgPrefillArgs 
     __shared__ int s_cu[kPgBatch], s_nq[kPgBatch], s_past[kPgBatch];
     __shared__ uint32_t upto[kPgBatch];                 // tiles of the sequences up to z
     __shared__ int cost[kPreSlots], first[kPreSlots];   // of a tile that may be cut: units, runs up to it
+    __shared__ uint16_t tile_z[kPreSlots];
     __shared__ int hist[kPlanThreads];
     __shared__ uint32_t wsum[5][kWaves];
     __shared__ int wmax[kWaves], fit[2][kWaves];
@@ -603,6 +609,7 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PgPrefillArgs 
         if (tid < nt) {
             own = tile(tid);
             cost[tid] = mx = sum = own.units;
+            tile_z[tid] = own.z;
         }
     } else {
         for (int t = tid; t < nt; t += kPlanThreads) mx = max(mx, tile(t).units);
@@ -622,7 +629,8 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PgPrefillArgs 
         for (int i = 0; lo < hi; i ^= 1) {
             const int step = (hi - lo + kWaves - 1) / kWaves, c = min(hi, lo + wave * step);
             int n = 0;
-            for (int t = lane; t < nt; t += 64) n += max(1, (cost[t] + c - 1) / c);
+            const float inv = __builtin_amdgcn_rcpf((float)c);
+            for (int t = lane; t < nt; t += 64) n += max(1, pg_div(cost[t] + c - 1, inv));
             n = wave_isum_dpp(n);
             if (lane == 0) fit[i][wave] = n <= a.slots;
             __syncthreads();
@@ -633,7 +641,7 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PgPrefillArgs 
         }
         per = max(hi, 1);
         // runs of the tiles up to each, and cut tiles above bit 16
-        const int k = tid < nt ? max(1, (own.units + per - 1) / per) : 0;
+        const int k = tid < nt ? max(1, pg_div(own.units + per - 1, __builtin_amdgcn_rcpf((float)per))) : 0;
         const int v = scan(k | (k > 1 ? 1 << 16 : 0), wsum[3], total);
         cuts = total >> 16;
         total &= 0xffff;
@@ -644,6 +652,7 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PgPrefillArgs 
     if (tid == 0) {
         a.counts[0] = total;
         a.counts[1] = cuts;
+        a.counts[2] = cut;
     }
     auto run = [&](int j) {
         int k = 1, i = 0, t = j;
@@ -659,22 +668,59 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PgPrefillArgs 
             k = first[l] - before;
             i = j - before;
         }
-        const Tile r = tile(t);
-        // (units < 2^20, runs <= 512)
-        return PgRun{r.i, r.units * i / k, r.units * (i + 1) / k, k > 1 ? j : -1, s_cu[r.z], s_nq[r.z], s_past[r.z],
-                     r.z, r.i * kPreRows / a.G, {0, 0, 0}};
+        Tile r;
+        if (cut) {
+            r.z = tile_z[t];
+            r.i = t - (r.z ? (int)upto[r.z - 1] : 0);
+            r.units = cost[t];
+        } else {
+            r = tile(t);
+        }
+        // units i / k, its whole part apart (units up to 2^19, k and i up to 512)
+        const float inv = __builtin_amdgcn_rcpf((float)k);
+        const int part = pg_div(r.units, inv), more = r.units - part * k;
+        auto start = [&](int i) { return part * i + pg_div(more * i, inv); };
+        return PgRun{r.i, start(i), start(i + 1), k > 1 ? j : -1, s_cu[r.z], s_nq[r.z], s_past[r.z],
+                     r.z, r.i * kPreRows / a.G, 0, {0, 0}};
     };
+    if (cut) {
+        // All run at once.  Workgroup b runs on XCD b % 8: each XCD takes an eighth of the
+        // (KV head, run) pairs as they follow one another, so that its runs share their
+        // sequence's K and V in its L2; there the longest first, and of a CU's two the
+        // second the other way round, so that it gets the longest and the shortest.
+        const int n = total * a.Hkv, each = (n + 7) / 8, half = (a.cus + 7) / 8;
+        const int x = each ? pg_div(tid, __builtin_amdgcn_rcpf((float)each)) : 0, lo = x * each;
+        constexpr int kSteps = kPlanThreads / 8;   // of a run's length, to an XCD
+        PgRun r{};
+        int bucket = 0, head = 0;
+        if (tid < n) {
+            head = pg_div(tid, __builtin_amdgcn_rcpf((float)total));
+            r = run(tid - head * total);
+            bucket = x * kSteps + (int)((float)(per - (r.u1 - r.u0)) * ((float)(kSteps - 1) / (float)per));
+            atomicAdd(&hist[bucket], 1);
+        }
+        __syncthreads();
+        const int h = hist[tid];
+        int all;
+        const int v = scan(h, wsum[4], all);
+        hist[tid] = v - h;
+        __syncthreads();
+        if (tid < each * 8) {
+            int at = tid - lo;
+            r.head = -1;
+            if (tid < n) {
+                at = atomicAdd(&hist[bucket], 1) - lo;
+                const int two = min(2 * half, min(each, n - lo));
+                if (at >= half && at < two) at = half + two - 1 - at;
+                r.head = head;
+            }
+            a.runs[at * 8 + x] = r;
+        }
+        return;
+    }
     // the longest first, to a thousandth of the longest
     const float scale = (float)(kPlanThreads - 1) / (float)per;
     auto bucket = [&](const PgRun &r) { return (int)((float)(per - min(per, r.u1 - r.u0)) * scale); };
-    const int two = min(2 * a.half, total);
-    auto put = [&](const PgRun &r) {
-        int at = atomicAdd(&hist[bucket(r)], 1);
-        // of those that run at once, the second half the other way round: a CU gets
-        // the longest and the shortest
-        if (at >= a.half && at < two) at = a.half + two - 1 - at;
-        a.runs[at] = r;
-    };
     PgRun mine{};
     if (tid < total) mine = run(tid);
     for (int j = tid; j < total; j += kPlanThreads) atomicAdd(&hist[bucket(j == tid ? mine : run(j))], 1);
@@ -684,7 +730,10 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PgPrefillArgs 
     const int v = scan(h, wsum[4], all);
     hist[tid] = v - h;
     __syncthreads();
-    for (int j = tid; j < total; j += kPlanThreads) put(j == tid ? mine : run(j));
+    for (int j = tid; j < total; j += kPlanThreads) {
+        const PgRun r = j == tid ? mine : run(j);
+        a.runs[atomicAdd(&hist[bucket(r)], 1)] = r;
+    }
 }
 
 // 16 bytes of each lane from base + off to LDS at m0 + 16 * lane (as lds_dma16, with a
@@ -726,16 +775,27 @@ __global__ __launch_bounds__(kPreThreads, 2) void paged_prefill_kernel(PgPrefill
     uint4(*sk)[kPreOps] = lds, (*sv)[kPreOps] = lds + kPreRing + PARTS - 1;
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int kvh = blockIdx.x % a.Hkv, item = blockIdx.x / a.Hkv;
-    // (the record with the count; past it, whatever is there)
-    const PgRun run = pg_uniform(a.runs + item);
-    if (item >= pg_uniform(a.counts)) return;
+    // Where tiles are cut, a record a workgroup, else one for all KV heads.  (Both are
+    // loaded with the counts; past them, whatever is there.)
+    struct Counts {
+        int runs, cuts, cut;
+    };
+    const Counts n = pg_uniform((const Counts *)a.counts);
+    const int each = blockIdx.x / a.Hkv;
+    PgRun run = pg_uniform(a.runs + each);
+    int kvh = blockIdx.x - each * a.Hkv;
+    if (n.cut) {
+        if ((int)blockIdx.x >= (n.runs * a.Hkv + 7) / 8 * 8) return;
+        run = pg_uniform(a.runs + min((int)blockIdx.x, kPreOrder - 1));
+        kvh = run.head;
+        if (kvh < 0) return;
+    } else if (each >= n.runs) {
+        return;
+    }
     const int r0 = run.tile * kPreRows, rows = min(kPreRows, run.nq * a.G - r0);   // of the tile
     const int b0 = run.u0, b1 = run.u1, h = lane >> 5;
-    // x / G for x below 2^22: x + 1/2 is 1 / 2G or more from every multiple of G, the
-    // product 2^-23 of it off at most
     const int rest = r0 - run.tok * a.G;
-    auto tok_of = [&](int r) { return (int)(((float)(rest + r) + 0.5f) * a.inv_G); };   // from run.tok on
+    auto tok_of = [&](int r) { return pg_div(rest + r, a.inv_G); };   // from run.tok on
     T *out = (T *)a.out + ((size_t)(run.cu + run.tok) * a.H + kvh * a.G) * kPgHd;
     const T *q = (const T *)a.q + ((size_t)(run.cu + run.tok) * a.H + kvh * a.G) * kPgHd;
     const int wrow = wave * 32, row = wrow + (lane & 31);   // of the tile
@@ -756,12 +816,13 @@ __global__ __launch_bounds__(kPreThreads, 2) void paged_prefill_kernel(PgPrefill
     const int wfull = past + tok_of(min(wrow, rows - 1)) + 1;
     const int wb = max(b0, min(b1, pg_units(max(wseen, 0))));
 
-    // Pages by lanes: of the run's first units, and of 64 from unit b0 + 3 on, which is
-    // the first that the loop brings.
+    // Pages: of the run's first units by scalar loads, which wait for no others, and by
+    // lanes those of 64 from unit b0 + 3 on, the first that the loop brings.
     const int *table = a.table + (size_t)run.z * a.table_stride;
-    auto load_ids = [&](int u) { return table[min(u + lane, b1 - 1) >> (a.page_log - 5)]; };
-    const int in_page = (1 << (a.page_log - 5)) - 1;
-    const int ids0 = load_ids(b0);
+    const int unit_log = a.page_log - 5, in_page = (1 << unit_log) - 1;
+    auto first_id = [&](int u) { return pg_uniform(table + (min(u, b1 - 1) >> unit_log)); };
+    auto load_ids = [&](int u) { return table[min(u + lane, b1 - 1) >> unit_log]; };
+    const int id0 = first_id(b0), id1 = first_id(b0 + 1), id2 = first_id(b0 + 2);
     int ids = load_ids(b0 + 3);
     uint32_t gone = 0;   // bit u % 32: unit u's page is none
     auto unit = [&](int id, int u) {
@@ -795,10 +856,6 @@ __global__ __launch_bounds__(kPreThreads, 2) void paged_prefill_kernel(PgPrefill
     // lane % 32
     half8_t qh[8], ql[8];
     float qs = kPgScore;
-    const _Float16 *u0 = unit(__builtin_amdgcn_readlane(ids0, 0), b0);
-    const _Float16 *u1 = unit(__builtin_amdgcn_readlane(ids0, 1), b0 + 1);
-    const _Float16 *u2 = unit(__builtin_amdgcn_readlane(ids0, 2), b0 + 2);
-    bring_k(u0, 0);
     uint4 *sq[2] = {&sv[0][0] + 512 * wave, &sk[1][0] + 512 * wave};
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
@@ -808,6 +865,8 @@ __global__ __launch_bounds__(kPreThreads, 2) void paged_prefill_kernel(PgPrefill
         for (int p = 0; p < PARTS; ++p)
             pg_dma16(q, off + 256 * p, lds0 - 2048 * wave + (uint32_t)((char *)(sq[p] + 64 * i) - (char *)&lds[0][0]));
     }
+    const _Float16 *u0 = unit(id0, b0), *u1 = unit(id1, b0 + 1), *u2 = unit(id2, b0 + 2);
+    bring_k(u0, 0);
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     if constexpr (PARTS == 1) {
 #pragma unroll
@@ -1169,8 +1228,8 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PgPrefillArgs a) {
 // last one may be short), runs that are resident at once, of a KV head, and the
 // parts' rows.
 struct PrefillPlan {
-    int most, slots, half, rows;
-    int64_t items;
+    int most, slots, rows;
+    int64_t wgs;
     size_t runs, cuts, ml, o, bytes;
 };
 static PrefillPlan prefill_plan(int n, int batch, int G, int Hkv) {
@@ -1178,16 +1237,15 @@ static PrefillPlan prefill_plan(int n, int batch, int G, int Hkv) {
     const int64_t rows = (int64_t)n * G;
     p.most = (int)(rows / kPreRows + std::min<int64_t>(batch, n));
     p.slots = std::min(2 * device_cus(), kPreSlots) / Hkv;
-    p.half = std::min(device_cus(), kPreSlots / 2) / Hkv;
     p.rows = (int)std::min<int64_t>(kPreRows, rows);
-    p.items = std::max(p.most, p.slots);
+    p.wgs = std::max<int64_t>((int64_t)p.most * Hkv, kPreOrder);
     size_t at = kPreHead + 256;
     auto take = [&](size_t b) {
         const size_t o = at;
         at += pg_align(b);
         return o;
     };
-    p.runs = take(p.items * sizeof(PgRun));
+    p.runs = take(std::max<int64_t>(p.most, kPreOrder) * sizeof(PgRun));
     p.cuts = take((size_t)(p.slots / 2 + 1) * sizeof(PgCut));
     p.ml = take((size_t)p.slots * Hkv * p.rows * 8);
     p.o = take((size_t)p.slots * Hkv * p.rows * kPgHd * 4);
@@ -1258,17 +1316,17 @@ extern "C" int oxb_attn_prefill_paged(const void *q, int dtype, const void *page
     const int G = H / Hkv;
     OXB_REQUIRE(n_tok >= 1 && (int64_t)n_tok * G <= kPreMost, "prefill attention: %d tokens", n_tok);
     const PrefillPlan p = prefill_plan(n_tok, batch, G, Hkv);
-    OXB_REQUIRE(p.items * Hkv < (1 << 24), "prefill attention: %d tokens of %d heads", n_tok, H);
+    OXB_REQUIRE(p.wgs < (1 << 24), "prefill attention: %d tokens of %d heads", n_tok, H);
     OXB_REQUIRE(ws && ((uintptr_t)ws & 255) == 0 && ws_bytes >= p.bytes,
                 "attention: workspace is NULL, not 256-byte aligned or %zu bytes < %zu", ws_bytes, p.bytes);
     char *w = (char *)ws;
     const PgPrefillArgs a{q, (const _Float16 *)pages, table, cu, len, n_pages, paged_log(page_size), table_stride,
-                          batch, n_tok, H, Hkv, G, p.most, p.slots, p.half, p.rows, 1.0f / G, out, (int *)(w + kPreHead),
+                          batch, n_tok, H, Hkv, G, p.most, p.slots, device_cus(), p.rows, 1.0f / G, out, (int *)(w + kPreHead),
                           (PgRun *)(w + p.runs), (PgCut *)(w + p.cuts), (float2 *)(w + p.ml), (float *)(w + p.o)};
     hipStream_t s = (hipStream_t)stream;
     hipLaunchKernelGGL(paged_plan_kernel, dim3(1), dim3(kPlanThreads), 0, s, a);
     OXB_CHECK_HIP(hipGetLastError());
-    const dim3 grid((unsigned)(p.items * Hkv)), th(kPreThreads);
+    const dim3 grid((unsigned)p.wgs), th(kPreThreads);
     if (dtype == OXB_F32) hipLaunchKernelGGL((paged_prefill_kernel<float>), grid, th, 0, s, a);
     else hipLaunchKernelGGL((paged_prefill_kernel<_Float16>), grid, th, 0, s, a);
     OXB_CHECK_HIP(hipGetLastError());
