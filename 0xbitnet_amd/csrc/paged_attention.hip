@@ -146,6 +146,7 @@ constexpr int kDecThreads = 64 * kDecWaves;
 constexpr int kDecRows = 8;            // query heads of a pass
 constexpr int kDecQs = kPgHd + 8;      // q row stride in LDS (f16)
 constexpr int kDecLeast = 4;           // units of a run
+constexpr int kDecUncut = 16;          // units of a sequence that is not cut
 constexpr int kDecSlots = 512;         // runs that are resident at once, at most
 constexpr int kDecParts = 2 * kDecSlots;
 
@@ -188,7 +189,7 @@ __global__ __launch_bounds__(kDecThreads, 2) void paged_decode_kernel(PgDecodeAr
         int base = 0, cut = 0;   // workgroups and parts before the 64 sequences
         for (int c = 0; c < a.batch; c += 64) {
             const int n = c ? length(c + lane) : len0, u = pg_units(n);
-            const int k = c + lane < a.batch ? max(1, (u + per - 1) / per) : 0;
+            const int k = c + lane < a.batch ? (u <= kDecUncut ? 1 : (u + per - 1) / per) : 0;
             const int upto = wave_iscan(k * a.Hkv), cutto = wave_iscan(k > 1 ? k * a.Hkv : 0);
             const int i = __popcll(__ballot(base + upto <= (int)blockIdx.x));
             if (i < 64) {
