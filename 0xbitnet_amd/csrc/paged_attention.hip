@@ -123,6 +123,19 @@ __device__ __forceinline__ void pg_store4(_Float16 *p, float x, float y, float z
 // A row's value from its parts' sum t and softmax sum l (0: nothing seen).
 __device__ __forceinline__ float pg_quot(float t, float l) { return l == 0.0f ? 0.0f : t / l; }
 
+// What all lanes read and no kernel in flight writes: by scalar loads.
+template <typename R>
+__device__ __forceinline__ R pg_uniform(const R *p) {
+    static_assert(sizeof(R) % 4 == 0, "whole words");
+    struct Words {
+        int w[sizeof(R) / 4];
+    } r;
+    const auto *c = (const __attribute__((address_space(4))) int *)p;
+#pragma unroll
+    for (unsigned i = 0; i < sizeof(R) / 4; ++i) r.w[i] = c[i];
+    return __builtin_bit_cast(R, r);
+}
+
 // ---------------------------------------------------------------------------
 // decode
 // ---------------------------------------------------------------------------
@@ -527,16 +540,25 @@ struct PgCut {
     int tile, part, runs, cu, nq, unused[3];
 };
 
+// A cut tile's units in even runs: units i / k, its whole part apart (units up to
+// 2^19, k and i up to 512).
+__device__ __forceinline__ int pg_run_start(int units, int k, int i) {
+    const float inv = __builtin_amdgcn_rcpf((float)k);
+    const int part = pg_div(units, inv), more = units - part * k;
+    return part * i + pg_div(more * i, inv);
+}
+
 struct PgPrefillArgs {
     const void *q;
     const _Float16 *pages;
     const int *table, *cu, *len;
-    int n_pages, page_log, table_stride, batch, n_tok, H, Hkv, G, most, slots, cus, rows;
+    int n_pages, page_log, table_stride, batch, n_tok, H, Hkv, G, most, slots, half, rows;
+    int few;        // no plan: the first step of a search among the batch's sequences (0: there is one)
     float inv_G;
     void *out;
-    int *counts;    // runs, cut tiles, whether tiles may be cut (then a record a workgroup)
+    int *counts;    // runs, `cuts`, whether tiles may be cut (then a record a workgroup)
     PgRun *runs;    // [most], or [kPreOrder] in the order of the workgroups
-    PgCut *cuts;    // [slots / 2 or most]
+    PgCut *cuts;    // cut tiles, or where there is no plan all tiles
     float2 *ml;     // [slots][Hkv][rows] a row's reference and sum
     float *o;       // [slots][Hkv][rows][128]
 };
@@ -677,11 +699,7 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PgPrefillArgs 
         } else {
             r = tile(t);
         }
-        // units i / k, its whole part apart (units up to 2^19, k and i up to 512)
-        const float inv = __builtin_amdgcn_rcpf((float)k);
-        const int part = pg_div(r.units, inv), more = r.units - part * k;
-        auto start = [&](int i) { return part * i + pg_div(more * i, inv); };
-        return PgRun{r.i, start(i), start(i + 1), k > 1 ? j : -1, s_cu[r.z], s_nq[r.z], s_past[r.z],
+        return PgRun{r.i, pg_run_start(r.units, k, i), pg_run_start(r.units, k, i + 1), k > 1 ? j : -1, s_cu[r.z], s_nq[r.z], s_past[r.z],
                      r.z, r.i * kPreRows / a.G, 0, {0, 0}};
     };
     if (cut) {
@@ -689,7 +707,7 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PgPrefillArgs 
         // (KV head, run) pairs as they follow one another, so that its runs share their
         // sequence's K and V in its L2; there the longest first, and of a CU's two the
         // second the other way round, so that it gets the longest and the shortest.
-        const int n = total * a.Hkv, each = (n + 7) / 8, half = (a.cus + 7) / 8;
+        const int n = total * a.Hkv, each = (n + 7) / 8, half = a.half;
         const int x = each ? pg_div(tid, __builtin_amdgcn_rcpf((float)each)) : 0, lo = x * each;
         constexpr int kSteps = kPlanThreads / 8;   // of a run's length, to an XCD
         PgRun r{};
@@ -737,28 +755,86 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PgPrefillArgs 
     }
 }
 
+// The same plan of a call of up to 64 sequences and kFewTiles tiles, which a wave
+// makes by itself: a lane a sequence, a lane a tile (two), so that no launch comes
+// before the attention's (its 4 to 7 us and the gap behind it).  All runs are
+// resident at once, so their order matters little: only each XCD's stretch of
+// them, and of a CU's two one from either end.
+constexpr int kFewTiles = 128;
+struct PgFew {
+    int nt, total;                     // tiles, runs
+    int cu, nq, past;                  // of sequence `lane`
+    int z[2], i[2], units[2], k[2], upto[2];   // of tiles `lane` and 64 + `lane`: runs, and up to it
+};
+__device__ __forceinline__ PgFew pg_few(const PgPrefillArgs &a) {
+    const int lane = threadIdx.x & 63;
+    PgFew p;
+    p.cu = p.nq = p.past = 0;
+    if (lane < a.batch) {
+        const int c0 = min(max(a.cu[lane], 0), a.n_tok), c1 = min(max(a.cu[lane + 1], 0), a.n_tok);
+        const int64_t cap = (int64_t)a.table_stride << a.page_log;
+        p.cu = c0;
+        p.nq = max(c1 - c0, 0);
+        p.past = (int)(min(max((int64_t)a.len[lane], (int64_t)0), cap) - p.nq);
+    }
+    const int tiles = wave_iscan((p.nq * a.G + kPreRows - 1) / kPreRows);
+    p.nt = min(__builtin_amdgcn_readlane(tiles, 63), min(a.most, kFewTiles));
+    int sum = 0, mx = 0;
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+        const int t = 64 * c + lane;
+        int z = 0;   // the first sequence with more than t tiles up to it
+        for (int step = a.few; step > 0; step >>= 1)
+            if (__shfl(tiles, z + step - 1, 64) <= t) z += step;
+        const int before = __shfl(tiles, z - 1, 64), nq = __shfl(p.nq, z, 64), past = __shfl(p.past, z, 64);
+        p.z[c] = z;
+        p.i[c] = t - (z ? before : 0);
+        const int last = min((p.i[c] + 1) * kPreRows, nq * a.G) - 1;
+        p.units[c] = t < p.nt ? pg_units(max(past + pg_div(last, a.inv_G) + 1, 0)) : 0;
+        sum += p.units[c];
+        mx = max(mx, p.units[c]);
+    }
+    sum = wave_isum_dpp(sum);
+#pragma unroll
+    for (int s = 32; s > 0; s >>= 1) mx = max(mx, __shfl_xor(mx, s, 64));
+    int lo = max(kPreLeast, sum / a.slots), hi = max(__builtin_amdgcn_readfirstlane(mx), 1);
+    if (p.nt < a.slots) hi = min(hi, max(lo, (sum + a.slots - p.nt - 1) / (a.slots - p.nt)));
+    auto runs = [&](int u, int t, int per) {
+        return t < p.nt ? max(1, pg_div(u + per - 1, __builtin_amdgcn_rcpf((float)per))) : 0;
+    };
+    while (lo < hi) {
+        const int per = (lo + hi) >> 1;
+        const int n = wave_isum_dpp(runs(p.units[0], lane, per) + runs(p.units[1], 64 + lane, per));
+        if (n <= a.slots) hi = per;
+        else lo = per + 1;
+    }
+    p.k[0] = runs(p.units[0], lane, hi);
+    p.k[1] = runs(p.units[1], 64 + lane, hi);
+    p.upto[0] = wave_iscan(p.k[0]);
+    const int half = __builtin_amdgcn_readlane(p.upto[0], 63);
+    p.upto[1] = half + wave_iscan(p.k[1]);
+    p.total = __builtin_amdgcn_readlane(p.upto[1], 63);
+    return p;
+}
+// Fields of tile t (uniform): of c = t / 64, lane t % 64.
+__device__ __forceinline__ int pg_of_tile(const int (&f)[2], int t) {
+    return __builtin_amdgcn_readlane(t < 64 ? f[0] : f[1], t & 63);
+}
+
 // 16 bytes of each lane from base + off to LDS at m0 + 16 * lane (as lds_dma16, with a
 // scalar base).
 __device__ __forceinline__ void pg_dma16(const void *base, uint32_t off, uint32_t lds) {
+    // (uniform as they are: for the compiler)
+    const uint64_t at = (uint64_t)base;
+    const uint64_t sbase = (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)at) |
+                           (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(at >> 32)) << 32;
+    const uint32_t slds = __builtin_amdgcn_readfirstlane((int)lds);
     uint32_t saved;
     asm volatile(
         "s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %2, %3\n\ts_mov_b32 m0, %0"
         : "=&s"(saved)
-        : "s"(lds), "v"(off), "s"(base)
+        : "s"(slds), "v"(off), "s"(sbase)
         : "memory");
-}
-
-// What all lanes read and no kernel in flight writes: by scalar loads.
-template <typename R>
-__device__ __forceinline__ R pg_uniform(const R *p) {
-    static_assert(sizeof(R) % 4 == 0, "whole words");
-    struct Words {
-        int w[sizeof(R) / 4];
-    } r;
-    const auto *c = (const __attribute__((address_space(4))) int *)p;
-#pragma unroll
-    for (unsigned i = 0; i < sizeof(R) / 4; ++i) r.w[i] = c[i];
-    return __builtin_bit_cast(R, r);
 }
 
 // A row's 16-byte pieces lie in LDS exchanged by the row's number, so that neither a
@@ -776,23 +852,61 @@ __global__ __launch_bounds__(kPreThreads, 2) void paged_prefill_kernel(PgPrefill
     uint4(*sk)[kPreOps] = lds, (*sv)[kPreOps] = lds + kPreRing + PARTS - 1;
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    // Where tiles are cut, a record a workgroup, else one for all KV heads.  (Both are
-    // loaded with the counts; past them, whatever is there.)
-    struct Counts {
-        int runs, cuts, cut;
-    };
-    const Counts n = pg_uniform((const Counts *)a.counts);
-    const int each = blockIdx.x / a.Hkv;
-    PgRun run = pg_uniform(a.runs + each);
-    int kvh = blockIdx.x - each * a.Hkv;
-    if (n.cut) {
-        if ((int)blockIdx.x >= (n.runs * a.Hkv + 7) / 8 * 8) return;
-        run = pg_uniform(a.runs + min((int)blockIdx.x, kPreOrder - 1));
-        kvh = run.head;
-        if (kvh < 0) return;
-    } else if (each >= n.runs) {
-        return;
+    PgRun run;
+    int kvh;
+    if (a.few) {
+        const PgFew p = pg_few(a);
+        if (blockIdx.x == 0 && tid == 0) a.counts[1] = p.nt;   // (for the join, of no tiles too)
+        const int n = p.total * a.Hkv, each = (n + 7) / 8, x = blockIdx.x & 7, i = blockIdx.x >> 3;
+        const int there = min(each, n - x * each);   // of this XCD
+        if (i >= there) return;
+        const int f = x * each + (i < a.half ? i : there - 1 - (i - a.half));
+        kvh = pg_div(f, __builtin_amdgcn_rcpf((float)p.total));
+        const int j = f - kvh * p.total;
+        const int t = __popcll(__ballot(p.upto[0] <= j)) + __popcll(__ballot(p.upto[1] <= j));
+        const int k = pg_of_tile(p.k, t), part = j - (pg_of_tile(p.upto, t) - k), units = pg_of_tile(p.units, t);
+        run.z = pg_of_tile(p.z, t);
+        run.tile = pg_of_tile(p.i, t);
+        run.u0 = pg_run_start(units, k, part);
+        run.u1 = pg_run_start(units, k, part + 1);
+        run.part = k > 1 ? j : -1;
+        run.cu = __builtin_amdgcn_readlane(p.cu, run.z);
+        run.nq = __builtin_amdgcn_readlane(p.nq, run.z);
+        run.past = __builtin_amdgcn_readlane(p.past, run.z);
+        run.tok = pg_div(run.tile * kPreRows, a.inv_G);
+        if (kvh == 0 && part == 0 && tid == 0)
+            a.cuts[t] = PgCut{run.tile, j, k, run.cu, run.nq, {0, 0, 0}};
+    } else {
+        // Where tiles are cut, a record a workgroup, else one for all KV heads.  (Both are
+        // loaded with the counts; past them, whatever is there.)
+        struct Counts {
+            int runs, cuts, cut;
+        };
+        const Counts n = pg_uniform((const Counts *)a.counts);
+        const int each = blockIdx.x / a.Hkv;
+        run = pg_uniform(a.runs + each);
+        kvh = blockIdx.x - each * a.Hkv;
+        if (n.cut) {
+            if ((int)blockIdx.x >= (n.runs * a.Hkv + 7) / 8 * 8) return;
+            run = pg_uniform(a.runs + min((int)blockIdx.x, kPreOrder - 1));
+            kvh = run.head;
+            if (kvh < 0) return;
+        } else if (each >= n.runs) {
+            return;
+        }
     }
+    // (uniform all of it: for the compiler)
+    auto first = [](int &v) { v = __builtin_amdgcn_readfirstlane(v); };
+    first(kvh);
+    first(run.tile);
+    first(run.u0);
+    first(run.u1);
+    first(run.part);
+    first(run.cu);
+    first(run.nq);
+    first(run.past);
+    first(run.z);
+    first(run.tok);
     const int r0 = run.tile * kPreRows, rows = min(kPreRows, run.nq * a.G - r0);   // of the tile
     const int b0 = run.u0, b1 = run.u1, h = lane >> 5;
     const int rest = r0 - run.tok * a.G;
@@ -1168,9 +1282,9 @@ __global__ __launch_bounds__(kPreThreads, 2) void paged_prefill_kernel(PgPrefill
         for (int k = 0; k < 4; ++k)
             pg_store4((float *)&so[pg_piece<32>(er, 8 * d + 2 * k + h)], o[d][4 * k] * f, o[d][4 * k + 1] * f,
                       o[d][4 * k + 2] * f, o[d][4 * k + 3] * f);
-    const size_t first = ((size_t)run.part * a.Hkv + kvh) * a.rows + wrow;   // (of a part)
-    if (!direct && h == 0 && row < rows) a.ml[first + er] = make_float2(ref.part(), lsum);
-    float *dst = direct ? (float *)out : a.o + first * kPgHd;
+    const size_t prow = ((size_t)run.part * a.Hkv + kvh) * a.rows + wrow;   // (of a part)
+    if (!direct && h == 0 && row < rows) a.ml[prow + er] = make_float2(ref.part(), lsum);
+    float *dst = direct ? (float *)out : a.o + prow * kPgHd;
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
         const int r = 2 * i + h, at = direct ? __shfl(qrow, r, 64) : r;
@@ -1184,7 +1298,7 @@ template <typename T>
 __global__ __launch_bounds__(256) void paged_join_kernel(PgPrefillArgs a) {
     const int c = blockIdx.x / (kPreRows / 8), kvh = blockIdx.y, d = (threadIdx.x & 31) * 4;
     const PgCut t = pg_uniform(a.cuts + c);   // (with the count; past it, whatever is there)
-    if (c >= pg_uniform(a.counts + 1)) return;
+    if (c >= pg_uniform(a.counts + 1) || t.runs == 1) return;   // (written by its only run)
     const int lrow = blockIdx.x % (kPreRows / 8) * 8 + (threadIdx.x >> 5), row = t.tile * kPreRows + lrow;
     if (row >= t.nq * a.G) return;
     const size_t step = (size_t)a.Hkv * a.rows, r = ((size_t)t.part * a.Hkv + kvh) * a.rows + lrow;
@@ -1247,7 +1361,7 @@ static PrefillPlan prefill_plan(int n, int batch, int G, int Hkv) {
         return o;
     };
     p.runs = take(std::max<int64_t>(p.most, kPreOrder) * sizeof(PgRun));
-    p.cuts = take((size_t)(p.slots / 2 + 1) * sizeof(PgCut));
+    p.cuts = take((size_t)std::max(p.slots / 2 + 1, kFewTiles) * sizeof(PgCut));
     p.ml = take((size_t)p.slots * Hkv * p.rows * 8);
     p.o = take((size_t)p.slots * Hkv * p.rows * kPgHd * 4);
     p.bytes = at;
@@ -1321,19 +1435,25 @@ extern "C" int oxb_attn_prefill_paged(const void *q, int dtype, const void *page
     OXB_REQUIRE(ws && ((uintptr_t)ws & 255) == 0 && ws_bytes >= p.bytes,
                 "attention: workspace is NULL, not 256-byte aligned or %zu bytes < %zu", ws_bytes, p.bytes);
     char *w = (char *)ws;
+    // a first step for a search of 0 .. batch - 1; without sequences to search, 1 too
+    int few = 0;
+    if (batch <= 64 && p.most <= std::min(p.slots, kFewTiles))
+        for (few = 1; 2 * few < batch;) few *= 2;
     const PgPrefillArgs a{q, (const _Float16 *)pages, table, cu, len, n_pages, paged_log(page_size), table_stride,
-                          batch, n_tok, H, Hkv, G, p.most, p.slots, device_cus(), p.rows, 1.0f / G, out, (int *)(w + kPreHead),
+                          batch, n_tok, H, Hkv, G, p.most, p.slots, (device_cus() + 7) / 8, p.rows, few, 1.0f / G, out, (int *)(w + kPreHead),
                           (PgRun *)(w + p.runs), (PgCut *)(w + p.cuts), (float2 *)(w + p.ml), (float *)(w + p.o)};
     hipStream_t s = (hipStream_t)stream;
-    hipLaunchKernelGGL(paged_plan_kernel, dim3(1), dim3(kPlanThreads), 0, s, a);
-    OXB_CHECK_HIP(hipGetLastError());
+    if (!few) {
+        hipLaunchKernelGGL(paged_plan_kernel, dim3(1), dim3(kPlanThreads), 0, s, a);
+        OXB_CHECK_HIP(hipGetLastError());
+    }
     const dim3 grid((unsigned)p.wgs), th(kPreThreads);
     if (dtype == OXB_F32) hipLaunchKernelGGL((paged_prefill_kernel<float>), grid, th, 0, s, a);
     else hipLaunchKernelGGL((paged_prefill_kernel<_Float16>), grid, th, 0, s, a);
     OXB_CHECK_HIP(hipGetLastError());
     // a tile is cut only where it has more than kPreLeast units
     if ((int64_t)table_stride * page_size > kPreLeast * kPgUnit && p.slots > 1) {
-        const dim3 jgrid((unsigned)std::min(p.most, p.slots / 2) * (kPreRows / 8), Hkv);
+        const dim3 jgrid((unsigned)(few ? p.most : std::min(p.most, p.slots / 2)) * (kPreRows / 8), Hkv);
         if (dtype == OXB_F32) hipLaunchKernelGGL((paged_join_kernel<float>), jgrid, dim3(256), 0, s, a);
         else hipLaunchKernelGGL((paged_join_kernel<_Float16>), jgrid, dim3(256), 0, s, a);
         OXB_CHECK_HIP(hipGetLastError());

@@ -408,6 +408,21 @@ def test_prefill_rows_with_nothing_to_see():
         assert not got[a:max(a, b - n)].any()
 
 
+@pytest.mark.parametrize("batch", [3, 70])
+def test_prefill_of_no_tokens(batch):
+    """A call whose sequences have no tokens, after one that left cut tiles in the
+    workspace: nothing is written."""
+    rng = rng_of("empty", batch)
+    lens = [900] + [40] * (batch - 1)
+    c, K, V = filled(rng, lens, 2, 32)
+    q = rng.standard_normal((batch + 40, 4 * HD)).astype(np.float32)
+    cu = np.minimum(np.arange(batch + 1) + 40, batch + 40) * (np.arange(batch + 1) > 0)
+    c.attn_prefill(q, cu)
+    before = np.full(q.shape, 3, np.float32)
+    for none in (np.zeros(batch + 1), np.full(batch + 1, 5), np.full(batch + 1, len(q))):
+        assert (c.attn_prefill(q, none, before) == 3).all()
+
+
 def test_cu_outside_the_buffer():
     """Values that do not ascend or lie outside 0..n_tok: whatever comes of them stays
     inside, and sequences with good ones are right."""
