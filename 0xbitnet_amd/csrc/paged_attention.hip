@@ -783,6 +783,8 @@ __device__ __forceinline__ PgFew pg_few(const PgPrefillArgs &a) {
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
         const int t = 64 * c + lane;
+        p.z[c] = p.i[c] = p.units[c] = 0;
+        if (64 * c >= p.nt) continue;   // (uniform)
         int z = 0;   // the first sequence with more than t tiles up to it
         for (int step = a.few; step > 0; step >>= 1)
             if (__shfl(tiles, z + step - 1, 64) <= t) z += step;

@@ -389,6 +389,105 @@ def test_prefill_larger(dtype, H, hkv, spec, page):
         ref.close_in_norm(got[at], want, q[at].reshape(-1, HD)[:200], K[z][:, 0], lens[z], f16)
 
 
+@pytest.mark.parametrize("seed", range(12))
+def test_prefill_and_decode_of_random_batches(seed):
+    """Batches, groups, pages and lengths at random: idle sequences, one token, more
+    tokens than lanes; every row."""
+    rng = rng_of("random", seed)
+    hkv = int(rng.choice([1, 2, 3, 5, 8]))
+    H = hkv * int(rng.choice([1, 2, 3, 4, 7, 8, 20]))
+    page, B = int(rng.choice([32, 64, 128, 512])), int(rng.choice([1, 2, 7, 30, 64, 65, 100]))
+    longest = int(rng.choice([3, 40, 150, 700])) if B < 30 else int(rng.choice([3, 40, 90]))
+    new = [int(x) for x in rng.integers(0, longest + 1, B)]
+    past = [int(x) for x in rng.integers(0, 2 * longest, B) * rng.integers(0, 2, B)]
+    if not sum(new):
+        new[0] = 1
+    lens = [a + b for a, b in zip(new, past)]
+    c, K, V = filled(rng, lens, hkv, page, table_pages=ref.pages(3 * longest, page) + 1)
+    cu = np.concatenate([[0], np.cumsum(new)])
+    dtype = np.float32 if seed % 3 else np.float16
+    q = rng.standard_normal((cu[-1], H * HD)).astype(dtype)
+    got, f16 = c.attn_prefill(q, cu), dtype == np.float16
+    dec = c.attn_decode(np.resize(q, (B, H * HD)))
+    for z, m in enumerate(new):
+        at = slice(cu[z], cu[z + 1])
+        want, tol = expect(q[at], K[z], V[z], hkv, lens[z] - m, f16, 1 if f16 else 2)
+        ref.check_rows(got[at], want, tol, (z, H, hkv, page, B))
+        one = np.resize(q, (B, H * HD))[z:z + 1]
+        want, tol = expect(one, K[z], V[z], hkv, lens[z] - 1, f16)
+        ref.check_rows(dec[z:z + 1], want, tol, (z, H, hkv, page, B))
+
+
+@pytest.mark.parametrize("H,hkv", [(200, 1), (300, 300), (600, 600)])
+def test_many_heads(H, hkv):
+    """A group larger than a tile of rows; more KV heads than resident workgroups."""
+    rng = rng_of("heads", H, hkv)
+    new, past = [3, 0, 9], [40, 5, 60]
+    lens = [a + b for a, b in zip(new, past)]
+    c, K, V = filled(rng, lens, hkv, 32)
+    q = rng.standard_normal((12, H * HD)).astype(np.float32)
+    got, dec = c.attn_prefill(q, [0, 3, 3, 12]), c.attn_decode(q[:3])
+    for z, (a, b) in enumerate(((0, 3), (3, 3), (3, 12))):
+        want, tol = expect(q[a:b], K[z], V[z], hkv, past[z])
+        ref.check_rows(got[a:b], want, tol, z)
+        want, tol = expect(q[z:z + 1], K[z], V[z], hkv, lens[z] - 1)
+        ref.check_rows(dec[z:z + 1], want, tol, z)
+
+
+def shared_pages(rng, B, hkv, n, page, none=()):
+    """A cache whose B sequences all hold the same n positions in one set of pages, the
+    pages of the numbers in `none` taken out of the table."""
+    c, K, V = filled(rng, [n], hkv, page)
+    t = c.table.download()
+    t[0, list(none)] = -1
+    c.batch = B
+    c.table, c.len = ops.DeviceArray.from_host(np.repeat(t, B, 0)), ops.DeviceArray.from_host(np.full(B, n, np.int32))
+    there = np.isin(np.arange(n) // page, list(none), invert=True)
+    return c, K[0], V[0], there
+
+
+def test_long_runs_over_shared_pages():
+    """Runs of more units than a wave looks pages up at once, over pages that all
+    sequences share, some of them none."""
+    rng = rng_of("shared")
+    B, page = 300, 32                                    # decode: 282 units a run, 70 a wave
+    c, K, V, there = shared_pages(rng, B, 1, 9000, page, (3, 70, 258, 270))
+    q = rng.standard_normal((B, 2 * HD)).astype(np.float32)
+    got = c.attn_decode(q)
+    for z in range(0, B, 23):
+        want, tol = expect(q[z:z + 1], K[there], V[there], 1, there.sum() - 1)
+        ref.check_rows(got[z:z + 1], want, tol, z)
+    B, n, m = 40, 4064, 64                               # prefill: 160 tiles of 127 units
+    c, K, V, there = shared_pages(rng, B, 8, n, page, (5, 66, 100))
+    H = 64
+    q = rng.standard_normal((B * m, H * HD)).astype(np.float32)
+    got = c.attn_prefill(q, np.arange(B + 1) * m)
+    for z in (0, 17, 39):
+        for i in (0, 31, 63):
+            seen = there & (np.arange(n) <= n - m + i)
+            r = z * m + i
+            want, tol = expect(q[r:r + 1], K[seen], V[seen], 8, seen.sum() - 1)
+            ref.check_rows(got[r:r + 1], want, tol, (z, i))
+
+
+def test_rows_of_q_that_are_not_finite():
+    """An Inf or NaN in a row of q makes that head's row NaN and no other."""
+    rng = rng_of("wild q")
+    lens, hkv, H = [90, 33], 2, 8
+    c, K, V = filled(rng, lens, hkv, 32)
+    for dtype in (np.float32, np.float16):
+        q = rng.standard_normal((50, H * HD)).astype(dtype)
+        clean = [c.attn_decode(q[:2]), c.attn_prefill(q, [0, 30, 50])]
+        q[1, 3 * HD + 5], q[20, 7 * HD] = np.inf, np.nan
+        for got, want in zip((c.attn_decode(q[:2]), c.attn_prefill(q, [0, 30, 50])), clean):
+            hit = np.zeros(got.shape, bool)
+            hit[1, 3 * HD:4 * HD] = True
+            if len(hit) > 2:
+                hit[20, 7 * HD:] = True
+            assert np.isnan(got[hit]).all()
+            assert np.array_equal(bits(got[~hit]), bits(want[~hit]))
+
+
 def test_prefill_rows_with_nothing_to_see():
     """More tokens than positions (the first rows see nothing), empty sequences between
     them, cu that begins past 0."""
