@@ -140,13 +140,13 @@ __device__ __forceinline__ R pg_uniform(const R *p) {
 // decode
 // ---------------------------------------------------------------------------
 // Workgroup: four waves over a run of a sequence's units of a KV head, wave w taking
-// every fourth, for up to 8 of its query heads at a time (more go round again over
-// the run).  16x16x32 MFMA, operands straight from memory to registers:
-//   the 16 columns are the 8 heads' hi and lo parts, for q and for p' alike, so the
-//   two-part products cost nothing over one;
-//   scores: A = 16 K rows x 32 dims, B = q; column c + (c ^ 8) is the score.  K
-//   rows are taken in an order that leaves lane group g (of 4) the scores of
-//   positions 8 g .. 8 g + 7;
+// every fourth, for ROWS of its query heads at a time (more go round again over the
+// run).  16x16x32 MFMA, operands straight from memory to registers:
+//   ROWS 8, for groups of up to 8: the 16 columns are the 8 heads' hi and lo parts, for
+//   q and for p' alike, so the two-part products cost nothing over one, and column
+//   c + (c ^ 8) is the score; ROWS 16: a product for each part;
+//   scores: A = 16 K rows x 32 dims, B = q.  K rows are taken in an order that
+//   leaves lane group g (of 4) the scores of positions 8 g .. 8 g + 7;
 //   P.V: A = 16 dims x 32 positions, B = the lane's own eight p'.
 // Bound by the cache's bytes.  The launch is as wide as the card holds, and each
 // workgroup finds its run from the lengths themselves: a run has `per` units at
@@ -156,7 +156,7 @@ __device__ __forceinline__ R pg_uniform(const R *p) {
 // joins them in order, so the sum does not depend on which is last.
 constexpr int kDecWaves = 4;
 constexpr int kDecThreads = 64 * kDecWaves;
-constexpr int kDecRows = 8;            // query heads of a pass
+constexpr int kDecRows = 8;            // query heads that the workgroup's threads hold a row of
 constexpr int kDecQs = kPgHd + 8;      // q row stride in LDS (f16)
 constexpr int kDecLeast = 4;           // units of a run
 constexpr int kDecUncut = 16;          // units of a sequence that is not cut
@@ -174,12 +174,13 @@ struct PgDecodeArgs {
     uint64_t *o;     // [kDecParts][G][64] pairs of dims
 };
 
-template <typename T>
+template <typename T, int ROWS>
 __global__ __launch_bounds__(kDecThreads, 2) void paged_decode_kernel(PgDecodeArgs a) {
-    __shared__ _Float16 sq[2 * kDecRows * kDecQs];
-    __shared__ float sqs[kDecRows];
-    __shared__ float2 sml[kDecWaves][kDecRows];
-    __shared__ float4 so[kDecWaves][kDecRows][kPgHd / 4];
+    constexpr int RT = ROWS / kDecRows;    // rows of a thread: orow, orow + 8
+    __shared__ _Float16 sq[2 * ROWS * kDecQs];
+    __shared__ float sqs[ROWS];
+    __shared__ float2 sml[kDecWaves][ROWS];
+    __shared__ float4 so[kDecWaves][ROWS][kPgHd / 4];
     __shared__ int s_last;
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -228,10 +229,15 @@ __global__ __launch_bounds__(kDecThreads, 2) void paged_decode_kernel(PgDecodeAr
         return;
     }
     const T *q = (const T *)a.q + ((size_t)z * a.H + (size_t)kvh * a.G) * kPgHd;
+    float4 qv[RT];
     auto load_q = [&](int hc) {
-        return hc + orow < a.G ? pg_load4(q + (size_t)(hc + orow) * kPgHd + od) : make_float4(0, 0, 0, 0);
+#pragma unroll
+        for (int i = 0; i < RT; ++i) {
+            const int r = hc + orow + 8 * i;
+            qv[i] = r < a.G ? pg_load4(q + (size_t)r * kPgHd + od) : make_float4(0, 0, 0, 0);
+        }
     };
-    float4 qv = load_q(0);
+    load_q(0);
     const int *table = a.table + (size_t)z * a.table_stride;
     const int in_page = (1 << (a.page_log - 5)) - 1;
     const int rr = lane & 15, g = lane >> 4;
@@ -247,8 +253,8 @@ __global__ __launch_bounds__(kDecThreads, 2) void paged_decode_kernel(PgDecodeAr
         return u < b1 ? table[u >> (a.page_log - 5)] : 0;
     };
 
-    for (int hc = 0; hc < a.G; hc += kDecRows) {
-        const int g0 = hc, ng = min(kDecRows, a.G - hc);
+    for (int hc = 0; hc < a.G; hc += ROWS) {
+        const int g0 = hc, ng = min(ROWS, a.G - hc);
         int ids = load_ids(b0 + wave), next = 0;   // unit b0 + wave + 4 next is lane next % 64's
         auto load = [&](int b) {
             Blk x;
@@ -264,8 +270,10 @@ __global__ __launch_bounds__(kDecThreads, 2) void paged_decode_kernel(PgDecodeAr
         };
         // the first unit is on its way while q is made ready
         Blk cur = load(min(b0 + wave, b1 - 1));
-        {   // q rows: scaled, split, and their score units
-            const float4 v = qv;
+#pragma unroll
+        for (int i = 0; i < RT; ++i) {   // q rows: scaled, split, and their score units
+            const float4 v = qv[i];
+            const int row = orow + 8 * i;
             float m = fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w)));
 #pragma unroll
             for (int s = 16; s > 0; s >>= 1) m = fmaxf(m, __shfl_xor(m, s, 64));
@@ -275,16 +283,19 @@ __global__ __launch_bounds__(kDecThreads, 2) void paged_decode_kernel(PgDecodeAr
             for (int j = 0; j < 4; ++j) {
                 const float x = ldexpf(f[j], -e);
                 const _Float16 hi = (_Float16)x;
-                sq[orow * kDecQs + od + j] = hi;
-                sq[(orow + kDecRows) * kDecQs + od + j] = (_Float16)(x - (float)hi);
+                sq[row * kDecQs + od + j] = hi;
+                sq[(row + ROWS) * kDecQs + od + j] = (_Float16)(x - (float)hi);
             }
-            if ((tid & 31) == 0) sqs[orow] = ldexpf(kPgScore, e);
+            if ((tid & 31) == 0) sqs[row] = ldexpf(kPgScore, e);
         }
         lds_barrier();
-        half8_t qf[4];
+        half8_t qf[RT][4];
 #pragma unroll
-        for (int s = 0; s < 4; ++s) qf[s] = *(const half8_t *)(sq + rr * kDecQs + 32 * s + 8 * g);
-        const float qs = sqs[rr & 7];
+        for (int i = 0; i < RT; ++i)
+#pragma unroll
+            for (int s = 0; s < 4; ++s)
+                qf[i][s] = *(const half8_t *)(sq + (rr + 16 * i) * kDecQs + 32 * s + 8 * g);
+        const float qs = sqs[rr & (ROWS - 1)];
 
         f32x4 o[8];
 #pragma unroll
@@ -297,15 +308,18 @@ __global__ __launch_bounds__(kDecThreads, 2) void paged_decode_kernel(PgDecodeAr
             if (b + kDecWaves < b1) nxt = load(b + kDecWaves);
             f32x4 s0{0, 0, 0, 0}, s1{0, 0, 0, 0};
 #pragma unroll
-            for (int s = 0; s < 4; ++s) {
-                s0 = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8_t, cur.k[2 * s]), qf[s], s0, 0, 0, 0);
-                s1 = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8_t, cur.k[2 * s + 1]), qf[s], s1, 0, 0, 0);
-            }
+            for (int s = 0; s < 4; ++s)
+#pragma unroll
+                for (int i = 0; i < RT; ++i) {
+                    s0 = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8_t, cur.k[2 * s]), qf[i][s], s0, 0, 0, 0);
+                    s1 = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8_t, cur.k[2 * s + 1]), qf[i][s], s1, 0, 0, 0);
+                }
+            auto whole = [](float v) { return RT == 1 ? v + pg_ror8(v) : v; };   // of both parts
             float x[8];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                x[i] = s0[i] + pg_ror8(s0[i]);
-                x[4 + i] = s1[i] + pg_ror8(s1[i]);
+                x[i] = whole(s0[i]);
+                x[4 + i] = whole(s1[i]);
             }
             // of the lane's positions 8 g .. 8 g + 7, the first `left` are there
             const bool partial = len - b * kPgUnit < kPgUnit || !cur.there;
@@ -321,14 +335,16 @@ __global__ __launch_bounds__(kDecThreads, 2) void paged_decode_kernel(PgDecodeAr
                 for (int i = 0; i < 8; ++i) o[i] *= al;
             }
             const float moff = ref.off();
-            half8_t pf;
+            half8_t pf[RT];
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 float p = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i], qs, -moff));
                 if (partial && i >= left) p = 0.0f;
                 lsum += p;
                 const _Float16 hi = (_Float16)p;
-                pf[i] = rr < kDecRows ? hi : (_Float16)(p - (float)hi);
+                const _Float16 lo = (_Float16)(p - (float)hi);
+                pf[0][i] = RT == 2 || rr < 8 ? hi : lo;
+                pf[RT - 1][i] = RT == 2 || rr >= 8 ? lo : hi;
             }
             if (partial) {   // what is not there may hold anything
                 uint32_t mk[4];
@@ -344,52 +360,54 @@ __global__ __launch_bounds__(kDecThreads, 2) void paged_decode_kernel(PgDecodeAr
             }
 #pragma unroll
             for (int i = 0; i < 8; ++i)
-                o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8_t, cur.v[i]), pf, o[i], 0, 0, 0);
+#pragma unroll
+                for (int j = 0; j < RT; ++j)
+                    o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8_t, cur.v[i]), pf[j], o[i], 0, 0, 0);
             cur = nxt;
         }
         // the four waves' parts
         lsum += __shfl_xor(lsum, 16, 64);
         lsum += __shfl_xor(lsum, 32, 64);
-        if (lane < kDecRows) sml[wave][lane] = make_float2(ref.part(), lsum);
+        if (lane < ROWS) sml[wave][lane] = make_float2(ref.part(), lsum);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            float4 t;
-            t.x = o[i][0] + pg_ror8(o[i][0]);
-            t.y = o[i][1] + pg_ror8(o[i][1]);
-            t.z = o[i][2] + pg_ror8(o[i][2]);
-            t.w = o[i][3] + pg_ror8(o[i][3]);
-            if (rr < kDecRows) so[wave][rr][4 * i + g] = t;
+            auto whole = [](float v) { return RT == 1 ? v + pg_ror8(v) : v; };
+            const float4 t = make_float4(whole(o[i][0]), whole(o[i][1]), whole(o[i][2]), whole(o[i][3]));
+            if (rr < ROWS) so[wave][rr][4 * i + g] = t;
         }
         lds_barrier();
-        float M = kPgNone;
 #pragma unroll
-        for (int w = 0; w < kDecWaves; ++w) M = fmaxf(M, sml[w][orow].x);
-        float lt = 0.0f;
-        float4 t = make_float4(0, 0, 0, 0);
+        for (int i = 0; i < RT; ++i) {
+            const int row = orow + 8 * i;
+            float M = kPgNone;
 #pragma unroll
-        for (int w = 0; w < kDecWaves; ++w) {
-            const float2 p = sml[w][orow];
-            const float f = p.x == kPgNone ? 0.0f : __builtin_amdgcn_exp2f(p.x - M);
-            const float4 v = so[w][orow][od >> 2];
-            lt = __builtin_fmaf(p.y, f, lt);
-            t.x = __builtin_fmaf(v.x, f, t.x);
-            t.y = __builtin_fmaf(v.y, f, t.y);
-            t.z = __builtin_fmaf(v.z, f, t.z);
-            t.w = __builtin_fmaf(v.w, f, t.w);
-        }
-        if (orow < ng) {
+            for (int w = 0; w < kDecWaves; ++w) M = fmaxf(M, sml[w][row].x);
+            float lt = 0.0f;
+            float4 t = make_float4(0, 0, 0, 0);
+#pragma unroll
+            for (int w = 0; w < kDecWaves; ++w) {
+                const float2 p = sml[w][row];
+                const float f = p.x == kPgNone ? 0.0f : __builtin_amdgcn_exp2f(p.x - M);
+                const float4 v = so[w][row][od >> 2];
+                lt = __builtin_fmaf(p.y, f, lt);
+                t.x = __builtin_fmaf(v.x, f, t.x);
+                t.y = __builtin_fmaf(v.y, f, t.y);
+                t.z = __builtin_fmaf(v.z, f, t.z);
+                t.w = __builtin_fmaf(v.w, f, t.w);
+            }
+            if (row >= ng) continue;
             if (runs == 1) {
-                pg_store4(out + (size_t)(g0 + orow) * kPgHd + od, pg_quot(t.x, lt), pg_quot(t.y, lt), pg_quot(t.z, lt),
+                pg_store4(out + (size_t)(g0 + row) * kPgHd + od, pg_quot(t.x, lt), pg_quot(t.y, lt), pg_quot(t.z, lt),
                           pg_quot(t.w, lt));
             } else {
-                const size_t at = (size_t)(part + run) * a.G + g0 + orow;
+                const size_t at = (size_t)(part + run) * a.G + g0 + row;
                 pg_put(a.o + at * 64 + (od >> 1), t.x, t.y);
                 pg_put(a.o + at * 64 + (od >> 1) + 1, t.z, t.w);
                 if (od == 0) pg_put(a.ml + at, M, lt);
             }
         }
         lds_barrier();   // LDS is free for the next heads
-        qv = load_q(hc + kDecRows);
+        load_q(hc + ROWS);
     }
     if (runs == 1) return;
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -1408,8 +1426,14 @@ extern "C" int oxb_attn_decode_paged(const void *q, int dtype, const void *pages
     const PgDecodeArgs a{q, (const _Float16 *)pages, table, len, n_pages, paged_log(page_size), table_stride, batch,
                          H, Hkv, G, p.denom, out, (int *)wp, (uint64_t *)(wp + w.ml), (uint64_t *)(wp + w.o)};
     const dim3 grid((unsigned)p.wgs), th(kDecThreads);
-    if (dtype == OXB_F32) hipLaunchKernelGGL((paged_decode_kernel<float>), grid, th, 0, (hipStream_t)stream, a);
-    else hipLaunchKernelGGL((paged_decode_kernel<_Float16>), grid, th, 0, (hipStream_t)stream, a);
+    hipStream_t s = (hipStream_t)stream;
+    if (dtype == OXB_F32) {
+        if (G <= 8) hipLaunchKernelGGL((paged_decode_kernel<float, 8>), grid, th, 0, s, a);
+        else hipLaunchKernelGGL((paged_decode_kernel<float, 16>), grid, th, 0, s, a);
+    } else {
+        if (G <= 8) hipLaunchKernelGGL((paged_decode_kernel<_Float16, 8>), grid, th, 0, s, a);
+        else hipLaunchKernelGGL((paged_decode_kernel<_Float16, 16>), grid, th, 0, s, a);
+    }
     OXB_CHECK_HIP(hipGetLastError());
     return 0;
 }
