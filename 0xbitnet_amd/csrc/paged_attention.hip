@@ -159,15 +159,16 @@ constexpr int kDecThreads = 64 * kDecWaves;
 constexpr int kDecRows = 8;            // query heads that the workgroup's threads hold a row of
 constexpr int kDecQs = kPgHd + 8;      // q row stride in LDS (f16)
 constexpr int kDecLeast = 4;           // units of a run
+constexpr int kDecFine = 24;           // units of a run, more of which are cut finer than one round of the card
 constexpr int kDecUncut = 16;          // units of a sequence that is not cut
 constexpr int kDecSlots = 512;         // runs that are resident at once, at most
-constexpr int kDecParts = 2 * kDecSlots;
+constexpr int kDecParts = 4 * kDecSlots;
 
 struct PgDecodeArgs {
     const void *q;
     const _Float16 *pages;
     const int *table, *len;
-    int n_pages, page_log, table_stride, batch, H, Hkv, G, denom;
+    int n_pages, page_log, table_stride, batch, H, Hkv, G, runs, most;   // runs beside one a sequence and head: wanted, at most
     void *out;
     int *cnt;        // [kDecParts] zero between calls
     uint64_t *ml;    // [kDecParts][G] reference and sum (two floats)
@@ -188,8 +189,8 @@ __global__ __launch_bounds__(kDecThreads, 2) void paged_decode_kernel(PgDecodeAr
     const int64_t cap = (int64_t)a.table_stride << a.page_log;
 
     // Each wave: the sum of all units, the runs' length from it, and the run of this
-    // workgroup.  sum ceil(n / per) <= sum n / per + batch, so per = sum / (runs that
-    // are wanted, less one a sequence) keeps within the launch.
+    // workgroup.  sum ceil(n / per) <= sum n / per + batch, so per >= sum / (runs beside
+    // one a sequence) keeps within the launch.
     auto length = [&](int z) { return z < a.batch ? (int)min(max((int64_t)a.len[z], (int64_t)0), cap) : 0; };
     const int len0 = length(lane);
     uint32_t total = pg_units(len0);
@@ -197,7 +198,8 @@ __global__ __launch_bounds__(kDecThreads, 2) void paged_decode_kernel(PgDecodeAr
 #pragma unroll
     for (int s = 32; s > 0; s >>= 1) total += __shfl_xor(total, s, 64);
     const uint64_t all = (uint64_t)total * a.Hkv;
-    const int per = max(kDecLeast, (int)min((all + a.denom - 1) / a.denom, (uint64_t)1 << 20));
+    auto share = [&](int runs) { return (int)min((all + runs - 1) / runs, (uint64_t)1 << 20); };
+    const int per = max(kDecLeast, max(share(a.most), min(share(a.runs), kDecFine)));
     int z = -1, len = 0, runs = 0, r = 0, part = 0;
     {
         int base = 0, cut = 0;   // workgroups and parts before the 64 sequences
@@ -486,24 +488,28 @@ __global__ __launch_bounds__(kDecThreads, 2) void paged_decode_kernel(PgDecodeAr
     }
 }
 
-// Workgroups of a launch and the runs that are wanted beside one a sequence and
-// head.  Where the sequences alone are half of the resident workgroups or more, half
-// as many are wanted beside them.
+// Workgroups of a launch, and the runs that are wanted beside one a sequence and head:
+// as many as are resident with them.  Where the sequences alone are half of the
+// resident workgroups or more, half as many beside them; there runs of more than
+// kDecFine units are cut further, as the rounds' ends cost more than a join then (up
+// to 4096 positions, H 20 over 5: 64 sequences 64.5 -> 61.2 us, 52 of up to 2304 34.3
+// -> 32.1; cut to 12 units 63.4 and 35.0).
 struct DecodePlan {
-    int denom;
+    int runs, most;
     int64_t wgs;
 };
 static DecodePlan decode_plan(int batch, int Hkv, int64_t units) {
     const int slots = std::min(2 * device_cus(), kDecSlots);
     const int64_t rows = (int64_t)batch * Hkv;
     DecodePlan p;
-    p.denom = rows < slots / 2 ? (int)(slots - rows) : slots / 2;
-    p.wgs = std::min(rows + p.denom, rows * ((units + kDecLeast - 1) / kDecLeast));
+    p.runs = rows < slots / 2 ? (int)(slots - rows) : slots / 2;
+    p.most = rows < slots / 2 ? p.runs : 2 * slots;
+    p.wgs = std::min(rows + p.most, rows * (units <= kDecUncut ? 1 : (units + kDecLeast - 1) / kDecLeast));
     return p;
 }
 
 // Parts: only a cut sequence's.  k runs where k > 1 are at most 2 (k - 1), and the
-// runs past one of each sequence and head are denom <= kDecSlots at most.
+// runs past one of each sequence and head are 2 kDecSlots at most.
 struct DecodeWs {
     size_t ml, o, bytes;
 };
@@ -1424,7 +1430,7 @@ extern "C" int oxb_attn_decode_paged(const void *q, int dtype, const void *pages
     char *wp = (char *)ws;
     const DecodePlan p = decode_plan(batch, Hkv, ((int64_t)table_stride * page_size + kPgUnit - 1) / kPgUnit);
     const PgDecodeArgs a{q, (const _Float16 *)pages, table, len, n_pages, paged_log(page_size), table_stride, batch,
-                         H, Hkv, G, p.denom, out, (int *)wp, (uint64_t *)(wp + w.ml), (uint64_t *)(wp + w.o)};
+                         H, Hkv, G, p.runs, p.most, out, (int *)wp, (uint64_t *)(wp + w.ml), (uint64_t *)(wp + w.o)};
     const dim3 grid((unsigned)p.wgs), th(kDecThreads);
     hipStream_t s = (hipStream_t)stream;
     if (dtype == OXB_F32) {

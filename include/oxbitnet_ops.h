@@ -449,7 +449,7 @@ int oxb_paged_append(void *pages, int n_pages, int page_size, int Hkv, int hd, c
  *            parts each, sums are f32 (22 bits of each value)
  *   OXB_F16  q and out f16, the same sums, rounded once
  * The result does not depend on timing.  ws: a device workspace of
- * oxb_attn_decode_paged_ws_bytes bytes, 256-byte aligned; its first 4 KB are arrival
+ * oxb_attn_decode_paged_ws_bytes bytes, 256-byte aligned; its first 8 KB are arrival
  * counters that must be zero before its first use (a zero-filled allocation) and that
  * every call leaves zero, so one serves calls of any batch and lengths in turn (the
  * size depends on H / Hkv alone).  Calls that share one must not run concurrently.
