@@ -540,8 +540,9 @@ static DecodeWs decode_ws(int G) {
 //
 // What the sequences' lengths are is known on the device only.  A first launch, of
 // one workgroup, makes the list of runs: the tiles, each a run where they fill the
-// card, else cut into runs of `per` units at most, the least that keeps all runs
-// resident at once; the longest first.  A last launch joins the cut tiles' parts.
+// card (but for the last few of equal ones), else cut into runs of `per` units at
+// most, the least that keeps all runs resident at once; the longest first.  A last
+// launch joins the cut tiles' parts.
 constexpr int kPreWaves = 4;
 constexpr int kPreThreads = 64 * kPreWaves;
 constexpr int kPreRows = 32 * kPreWaves;
@@ -581,7 +582,7 @@ struct PgPrefillArgs {
     float inv_G;
     void *out;
     int *counts;    // runs, `cuts`, whether tiles may be cut (then a record a workgroup)
-    PgRun *runs;    // [most], or [kPreOrder] in the order of the workgroups
+    PgRun *runs;    // [most + slots], or [kPreOrder] in the order of the workgroups
     PgCut *cuts;    // cut tiles, or where there is no plan all tiles
     float2 *ml;     // [slots][Hkv][rows] a row's reference and sum
     float *o;       // [slots][Hkv][rows][128]
@@ -599,7 +600,8 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PgPrefillArgs 
     __shared__ uint16_t tile_z[kPreSlots];
     __shared__ int hist[kPlanThreads];
     __shared__ uint32_t wsum[5][kWaves];
-    __shared__ int wmax[kWaves], fit[2][kWaves];
+    __shared__ int wmax[kWaves], wmin[kWaves], fit[2][kWaves];
+    __shared__ float wfsum[kWaves];
     const int tid = threadIdx.x, lane = tid & 63, B = a.batch;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int64_t cap = (int64_t)a.table_stride << a.page_log;
@@ -652,6 +654,7 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PgPrefillArgs 
     };
     Tile own{0, 0, 0};   // of a tile a thread, where they may be cut
     int mx = 0, sum = 0;
+    float fsum = 0.0f;
     if (cut) {
         if (tid < nt) {
             own = tile(tid);
@@ -659,16 +662,47 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PgPrefillArgs 
             tile_z[tid] = own.z;
         }
     } else {
-        for (int t = tid; t < nt; t += kPlanThreads) mx = max(mx, tile(t).units);
+        for (int t = tid; t < nt; t += kPlanThreads) {
+            const int u = tile(t).units;
+            mx = max(mx, u);
+            fsum += (float)u;
+        }
+        fsum = wave_sum(fsum);
     }
 #pragma unroll
     for (int s = 32; s > 0; s >>= 1) mx = max(mx, __shfl_xor(mx, s, 64));
-    if (lane == 0) wmax[wave] = mx;
+    if (lane == 0) {
+        wmax[wave] = mx;
+        wfsum[wave] = fsum;
+    }
     scan(sum, wsum[2], sum);
     mx = lane < kWaves ? wmax[lane] : 0;
 #pragma unroll
     for (int s = 32; s > 0; s >>= 1) mx = max(mx, __shfl_xor(mx, s, 64));
-    int per = max(mx, 1), total = nt, cuts = 0;
+    int per = max(mx, 1), total = nt, cuts = 0, pieces = 1;
+    const int rest = a.slots > 1 ? nt % a.slots : 0;
+    if (!cut && rest && 2 * rest <= a.slots) {   // (uniform)
+        // Whole rounds of tiles that are nearly equal, and a few more: those are cut so
+        // that they fill a round of their own together.
+        fsum = wave_sum(lane < kWaves ? wfsum[lane] : 0.0f);
+        if (fsum > 0.75f * (float)mx * (float)nt) {
+            int least = tid < rest ? tile(nt - rest + tid).units : INT32_MAX;
+#pragma unroll
+            for (int s = 32; s > 0; s >>= 1) least = min(least, __shfl_xor(least, s, 64));
+            if (lane == 0) wmin[wave] = least;
+            __syncthreads();
+            for (int w = 0; w < kWaves; ++w) least = min(least, wmin[w]);
+            pieces = min(a.slots / rest, least / kPreLeast);
+            if (pieces > 1) {
+                cuts = rest;
+                total = nt + rest * (pieces - 1);
+                if (tid < rest) {
+                    const Tile r = tile(nt - rest + tid);
+                    a.cuts[tid] = PgCut{r.i, tid * pieces, pieces, s_cu[r.z], s_nq[r.z], {0, 0, 0}};
+                }
+            }
+        }
+    }
     if (cut) {
         // the least run length whose runs all are resident: a candidate a wave
         int lo = max(kPreLeast, nt ? sum / a.slots : 0), hi = per;
@@ -702,7 +736,14 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PgPrefillArgs 
         a.counts[2] = cut;
     }
     auto run = [&](int j) {
-        int k = 1, i = 0, t = j;
+        int k = 1, i = 0, t = j, part = j;
+        if (!cut && j >= nt - cuts) {
+            part = j - (nt - cuts);
+            k = pieces;
+            t = part / k;
+            i = part - t * k;
+            t += nt - cuts;
+        }
         if (cut) {
             int l = 0, h = nt - 1;
             while (l < h) {
@@ -723,7 +764,7 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PgPrefillArgs 
         } else {
             r = tile(t);
         }
-        return PgRun{r.i, pg_run_start(r.units, k, i), pg_run_start(r.units, k, i + 1), k > 1 ? j : -1, s_cu[r.z], s_nq[r.z], s_past[r.z],
+        return PgRun{r.i, pg_run_start(r.units, k, i), pg_run_start(r.units, k, i + 1), k > 1 ? part : -1, s_cu[r.z], s_nq[r.z], s_past[r.z],
                      r.z, r.i * kPreRows / a.G, 0, {0, 0}};
     };
     if (cut) {
@@ -1379,14 +1420,14 @@ static PrefillPlan prefill_plan(int n, int batch, int G, int Hkv) {
     p.most = (int)(rows / kPreRows + std::min<int64_t>(batch, n));
     p.slots = std::min(2 * device_cus(), kPreSlots) / Hkv;
     p.rows = (int)std::min<int64_t>(kPreRows, rows);
-    p.wgs = std::max<int64_t>((int64_t)p.most * Hkv, kPreOrder);
+    p.wgs = std::max<int64_t>((int64_t)(p.most + p.slots) * Hkv, kPreOrder);
     size_t at = kPreHead + 256;
     auto take = [&](size_t b) {
         const size_t o = at;
         at += pg_align(b);
         return o;
     };
-    p.runs = take(std::max<int64_t>(p.most, kPreOrder) * sizeof(PgRun));
+    p.runs = take(std::max<int64_t>(p.most + p.slots, kPreOrder) * sizeof(PgRun));
     p.cuts = take((size_t)std::max(p.slots / 2 + 1, kFewTiles) * sizeof(PgCut));
     p.ml = take((size_t)p.slots * Hkv * p.rows * 8);
     p.o = take((size_t)p.slots * Hkv * p.rows * kPgHd * 4);

@@ -470,6 +470,24 @@ def test_long_runs_over_shared_pages():
             ref.check_rows(got[r:r + 1], want, tol, (z, i))
 
 
+@pytest.mark.parametrize("n,past", [(1056, 3000), (1100, 300), (1500, 2000), (1030, 2500)])
+def test_tiles_past_a_round(n, past):
+    """A few tiles more than workgroups that are resident: cut where all are nearly equal;
+    every token of some heads, some tokens of all."""
+    rng = rng_of("round", n, past)
+    hkv, H = 8, 64
+    c, K, V = filled(rng, [past + n], hkv, 64)
+    q = rng.standard_normal((n, H * HD)).astype(np.float32)
+    got = c.attn_prefill(q, [0, n])
+    for i in [0, 1, n // 2, n - 1]:
+        want, tol = expect(q[i:i + 1], K[0], V[0], hkv, past + i)
+        ref.check_rows(got[i:i + 1], want, tol, i)
+    for h in (0, 63):
+        at = slice(h * HD, (h + 1) * HD)
+        out, tol = ref.attend(q[::5, at], K[0][:, h // 8], V[0][:, h // 8], past + 1 + np.arange(n)[::5])
+        ref.check_rows(got[::5, at], out, tol, h)
+
+
 def test_rows_of_q_that_are_not_finite():
     """An Inf or NaN in a row of q makes that head's row NaN and no other."""
     rng = rng_of("wild q")
