@@ -281,13 +281,15 @@ __global__ __launch_bounds__(kDecThreads, 2) void paged_decode_kernel(PgDecodeAr
             for (int s = 16; s > 0; s >>= 1) m = fmaxf(m, __shfl_xor(m, s, 64));
             const int e = pg_row_exp(m);
             const float f[4] = {v.x, v.y, v.z, v.w};
+            half4_t hi, lo;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 const float x = ldexpf(f[j], -e);
-                const _Float16 hi = (_Float16)x;
-                sq[row * kDecQs + od + j] = hi;
-                sq[(row + ROWS) * kDecQs + od + j] = (_Float16)(x - (float)hi);
+                hi[j] = (_Float16)x;
+                lo[j] = (_Float16)(x - (float)hi[j]);
             }
+            *(half4_t *)(sq + row * kDecQs + od) = hi;
+            *(half4_t *)(sq + (row + ROWS) * kDecQs + od) = lo;
             if ((tid & 31) == 0) sqs[row] = ldexpf(kPgScore, e);
         }
         lds_barrier();
@@ -375,7 +377,7 @@ __global__ __launch_bounds__(kDecThreads, 2) void paged_decode_kernel(PgDecodeAr
         for (int i = 0; i < 8; ++i) {
             auto whole = [](float v) { return RT == 1 ? v + pg_ror8(v) : v; };
             const float4 t = make_float4(whole(o[i][0]), whole(o[i][1]), whole(o[i][2]), whole(o[i][3]));
-            if (rr < ROWS) so[wave][rr][4 * i + g] = t;
+            if (rr < ROWS) so[wave][rr][(4 * i + g) ^ (4 * (rr & 7))] = t;   // (no two rows in a bank)
         }
         lds_barrier();
 #pragma unroll
@@ -390,7 +392,7 @@ __global__ __launch_bounds__(kDecThreads, 2) void paged_decode_kernel(PgDecodeAr
             for (int w = 0; w < kDecWaves; ++w) {
                 const float2 p = sml[w][row];
                 const float f = p.x == kPgNone ? 0.0f : __builtin_amdgcn_exp2f(p.x - M);
-                const float4 v = so[w][row][od >> 2];
+                const float4 v = so[w][row][(od >> 2) ^ (4 * orow)];
                 lt = __builtin_fmaf(p.y, f, lt);
                 t.x = __builtin_fmaf(v.x, f, t.x);
                 t.y = __builtin_fmaf(v.y, f, t.y);
