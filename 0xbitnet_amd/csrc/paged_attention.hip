@@ -154,6 +154,13 @@ __device__ __forceinline__ R pg_uniform(const R *p) {
 // ragged batch is spread evenly whatever its longest sequence is.  A sequence's
 // runs meet in the workspace: each stores its part and counts in, and the last one
 // joins them in order, so the sum does not depend on which is last.
+// H 20 over 5, pages of 32: 64 sequences of up to 4096, 284 MB, 60.5 us (4.7 TB/s);
+// four of up to 100001, 527 MB, 98.5 us (5.3 TB/s, a copy 4.9); one of 2304, 6 MB, 8.6
+// us, a chain of loads (length, page, K and V, parts) of 0.5 to 1 us each.  Sequences
+// of up to 512 positions are not cut: 32 of them 9.4 -> 8.4 us, 8 of 300 8.0 -> 7.0,
+// one of 500 7.9 -> 8.1.  H 32 over 2, 13 of up to 49812: 68 us, in two passes of 8
+// heads 107.  Joining 32 runs at once instead of 16 gave nothing (100000 positions
+// 47.8, 47.1 us; 2304 8.6, 9.3).
 constexpr int kDecWaves = 4;
 constexpr int kDecThreads = 64 * kDecWaves;
 constexpr int kDecRows = 8;            // query heads that the workgroup's threads hold a row of
@@ -539,12 +546,23 @@ static DecodeWs decode_ws(int G) {
 // unit's score products alternate with this unit's exponentials, and P.V with the
 // rest of them.  K runs a unit ahead of V; rings of four units of each leave one
 // barrier per two units.
+// H 20 over 5: 8192 tokens 598 us f32 (1152 TFLOP/s of MFMA work, both parts; a large
+// f16 product of the library 1153); 12 prompts of up to 4096 510-525 us f32, 320-335
+// f16 (1050, 850 TFLOP/s), of which an f16 tile's beginning and end are 14k cycles, 12%
+// (20k with q and the output straight from and to memory); the MFMAs are busy for 62%
+// (f32) and 46% (f16) of all cycles.  101 tokens 12 us; 23 drafts of up to 5 tokens
+// behind up to 4000 33 us; 333 tokens behind 30011 and two shorter turns, f16, 149-157.
+// Not kept (f32, f16 of the 12 prompts; then 519, 320): 64 rows a wave, one wave a SIMD
+// (859, 409: the compiler moves accumulators to and fro); tiles of 256 rows, eight
+// waves (532, 317; the 333 tokens 160 against 152); the loads of K and V spread over the
+// products (522, 326) or V through registers (531, 343).
 //
 // What the sequences' lengths are is known on the device only.  A first launch, of
 // one workgroup, makes the list of runs: the tiles, each a run where they fill the
 // card (but for the last few of equal ones), else cut into runs of `per` units at
 // most, the least that keeps all runs resident at once; the longest first.  A last
-// launch joins the cut tiles' parts.
+// launch joins the cut tiles' parts.  (The tiles past whole rounds of equal ones: 3300
+// tokens behind 20000 1622 -> 1228 us, where 3264 take 1213; 4096 1704 -> 1560.)
 constexpr int kPreWaves = 4;
 constexpr int kPreThreads = 64 * kPreWaves;
 constexpr int kPreRows = 32 * kPreWaves;
@@ -593,7 +611,8 @@ struct PgPrefillArgs {
 // Latency is all that counts here: lengths are loaded once and kept in LDS, a sum over
 // the workgroup takes one barrier, and the search for `per` starts between the bounds
 // that the units' sum gives (sum ceil(n / per) lies between sum n / per and that plus
-// the tiles), so that one round of candidates decides as a rule.
+// the tiles), so that one round of candidates decides as a rule.  The 12 prompts' plan
+// of 664 tiles: 8.0 us (12.0 with lengths and tiles looked up in memory by each step).
 __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PgPrefillArgs a) {
     constexpr int kWaves = kPlanThreads / 64;
     __shared__ int s_cu[kPgBatch], s_nq[kPgBatch], s_past[kPgBatch];
@@ -826,7 +845,9 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PgPrefillArgs 
 // makes by itself: a lane a sequence, a lane a tile (two), so that no launch comes
 // before the attention's (its 4 to 7 us and the gap behind it).  All runs are
 // resident at once, so their order matters little: only each XCD's stretch of
-// them, and of a CU's two one from either end.
+// them, and of a CU's two one from either end.  (101 tokens 16.4 -> 12.2 us, the
+// drafts 37 -> 33.  The join reads what the first run of each tile leaves: with a plan of
+// its own it took 11.3 us for 6.3.)
 constexpr int kFewTiles = 128;
 struct PgFew {
     int nt, total;                     // tiles, runs
@@ -1362,7 +1383,9 @@ __global__ __launch_bounds__(kPreThreads, 2) void paged_prefill_kernel(PgPrefill
     }
 }
 
-// Joins a cut tile's parts: 32 threads a row, 4 dims each.
+// Joins a cut tile's parts: 32 threads a row, 4 dims each.  Bound by the parts' bytes
+// where there are many (the 333 tokens: 31 MB in 8.2 us), else by the launch (the
+// drafts 6.3; 32 rows a workgroup the same).
 template <typename T>
 __global__ __launch_bounds__(256) void paged_join_kernel(PgPrefillArgs a) {
     const int c = blockIdx.x / (kPreRows / 8), kvh = blockIdx.y, d = (threadIdx.x & 31) * 4;
