@@ -80,7 +80,8 @@ def test_attention_refusals():
     common[12] = (dict(ln=None), "cu or len")
     refused(pre, common + [(dict(wsb=need - 1), "workspace"), (dict(cu=None), "cu or len"), (dict(n=0), "0 tokens"),
                            (dict(n=-3), "-3 tokens"), (dict(n=1 << 29), "tokens"),
-                           (dict(n=1 << 28, H=4096, hkv=4096), "4096 heads")])
+                           (dict(n=(1 << 27) + 1, H=1), "tokens"),
+                           (dict(n=1 << 20, H=4096, hkv=4096), "4096 heads")])
     for args in ((0, 4, 1, 128), (1, 5, 2, 128), (1, 4, 1, 64), (4097, 4, 1, 128), (1, 4, 0, 128)):
         assert L().oxb_attn_decode_paged_ws_bytes(*args) == 0
         assert L().oxb_attn_prefill_paged_ws_bytes(1, *args) == 0
