@@ -175,7 +175,8 @@ struct PgDecodeArgs {
     const void *q;
     const _Float16 *pages;
     const int *table, *len;
-    int n_pages, page_log, table_stride, batch, H, Hkv, G, runs, most;   // runs beside one a sequence and head: wanted, at most
+    int n_pages, page_log, table_stride, batch, H, Hkv, G;
+    int runs, most, slots;   // runs beside one a sequence and head: wanted, at most; resident ones, to be filled
     void *out;
     int *cnt;        // [kDecParts] zero between calls
     uint64_t *ml;    // [kDecParts][G] reference and sum (two floats)
@@ -206,13 +207,26 @@ __global__ __launch_bounds__(kDecThreads, 2) void paged_decode_kernel(PgDecodeAr
     for (int s = 32; s > 0; s >>= 1) total += __shfl_xor(total, s, 64);
     const uint64_t all = (uint64_t)total * a.Hkv;
     auto share = [&](int runs) { return (int)min((all + runs - 1) / runs, (uint64_t)1 << 20); };
-    const int per = max(kDecLeast, max(share(a.most), min(share(a.runs), kDecFine)));
+    int per = max(kDecLeast, max(share(a.most), min(share(a.runs), kDecFine)));
+    auto runs_of = [&](int units, int per) {
+        return units <= kDecUncut ? 1 : pg_div(units + per - 1, __builtin_amdgcn_rcpf((float)per));
+    };
+    // few sequences, which are in the lanes: the least length that fits (48 of up to 2304
+    // 32.0 -> 30.6 us, 32 23.4 -> 22.5)
+    if (a.slots) {
+        for (int lo = max(kDecLeast, share(a.slots)); lo < per;) {
+            const int c = (lo + per) >> 1;
+            const int n = wave_isum_dpp(lane < a.batch ? runs_of(pg_units(len0), c) : 0) * a.Hkv;
+            if (n <= a.slots) per = c;
+            else lo = c + 1;
+        }
+    }
     int z = -1, len = 0, runs = 0, r = 0, part = 0;
     {
         int base = 0, cut = 0;   // workgroups and parts before the 64 sequences
         for (int c = 0; c < a.batch; c += 64) {
             const int n = c ? length(c + lane) : len0, u = pg_units(n);
-            const int k = c + lane < a.batch ? (u <= kDecUncut ? 1 : (u + per - 1) / per) : 0;
+            const int k = c + lane < a.batch ? runs_of(u, per) : 0;
             const int upto = wave_iscan(k * a.Hkv), cutto = wave_iscan(k > 1 ? k * a.Hkv : 0);
             const int i = __popcll(__ballot(base + upto <= (int)blockIdx.x));
             if (i < 64) {
@@ -504,7 +518,7 @@ __global__ __launch_bounds__(kDecThreads, 2) void paged_decode_kernel(PgDecodeAr
 // to 4096 positions, H 20 over 5: 64 sequences 64.5 -> 61.2 us, 52 of up to 2304 34.3
 // -> 32.1; cut to 12 units 63.4 and 35.0).
 struct DecodePlan {
-    int runs, most;
+    int runs, most, slots;
     int64_t wgs;
 };
 static DecodePlan decode_plan(int batch, int Hkv, int64_t units) {
@@ -513,6 +527,7 @@ static DecodePlan decode_plan(int batch, int Hkv, int64_t units) {
     DecodePlan p;
     p.runs = rows < slots / 2 ? (int)(slots - rows) : slots / 2;
     p.most = rows < slots / 2 ? p.runs : 2 * slots;
+    p.slots = rows < slots / 2 && batch <= 64 ? slots : 0;
     p.wgs = std::min(rows + p.most, rows * (units <= kDecUncut ? 1 : (units + kDecLeast - 1) / kDecLeast));
     return p;
 }
@@ -1496,7 +1511,7 @@ extern "C" int oxb_attn_decode_paged(const void *q, int dtype, const void *pages
     char *wp = (char *)ws;
     const DecodePlan p = decode_plan(batch, Hkv, ((int64_t)table_stride * page_size + kPgUnit - 1) / kPgUnit);
     const PgDecodeArgs a{q, (const _Float16 *)pages, table, len, n_pages, paged_log(page_size), table_stride, batch,
-                         H, Hkv, G, p.runs, p.most, out, (int *)wp, (uint64_t *)(wp + w.ml), (uint64_t *)(wp + w.o)};
+                         H, Hkv, G, p.runs, p.most, p.slots, out, (int *)wp, (uint64_t *)(wp + w.ml), (uint64_t *)(wp + w.o)};
     const dim3 grid((unsigned)p.wgs), th(kDecThreads);
     hipStream_t s = (hipStream_t)stream;
     if (dtype == OXB_F32) {
