@@ -80,6 +80,14 @@ __device__ __forceinline__ float pg_ror8(float v) {   // lane i of 16 takes lane
 // every multiple of d, the product less than that off.
 __device__ __forceinline__ int pg_div(int x, float inv) { return (int)(((float)x + 0.5f) * inv); }
 
+// Units before run i of k even runs: units i / k, its whole part apart (units up to
+// 2^19, k and i up to 1025).
+__device__ __forceinline__ int pg_run_start(int units, int k, int i) {
+    const float inv = __builtin_amdgcn_rcpf((float)k);
+    const int part = pg_div(units, inv), more = units - part * k;
+    return part * i + pg_div(more * i, inv);
+}
+
 __device__ __forceinline__ int pg_units(int64_t positions) { return (int)((positions + kPgUnit - 1) >> 5); }
 
 // Sums over the lanes up to this one.
@@ -91,6 +99,17 @@ __device__ __forceinline__ int wave_iscan(int v) {
     v += dpp0<0x142, 0xa>(v);
     v += dpp0<0x143, 0xc>(v);
     return v;
+}
+
+// The largest of the lanes' values (not negative).
+__device__ __forceinline__ int wave_imax(int v) {
+    v = max(v, dpp0<0x111, 0xf>(v));
+    v = max(v, dpp0<0x112, 0xf>(v));
+    v = max(v, dpp0<0x114, 0xf>(v));
+    v = max(v, dpp0<0x118, 0xf>(v));
+    v = max(v, dpp0<0x142, 0xa>(v));
+    v = max(v, dpp0<0x143, 0xc>(v));
+    return __builtin_amdgcn_readlane(v, 63);
 }
 
 // Hand-over between workgroups goes through agent-scope stores and loads.
@@ -201,12 +220,13 @@ __global__ __launch_bounds__(kDecThreads, 2) void paged_decode_kernel(PgDecodeAr
     // one a sequence) keeps within the launch.
     auto length = [&](int z) { return z < a.batch ? (int)min(max((int64_t)a.len[z], (int64_t)0), cap) : 0; };
     const int len0 = length(lane);
-    uint32_t total = pg_units(len0);
+    uint32_t total = pg_units(len0);   // (2^31 at most)
     for (int c = 64; c < a.batch; c += 64) total += pg_units(length(c + lane));
-#pragma unroll
-    for (int s = 32; s > 0; s >>= 1) total += __shfl_xor(total, s, 64);
-    const uint64_t all = (uint64_t)total * a.Hkv;
-    auto share = [&](int runs) { return (int)min((all + runs - 1) / runs, (uint64_t)1 << 20); };
+    total = (uint32_t)wave_isum_dpp((int)total);
+    // all / runs or up to 1 more (the product is within 2^-21 of it; whole divisions of 64
+    // bits would be a tenth of a short call's time)
+    const float all = (float)total * (float)a.Hkv * 1.000001f;
+    auto share = [&](int runs) { return (int)fminf(all * __builtin_amdgcn_rcpf((float)runs), 1 << 20) + 1; };
     int per = max(kDecLeast, max(share(a.most), min(share(a.runs), kDecFine)));
     auto runs_of = [&](int units, int per) {
         return units <= kDecUncut ? 1 : pg_div(units + per - 1, __builtin_amdgcn_rcpf((float)per));
@@ -242,10 +262,10 @@ __global__ __launch_bounds__(kDecThreads, 2) void paged_decode_kernel(PgDecodeAr
         }
     }
     if (z < 0 || z >= a.batch) return;
-    const int kvh = r % a.Hkv, run = r / a.Hkv;
+    const int run = r / a.Hkv, kvh = r - run * a.Hkv;
     part += kvh * runs;   // the parts of this sequence and head
     const int units = pg_units(len);
-    const int b0 = (int)((int64_t)units * run / runs), b1 = (int)((int64_t)units * (run + 1) / runs);
+    const int b0 = pg_run_start(units, runs, run), b1 = pg_run_start(units, runs, run + 1);
     T *out = (T *)a.out + ((size_t)z * a.H + (size_t)kvh * a.G) * kPgHd;
     if (b0 >= b1) {   // (an idle sequence)
         for (int i = tid; i < a.G * kPgHd; i += kDecThreads) out[i] = (T)0.0f;
@@ -600,14 +620,6 @@ struct PgCut {
     int tile, part, runs, cu, nq, unused[3];
 };
 
-// A cut tile's units in even runs: units i / k, its whole part apart (units up to
-// 2^19, k and i up to 512).
-__device__ __forceinline__ int pg_run_start(int units, int k, int i) {
-    const float inv = __builtin_amdgcn_rcpf((float)k);
-    const int part = pg_div(units, inv), more = units - part * k;
-    return part * i + pg_div(more * i, inv);
-}
-
 struct PgPrefillArgs {
     const void *q;
     const _Float16 *pages;
@@ -900,10 +912,10 @@ __device__ __forceinline__ PgFew pg_few(const PgPrefillArgs &a) {
         mx = max(mx, p.units[c]);
     }
     sum = wave_isum_dpp(sum);
-#pragma unroll
-    for (int s = 32; s > 0; s >>= 1) mx = max(mx, __shfl_xor(mx, s, 64));
-    int lo = max(kPreLeast, sum / a.slots), hi = max(__builtin_amdgcn_readfirstlane(mx), 1);
-    if (p.nt < a.slots) hi = min(hi, max(lo, (sum + a.slots - p.nt - 1) / (a.slots - p.nt)));
+    // (bounds, the lower from below, the upper from above)
+    auto share = [&](int n) { return (float)sum * __builtin_amdgcn_rcpf((float)n); };
+    int lo = max(kPreLeast, (int)(share(a.slots) * 0.999999f)), hi = max(wave_imax(mx), 1);
+    if (p.nt < a.slots) hi = min(hi, max(lo, (int)(share(a.slots - p.nt) * 1.000001f) + 1));
     auto runs = [&](int u, int t, int per) {
         return t < p.nt ? max(1, pg_div(u + per - 1, __builtin_amdgcn_rcpf((float)per))) : 0;
     };
