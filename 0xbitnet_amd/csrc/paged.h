@@ -12,6 +12,7 @@ constexpr int kPgUnit = OXB_PAGED_UNIT;        // positions of a layout unit
 constexpr int kPgHalf = kPgUnit * kPgHd;       // elements of a unit's K (or V)
 constexpr int kPgElems = 2 * kPgHalf;          // elements of a unit: K, then V
 constexpr int kPgBatch = OXB_PAGED_MAX_BATCH;
+constexpr int kPgPrefill = OXB_PAGED_MAX_PREFILL;   // sequences of a prefill call
 
 // Elements inside a unit (include/oxbitnet_ops.h): 8 dims of a K row, 8
 // positions of a V dim are 16 bytes, an MFMA operand's share of a lane.

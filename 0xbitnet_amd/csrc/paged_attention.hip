@@ -642,19 +642,19 @@ struct PgPrefillArgs {
 // of 664 tiles: 8.0 us (12.0 with lengths and tiles looked up in memory by each step).
 __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PgPrefillArgs a) {
     constexpr int kWaves = kPlanThreads / 64;
-    __shared__ int s_cu[kPgBatch], s_nq[kPgBatch], s_past[kPgBatch];
-    __shared__ uint32_t upto[kPgBatch];                 // tiles of the sequences up to z
+    static_assert(kPgPrefill <= kPlanThreads, "a thread a sequence");
+    __shared__ int s_cu[kPgPrefill], s_nq[kPgPrefill], s_past[kPgPrefill];
+    __shared__ uint32_t upto[kPgPrefill];               // tiles of the sequences up to z
     __shared__ int cost[kPreSlots], first[kPreSlots];   // of a tile that may be cut: units, runs up to it
     __shared__ uint16_t tile_z[kPreSlots];
     __shared__ int hist[kPlanThreads];
-    __shared__ uint32_t wsum[5][kWaves];
+    __shared__ uint32_t wsum[4][kWaves];
     __shared__ int wmax[kWaves], wmin[kWaves], fit[2][kWaves];
     __shared__ float wfsum[kWaves];
     const int tid = threadIdx.x, lane = tid & 63, B = a.batch;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int64_t cap = (int64_t)a.table_stride << a.page_log;
-    // Inclusive sum over the threads; `all` is the whole one.  `to` is free again after
-    // the next barrier but one.
+    // Inclusive sum over the threads; `all` is the whole one.
     auto scan = [&](int v, uint32_t *to, int &all) {
         v = wave_iscan(v);
         if (lane == 63) to[wave] = v;
@@ -664,23 +664,18 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PgPrefillArgs 
         return v + (wave ? __builtin_amdgcn_readlane(w, wave - 1) : 0);
     };
     hist[tid] = 0;
-    int nt = 0;   // (cut off at what a cu that ascends has at most)
-    for (int c = 0, i = 0; c < B; c += kPlanThreads, i ^= 1) {   // (uniform)
-        const int z = c + tid;
-        int tiles = 0;
-        if (z < B) {
-            const int c0 = min(max(a.cu[z], 0), a.n_tok), c1 = min(max(a.cu[z + 1], 0), a.n_tok);
-            const int nq = max(c1 - c0, 0);
-            s_cu[z] = c0;
-            s_nq[z] = nq;
-            s_past[z] = (int)(min(max((int64_t)a.len[z], (int64_t)0), cap) - nq);
-            tiles = (nq * a.G + kPreRows - 1) / kPreRows;
-        }
-        int all;
-        const int v = scan(tiles, wsum[i], all);
-        if (z < B) upto[z] = nt + v;
-        nt = min(nt + all, a.most);
+    int nt = 0;
+    if (tid < B) {
+        const int c0 = min(max(a.cu[tid], 0), a.n_tok), c1 = min(max(a.cu[tid + 1], 0), a.n_tok);
+        const int nq = max(c1 - c0, 0);
+        s_cu[tid] = c0;
+        s_nq[tid] = nq;
+        s_past[tid] = (int)(min(max((int64_t)a.len[tid], (int64_t)0), cap) - nq);
+        nt = (nq * a.G + kPreRows - 1) / kPreRows;
     }
+    const int tiles = scan(nt, wsum[0], nt);
+    if (tid < B) upto[tid] = tiles;
+    nt = min(nt, a.most);   // (what a cu that ascends has at most)
     __syncthreads();
     const bool cut = nt <= a.slots;
     struct Tile {
@@ -723,7 +718,7 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PgPrefillArgs 
         wmax[wave] = mx;
         wfsum[wave] = fsum;
     }
-    scan(sum, wsum[2], sum);
+    scan(sum, wsum[1], sum);
     mx = lane < kWaves ? wmax[lane] : 0;
 #pragma unroll
     for (int s = 32; s > 0; s >>= 1) mx = max(mx, __shfl_xor(mx, s, 64));
@@ -771,7 +766,7 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PgPrefillArgs 
         per = max(hi, 1);
         // runs of the tiles up to each, and cut tiles above bit 16
         const int k = tid < nt ? max(1, pg_div(own.units + per - 1, __builtin_amdgcn_rcpf((float)per))) : 0;
-        const int v = scan(k | (k > 1 ? 1 << 16 : 0), wsum[3], total);
+        const int v = scan(k | (k > 1 ? 1 << 16 : 0), wsum[2], total);
         cuts = total >> 16;
         total &= 0xffff;
         if (tid < nt) first[tid] = v & 0xffff;
@@ -834,7 +829,7 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PgPrefillArgs 
         __syncthreads();
         const int h = hist[tid];
         int all;
-        const int v = scan(h, wsum[4], all);
+        const int v = scan(h, wsum[3], all);
         hist[tid] = v - h;
         __syncthreads();
         if (tid < each * 8) {
@@ -859,7 +854,7 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PgPrefillArgs 
     __syncthreads();
     const int h = hist[tid];
     int all;
-    const int v = scan(h, wsum[4], all);
+    const int v = scan(h, wsum[3], all);
     hist[tid] = v - h;
     __syncthreads();
     for (int j = tid; j < total; j += kPlanThreads) {
@@ -939,7 +934,8 @@ __device__ __forceinline__ int pg_of_tile(const int (&f)[2], int t) {
 }
 
 // 16 bytes of each lane from base + off to LDS at m0 + 16 * lane (as lds_dma16, with a
-// scalar base).
+// scalar base).  The load reads m0 a wait state after its write at the earliest, and
+// the base five after one by v_readfirstlane; the compiler adds neither inside asm.
 __device__ __forceinline__ void pg_dma16(const void *base, uint32_t off, uint32_t lds) {
     // (uniform as they are: for the compiler)
     const uint64_t at = (uint64_t)base;
@@ -948,7 +944,7 @@ __device__ __forceinline__ void pg_dma16(const void *base, uint32_t off, uint32_
     const uint32_t slds = __builtin_amdgcn_readfirstlane((int)lds);
     uint32_t saved;
     asm volatile(
-        "s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %2, %3\n\ts_mov_b32 m0, %0"
+        "s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 2\n\tglobal_load_lds_dwordx4 %2, %3\n\ts_mov_b32 m0, %0"
         : "=&s"(saved)
         : "s"(slds), "v"(off), "s"(sbase)
         : "memory");
@@ -1538,7 +1534,7 @@ extern "C" int oxb_attn_decode_paged(const void *q, int dtype, const void *pages
 }
 
 extern "C" size_t oxb_attn_prefill_paged_ws_bytes(int n_tok, int batch, int H, int Hkv, int hd) {
-    if (n_tok < 1 || batch < 1 || batch > kPgBatch || Hkv < 1 || Hkv > 4096 || H < 1 || H % Hkv || H > 65535 ||
+    if (n_tok < 1 || batch < 1 || batch > kPgPrefill || Hkv < 1 || Hkv > 4096 || H < 1 || H % Hkv || H > 65535 ||
         hd != kPgHd || (int64_t)n_tok * (H / Hkv) > kPreMost)
         return 0;
     return prefill_plan(n_tok, batch, H / Hkv, Hkv).bytes;
@@ -1552,6 +1548,7 @@ extern "C" int oxb_attn_prefill_paged(const void *q, int dtype, const void *page
     if (paged_check(pages, n_pages, page_size, Hkv, hd) || paged_table_check(table, table_stride, page_size, batch) ||
         heads_check(H, Hkv) || dtype_check(dtype, q, out))
         return -1;
+    OXB_REQUIRE(batch <= kPgPrefill, "prefill attention: batch %d", batch);
     OXB_REQUIRE(cu && len, "prefill attention: cu or len is NULL");
     const int G = H / Hkv;
     OXB_REQUIRE(n_tok >= 1 && (int64_t)n_tok * G <= kPreMost, "prefill attention: %d tokens", n_tok);

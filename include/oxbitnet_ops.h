@@ -59,11 +59,12 @@ extern "C" {
 #define OXB_F16 1
 
 /* The paged KV cache (oxb_paged_*): positions of its layout unit, the largest
- * page, the longest sequence and the largest batch. */
+ * page, the longest sequence, the largest batch, and that of a prefill call. */
 #define OXB_PAGED_UNIT 32
 #define OXB_PAGED_MAX_PAGE 4096
 #define OXB_PAGED_MAX_SEQ (1 << 24)
 #define OXB_PAGED_MAX_BATCH 4096
+#define OXB_PAGED_MAX_PREFILL 128
 
 /* ---- errors, device memory, streams, events (plumbing) ----------------- */
 const char *oxb_last_error(void);
@@ -445,6 +446,7 @@ int oxb_paged_append(void *pages, int n_pages, int page_size, int Hkv, int hd, c
  * of a page id outside 0..n_pages-1 are not there.  What lies behind the length, and
  * in other pages, may hold anything; a visible Inf or NaN makes what it reaches NaN
  * or Inf.
+ * out may be q.
  *   OXB_F32  q and out f32: q and the softmax weights go through f16 MFMA as two
  *            parts each, sums are f32 (22 bits of each value)
  *   OXB_F16  q and out f16, the same sums, rounded once
@@ -467,8 +469,10 @@ int oxb_attn_decode_paged(const void *q, int dtype, const void *pages, int n_pag
  * they were.  Types, pages and what is not there as above; with OXB_F16 the softmax
  * weights are f16.  ws: oxb_attn_prefill_paged_ws_bytes bytes, 256-byte aligned, any
  * contents (one workspace may serve decode too, whose counters this call leaves
- * alone); the size grows with n_tok and batch.  n_tok * H / Hkv is 2^27 at most.  Calls that share one must not run
- * concurrently. */
+ * alone); the size grows with n_tok and batch.  Calls that share one must not run
+ * concurrently.  n_tok * H / Hkv is 2^27 at most, batch OXB_PAGED_MAX_PREFILL: more
+ * sequences go in several calls, each with the rows of table, cu and len from its first
+ * sequence on. */
 size_t oxb_attn_prefill_paged_ws_bytes(int n_tok, int batch, int H, int Hkv, int hd);
 int oxb_attn_prefill_paged(const void *q, int dtype, const void *pages, int n_pages, int page_size,
                            const int *table, int table_stride, const int *cu, const int *len,

@@ -88,6 +88,15 @@ def test_attention_refusals():
     assert L().oxb_attn_prefill_paged_ws_bytes(0, 1, 4, 1, 128) == 0
 
 
+def test_sequences_of_a_prefill_call():
+    """128 at most; decode takes 4096."""
+    f, need = L().oxb_attn_prefill_paged_ws_bytes, L().oxb_attn_prefill_paged_ws_bytes(4096, 128, 4, 2, 128)
+    assert need > 0 and f(4096, 129, 4, 2, 128) == 0 and f(4096, 4096, 4, 2, 128) == 0
+    assert L().oxb_attn_decode_paged_ws_bytes(4096, 4, 2, 128) > 0
+    refused(lambda b: L().oxb_attn_prefill_paged(P, 0, P, 4, 32, P, 2, P, P, 4096, b, 4, 2, 128, P, P, 1 << 40, None),
+            [(dict(b=129), "batch 129"), (dict(b=4096), "batch 4096")])
+
+
 def test_workspace_grows_with_the_call():
     """One workspace of the largest call serves every smaller one; decode's depends on
     the group alone."""
