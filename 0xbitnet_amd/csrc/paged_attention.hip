@@ -173,12 +173,12 @@ __device__ __forceinline__ R pg_uniform(const R *p) {
 // ragged batch is spread evenly whatever its longest sequence is.  A sequence's
 // runs meet in the workspace: each stores its part and counts in, and the last one
 // joins them in order, so the sum does not depend on which is last.
-// H 20 over 5, pages of 32: 64 sequences of up to 4096, 284 MB, 60.5 us (4.7 TB/s);
-// four of up to 100001, 527 MB, 98.5 us (5.3 TB/s, a copy 4.9); one of 2304, 6 MB, 8.6
+// H 20 over 5, pages of 32: 64 sequences of up to 4096, 284 MB, 60 us (4.7 TB/s);
+// four of up to 100001, 527 MB, 98.5 us (5.35 TB/s, a copy 4.9); one of 2304, 6 MB, 8.2
 // us, a chain of loads (length, page, K and V, parts) of 0.5 to 1 us each.  Sequences
 // of up to 512 positions are not cut: 32 of them 9.4 -> 8.4 us, 8 of 300 8.0 -> 7.0,
-// one of 500 7.9 -> 8.1.  H 32 over 2, 13 of up to 49812: 68 us, in two passes of 8
-// heads 107.  Joining 32 runs at once instead of 16 gave nothing (100000 positions
+// one of 500 7.9 -> 8.1 (since then 8.3, 6.7, 7.5).  H 32 over 2, 13 of up to 49812: 67
+// us, in two passes of 8 heads 107.  Joining 32 runs at once instead of 16 gave nothing (100000 positions
 // 47.8, 47.1 us; 2304 8.6, 9.3).
 constexpr int kDecWaves = 4;
 constexpr int kDecThreads = 64 * kDecWaves;
@@ -232,7 +232,7 @@ __global__ __launch_bounds__(kDecThreads, 2) void paged_decode_kernel(PgDecodeAr
         return units <= kDecUncut ? 1 : pg_div(units + per - 1, __builtin_amdgcn_rcpf((float)per));
     };
     // few sequences, which are in the lanes: the least length that fits (48 of up to 2304
-    // 32.0 -> 30.6 us, 32 23.4 -> 22.5)
+    // 32.0 -> 30.6 us, 32 23.4 -> 22.0)
     if (a.slots) {
         for (int lo = max(kDecLeast, share(a.slots)); lo < per;) {
             const int c = (lo + per) >> 1;
@@ -582,11 +582,11 @@ static DecodeWs decode_ws(int G) {
 // rest of them.  K runs a unit ahead of V; rings of four units of each leave one
 // barrier per two units.
 // H 20 over 5: 8192 tokens 598 us f32 (1152 TFLOP/s of MFMA work, both parts; a large
-// f16 product of the library 1153); 12 prompts of up to 4096 510-525 us f32, 320-335
+// f16 product of the library 1153); 12 prompts of up to 4096 510-535 us f32, 320-335
 // f16 (1050, 850 TFLOP/s), of which an f16 tile's beginning and end are 14k cycles, 12%
 // (20k with q and the output straight from and to memory); the MFMAs are busy for 62%
 // (f32) and 46% (f16) of all cycles.  101 tokens 12 us; 23 drafts of up to 5 tokens
-// behind up to 4000 33 us; 333 tokens behind 30011 and two shorter turns, f16, 149-157.
+// behind up to 4000 32 us; 333 tokens behind 30011 and two shorter turns, f16, 149-160.
 // Not kept (f32, f16 of the 12 prompts; then 519, 320): 64 rows a wave, one wave a SIMD
 // (859, 409: the compiler moves accumulators to and fro); tiles of 256 rows, eight
 // waves (532, 317; the 333 tokens 160 against 152); the loads of K and V spread over the

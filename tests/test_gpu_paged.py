@@ -854,6 +854,34 @@ def test_longest_sequence():
         ref.close_in_norm(got, want, q.reshape(3, HD), K[0][:, 0], page * W)
 
 
+@pytest.mark.parametrize("B", [128, 200])
+def test_sequences_of_several_calls(B):
+    """As many sequences as a prefill call takes, and more in two calls: table, lengths and
+    cu from a sequence on, one buffer of q and out."""
+    rng = rng_of("calls", B)
+    L, H, hkv, page, most = ops.lib(), 6, 2, 32, 128
+    new = [int(x) for x in rng.integers(0, 40, B)]
+    lens = [a + int(b) for a, b in zip(new, rng.integers(0, 90, B))]
+    c, K, V = filled(rng, lens, hkv, page)
+    cu = np.concatenate([[0], np.cumsum(new)]).astype(np.int32)
+    n = int(cu[-1])
+    q = rng.standard_normal((n, H * HD)).astype(np.float32)
+    dq, dc, out = ops.DeviceArray.from_host(q), ops.DeviceArray.from_host(cu), ops.DeviceArray(q.shape, np.float32)
+    for z in range(0, B, most):
+        b = min(most, B - z)
+        need = L.oxb_attn_prefill_paged_ws_bytes(n, b, H, hkv, HD)
+        ws = ops.DeviceArray((need,), np.uint8)
+        ops.check(L.oxb_attn_prefill_paged(dq.ptr, 0, c.pool.ptr, c.n_pages, page, c.table.offset(4 * z * c.table.shape[1]),
+                                           c.table.shape[1], dc.offset(4 * z), c.len.offset(4 * z), n, b, H, hkv, HD,
+                                           out.ptr, ws.ptr, need, None))
+        ops.sync()
+    got = out.download()
+    for z, m in enumerate(new):
+        at = slice(cu[z], cu[z + 1])
+        want, tol = expect(q[at], K[z], V[z], hkv, lens[z] - m)
+        ref.check_rows(got[at], want, tol, z)
+
+
 @pytest.mark.skip(reason="the packed prefill of 4096 sequences faulted and its cause is not known: such calls "
                          "are refused (128 at most)")
 def test_largest_batch():
