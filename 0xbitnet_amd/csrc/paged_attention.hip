@@ -23,7 +23,10 @@
 //
 // What a row does not see has no part in it, whatever its bytes are: hidden scores
 // become -inf by selection, and V elements that are not finite are taken out of
-// units that some row does not see whole (0 times them would be NaN).
+// units that some row does not see whole (0 times them would be NaN).  A reference
+// of -inf says that a row has seen nothing, and its output is zeros; what it does see
+// raises the reference to kPgLow at least, so that a row whose scores all are -inf
+// has weights and a sum of 0 and ends as 0 / 0, NaN, as a softmax does.
 #include "paged.h"
 
 #include <algorithm>
@@ -42,6 +45,7 @@ constexpr float kPgStep = 8.0f;       // a score may pass the reference by this 
 constexpr float kPgBase = 6.0f;       // p' <= 2^(6 + kPgStep)
 constexpr int kPgQExp = 14;           // q rows are scaled below 2^kPgQExp
 constexpr float kPgNone = -__builtin_inff();
+constexpr float kPgLow = -0x1.fffffep127f;   // the lowest f32
 
 // A row's reference.  mx is the lane's largest score; where any row of the wave
 // passes its reference by kPgStep, all take their row's maxima (over LANES lane
@@ -139,8 +143,8 @@ __device__ __forceinline__ void pg_store4(_Float16 *p, float x, float y, float z
     *(half4_t *)p = half4_t{(_Float16)x, (_Float16)y, (_Float16)z, (_Float16)w};
 }
 
-// A row's value from its parts' sum t and softmax sum l (0: nothing seen).
-__device__ __forceinline__ float pg_quot(float t, float l) { return l == 0.0f ? 0.0f : t / l; }
+// A row's value from its parts' sum t, softmax sum l and reference m (nothing seen: 0).
+__device__ __forceinline__ float pg_quot(float t, float l, float m) { return m == kPgNone ? 0.0f : t / l; }
 
 // What all lanes read and no kernel in flight writes: by scalar loads.
 template <typename R>
@@ -373,6 +377,7 @@ __global__ __launch_bounds__(kDecThreads, 2) void paged_decode_kernel(PgDecodeAr
 #pragma unroll
             for (int i = 0; i < 8; ++i)
                 if (!partial || i < left) mx = fmaxf(mx, x[i] * qs);
+            if (!partial || left > 0) mx = fmaxf(mx, kPgLow);
             if (ref.passed(mx)) {
                 const float al = ref.raise<4>(mx);
                 lsum *= al;
@@ -442,8 +447,8 @@ __global__ __launch_bounds__(kDecThreads, 2) void paged_decode_kernel(PgDecodeAr
             }
             if (row >= ng) continue;
             if (runs == 1) {
-                pg_store4(out + (size_t)(g0 + row) * kPgHd + od, pg_quot(t.x, lt), pg_quot(t.y, lt), pg_quot(t.z, lt),
-                          pg_quot(t.w, lt));
+                pg_store4(out + (size_t)(g0 + row) * kPgHd + od, pg_quot(t.x, lt, M), pg_quot(t.y, lt, M),
+                          pg_quot(t.z, lt, M), pg_quot(t.w, lt, M));
             } else {
                 const size_t at = (size_t)(part + run) * a.G + g0 + row;
                 pg_put(a.o + at * 64 + (od >> 1), t.x, t.y);
@@ -524,8 +529,8 @@ __global__ __launch_bounds__(kDecThreads, 2) void paged_decode_kernel(PgDecodeAr
                 t.z = __builtin_fmaf(v.z, f, t.z);
                 t.w = __builtin_fmaf(v.w, f, t.w);
             }
-            pg_store4(out + (size_t)(hc + orow) * kPgHd + od, pg_quot(t.x, lt), pg_quot(t.y, lt), pg_quot(t.z, lt),
-                      pg_quot(t.w, lt));
+            pg_store4(out + (size_t)(hc + orow) * kPgHd + od, pg_quot(t.x, lt, M), pg_quot(t.y, lt, M),
+                      pg_quot(t.z, lt, M), pg_quot(t.w, lt, M));
         }
         lds_barrier();
     }
@@ -1171,14 +1176,16 @@ __global__ __launch_bounds__(kPreThreads, 2) void paged_prefill_kernel(PgPrefill
         constexpr bool some_hidden = decltype(SOME)::value;
         const int p0 = b * kPgUnit;
         const bool there = !((gone >> (b & 31)) & 1);
+        float low = kPgLow;
         if constexpr (some_hidden) {
             // positions of the lane's scores: 16 (i / 8) + 8 h + i % 8
             const int left = there ? qpos + 1 - p0 - 8 * h : 0;
 #pragma unroll
             for (int i = 0; i < 16; ++i) s[i] = (i & 7) + 16 * (i >> 3) < left ? s[i] : kPgNone;
             smax = top(top(top(top(kPgNone, s, 0), s, 4), s, 8), s, 12);
+            if (left <= 0) low = kPgNone;
         }
-        const float mx = smax * qs;
+        const float mx = fmaxf(smax * qs, low);
         if (ref.passed(mx)) {
             const float al = ref.raise<2>(mx);
             lsum *= al;
@@ -1371,7 +1378,7 @@ __global__ __launch_bounds__(kPreThreads, 2) void paged_prefill_kernel(PgPrefill
     // of its row.  (Stored from there, 16 or 32 bytes a row with each store: twice the
     // time.)
     const bool direct = run.part < 0;
-    const float f = !direct ? 1.0f : lsum == 0.0f ? 0.0f : 1.0f / lsum;
+    const float f = !direct ? 1.0f : ref.m == kPgNone ? 0.0f : 1.0f / lsum;
     uint4 *so = &lds[0][0] + 1024 * wave;
     const int er = lane & 31;
     if (direct && PARTS == 1) {
@@ -1450,8 +1457,8 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PgPrefillArgs a) {
             s.w = __builtin_fmaf(v[i].w, f, s.w);
         }
     }
-    pg_store4((T *)a.out + ((size_t)(t.cu + row / a.G) * a.H + kvh * a.G + row % a.G) * kPgHd + d, pg_quot(s.x, lt),
-              pg_quot(s.y, lt), pg_quot(s.z, lt), pg_quot(s.w, lt));
+    pg_store4((T *)a.out + ((size_t)(t.cu + row / a.G) * a.H + kvh * a.G + row % a.G) * kPgHd + d, pg_quot(s.x, lt, M),
+              pg_quot(s.y, lt, M), pg_quot(s.z, lt, M), pg_quot(s.w, lt, M));
 }
 
 // Launch shapes and workspace of a call of n tokens: tiles at most (a sequence's

@@ -444,8 +444,10 @@ int oxb_paged_append(void *pages, int n_pages, int page_size, int Hkv, int hd, c
  * over positions 0..len[z]-1 (append first; 0 or less: the output is zeros; more than
  * the table's row holds: what it holds), any H that is a multiple of Hkv.  Positions
  * of a page id outside 0..n_pages-1 are not there.  What lies behind the length, and
- * in other pages, may hold anything; a visible Inf or NaN makes what it reaches NaN
- * or Inf.
+ * in other pages, may hold anything.  A visible Inf or NaN in V makes its dim NaN or
+ * Inf in the rows that see it, one in K those rows NaN; but a position whose score
+ * comes out as -Inf has weight 0 beside finite ones, and rows that see no other are
+ * NaN.
  * out may be q.
  *   OXB_F32  q and out f32: q and the softmax weights go through f16 MFMA as two
  *            parts each, sums are f32 (22 bits of each value)
