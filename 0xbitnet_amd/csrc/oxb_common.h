@@ -218,6 +218,28 @@ __device__ inline int wave_isum_dpp(int v) {
     return __builtin_amdgcn_readlane(v, 63);
 }
 
+// Sums over the lanes up to this one.
+__device__ inline int wave_iscan(int v) {
+    v += dpp0<0x111, 0xf>(v);
+    v += dpp0<0x112, 0xf>(v);
+    v += dpp0<0x114, 0xf>(v);
+    v += dpp0<0x118, 0xf>(v);
+    v += dpp0<0x142, 0xa>(v);
+    v += dpp0<0x143, 0xc>(v);
+    return v;
+}
+
+// The largest of the lanes' values (not negative).
+__device__ inline int wave_imax(int v) {
+    v = max(v, dpp0<0x111, 0xf>(v));
+    v = max(v, dpp0<0x112, 0xf>(v));
+    v = max(v, dpp0<0x114, 0xf>(v));
+    v = max(v, dpp0<0x118, 0xf>(v));
+    v = max(v, dpp0<0x142, 0xa>(v));
+    v = max(v, dpp0<0x143, 0xc>(v));
+    return __builtin_amdgcn_readlane(v, 63);
+}
+
 __device__ inline float wave_nonneg_max_dpp(float f) {
     int v = __float_as_int(f);
     v = __float_as_int(fmaxf(__int_as_float(v), __int_as_float(dpp0<0x111, 0xf>(v))));
