@@ -618,6 +618,8 @@ __global__ __launch_bounds__(kPreThreads, 2) void paged_prefill_kernel(PgPrefill
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     PgRun run;
     int kvh;
+    // (loaded with the list's arguments, not behind it: 101 tokens 12.1 -> 11.9 us)
+    asm volatile("" ::"s"(a.q), "s"(a.pages), "s"(a.table), "s"(a.n_pages), "s"(a.H), "s"(a.out));
     if (a.few) {
         const PgFew p = pg_few(a);
         if (blockIdx.x == 0 && tid == 0) a.counts[1] = p.nt;   // (for the join, of no tiles too)
@@ -1090,7 +1092,8 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PgPrefillArgs a) {
               pg_quot(s.y, lt, M), pg_quot(s.z, lt, M), pg_quot(s.w, lt, M));
 }
 
-// Workspace of a call of n tokens: the lists and the parts' rows.
+// Workspace of a call of n tokens (of its largest launch, whose sizes an n of the whole
+// call gives too): the lists and the parts' rows.
 struct PrefillPlan : PgSizes {
     int rows;
     size_t runs_at, cuts_at, ml, o, bytes;
@@ -1181,32 +1184,38 @@ extern "C" int oxb_attn_prefill_paged(const void *q, int dtype, const void *page
     OXB_REQUIRE(cu && len, "prefill attention: cu or len is NULL");
     const int G = H / Hkv;
     OXB_REQUIRE(n_tok >= 1 && (int64_t)n_tok * G <= kPreMost, "prefill attention: %d tokens", n_tok);
+    // (q's bytes would pass any device's memory)
+    OXB_REQUIRE((int64_t)n_tok * H <= INT32_MAX, "prefill attention: %d tokens of %d heads", n_tok, H);
     const PrefillPlan p = prefill_plan(n_tok, batch, G, Hkv);
-    OXB_REQUIRE(p.wgs < (1 << 24), "prefill attention: %d tokens of %d heads", n_tok, H);
     OXB_REQUIRE(ws && ((uintptr_t)ws & 255) == 0 && ws_bytes >= p.bytes,
                 "attention: workspace is NULL, not 256-byte aligned or %zu bytes < %zu", ws_bytes, p.bytes);
     char *w = (char *)ws;
-    const int few = pg_few_step(p, batch);
-    const PgPrefillArgs a{{cu, len, paged_log(page_size), table_stride, batch, n_tok, G, Hkv, p.most, p.slots,
-                           (device_cus() + 7) / 8, few, 1.0f / G, (int *)(w + kPreHead), (PgRun *)(w + p.runs_at),
-                           (PgCut *)(w + p.cuts_at)},
-                          q, (const _Float16 *)pages, table, n_pages, H, p.rows, out, (float2 *)(w + p.ml),
-                          (float *)(w + p.o)};
     hipStream_t s = (hipStream_t)stream;
-    if (!few) {
-        hipLaunchKernelGGL(paged_plan_kernel, dim3(1), dim3(kPlanThreads), 0, s, (const PgList &)a);
+    const int window = pg_window(n_tok, batch, G);
+    for (int t = 0; t < n_tok; t += std::min(window, n_tok - t)) {
+        const int n = std::min(window, n_tok - t);
+        const PgSizes z = pg_sizes(n, batch, G, Hkv, device_cus());
+        const int few = pg_few_step(z, batch);
+        const PgPrefillArgs a{{cu, len, paged_log(page_size), table_stride, batch, n_tok, t, t + n, G, Hkv, z.most, z.slots,
+                               (device_cus() + 7) / 8, few, 1.0f / G, (int *)(w + kPreHead), (PgRun *)(w + p.runs_at),
+                               (PgCut *)(w + p.cuts_at)},
+                              q, (const _Float16 *)pages, table, n_pages, H, p.rows, out, (float2 *)(w + p.ml),
+                              (float *)(w + p.o)};
+        if (!few) {
+            hipLaunchKernelGGL(paged_plan_kernel, dim3(1), dim3(kPlanThreads), 0, s, (const PgList &)a);
+            OXB_CHECK_HIP(hipGetLastError());
+        }
+        const dim3 grid((unsigned)z.wgs), th(kPreThreads);
+        if (dtype == OXB_F32) hipLaunchKernelGGL((paged_prefill_kernel<float>), grid, th, 0, s, a);
+        else hipLaunchKernelGGL((paged_prefill_kernel<_Float16>), grid, th, 0, s, a);
         OXB_CHECK_HIP(hipGetLastError());
-    }
-    const dim3 grid((unsigned)p.wgs), th(kPreThreads);
-    if (dtype == OXB_F32) hipLaunchKernelGGL((paged_prefill_kernel<float>), grid, th, 0, s, a);
-    else hipLaunchKernelGGL((paged_prefill_kernel<_Float16>), grid, th, 0, s, a);
-    OXB_CHECK_HIP(hipGetLastError());
-    // a tile is cut only where it has more than kPreLeast units
-    if ((int64_t)table_stride * page_size > kPreLeast * kPgUnit && p.slots > 1) {
-        const dim3 jgrid((unsigned)(few ? p.most : std::min(p.most, p.slots / 2)) * (kPreRows / 8), Hkv);
-        if (dtype == OXB_F32) hipLaunchKernelGGL((paged_join_kernel<float>), jgrid, dim3(256), 0, s, a);
-        else hipLaunchKernelGGL((paged_join_kernel<_Float16>), jgrid, dim3(256), 0, s, a);
-        OXB_CHECK_HIP(hipGetLastError());
+        // a tile is cut only where it has more than kPreLeast units
+        if ((int64_t)table_stride * page_size > kPreLeast * kPgUnit && z.slots > 1) {
+            const dim3 jgrid((unsigned)(few ? z.most : std::min(z.most, z.slots / 2)) * (kPreRows / 8), Hkv);
+            if (dtype == OXB_F32) hipLaunchKernelGGL((paged_join_kernel<float>), jgrid, dim3(256), 0, s, a);
+            else hipLaunchKernelGGL((paged_join_kernel<_Float16>), jgrid, dim3(256), 0, s, a);
+            OXB_CHECK_HIP(hipGetLastError());
+        }
     }
     return 0;
 }

@@ -31,8 +31,9 @@ constexpr int kPreLeast = 8;                 // units of a run
 constexpr int kPreSlots = 512;               // resident workgroups, at most
 constexpr int kPreOrder = kPreSlots;         // (a multiple of 8)
 constexpr int kPlanThreads = 1024;
+constexpr int kPreList = kPlanThreads;       // tiles and runs of a list, a thread each
 constexpr int kFewTiles = 128;
-constexpr int64_t kPreMost = 1 << 27;        // rows of a call: 2^20 tiles, 1024 times which is in 32 bits
+constexpr int64_t kPreMost = 1 << 27;        // rows of a call
 
 // A run: a tile's units u0 .. u1, and a cut tile: its parts.
 struct PgRun {
@@ -47,13 +48,26 @@ struct PgCut {
 // What a list is made from, and where it goes.
 struct PgList {
     const int *cu, *len;
-    int page_log, table_stride, batch, n_tok, G, Hkv, most, slots, half;
+    int page_log, table_stride, batch, n_tok, begin, end;   // of the call's n_tok tokens the launch's begin .. end - 1
+    int G, Hkv, most, slots, half;
     int few;        // no plan: the first step of a search among the batch's sequences (0: there is one)
     float inv_G;
     int *counts;    // runs, `cuts`, whether tiles may be cut (then a record a workgroup)
-    PgRun *runs;    // [most + slots], or [kPreOrder] in the order of the workgroups
+    PgRun *runs;    // [kPreList], or [kPreOrder] in the order of the workgroups
     PgCut *cuts;    // cut tiles, or where there is no plan all tiles
 };
+
+// Sequence z's tokens of the launch: the first one's place, their number, positions
+// that come before them.
+struct PgTokens {
+    int cu, nq, past;
+};
+__device__ __forceinline__ PgTokens pg_tokens(const PgList &a, int z) {
+    const int64_t cap = (int64_t)a.table_stride << a.page_log;
+    const int end = min(max(a.cu[z + 1], 0), a.n_tok);   // (of all that the call has)
+    const int c0 = min(max(a.cu[z], a.begin), a.end), c1 = min(max(end, a.begin), a.end);
+    return PgTokens{c0, max(c1 - c0, 0), (int)(min(max((int64_t)a.len[z], (int64_t)0), cap) - (end - c0))};
+}
 
 // Latency is all that counts here: lengths are loaded once and kept in LDS, a sum over
 // the workgroup takes one barrier, and the search for `per` starts between the bounds
@@ -62,7 +76,7 @@ struct PgList {
 // of 664 tiles: 8.0 us (12.0 with lengths and tiles looked up in memory by each step).
 __device__ __forceinline__ void pg_list(const PgList &a) {
     constexpr int kWaves = kPlanThreads / 64;
-    static_assert(kPgPrefill <= kPlanThreads, "a thread a sequence");
+    static_assert(kPgPrefill <= kPlanThreads && kPreSlots <= kPreList, "a thread a sequence, and a run");
     __shared__ int s_cu[kPgPrefill], s_nq[kPgPrefill], s_past[kPgPrefill];
     __shared__ uint32_t upto[kPgPrefill];               // tiles of the sequences up to z
     __shared__ int cost[kPreSlots], first[kPreSlots];   // of a tile that may be cut: units, runs up to it
@@ -70,10 +84,8 @@ __device__ __forceinline__ void pg_list(const PgList &a) {
     __shared__ int hist[kPlanThreads];
     __shared__ uint32_t wsum[4][kWaves];
     __shared__ int wmax[kWaves], wmin[kWaves], fit[2][kWaves];
-    __shared__ float wfsum[kWaves];
     const int tid = threadIdx.x, lane = tid & 63, B = a.batch;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int64_t cap = (int64_t)a.table_stride << a.page_log;
     // Inclusive sum over the threads; `all` is the whole one.
     auto scan = [&](int v, uint32_t *to, int &all) {
         v = wave_iscan(v);
@@ -86,12 +98,11 @@ __device__ __forceinline__ void pg_list(const PgList &a) {
     hist[tid] = 0;
     int nt = 0;
     if (tid < B) {
-        const int c0 = min(max(a.cu[tid], 0), a.n_tok), c1 = min(max(a.cu[tid + 1], 0), a.n_tok);
-        const int nq = max(c1 - c0, 0);
-        s_cu[tid] = c0;
-        s_nq[tid] = nq;
-        s_past[tid] = (int)(min(max((int64_t)a.len[tid], (int64_t)0), cap) - nq);
-        nt = (nq * a.G + kPreRows - 1) / kPreRows;
+        const PgTokens k = pg_tokens(a, tid);
+        s_cu[tid] = k.cu;
+        s_nq[tid] = k.nq;
+        s_past[tid] = k.past;
+        nt = (k.nq * a.G + kPreRows - 1) / kPreRows;
     }
     const int tiles = scan(nt, wsum[0], nt);
     if (tid < B) upto[tid] = tiles;
@@ -115,29 +126,19 @@ __device__ __forceinline__ void pg_list(const PgList &a) {
         r.units = pg_units(max(s_past[lo] + last / a.G + 1, 0));
         return r;
     };
-    Tile own{0, 0, 0};   // of a tile a thread, where they may be cut
+    Tile own{0, 0, 0};   // a thread's
     int mx = 0, sum = 0;
-    float fsum = 0.0f;
-    if (cut) {
-        if (tid < nt) {
-            own = tile(tid);
-            cost[tid] = mx = sum = own.units;
+    if (tid < nt) {
+        own = tile(tid);
+        mx = sum = own.units;
+        if (cut) {
+            cost[tid] = own.units;
             tile_z[tid] = own.z;
         }
-    } else {
-        for (int t = tid; t < nt; t += kPlanThreads) {
-            const int u = tile(t).units;
-            mx = max(mx, u);
-            fsum += (float)u;
-        }
-        fsum = wave_sum(fsum);
     }
 #pragma unroll
     for (int s = 32; s > 0; s >>= 1) mx = max(mx, __shfl_xor(mx, s, 64));
-    if (lane == 0) {
-        wmax[wave] = mx;
-        wfsum[wave] = fsum;
-    }
+    if (lane == 0) wmax[wave] = mx;
     scan(sum, wsum[1], sum);
     mx = lane < kWaves ? wmax[lane] : 0;
 #pragma unroll
@@ -147,22 +148,20 @@ __device__ __forceinline__ void pg_list(const PgList &a) {
     if (!cut && rest && 2 * rest <= a.slots) {   // (uniform)
         // Whole rounds of tiles that are nearly equal, and a few more: those are cut so
         // that they fill a round of their own together.
-        fsum = wave_sum(lane < kWaves ? wfsum[lane] : 0.0f);
-        if (fsum > 0.75f * (float)mx * (float)nt) {
-            int least = tid < rest ? tile(nt - rest + tid).units : INT32_MAX;
+        if ((float)sum > 0.75f * (float)mx * (float)nt) {
+            int least = tid >= nt - rest && tid < nt ? own.units : INT32_MAX;
 #pragma unroll
             for (int s = 32; s > 0; s >>= 1) least = min(least, __shfl_xor(least, s, 64));
             if (lane == 0) wmin[wave] = least;
             __syncthreads();
             for (int w = 0; w < kWaves; ++w) least = min(least, wmin[w]);
-            pieces = min(a.slots / rest, least / kPreLeast);
+            pieces = min(min(a.slots / rest, least / kPreLeast), 1 + (kPreList - nt) / rest);
             if (pieces > 1) {
                 cuts = rest;
                 total = nt + rest * (pieces - 1);
-                if (tid < rest) {
-                    const Tile r = tile(nt - rest + tid);
-                    a.cuts[tid] = PgCut{r.i, tid * pieces, pieces, s_cu[r.z], s_nq[r.z], {0, 0, 0}};
-                }
+                const int i = tid - (nt - rest);
+                if (i >= 0 && i < rest)
+                    a.cuts[i] = PgCut{own.i, i * pieces, pieces, s_cu[own.z], s_nq[own.z], {0, 0, 0}};
             }
         }
     }
@@ -269,18 +268,17 @@ __device__ __forceinline__ void pg_list(const PgList &a) {
     const float scale = (float)(kPlanThreads - 1) / (float)per;
     auto bucket = [&](const PgRun &r) { return (int)((float)(per - min(per, r.u1 - r.u0)) * scale); };
     PgRun mine{};
-    if (tid < total) mine = run(tid);
-    for (int j = tid; j < total; j += kPlanThreads) atomicAdd(&hist[bucket(j == tid ? mine : run(j))], 1);
+    if (tid < total) {
+        mine = run(tid);
+        atomicAdd(&hist[bucket(mine)], 1);
+    }
     __syncthreads();
     const int h = hist[tid];
     int all;
     const int v = scan(h, wsum[3], all);
     hist[tid] = v - h;
     __syncthreads();
-    for (int j = tid; j < total; j += kPlanThreads) {
-        const PgRun r = j == tid ? mine : run(j);
-        a.runs[atomicAdd(&hist[bucket(r)], 1)] = r;
-    }
+    if (tid < total) a.runs[atomicAdd(&hist[bucket(mine)], 1)] = mine;
 }
 
 // The same plan of a call of up to 64 sequences and kFewTiles tiles, which a wave
@@ -298,14 +296,10 @@ struct PgFew {
 __device__ __forceinline__ PgFew pg_few(const PgList &a) {
     const int lane = threadIdx.x & 63;
     PgFew p;
-    p.cu = p.nq = p.past = 0;
-    if (lane < a.batch) {
-        const int c0 = min(max(a.cu[lane], 0), a.n_tok), c1 = min(max(a.cu[lane + 1], 0), a.n_tok);
-        const int64_t cap = (int64_t)a.table_stride << a.page_log;
-        p.cu = c0;
-        p.nq = max(c1 - c0, 0);
-        p.past = (int)(min(max((int64_t)a.len[lane], (int64_t)0), cap) - p.nq);
-    }
+    const PgTokens own = pg_tokens(a, min(lane, a.batch - 1));   // (without a branch that loads wait for)
+    p.cu = own.cu;
+    p.nq = lane < a.batch ? own.nq : 0;
+    p.past = own.past;
     const int tiles = wave_iscan((p.nq * a.G + kPreRows - 1) / kPreRows);
     p.nt = min(__builtin_amdgcn_readlane(tiles, 63), min(a.most, kFewTiles));
     int sum = 0, mx = 0;
@@ -376,8 +370,23 @@ __device__ __forceinline__ bool pg_few_run(const PgList &a, const PgFew &p, int 
     return true;
 }
 
-// Sizes of a call of n tokens on `cus` CUs: tiles at most (a sequence's last one may be
-// short), runs that are resident at once, of a KV head, workgroups, and the records'
+// A call's tokens go in launches of `window` each, so that a list has kPreList tiles at
+// most, the longest that has run: a call of 4096 tiles, of as many sequences, ended in a
+// memory fault, and why is not known.  Even windows, of whole tiles of a sequence where
+// one fits.
+inline int pg_window(int n, int batch, int G) {
+    int64_t whole = kPreRows;   // tokens of whole tiles
+    while (whole > 1 && whole / 2 * G % kPreRows == 0) whole /= 2;
+    int64_t most = std::max<int64_t>(1, (int64_t)(kPreList - std::min(batch, n)) * kPreRows / G);
+    if (n <= most) return n;
+    if (most < whole) return (int)most;
+    most -= most % whole;
+    const int64_t parts = (n + most - 1) / most, even = (n + parts - 1) / parts;
+    return (int)((even + whole - 1) / whole * whole);
+}
+
+// Sizes of a launch of n tokens on `cus` CUs: tiles at most (a sequence's last one may
+// be short), runs that are resident at once, of a KV head, workgroups, and the records'
 // entries.
 struct PgSizes {
     int most, slots;
@@ -386,10 +395,10 @@ struct PgSizes {
 };
 inline PgSizes pg_sizes(int n, int batch, int G, int Hkv, int cus) {
     PgSizes p;
-    p.most = (int)((int64_t)n * G / kPreRows + std::min<int64_t>(batch, n));
+    p.most = (int)std::min<int64_t>((int64_t)n * G / kPreRows + std::min(batch, n), kPreList);
     p.slots = std::min(2 * cus, kPreSlots) / Hkv;
-    p.wgs = std::max<int64_t>((int64_t)(p.most + p.slots) * Hkv, kPreOrder);
-    p.runs = std::max(p.most + p.slots, kPreOrder);
+    p.runs = std::max(std::min(p.most + p.slots, kPreList), kPreOrder);
+    p.wgs = std::max<int64_t>((int64_t)std::min(p.most + p.slots, kPreList) * Hkv, kPreOrder);
     p.cuts = std::max(p.slots / 2 + 1, kFewTiles);
     return p;
 }

@@ -472,9 +472,12 @@ int oxb_attn_decode_paged(const void *q, int dtype, const void *pages, int n_pag
  * weights are f16.  ws: oxb_attn_prefill_paged_ws_bytes bytes, 256-byte aligned, any
  * contents (one workspace may serve decode too, whose counters this call leaves
  * alone); the size grows with n_tok and batch.  Calls that share one must not run
- * concurrently.  n_tok * H / Hkv is 2^27 at most, batch OXB_PAGED_MAX_PREFILL: more
- * sequences go in several calls, each with the rows of table, cu and len from its first
- * sequence on. */
+ * concurrently.  n_tok * H / Hkv is 2^27 at most, n_tok * H below 2^31; calls of more
+ * than 1024 tiles of 128 rows go in several launches.  batch is OXB_PAGED_MAX_PREFILL
+ * at most: that many are tested, a call of 4096 sequences once ended in a memory fault
+ * whose cause is not known, and lists of sequences and tiles as long as that one's have
+ * been closed since.  More sequences go in several calls, each with the rows of table,
+ * cu and len from its first sequence on. */
 size_t oxb_attn_prefill_paged_ws_bytes(int n_tok, int batch, int H, int Hkv, int hd);
 int oxb_attn_prefill_paged(const void *q, int dtype, const void *pages, int n_pages, int page_size,
                            const int *table, int table_stride, const int *cu, const int *len,

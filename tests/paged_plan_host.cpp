@@ -3,8 +3,8 @@
 // values.  Arguments: -1, 0 or 1, the steps that reciprocals are off by, and 1 for
 // threads that run in descending order.  Reads calls from standard input, whole numbers:
 //   cus n_tok batch G Hkv page_log table_stride  cu[batch + 1]  len[batch]
-// and writes for each, as int32: the sizes (most, slots, wgs, runs, cuts), the counts
-// and the entries of runs and of cuts that were written, [index, record ...] and -1 at
+// and writes for each, as int32: its launches' number and for each of these its tokens
+// (begin, end), the sizes (most, slots, wgs, runs, cuts), the counts and the entries of runs and of cuts that were written, [index, record ...] and -1 at
 // their end.  Where no list is made, count 2 is 2 and the runs are those that the
 // workgroups find themselves.  A write outside the entries ends the program.
 #include <ucontext.h>
@@ -195,23 +195,29 @@ int main(int argc, char **argv) {
             if (scanf("%d", &x) != 1) return 2;
         for (int &x : len)
             if (scanf("%d", &x) != 1) return 2;
-        const PgSizes p = pg_sizes(n, B, G, Hkv, cus);
-        const int sizes[5] = {p.most, p.slots, (int)p.wgs, (int)p.runs, (int)p.cuts};
-        put(sizes, 5);
-        int counts[4] = {-7, -7, -7, -7};
-        auto runs = blank<PgRun>(p.runs);
-        auto cuts = blank<PgCut>(p.cuts);
-        args = PgList{cu.data(), len.data(), plog, W, B, n, G, Hkv, p.most, p.slots, (cus + 7) / 8,
-                      pg_few_step(p, B), 1.0f / G, counts, runs.data(), cuts.data()};
-        few_runs.assign(args.few ? p.wgs : 0, PgRun{});
-        few_has.assign(few_runs.size(), 0);
-        launch(args.few ? 64 : kPlanThreads);
-        if (counts[3] != -7) return 3;
-        put(counts, 3);
-        for (size_t b = 0; b < few_runs.size(); ++b)   // (as the lists of a launch that has them)
-            if (few_has[b]) runs[b] = few_runs[b];
-        put_written(runs, args.few ? p.wgs : p.runs, "run");
-        put_written(cuts, p.cuts, "cut");
+        const PgSizes whole = pg_sizes(n, B, G, Hkv, cus);   // (the workspace's)
+        const int window = pg_window(n, B, G);
+        put((n + window - 1) / window);
+        for (int t = 0; t < n; t += window) {
+            const int end = min(n, t + window);
+            const PgSizes p = pg_sizes(end - t, B, G, Hkv, cus);
+            const int sizes[7] = {t, end, p.most, p.slots, (int)p.wgs, (int)whole.runs, (int)whole.cuts};
+            put(sizes, 7);
+            int counts[4] = {-7, -7, -7, -7};
+            auto runs = blank<PgRun>(whole.runs);
+            auto cuts = blank<PgCut>(whole.cuts);
+            args = PgList{cu.data(), len.data(), plog, W, B, n, t, end, G, Hkv, p.most, p.slots, (cus + 7) / 8,
+                          pg_few_step(p, B), 1.0f / G, counts, runs.data(), cuts.data()};
+            few_runs.assign(args.few ? p.wgs : 0, PgRun{});
+            few_has.assign(few_runs.size(), 0);
+            launch(args.few ? 64 : kPlanThreads);
+            if (counts[3] != -7) return 3;
+            put(counts, 3);
+            for (size_t b = 0; b < few_runs.size(); ++b)   // (as the lists of a launch that has them)
+                if (few_has[b]) runs[b] = few_runs[b];
+            put_written(runs, args.few ? p.wgs : whole.runs, "run");
+            put_written(cuts, whole.cuts, "cut");
+        }
     }
     return 0;
 }

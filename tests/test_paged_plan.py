@@ -9,7 +9,7 @@ import numpy as np
 import pytest
 
 HERE = os.path.dirname(os.path.abspath(__file__))
-ROWS, UNIT = 128, 32
+ROWS, UNIT, LIST = 128, 32, 1024
 RUN = ("tile", "u0", "u1", "part", "cu", "nq", "past", "z", "tok", "head")
 
 
@@ -42,17 +42,31 @@ def ceil(a, b):
 
 
 def check(call, words):
-    """One call's output; returns (tiles, whether tiles could be cut, cut tiles)."""
+    """One call's output: (tiles, whether tiles could be cut, cut tiles) of each launch."""
+    launches = words.take(1)[0]
+    out, at = [], 0
+    for _ in range(launches):
+        begin, end, *sizes = words.take(7)
+        assert begin == at < end
+        at = end
+        out.append(check_launch(call, begin, end, sizes, words))
+    assert at == call["head"][1]
+    return out
+
+
+def check_launch(call, begin, end, sizes, words):
     cus, n, B, G, hkv, log, W = call["head"]
-    cu, length = call["cu"], call["len"]
-    most, slots, wgs, n_runs, n_cuts = words.take(5)
+    length = call["len"]
+    cu = np.clip(call["cu"], begin, end).tolist()
+    most, slots, wgs, n_runs, n_cuts = sizes
     total, cuts, kind = words.take(3)
+    assert most <= LIST and n_runs <= LIST and total <= LIST
     runs, cut = words.entries(12), words.entries(8)
     cap = W << log
     tiles = {}
     for z in range(B):
         nq = cu[z + 1] - cu[z]
-        past = min(max(length[z], 0), cap) - nq
+        past = min(max(length[z], 0), cap) - (call["cu"][z + 1] - cu[z])
         for t in range(ceil(nq * G, ROWS)):
             last = min((t + 1) * ROWS, nq * G) - 1
             tiles[z, t] = ceil(max(past + last // G + 1, 0), UNIT), nq, past
@@ -133,21 +147,21 @@ CALLS = {
     "a group of more heads than rows": make([3, 0, 9], [40, 5, 60], 200, 1),
     "nothing to see": make([40, 6, 10], [-37, -6, -9], 2, 2),
     "few CUs": make([900, 70], [100, 3000], 4, 2, cus=3),
-    "1024 tiles": make([4096] * 8, [0] * 8, 4, 5),
+    "1016 tiles": make([4064] * 8, [0] * 8, 4, 5),
 }
 
 
 @pytest.mark.parametrize("descending", [0, 1])
 @pytest.mark.parametrize("rcp", [-1, 0, 1])
 def test_calls(program, rcp, descending):
-    for (name, call), (tiles, kind, cut) in zip(CALLS.items(), run(program, CALLS.values(), rcp, descending)):
+    for (name, call), [(tiles, kind, cut)] in zip(CALLS.items(), run(program, CALLS.values(), rcp, descending)):
         if name in ("one token", "a first turn", "drafts"):
             assert kind == 2, name                  # no list
-        if name in ("whole rounds", "packed prompts", "1024 tiles"):
+        if name in ("whole rounds", "packed prompts", "1016 tiles"):
             assert kind == 0 and not cut, name
         if "past a round" in name:
             assert kind == 0 and cut, name
-    assert tiles == 1024
+    assert tiles == 1016
 
 
 def test_calls_at_random(program):
@@ -162,5 +176,28 @@ def test_calls_at_random(program):
         past = (rng.integers(0, int(2 ** rng.uniform(0, 14)) + 1, B) * rng.integers(0, 2, B)).tolist()
         calls.append(make(new, past, G, hkv, int(rng.choice([32, 64, 256])), int(rng.choice([256, 256, 64])),
                           begin=int(rng.integers(0, 3)), behind=int(rng.integers(0, 40))))
-    kinds = [k for _, k, _ in run(program, calls)]
+    kinds = [k for r in run(program, calls) for _, k, _ in r]
     assert {0, 1, 2} == set(kinds)
+
+
+LONG = {
+    "1025 tiles": make([32800], [0], 4, 5),
+    "1025 tiles of 16 heads": make([8200], [700], 16, 2),
+    "prompts of many launches": make([30000, 0, 70001, 1, 4000], [0, 9, 100, 5, 20000], 4, 5),
+    "a whole batch": make([1000, 1, 90] * 42, [0, 3000, 40] * 42, 6, 2, begin=5, behind=300),
+    "one KV head": make([140000], [2000], 1, 1, page=256),
+    "four times the list": make([32] * 128, list(range(128)), 128, 1),
+    "a token is 512 tiles": make([3, 2], [50, 900], 65535, 1),
+    "few CUs": make([9000, 300], [0, 70], 16, 3, cus=7),
+    "behind the last token": make([40], [0], 4, 5, behind=40000),
+}
+
+
+@pytest.mark.parametrize("descending", [0, 1])
+def test_long_lists_go_in_several(program, descending):
+    """More tiles than a list takes: launches that follow one another, each a list of
+    1024 at most, every token in one of them."""
+    for (name, call), out in zip(LONG.items(), run(program, LONG.values(), 0, descending)):
+        most = call["head"][1] * call["head"][3] // ROWS + len(call["len"])
+        assert 1 < len(out) <= 2 * most // LIST + 2, name
+        assert sum(t for t, _, _ in out) >= sum(ceil(a * call["head"][3], ROWS) for a in np.diff(call["cu"])), name
