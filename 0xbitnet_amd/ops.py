@@ -370,7 +370,7 @@ class Kv8Cache:
 
 
 F32, F16 = 0, 1   # include/oxbitnet_ops.h OXB_F32, OXB_F16
-PAGED_UNIT = 32   # OXB_PAGED_UNIT
+PAGED_UNIT, PAGED_MAX_PREFILL = 32, 128   # OXB_PAGED_UNIT, OXB_PAGED_MAX_PREFILL
 
 
 class PagedCache:
@@ -454,11 +454,15 @@ class PagedCache:
         dq, dc = DeviceArray.from_host(q), DeviceArray.from_host(cu)
         do = DeviceArray.from_host(np.zeros_like(q) if out is None else np.ascontiguousarray(out, q.dtype))
         _require(do.shape == q.shape, f"out {do.shape} for {q.shape}")
-        ws = self._workspace(lib().oxb_attn_prefill_paged_ws_bytes(q.shape[0], self.batch, H, self.Hkv, self.hd))
-        check(lib().oxb_attn_prefill_paged(dq.ptr, dtype, self.pool.ptr, self.n_pages, self.page_size,
-                                           self.table.ptr, self.table.shape[1], dc.ptr, self.len.ptr, q.shape[0],
-                                           self.batch, H, self.Hkv, self.hd, do.ptr, *ws, None),
-              "attn_prefill_paged")
+        # as many sequences a call as one takes
+        parts = [(z, min(PAGED_MAX_PREFILL, self.batch - z)) for z in range(0, self.batch, PAGED_MAX_PREFILL)]
+        ws = self._workspace(max(lib().oxb_attn_prefill_paged_ws_bytes(q.shape[0], b, H, self.Hkv, self.hd)
+                                 for _, b in parts))
+        for z, b in parts:
+            check(lib().oxb_attn_prefill_paged(dq.ptr, dtype, self.pool.ptr, self.n_pages, self.page_size,
+                                               self.table.offset(4 * z * self.table.shape[1]), self.table.shape[1],
+                                               dc.offset(4 * z), self.len.offset(4 * z), q.shape[0], b, H, self.Hkv,
+                                               self.hd, do.ptr, *ws, None), "attn_prefill_paged")
         sync()
         return do.download()
 
