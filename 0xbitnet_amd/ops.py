@@ -387,13 +387,18 @@ class PagedCache:
         self.free = DeviceArray.from_host(np.arange(n_pages, dtype=np.int32)[::-1])
         self.n_free = DeviceArray.from_host(np.array([n_pages], np.int32))
         self.len = DeviceArray((batch,), np.int32, zero=True)
-        self._ws = {}
+        self._ws = None
 
     def _workspace(self, n: int) -> tuple:
+        """One for all calls, of the largest so far."""
         _require(n > 0, "no workspace for this shape")
-        if n not in self._ws:
-            self._ws[n] = DeviceArray((n,), np.uint8, zero=True)
-        return self._ws[n].ptr, n
+        if self._ws is None or self._ws.nbytes < n:
+            if self._ws is not None:
+                sync()
+                self._ws.free()
+            self._ws = None   # (should the allocation fail)
+            self._ws = DeviceArray((n,), np.uint8, zero=True)
+        return self._ws.ptr, self._ws.nbytes
 
     def step(self, delta, n_max: int | None = None) -> dict:
         """Grow, keep or shrink each sequence: granted tokens, and the packed tokens'
