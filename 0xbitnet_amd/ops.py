@@ -370,7 +370,8 @@ class Kv8Cache:
 
 
 F32, F16 = 0, 1   # include/oxbitnet_ops.h OXB_F32, OXB_F16
-PAGED_UNIT, PAGED_MAX_PREFILL = 32, 128   # OXB_PAGED_UNIT, OXB_PAGED_MAX_PREFILL
+# OXB_PAGED_UNIT, OXB_PAGED_MAX_SEQ, OXB_PAGED_MAX_BATCH, OXB_PAGED_MAX_PREFILL
+PAGED_UNIT, PAGED_MAX_SEQ, PAGED_MAX_BATCH, PAGED_MAX_PREFILL = 32, 1 << 24, 4096, 128
 
 
 class PagedCache:
@@ -382,6 +383,8 @@ class PagedCache:
         n = lib().oxb_paged_bytes(n_pages, page_size, Hkv, hd)
         if not n:
             raise NativeError(f"no pool of {n_pages} pages of {page_size} positions, {Hkv} heads of {hd}")
+        _require(1 <= batch <= PAGED_MAX_BATCH, f"batch {batch}")
+        _require(1 <= table_pages <= PAGED_MAX_SEQ // page_size, f"block table of {table_pages} pages a sequence")
         self.pool = DeviceArray((n // 2,), np.uint16)
         self.table = DeviceArray.from_host(np.full((batch, table_pages), -1, np.int32))
         self.free = DeviceArray.from_host(np.arange(n_pages, dtype=np.int32)[::-1])

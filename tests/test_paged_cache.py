@@ -44,3 +44,17 @@ def test_one_workspace(counted):
         assert sum(counted.values()) - before == max(sizes)
     with pytest.raises(ValueError):
         c._workspace(0)
+
+
+def test_shapes_are_checked_before_anything_is_allocated(counted):
+    for batch, table_pages in ((0, 8), (-1, 8), (4097, 8), (4, 0), (4, -3), (4, (1 << 19) + 1)):
+        with pytest.raises(ValueError):
+            ops.PagedCache(batch, 2, 40, 32, table_pages)
+    with pytest.raises(ops.NativeError):
+        ops.PagedCache(4, 2, 40, 33, 8)
+    assert not counted
+    ops.PagedCache(4096, 2, 40, 32, 8), ops.PagedCache(1, 2, 40, 32, 1 << 19)
+    header = open(ops.__file__.replace("0xbitnet_amd/ops.py", "include/oxbitnet_ops.h")).read()
+    for name, value in (("UNIT 32", ops.PAGED_UNIT), ("MAX_SEQ (1 << 24)", ops.PAGED_MAX_SEQ),
+                        ("MAX_BATCH 4096", ops.PAGED_MAX_BATCH), ("MAX_PREFILL 128", ops.PAGED_MAX_PREFILL)):
+        assert f"#define OXB_PAGED_{name}\n" in header and value == eval(name.split(" ", 1)[1])
