@@ -347,7 +347,8 @@ extern "C" int oxb_paged_append(void *pages, int n_pages, int page_size, int Hkv
                                 const int *slots, int n_tok, void *stream) {
     clear_error();
     if (paged_check(pages, n_pages, page_size, Hkv, hd)) return -1;
-    OXB_REQUIRE(n_tok >= 0 && n_tok < (1 << 30), "paged append: %d tokens", n_tok);
+    // (a launch has less than 2^32 threads)
+    OXB_REQUIRE(n_tok >= 0 && n_tok <= (1 << 29) - kAppTokens, "paged append: %d tokens", n_tok);
     if (n_tok == 0) return 0;
     OXB_REQUIRE(k && v && slots && (((uintptr_t)k | (uintptr_t)v) & 15) == 0,
                 "paged append: k, v or slots is NULL or rows are not 16-byte aligned");

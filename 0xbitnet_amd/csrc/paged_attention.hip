@@ -1152,6 +1152,7 @@ extern "C" int oxb_attn_decode_paged(const void *q, int dtype, const void *pages
     const DecodePlan p = decode_plan(batch, Hkv, ((int64_t)table_stride * page_size + kPgUnit - 1) / kPgUnit);
     const PgDecodeArgs a{q, (const _Float16 *)pages, table, len, n_pages, paged_log(page_size), table_stride, batch,
                          H, Hkv, G, p.runs, p.most, p.slots, out, (int *)wp, (uint64_t *)(wp + w.ml), (uint64_t *)(wp + w.o)};
+    OXB_REQUIRE(p.wgs < (int64_t)1 << 24, "attention: batch %d of %d kv heads", batch, Hkv);   // (2^32 threads)
     const dim3 grid((unsigned)p.wgs), th(kDecThreads);
     hipStream_t s = (hipStream_t)stream;
     if (dtype == OXB_F32) {

@@ -435,7 +435,8 @@ int oxb_paged_update(int page_size, int batch, const int *len, const int *delta,
  * k + t*tok_stride + h*head_stride (f16; strides in elements, multiples of 8,
  * 16-byte aligned rows), or, with src_pos, src_pos[t]*128 elements further: the row
  * where the q|k|v projections leave a position in a f16 cache [Hkv][max_seq][128]
- * that serves as scratch (src_pos is then oxb_paged_update's pos; below 0: skipped). */
+ * that serves as scratch (src_pos is then oxb_paged_update's pos; below 0: skipped).
+ * n_tok is 2^29 - 32 at most. */
 int oxb_paged_append(void *pages, int n_pages, int page_size, int Hkv, int hd, const uint16_t *k,
                      const uint16_t *v, size_t tok_stride, size_t head_stride, const int *src_pos,
                      const int *slots, int n_tok, void *stream);
@@ -457,6 +458,7 @@ int oxb_paged_append(void *pages, int n_pages, int page_size, int Hkv, int hd, c
  * counters that must be zero before its first use (a zero-filled allocation) and that
  * every call leaves zero, so one serves calls of any batch and lengths in turn (the
  * size depends on H / Hkv alone).  Calls that share one must not run concurrently.
+ * batch * Hkv is 2^24 - 1025 at most.
  * Replaces nn/attention.rs:109-118 over this cache. */
 size_t oxb_attn_decode_paged_ws_bytes(int batch, int H, int Hkv, int hd);
 int oxb_attn_decode_paged(const void *q, int dtype, const void *pages, int n_pages, int page_size,

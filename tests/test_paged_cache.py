@@ -1,8 +1,11 @@
-"""ops.PagedCache's own bookkeeping on the CPU, its device arrays counted and not made."""
+"""ops.PagedCache's own bookkeeping on the CPU, its device arrays counted and not made, and
+refusals of calls larger than a launch."""
+import ctypes as C
+
 import numpy as np
 import pytest
 
-from helpers import ops
+from helpers import ops, pkg
 
 
 class Counted:
@@ -58,3 +61,15 @@ def test_shapes_are_checked_before_anything_is_allocated(counted):
     for name, value in (("UNIT 32", ops.PAGED_UNIT), ("MAX_SEQ (1 << 24)", ops.PAGED_MAX_SEQ),
                         ("MAX_BATCH 4096", ops.PAGED_MAX_BATCH), ("MAX_PREFILL 128", ops.PAGED_MAX_PREFILL)):
         assert f"#define OXB_PAGED_{name}\n" in header and value == eval(name.split(" ", 1)[1])
+
+
+def test_calls_larger_than_a_launch():
+    """2^32 threads or more are refused before any device call."""
+    L, P = ops.lib(), C.c_void_p(4096)
+    last = pkg._native.last_error
+    for n in ((1 << 29) - 31, (1 << 30) - 1, 2 ** 31 - 1):
+        assert L.oxb_paged_append(P, 4, 32, 1, 128, P, P, 128, 128, None, P, n, None) == -1
+        assert f"{n} tokens" in last()
+    for w in (1, 1 << 10):      # uncut or cut
+        assert L.oxb_attn_decode_paged(P, 0, P, 4, 32, P, w, P, 4096, 4096, 4096, 128, P, P, 1 << 40, None) == -1
+        assert "batch 4096 of 4096 kv heads" in last()
