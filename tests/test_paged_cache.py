@@ -1,5 +1,5 @@
 """ops.PagedCache's own bookkeeping on the CPU, its device arrays counted and not made, and
-refusals of calls larger than a launch."""
+refusals of calls larger than a launch, and workspaces over all batches."""
 import ctypes as C
 
 import numpy as np
@@ -73,3 +73,17 @@ def test_calls_larger_than_a_launch():
     for w in (1, 1 << 10):      # uncut or cut
         assert L.oxb_attn_decode_paged(P, 0, P, 4, 32, P, w, P, 4096, 4096, 4096, 128, P, P, 1 << 40, None) == -1
         assert "batch 4096 of 4096 kv heads" in last()
+
+
+def test_workspace_grows_with_the_batch():
+    """Up to the most sequences that a call takes, every size there is."""
+    f = ops.lib().oxb_attn_prefill_paged_ws_bytes
+    for H, hkv in ((20, 5), (8, 8), (32, 2), (7, 1), (640, 640)):
+        for n in (1, 33, 129, 1000, 4096, 33000, 100000):
+            last = 1
+            for b in (1, 2, 64, 65, 127, 128):
+                assert f(n, b, H, hkv, 128) >= last
+                last = f(n, b, H, hkv, 128)
+            assert f(n, 129, H, hkv, 128) == 0
+        sizes = [f(n, 128, H, hkv, 128) for n in (1, 2, 500, 8000, 33000, 500000, 4000000)]
+        assert sizes[0] > 0 and sizes == sorted(sizes) and sizes[-1] == sizes[-2]
