@@ -143,12 +143,13 @@ __device__ __forceinline__ R pg_uniform(const R *p) {
 // runs meet in the workspace: each stores its part and counts in, and the last one
 // joins them in order, so the sum does not depend on which is last.
 // H 20 over 5, pages of 32: 64 sequences of up to 4096, 284 MB, 60 us (4.7 TB/s);
-// four of up to 100001, 527 MB, 98.5 us (5.35 TB/s, a copy 4.9); one of 2304, 6 MB, 8.2
-// us, a chain of loads (length, page, K and V, parts) of 0.5 to 1 us each.  Sequences
-// of up to 512 positions are not cut: 32 of them 9.4 -> 8.4 us, 8 of 300 8.0 -> 7.0,
-// one of 500 7.9 -> 8.1 (since then 8.3, 6.7, 7.5).  H 32 over 2, 13 of up to 49812: 67
-// us, in two passes of 8 heads 107.  Joining 32 runs at once instead of 16 gave nothing (100000 positions
-// 47.8, 47.1 us; 2304 8.6, 9.3).
+// four of up to 100001, 527 MB, 98.5 us (5.35 TB/s, a copy 4.9); one of 100000 55.5 (4.6);
+// one of 2304, 6 MB, 8.2 us, a chain of loads (length, page, K and V, parts) of 0.5 to 1
+// us each.  Sequences of up to 16 units are not cut, which saves them the join: 32 of
+// 512 positions 8.5 us (cut from 4 units on 10.2), 8 of 300 7.1 (7.7), one of 500 7.6 (7.5);
+// uncut up to 32 units, 16 of 1000 take 11.3 for 9.2.  H 32 over 2, 13 of up to 49812: 67
+// us, in two passes of 8 heads 107.  Joining 32 runs at once instead of 16 gave nothing
+// (one of 100000, its bytes in the 256 MB cache, 47.1 for 47.8 us; 2304 9.3 for 8.6).
 constexpr int kDecWaves = 4;
 constexpr int kDecThreads = 64 * kDecWaves;
 constexpr int kDecRows = 8;            // query heads that the workgroup's threads hold a row of
@@ -504,9 +505,9 @@ __global__ __launch_bounds__(kDecThreads, 2) void paged_decode_kernel(PgDecodeAr
 // Workgroups of a launch, and the runs that are wanted beside one a sequence and head:
 // as many as are resident with them.  Where the sequences alone are half of the
 // resident workgroups or more, half as many beside them; there runs of more than
-// kDecFine units are cut further, as the rounds' ends cost more than a join then (up
-// to 4096 positions, H 20 over 5: 64 sequences 64.5 -> 61.2 us, 52 of up to 2304 34.3
-// -> 32.1; cut to 12 units 63.4 and 35.0).
+// kDecFine units are cut further, as the rounds' ends cost more than a join then (H 20
+// over 5, 52 sequences of up to 2304: 31.8 us, cut to 12 units 34.2, to 48 33.9; 96 of
+// them 55.0, 56.3, 57.6; 64 of up to 4096 60.4, 62.0, 58.6).
 struct DecodePlan {
     int runs, most, slots;
     int64_t wgs;
@@ -551,12 +552,15 @@ static DecodeWs decode_ws(int G) {
 // unit's score products alternate with this unit's exponentials, and P.V with the
 // rest of them.  K runs a unit ahead of V; rings of four units of each leave one
 // barrier per two units.
-// H 20 over 5: 8192 tokens 598 us f32 (1152 TFLOP/s of MFMA work, both parts; a large
-// f16 product of the library 1153); 12 prompts of up to 4096 510-535 us f32, 320-335
+// H 20 over 5: 8192 tokens 588 us f32 (1170 TFLOP/s of MFMA work, both parts; a large
+// f16 product of the library 1153); 12 prompts of up to 4096 507-535 us f32, 320-340
 // f16 (1050, 850 TFLOP/s), of which an f16 tile's beginning and end are 14k cycles, 12%
-// (20k with q and the output straight from and to memory); the MFMAs are busy for 62%
+// (20k with q and the output straight from and to memory); the MFMAs are busy for 62-65%
 // (f32) and 46% (f16) of all cycles.  101 tokens 12 us; 23 drafts of up to 5 tokens
-// behind up to 4000 32 us; 333 tokens behind 30011 and two shorter turns, f16, 149-160.
+// behind up to 4000 32 us; 333 tokens behind 30011 and two shorter turns, f16, 148-160.
+// With p' in two parts too, f16 takes 416 us for the prompts and 205 for the 333, and is
+// as near to 64 bits as its output's rounding (2.0e-4 in the norm; 2.6e-4 to 2.9e-4 as
+// it is, half a step of f16 being 4.9e-4).
 // Not kept (f32, f16 of the 12 prompts; then 519, 320): 64 rows a wave, one wave a SIMD
 // (859, 409: the compiler moves accumulators to and fro); tiles of 256 rows, eight
 // waves (532, 317; the 333 tokens 160 against 152); the loads of K and V spread over the
@@ -566,8 +570,8 @@ static DecodeWs decode_ws(int G) {
 // one workgroup, makes the list of runs: the tiles, each a run where they fill the
 // card (but for the last few of equal ones), else cut into runs of `per` units at
 // most, the least that keeps all runs resident at once; the longest first.  A last
-// launch joins the cut tiles' parts.  (The tiles past whole rounds of equal ones: 3300
-// tokens behind 20000 1622 -> 1228 us, where 3264 take 1213; 4096 1704 -> 1560.)
+// launch joins the cut tiles' parts.  (The tiles past whole rounds of equal ones, cut and
+// uncut: 3300 tokens behind 20000 1195 and 1622 us, where 3264 take 1174; 4096 1518 and 1704.)
 constexpr int kPreRing = 4;
 constexpr int kPreOps = kPgHalf * 2 / 16;    // 16-byte operands of a unit's K (or V)
 constexpr size_t kPreHead = kDecParts * 4;   // decode's counters, in a workspace of both, then the counts

@@ -27,7 +27,7 @@ __device__ __forceinline__ int pg_units(int64_t positions) { return (int)((posit
 constexpr int kPreWaves = 4;
 constexpr int kPreThreads = 64 * kPreWaves;
 constexpr int kPreRows = 32 * kPreWaves;
-constexpr int kPreLeast = 8;                 // units of a run
+constexpr int kPreLeast = 8;                 // units of a run (8 x 40 tokens behind 2000 36.5 us; 4 37.3, 16 39.0)
 constexpr int kPreSlots = 512;               // resident workgroups, at most
 constexpr int kPreOrder = kPreSlots;         // (a multiple of 8)
 constexpr int kPlanThreads = 1024;
@@ -73,7 +73,7 @@ __device__ __forceinline__ PgTokens pg_tokens(const PgList &a, int z) {
 // the workgroup takes one barrier, and the search for `per` starts between the bounds
 // that the units' sum gives (sum ceil(n / per) lies between sum n / per and that plus
 // the tiles), so that one round of candidates decides as a rule.  The 12 prompts' plan
-// of 664 tiles: 8.0 us (12.0 with lengths and tiles looked up in memory by each step).
+// of 664 tiles: 7.3 us (12.0 with lengths and tiles looked up in memory by each step).
 __device__ __forceinline__ void pg_list(const PgList &a) {
     constexpr int kWaves = kPlanThreads / 64;
     static_assert(kPgPrefill <= kPlanThreads && kPreSlots <= kPreList, "a thread a sequence, and a run");
@@ -146,8 +146,12 @@ __device__ __forceinline__ void pg_list(const PgList &a) {
     int per = max(mx, 1), total = nt, cuts = 0, pieces = 1;
     const int rest = a.slots > 1 ? nt % a.slots : 0;
     if (!cut && rest && 2 * rest <= a.slots) {   // (uniform)
-        // Whole rounds of tiles that are nearly equal, and a few more: those are cut so
-        // that they fill a round of their own together.
+        // Whole rounds of tiles that are nearly equal, and a few more, no more than half a
+        // round: those are cut so that they fill a round of their own together.  (H 20 over
+        // 5.  Up to a quarter of a round only: 4096 tokens behind 20000 1660 us for 1522; up
+        // to three quarters: the same, for lack of pieces.  Nearly equal, a mean of 3/4 of the
+        // longest: 4500 tokens from 0, whose mean is half of it, 203.5 us, cut too 210; at
+        // 0.9, 4200 behind 8000, f16, 485 for 458.)
         if ((float)sum > 0.75f * (float)mx * (float)nt) {
             int least = tid >= nt - rest && tid < nt ? own.units : INT32_MAX;
 #pragma unroll
